@@ -494,6 +494,178 @@ int hn_silu_mul_quant(const void *g, int64_t ldg, const void *u, int64_t ldu, in
                     "hn_silu_mul_quant launch");
 }
 
+int hn_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr, const void *weight, int64_t rows,
+                         int64_t D, float eps, int kind, int flags, void *out, int64_t ldo, void *q, int64_t ldq,
+                         float *s, int64_t s_rs, int64_t s_gs, void *stream) {
+    REQUIRE(rows == 0 || (x && r && weight && out && q && s), HN_ERR_ARG, "hn_add_rmsnorm_quant: null pointer");
+    REQUIRE(kind == HN_KIND_INT8 || kind == HN_KIND_FP8E4M3, HN_ERR_ARG, "hn_add_rmsnorm_quant: unknown kind %d", kind);
+    REQUIRE((flags & ~HN_QUANT_PER_ROW) == 0, HN_ERR_ARG, "hn_add_rmsnorm_quant: unknown flags %d", flags);
+    const bool per_row = (flags & HN_QUANT_PER_ROW) != 0;
+    REQUIRE(rows >= 0 && rows < (1LL << 31) && D > 0 && D % 128 == 0 && D <= 16384, HN_ERR_SHAPE,
+            "hn_add_rmsnorm_quant: need D %% 128 == 0 and D <= 16384 (rows=%lld D=%lld)", (long long)rows, (long long)D);
+    if (rows == 0) return HN_OK;
+    REQUIRE(ldx >= D && ldr >= D && ldo >= D && ldq >= D, HN_ERR_SHAPE, "hn_add_rmsnorm_quant: leading dimension too small");
+    REQUIRE(scale_strides_ok(rows, per_row ? 1 : D / 128, s_rs, s_gs), HN_ERR_SHAPE,
+            "hn_add_rmsnorm_quant: scale strides overlap");
+    REQUIRE(al16(x) && al16(r) && al16(weight) && al16(out) && al16(q) && ldx % 8 == 0 && ldr % 8 == 0 && ldo % 8 == 0 &&
+                ldq % 16 == 0, HN_ERR_ALIGN, "hn_add_rmsnorm_quant: 16-byte aligned pointers and row pitches needed");
+    CHECK_DEVICE(x);
+    return launched(launch_add_rmsnorm_quant(x, ldx, r, ldr, weight, rows, D, eps, kind, per_row, out, ldo, q, ldq, s, s_rs,
+                                             s_gs, (cudaStream_t)stream), "hn_add_rmsnorm_quant launch");
+}
+
+// the cache's own checks, then `a` filled in
+static int cache_args(const hn_kv_cache *c, const char *what, CacheArgs &a) {
+    REQUIRE(c && c->k && c->v && c->table && c->lengths && c->refs && c->failed, HN_ERR_ARG, "%s: null pointer in the cache", what);
+    REQUIRE((c->k_scale == nullptr) == (c->v_scale == nullptr), HN_ERR_ARG, "%s: one of the two scale pools is missing", what);
+    REQUIRE(c->layers > 0 && c->pages > 0 && c->heads > 0 && c->slots > 0 && c->width > 0, HN_ERR_SHAPE,
+            "%s: layers, pages, heads, slots and width must be positive", what);
+    REQUIRE(c->page >= 16 && c->page % 16 == 0, HN_ERR_SHAPE, "%s: the page must be a multiple of 16 tokens (%lld)", what,
+            (long long)c->page);
+    const int64_t most = 0x7fffffff;
+    REQUIRE(c->layers <= most && c->pages <= most / 4 && c->heads <= 65536 && c->slots <= most / 4 && c->page <= most &&
+                c->width <= most / c->page && c->heads * c->page <= most, HN_ERR_SHAPE, "%s: the cache is too large", what);
+    REQUIRE(al16(c->k) && al16(c->v) && al16(c->k_scale) && al16(c->v_scale), HN_ERR_ALIGN,
+            "%s: the pools must be 16-byte aligned", what);
+    a.k = c->k; a.v = c->v; a.ks = c->k_scale; a.vs = c->v_scale;
+    a.layers = (int)c->layers; a.heads = (int)c->heads;
+    a.meta.table = c->table; a.meta.lengths = c->lengths; a.meta.refs = c->refs; a.meta.failed = c->failed;
+    a.meta.slots = (int)c->slots; a.meta.width = (int)c->width; a.meta.pages = (int)c->pages; a.meta.page = (int)c->page;
+    return HN_OK;
+}
+// at most so many requests a call (their number is a grid or a loop count of int)
+constexpr int64_t MAX_REQUESTS = 1 << 24;
+
+int hn_cache_workspace(const hn_kv_cache *cache, int64_t n, int64_t *words_host) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_workspace", a)) return rc;
+    REQUIRE(words_host && n >= 0 && n <= MAX_REQUESTS, HN_ERR_ARG, "hn_cache_workspace: bad arguments");
+    const int64_t requests = cache->slots + cache->pages + 4 * n, moves = 4 + 3 * cache->pages;
+    *words_host = requests > moves ? requests : moves;
+    t_last_error.clear();
+    return HN_OK;
+}
+
+int hn_cache_extend(const hn_kv_cache *cache, const int32_t *rows, int64_t n, int64_t tokens, int32_t *ws, void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_extend", a)) return rc;
+    REQUIRE(n >= 0 && n <= MAX_REQUESTS && tokens >= 0 && tokens <= 0x3fffffff, HN_ERR_SHAPE,
+            "hn_cache_extend: bad count (n=%lld tokens=%lld)", (long long)n, (long long)tokens);
+    if (n == 0) return HN_OK;
+    REQUIRE(rows && ws, HN_ERR_ARG, "hn_cache_extend: null pointer");
+    CHECK_DEVICE(cache->k);
+    return launched(launch_cache_extend(a.meta, rows, (int)n, (int)tokens, ws, (cudaStream_t)stream), "hn_cache_extend launch");
+}
+
+int hn_cache_append(const hn_kv_cache *cache, int64_t layer, const void *k, int64_t k_bs, int64_t k_ts, int64_t k_hs,
+                    const void *v, int64_t v_bs, int64_t v_ts, int64_t v_hs, const int32_t *rows, int64_t B, int64_t n,
+                    void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_append", a)) return rc;
+    REQUIRE(layer >= 0 && layer < cache->layers, HN_ERR_SHAPE, "hn_cache_append: layer %lld of %lld", (long long)layer,
+            (long long)cache->layers);
+    REQUIRE(B >= 0 && n >= 0 && B <= MAX_REQUESTS && n <= 0x3fffffff, HN_ERR_SHAPE, "hn_cache_append: bad count");
+    if (B == 0 || n == 0) return HN_OK;
+    REQUIRE(k && v && rows, HN_ERR_ARG, "hn_cache_append: null pointer");
+    REQUIRE(al16(k) && al16(v) && (k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0, HN_ERR_ALIGN,
+            "hn_cache_append: k and v need 16-byte aligned rows of 128");
+    CHECK_DEVICE(k);
+    return launched(launch_cache_append(a, (int)layer, k, k_bs, k_ts, k_hs, v, v_bs, v_ts, v_hs, rows, (int)B, (int)n,
+                                        (cudaStream_t)stream), "hn_cache_append launch");
+}
+
+int hn_cache_free(const hn_kv_cache *cache, const int32_t *rows, int64_t n, void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_free", a)) return rc;
+    REQUIRE(n >= 0 && n <= MAX_REQUESTS, HN_ERR_SHAPE, "hn_cache_free: bad count %lld", (long long)n);
+    if (n == 0) return HN_OK;
+    REQUIRE(rows, HN_ERR_ARG, "hn_cache_free: null pointer");
+    CHECK_DEVICE(cache->k);
+    return launched(launch_cache_free(a.meta, rows, (int)n, (cudaStream_t)stream), "hn_cache_free launch");
+}
+
+int hn_cache_fork(const hn_kv_cache *cache, const int32_t *parents, const int32_t *children, int64_t n, int32_t *ws,
+                  void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_fork", a)) return rc;
+    REQUIRE(n >= 0 && n <= MAX_REQUESTS, HN_ERR_SHAPE, "hn_cache_fork: bad count %lld", (long long)n);
+    if (n == 0) return HN_OK;
+    REQUIRE(parents && children && ws, HN_ERR_ARG, "hn_cache_fork: null pointer");
+    CHECK_DEVICE(cache->k);
+    return launched(launch_cache_fork(a, parents, children, (int)n, ws, (cudaStream_t)stream), "hn_cache_fork launch");
+}
+
+int hn_cache_compact(const hn_kv_cache *cache, int32_t *ws, void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_compact", a)) return rc;
+    REQUIRE(ws, HN_ERR_ARG, "hn_cache_compact: null pointer");
+    CHECK_DEVICE(cache->k);
+    return launched(launch_cache_compact(a, ws, (cudaStream_t)stream), "hn_cache_compact launch");
+}
+
+int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {
+    CacheArgs a;
+    if (int rc = cache_args(cache, "hn_cache_copy", a)) return rc;
+    REQUIRE(n >= 0 && n <= MAX_REQUESTS, HN_ERR_SHAPE, "hn_cache_copy: bad count %lld", (long long)n);
+    if (n == 0) return HN_OK;
+    REQUIRE(src && dst, HN_ERR_ARG, "hn_cache_copy: null pointer");
+    CHECK_DEVICE(cache->k);
+    return launched(launch_cache_copy(a, src, dst, (int)n, (cudaStream_t)stream), "hn_cache_copy launch");
+}
+
+// the shape checks of hn_paged_attention and of its workspace
+static int paged_args(const hn_kv_cache *cache, const char *what, int64_t B, int64_t Lq, int64_t H, int64_t shared, int causal,
+                      PagedAttnArgs &a) {
+    if (int rc = cache_args(cache, what, a.cache)) return rc;
+    REQUIRE(B >= 0 && B <= 4096 && Lq >= 0 && H > 0 && H % cache->heads == 0, HN_ERR_SHAPE,
+            "%s: need 0 <= B <= 4096 and H a multiple of the cache's %lld heads (B=%lld Lq=%lld H=%lld)", what,
+            (long long)cache->heads, (long long)B, (long long)Lq, (long long)H);
+    REQUIRE(H <= 65536 && Lq <= (1LL << 24) && B * Lq * H <= (1LL << 29), HN_ERR_SHAPE, "%s: too many queries", what);
+    REQUIRE(shared >= 0 && shared % cache->page == 0 && shared <= cache->width * cache->page, HN_ERR_SHAPE,
+            "%s: shared must be whole pages within the table (%lld, page %lld)", what, (long long)shared, (long long)cache->page);
+    REQUIRE(causal == 0 || causal == 1, HN_ERR_ARG, "%s: causal is 0 or 1", what);
+    a.B = (int)B; a.Lq = (int)Lq; a.H = (int)H; a.shared = (int)shared; a.causal = causal;
+    return HN_OK;
+}
+
+int hn_paged_attention_workspace(const hn_kv_cache *cache, int64_t B, int64_t Lq, int64_t H, int64_t shared, int causal,
+                                 int64_t *bytes_host) {
+    PagedAttnArgs a;
+    if (int rc = paged_args(cache, "hn_paged_attention_workspace", B, Lq, H, shared, causal, a)) return rc;
+    REQUIRE(bytes_host, HN_ERR_ARG, "hn_paged_attention_workspace: null pointer");
+    *bytes_host = B == 0 || Lq == 0 ? 0 : paged_attention_ws(a);
+    t_last_error.clear();
+    return HN_OK;
+}
+
+int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, int64_t q_bs, int64_t q_ls, int64_t q_hs,
+                       const int32_t *rows, int64_t B, int64_t Lq, int64_t H, int64_t D, int64_t shared, int causal,
+                       float scale, void *out, int64_t o_bs, int64_t o_ls, int64_t o_hs, float *lse, void *ws,
+                       int64_t ws_bytes, void *stream) {
+    PagedAttnArgs a;
+    if (int rc = paged_args(cache, "hn_paged_attention", B, Lq, H, shared, causal, a)) return rc;
+    REQUIRE(D == 128, HN_ERR_UNSUPPORTED, "hn_paged_attention: head dim %lld (128 is supported)", (long long)D);
+    REQUIRE(layer >= 0 && layer < cache->layers, HN_ERR_SHAPE, "hn_paged_attention: layer %lld of %lld", (long long)layer,
+            (long long)cache->layers);
+    if (B == 0 || Lq == 0) return HN_OK;
+    REQUIRE(q && rows && out && ws, HN_ERR_ARG, "hn_paged_attention: null pointer");
+    REQUIRE(al16(q) && al16(out) && al16(ws) && (q_bs | q_ls | q_hs | o_bs | o_ls | o_hs) % 8 == 0, HN_ERR_ALIGN,
+            "hn_paged_attention: q, out and ws must be 16-byte aligned, strides multiples of 8 elements");
+    CHECK_DEVICE(q);
+    const int64_t tokens = layer * cache->pages * cache->heads * cache->page;
+    const int64_t row_bytes = cache->k_scale ? 128 : 256;
+    a.cache.k = static_cast<uint8_t *>(cache->k) + tokens * row_bytes;
+    a.cache.v = static_cast<uint8_t *>(cache->v) + tokens * row_bytes;
+    if (cache->k_scale) { a.cache.ks += tokens; a.cache.vs += tokens; }
+    a.q = q; a.q_bs = q_bs; a.q_ls = q_ls; a.q_hs = q_hs;
+    a.out = out; a.o_bs = o_bs; a.o_ls = o_ls; a.o_hs = o_hs;
+    a.lse = lse; a.rows = rows; a.scale = scale; a.ws = ws; a.ws_bytes = ws_bytes;
+    const int64_t need = paged_attention_ws(a);
+    REQUIRE(ws_bytes >= need, HN_ERR_ARG, "hn_paged_attention: the workspace has %lld bytes, %lld are needed",
+            (long long)ws_bytes, (long long)need);
+    return launched(launch_paged_attention(a, (cudaStream_t)stream), "hn_paged_attention launch");
+}
+
 int hn_quantize_fp8_block(const void *w, int w_dtype, int64_t N, int64_t K, void *q, float *s, void *stream) {
     REQUIRE(w && q && s, HN_ERR_ARG, "hn_quantize_fp8_block: null pointer");
     REQUIRE(w_dtype == HN_DTYPE_FP32 || w_dtype == HN_DTYPE_BF16, HN_ERR_ARG,

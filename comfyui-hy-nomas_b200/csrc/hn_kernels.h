@@ -100,4 +100,41 @@ cudaError_t launch_attn_merge(const MergeArgs &a, cudaStream_t st);
 cudaError_t launch_wait_flags(const uint32_t *flags, int groups, int count, int group_stride, int skip,
                               uint32_t value, uint32_t timeout_us, cudaStream_t st);
 
+// the paged K/V cache (cache.cu, paged_attention.cu): page table, lengths, reference counts, failure counter
+struct Meta {
+    int *table, *lengths, *refs, *failed;
+    int slots, width, pages, page;
+};
+struct CacheArgs {
+    void *k, *v;            // [layers][pages][heads][page][128], bf16, or int8 with scales
+    float *ks, *vs;         // [layers][pages][heads][page], or null: bf16
+    int layers, heads;
+    Meta meta;
+};
+cudaError_t launch_cache_extend(const Meta &m, const int *rows, int n, int tokens, int *ws, cudaStream_t st);
+cudaError_t launch_cache_free(const Meta &m, const int *rows, int n, cudaStream_t st);
+cudaError_t launch_cache_fork(const CacheArgs &a, const int *parents, const int *children, int n, int *ws, cudaStream_t st);
+cudaError_t launch_cache_compact(const CacheArgs &a, int *ws, cudaStream_t st);
+cudaError_t launch_cache_copy(const CacheArgs &a, const int *src, const int *dst, int n, cudaStream_t st);
+cudaError_t launch_cache_append(const CacheArgs &a, int layer, const void *k, int64_t k_bs, int64_t k_ts, int64_t k_hs,
+                                const void *v, int64_t v_bs, int64_t v_ts, int64_t v_hs, const int *rows, int B, int n,
+                                cudaStream_t st);
+
+struct PagedAttnArgs {
+    const void *q; int64_t q_bs, q_ls, q_hs;
+    void *out; int64_t o_bs, o_ls, o_hs;
+    float *lse;             // [B, H, Lq] or null
+    CacheArgs cache;        // pools of the one layer that is read
+    const int *rows;
+    int B, Lq, H, shared, causal;
+    float scale;
+    void *ws; int64_t ws_bytes;
+};
+int64_t paged_attention_ws(const PagedAttnArgs &a);
+cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st);
+
+cudaError_t launch_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr, const void *weight,
+                                     int64_t rows, int64_t D, float eps, int kind, bool per_row, void *out, int64_t ldo,
+                                     void *q, int64_t ldq, float *s, int64_t s_rs, int64_t s_gs, cudaStream_t st);
+
 } // namespace hn

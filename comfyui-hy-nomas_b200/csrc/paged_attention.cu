@@ -1,0 +1,666 @@
+// paged_attention.cu - attention over the paged K/V cache of sequences that share their first tokens:
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale * q_i . k_j - m_i),  j < limit_i
+// limit_i = the sequence's length, or (causal) length - Lq + i + 1. A row that sees no key gives 0. With a shared part
+// (the first `shared` tokens of every listed sequence are on the same pages) the rows of all sequences attend to it
+// together - its K and V are read once, not once per sequence - and each sequence's rows to its own tokens; the
+// two results are joined by their maxima and sums.
+//
+// Heads of 128, H query heads on Hkv K/V heads (H / Hkv rows per token share a head's K and V). Rows of a tile:
+// (sequence,) token, group member. A tile of 16, 32 or 64 rows walks its keys in blocks of 64; the blocks of all tiles
+// form one line, cut into equal parts for the CTAs, so that long and short sequences load them evenly (every CTA
+// computes the cut itself from the lengths on the device). A tile that spans CTAs leaves a partial result per CTA
+// (fp32 sums, maximum, normaliser), joined by k_paged_join.
+//
+// Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head).
+// Per warp: 16 rows; m16n8k16 products, S and O in registers. The four warps split a block's keys (16-row tiles), its
+// rows (64), or both (32). Blocks arrive by cp.async, STAGES deep; the smem chunks are permuted so that no read conflicts.
+//  - bf16 cache: K by ldmatrix, V by its transposing form, P rounded to bf16.
+//  - int8 cache: codes become fp16 integers (exact: 0x6400 | (code + 128) is 1152 + code), so the scales stay outside the
+//    products: x_j = (q . ck_j) * sk_j * scale + log2 sv_j (base 2), P'_j = 2^(x_j - m + 14) multiplies cv_j, and the
+//    normaliser sums P'_j / sv_j. Taking the maximum over x_j keeps P' in fp16's range whatever the scales are.
+//    q is brought to fp16 by a power of two per row (exact but for values 2^-24 below the row's largest).
+#include <cuda_fp16.h>
+
+#include "hn_common.cuh"
+#include "hn_kernels.h"
+
+namespace hn {
+namespace paged {
+
+constexpr int HD = 128;
+constexpr int BK = 64;                  // keys per block
+constexpr int THREADS = 128;
+constexpr int MAX_B = 4096;             // sequences (their block counts' prefix sums sit in shared memory)
+constexpr float P_SHIFT = 14.0f;        // int8: P' <= 2^14
+
+struct Params {
+    const __nv_bfloat16 *q; int64_t q_bs, q_ls, q_hs;
+    __nv_bfloat16 *out; int64_t o_bs, o_ls, o_hs;
+    float *lse;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    const int *table, *lengths, *rows;
+    int slots, width, pages, page;
+    int B, Lq, H, Hkv, G, shared, causal;
+    float sl2;                          // scale * log2 e
+    int nbA, nrtA, ta, nrtB, tb;        // shared part: blocks, row tiles per head, rows per tile; own part
+    float *part_o, *part_ml;            // [slots][rows per slot][128], [slots][rows per slot][2]
+    int *sched;                         // [B + 1] prefix sums of the own blocks, written for the join
+    int part_rows, min_quota;
+};
+
+__device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+    return r;
+}
+// c += a b, 16 x 8 x 16, fp32 sums
+template <bool I8>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+    if (I8)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two biased code bytes (code + 128) selected from w -> two fp16 integers
+template <uint32_t SEL> __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+    const uint32_t u = __byte_perm(w, 0x64646464u, SEL);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));       // 1152
+    __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&u), off);
+    return *reinterpret_cast<uint32_t *>(&x);
+}
+
+// Bytes of one stage: K and V blocks, and the int8 scales
+template <bool I8> constexpr int tile_bytes() { return BK * (I8 ? HD : 2 * HD); }
+template <bool I8> constexpr int stage_bytes() { return 2 * tile_bytes<I8>() + (I8 ? 2 * BK * 4 : 0); }
+template <bool I8> constexpr int stages() { return I8 ? 4 : 3; }
+// the ring also holds the four warps' sums when a tile ends (4 x 16 rows x 128 fp32 + maxima and normalisers)
+constexpr int END_BYTES = 4 * 16 * HD * 4 + 4 * 16 * 2 * 4;
+template <bool I8> constexpr int smem_bytes() {
+    return stages<I8>() * stage_bytes<I8>() > END_BYTES ? stages<I8>() * stage_bytes<I8>() : END_BYTES;
+}
+
+// One piece: rows [row0, row0 + 16 * RG) of a tile, key blocks [blk0, blk0 + nblk) of [kbeg, kend).
+struct Piece {
+    int own_b;          // the sequence, or -1: the shared part, rows over all sequences
+    int h, row0;        // K/V head, first row
+    int kbeg, kend;     // keys of the part
+    int blk0, nblk;
+    int slot;           // of the partial result, or -1: the rows end here
+};
+
+__device__ __forceinline__ void split_row(const Params &p, const Piece &w, int r, int &b, int &l, int &g) {
+    const int r1 = p.Lq * p.G;
+    b = w.own_b;
+    if (b < 0) { b = r / r1; r -= b * r1; }
+    l = r / p.G;
+    g = r - l * p.G;
+}
+
+template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piece &w, uint8_t *smem) {
+    constexpr int KG = 4 / RG, KW = BK / KG, NT = KW / 8;        // key groups, keys and 8-key tiles per warp and block
+    constexpr int ST = stages<I8>(), TILE = tile_bytes<I8>(), STAGE = stage_bytes<I8>();
+    constexpr int CPR = I8 ? 8 : 16;                             // 16-byte chunks per row
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rg = warp % RG, kg = warp / RG, gid = lane >> 2, tq = lane & 3;
+    const uint32_t sb = saddr(smem);
+    const int rows = w.own_b < 0 ? p.B * p.Lq * p.G : p.Lq * p.G;
+
+    // --- the two rows of this lane: their key limits and q
+    int lim[2];
+    float rowscale[2];
+    uint32_t qf[8][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = w.row0 + 16 * rg + gid + 8 * i;
+        lim[i] = w.kend;                        // a row past the tile's end: q = 0, computed and dropped
+        const __nv_bfloat16 *qp = p.q;
+        const bool valid = r < rows;
+        if (valid) {
+            int b, l, g;
+            split_row(p, w, r, b, l, g);
+            const int seq = p.rows[b];
+            const int len = (unsigned)seq < (unsigned)p.slots ? p.lengths[seq] : 0;
+            lim[i] = p.causal ? len - p.Lq + l + 1 : len;
+            if (lim[i] > w.kend) lim[i] = w.kend;
+            qp += b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + g) * p.q_hs;
+        }
+        rowscale[i] = p.sl2;
+        if (!I8) {
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                qf[s][i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 2 * tq) : 0u;
+                qf[s][2 + i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 8 + 2 * tq) : 0u;
+            }
+        } else {
+            // k-step s, element j of this lane's four: d = 64 (s / 4) + 16 tq + 4 (s % 4) + j, on both operands
+            uint32_t raw[16];
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (valid) x = *reinterpret_cast<const uint4 *>(qp + 64 * c + 16 * tq + 8 * u);
+                    raw[8 * c + 4 * u] = x.x; raw[8 * c + 4 * u + 1] = x.y;
+                    raw[8 * c + 4 * u + 2] = x.z; raw[8 * c + 4 * u + 3] = x.w;
+                }
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(fabsf(bf16_lo(raw[j])), fabsf(bf16_hi(raw[j]))));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^-e brings the largest into [1, 2); e in [-126, 126] so that both powers are normal numbers
+            int e = (int)(__float_as_uint(top) >> 23) - 127;
+            e = e < -126 ? -126 : e > 126 ? 126 : e;
+            const float down = pow2i(-e);
+            rowscale[i] *= pow2i(e);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const uint32_t x0 = raw[2 * s], x1 = raw[2 * s + 1];
+                qf[s][i] = pack_f16_rn(bf16_lo(x0) * down, bf16_hi(x0) * down);
+                qf[s][2 + i] = pack_f16_rn(bf16_lo(x1) * down, bf16_hi(x1) * down);
+            }
+        }
+    }
+    int minlim = lim[0] < lim[1] ? lim[0] : lim[1];
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+        const int y = __shfl_xor_sync(0xffffffffu, minlim, o);
+        minlim = y < minlim ? y : minlim;
+    }
+
+    // --- loader: block i of the piece into stage i % ST. A thread's chunks of step `it` are all in 16-key group
+    // it * (128 / CPR) / 16, which lies in one page (pages and the parts' first keys are multiples of 16 tokens).
+    const int seq = p.rows[w.own_b < 0 ? 0 : w.own_b];
+    const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
+    constexpr int RPI = THREADS / CPR;                           // rows per step: 8 (bf16), 16 (int8)
+    auto load = [&](int i) {
+        if (i < w.nblk) {
+            const uint32_t st = sb + (uint32_t)(i % ST) * STAGE;
+            const int k0 = w.kbeg + (w.blk0 + i) * BK;
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub) {
+                const int kk = k0 + 16 * sub, pg = kk / p.page, off = kk - pg * p.page;
+                int id = kk < w.kend && pg < p.width ? tab[pg] : -1;
+                if ((unsigned)id >= (unsigned)p.pages) id = -1;
+                const int64_t tok = ((int64_t)(id < 0 ? 0 : id) * p.Hkv + w.h) * p.page + off;
+#pragma unroll
+                for (int it = 0; it < 16 / RPI; ++it) {
+                    const int r = it * RPI + tid / CPR, c = tid % CPR, row = 16 * sub + r;
+                    const bool ok = id >= 0 && kk + r < w.kend;
+                    const int64_t src = (tok + (ok ? r : 0)) * (CPR * 16) + c * 16;
+                    const int ck = I8 ? c ^ ((row & 1) << 2) : c ^ (row & 7);
+                    const int cv = I8 ? c ^ (((row >> 1) & 3) << 1) : c ^ (row & 7);
+                    cp16(st + row * (CPR * 16) + ck * 16, p.k + (ok ? src : 0), ok);
+                    cp16(st + TILE + row * (CPR * 16) + cv * 16, p.v + (ok ? src : 0), ok);
+                }
+                if (I8 && tid < 32) {
+                    const int r = tid & 15;
+                    const bool ok = id >= 0 && kk + r < w.kend;
+                    const float *sc = tid < 16 ? p.ks : p.vs;
+                    cp4(st + 2 * TILE + (tid < 16 ? 0 : BK * 4) + (16 * sub + r) * 4, sc + (ok ? tok + r : 0), ok);
+                }
+            }
+        }
+        cp_commit();
+    };
+
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    for (int i = 0; i < ST - 1; ++i) load(i);
+    for (int i = 0; i < w.nblk; ++i) {
+        cp_wait<ST - 2>();
+        __syncthreads();                        // block i is here, and every warp is done with block i - 1
+        load(i + ST - 1);
+        const uint32_t st = sb + (uint32_t)(i % ST) * STAGE;
+        const int kw = kg * KW;                 // this warp's keys in the block
+        const int key0 = w.kbeg + (w.blk0 + i) * BK + kw;
+
+        // --- S = Q K^T
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        if (!I8) {
+#pragma unroll
+            for (int n = 0; n < NT; n += 2)
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    uint32_t b[4];
+                    const int row = kw + 8 * n + ((lane >> 4) << 3) + (lane & 7), c = 2 * ks + ((lane >> 3) & 1);
+                    ldsm4(b, st + row * 256 + ((c ^ (row & 7)) << 4));
+                    mma<I8>(s[n], qf[ks], b[0], b[1]);
+                    mma<I8>(s[n + 1], qf[ks], b[2], b[3]);
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int row = kw + 8 * n + gid;
+                    const uint4 x = lds16(st + row * 128 + (((4 * c + tq) ^ ((row & 1) << 2)) << 4));
+                    const uint32_t xs[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        mma<I8>(s[n], qf[4 * c + u], codes_f16<0x4140>(xs[u]), codes_f16<0x4342>(xs[u]));
+                }
+        }
+
+        // --- base-2 logits, masked; running maximum
+        float inv[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (I8) {
+                const float *sc = reinterpret_cast<const float *>(smem + (i % ST) * STAGE + 2 * TILE) + kw + 8 * n + 2 * tq;
+                const float2 sk = *reinterpret_cast<const float2 *>(sc);
+                float2 sv = *reinterpret_cast<const float2 *>(sc + BK);
+                // a scale below 2^-100 (an all but zero row) counts as 2^-100: its values then are below 2^-93
+                sv.x = sv.x < 0x1p-100f ? 0x1p-100f : sv.x;
+                sv.y = sv.y < 0x1p-100f ? 0x1p-100f : sv.y;
+                inv[n][0] = __frcp_rn(sv.x);
+                inv[n][1] = __frcp_rn(sv.y);
+                const float l0 = lg2(sv.x), l1 = lg2(sv.y);
+                s[n][0] = fmaf(s[n][0], sk.x * rowscale[0], l0);
+                s[n][1] = fmaf(s[n][1], sk.y * rowscale[0], l1);
+                s[n][2] = fmaf(s[n][2], sk.x * rowscale[1], l0);
+                s[n][3] = fmaf(s[n][3], sk.y * rowscale[1], l1);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= rowscale[e >> 1];
+            }
+        }
+        if (key0 + KW > minlim) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (key0 + 8 * n + 2 * tq + (e & 1) >= lim[e >> 1]) s[n][e] = -INFINITY;
+        }
+        float al[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float mn = fmaxf(m[r], top), ref = mn == -INFINITY ? 0.0f : mn;
+            al[r] = ex2(m[r] - ref);
+            m[r] = mn;
+            const float sub = I8 ? ref - P_SHIFT : ref;
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x = ex2(s[n][2 * r + e] - sub);
+                    s[n][2 * r + e] = x;
+                    sum = I8 ? fmaf(x, inv[n][e], sum) : sum + x;
+                }
+            l[r] = fmaf(l[r], al[r], sum);
+        }
+        if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                o[j][0] *= al[0]; o[j][1] *= al[0];
+                o[j][2] *= al[1]; o[j][3] *= al[1];
+            }
+        }
+
+        // --- O += P V, 16 keys at a time
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            uint32_t a[4];
+            if (I8) {
+                a[0] = pack_f16_rn(s[n][0], s[n][1]); a[1] = pack_f16_rn(s[n][2], s[n][3]);
+                a[2] = pack_f16_rn(s[n + 1][0], s[n + 1][1]); a[3] = pack_f16_rn(s[n + 1][2], s[n + 1][3]);
+            } else {
+                a[0] = bf16x2_rn(s[n][0], s[n][1]); a[1] = bf16x2_rn(s[n][2], s[n][3]);
+                a[2] = bf16x2_rn(s[n + 1][0], s[n + 1][1]); a[3] = bf16x2_rn(s[n + 1][2], s[n + 1][3]);
+            }
+            const uint32_t vt = st + TILE;
+            const int kr = kw + 8 * n;
+            if (!I8) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    uint32_t b[4];
+                    const int row = kr + (lane & 15), c = j + (lane >> 4);
+                    ldsm4t(b, vt + row * 256 + ((c ^ (row & 7)) << 4));
+                    mma<I8>(o[j], a, b[0], b[1]);
+                    mma<I8>(o[j + 1], a, b[2], b[3]);
+                }
+            } else {
+                // rows 2 tq, 2 tq + 1, 8 + 2 tq, 9 + 2 tq of the 16; chunk gid: n index gid of tile j is d = 16 gid + j
+                uint32_t x[4][4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int row = kr + 8 * (u >> 1) + 2 * tq + (u & 1);
+                    const uint4 y = lds16(vt + row * 128 + ((gid ^ (((row >> 1) & 3) << 1)) << 4));
+                    x[u][0] = y.x ^ 0x80808080u; x[u][1] = y.y ^ 0x80808080u;
+                    x[u][2] = y.z ^ 0x80808080u; x[u][3] = y.w ^ 0x80808080u;
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t lo0 = __byte_perm(x[0][c], x[1][c], 0x5140), hi0 = __byte_perm(x[0][c], x[1][c], 0x7362);
+                    const uint32_t lo1 = __byte_perm(x[2][c], x[3][c], 0x5140), hi1 = __byte_perm(x[2][c], x[3][c], 0x7362);
+                    mma<I8>(o[4 * c], a, codes_f16<0x4140>(lo0), codes_f16<0x4140>(lo1));
+                    mma<I8>(o[4 * c + 1], a, codes_f16<0x4342>(lo0), codes_f16<0x4342>(lo1));
+                    mma<I8>(o[4 * c + 2], a, codes_f16<0x4140>(hi0), codes_f16<0x4140>(hi1));
+                    mma<I8>(o[4 * c + 3], a, codes_f16<0x4342>(hi0), codes_f16<0x4342>(hi1));
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // --- the warps' sums through shared memory, joined over the key groups
+    float *so = reinterpret_cast<float *>(smem), *sm = so + 4 * 16 * HD;     // [warp][16][128], [warp][16][2]
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        const int row = 16 * warp + gid + 8 * r;
+        if (tq == 0) { sm[2 * row] = m[r]; sm[2 * row + 1] = l[r]; }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (I8) {
+                so[row * HD + 32 * tq + j] = o[j][2 * r];
+                so[row * HD + 32 * tq + 16 + j] = o[j][2 * r + 1];
+            } else {
+                so[row * HD + 8 * j + 2 * tq] = o[j][2 * r];
+                so[row * HD + 8 * j + 2 * tq + 1] = o[j][2 * r + 1];
+            }
+        }
+    }
+    __syncthreads();
+    // each warp finishes RG * 16 / 4 rows, 4 values per lane
+    for (int rr = warp; rr < 16 * RG; rr += 4) {
+        const int r = w.row0 + rr;
+        if (r >= rows) break;
+        float M = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) M = fmaxf(M, sm[2 * ((g * RG + rr / 16) * 16 + rr % 16)]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            const int row = (g * RG + rr / 16) * 16 + rr % 16;
+            const float f = ex2(sm[2 * row] - ref);
+            const float4 x = *reinterpret_cast<const float4 *>(so + row * HD + 4 * lane);
+            L = fmaf(f, sm[2 * row + 1], L);
+            acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
+            acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+        }
+        if (w.slot >= 0) {
+            const int64_t at = (int64_t)w.slot * p.part_rows + rr;
+            *reinterpret_cast<float4 *>(p.part_o + at * HD + 4 * lane) = acc;
+            if (lane == 0) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(M, L);
+        } else {
+            int b, ll, g;
+            split_row(p, w, r, b, ll, g);
+            const int head = w.h * p.G + g;
+            const float inv = L > 0.0f ? __frcp_rn(L) : L == 0.0f ? 0.0f : L;     // a NaN stays one
+            uint2 y;
+            y.x = bf16x2_rn(acc.x * inv, acc.y * inv);
+            y.y = bf16x2_rn(acc.z * inv, acc.w * inv);
+            *reinterpret_cast<uint2 *>(p.out + b * p.o_bs + ll * p.o_ls + head * p.o_hs + 4 * lane) = y;
+            if (p.lse != nullptr && lane == 0)
+                p.lse[((int64_t)b * p.H + head) * p.Lq + ll] = (M + lg2(L) - (I8 ? P_SHIFT : 0.0f)) * 0.6931471805599453f;
+        }
+    }
+    __syncthreads();                        // the ring is free for the next piece
+}
+
+__device__ __forceinline__ int own_blocks(const Params &p, int b, int &len) {
+    const int seq = p.rows[b];
+    len = (unsigned)seq < (unsigned)p.slots ? p.lengths[seq] : 0;
+    const int most = p.width * p.page;
+    if (len > most) len = most;
+    const int first = p.nbA ? p.shared : 0;
+    return len > first ? (len - first + BK - 1) / BK : 0;
+}
+
+// pre[b] = own blocks of the sequences before b (every CTA computes it; B <= MAX_B)
+__device__ void prefix_blocks(const Params &p, int *pre) {
+    __shared__ int sums[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+        int len;
+        const int n = b0 + tid < p.B ? own_blocks(p, b0 + tid, len) : 0;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        for (int i = 0; i < warp; ++i) x += sums[i];
+        const int total = sums[0] + sums[1] + sums[2] + sums[3];
+        if (b0 + tid < p.B) pre[b0 + tid] = base + x - n;
+        base += total;
+        __syncthreads();
+    }
+    if (tid == 0) pre[p.B] = base;
+    __syncthreads();
+}
+
+__device__ __forceinline__ int64_t quota_of(const Params &p, int64_t total, int ctas) {
+    const int64_t q = (total + ctas - 1) / ctas;
+    return q < p.min_quota ? p.min_quota : q;
+}
+
+template <bool I8> __global__ void __launch_bounds__(THREADS) k_paged_attention(const Params p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    int *pre = reinterpret_cast<int *>(smem + smem_bytes<I8>());
+    prefix_blocks(p, pre);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= p.B; b += THREADS) p.sched[b] = pre[b];
+    const int tilesA = p.nbA ? p.Hkv * p.nrtA : 0, tilesB = p.Hkv * p.nrtB;      // tilesB: per sequence
+    const int64_t blocksA = (int64_t)tilesA * p.nbA, total = blocksA + (int64_t)pre[p.B] * tilesB;
+    const int64_t quota = quota_of(p, total, gridDim.x);
+    int64_t x = quota * blockIdx.x;
+    const int64_t end = x + quota < total ? x + quota : total;
+    while (x < end) {
+        Piece w;
+        int64_t tile_end;
+        int tile, rows_per;
+        if (x < blocksA) {
+            tile = (int)(x / p.nbA);
+            w.own_b = -1;
+            w.h = tile / p.nrtA;
+            rows_per = p.ta;
+            w.row0 = (tile - w.h * p.nrtA) * p.ta;
+            w.kbeg = 0; w.kend = p.shared;
+            w.blk0 = (int)(x - (int64_t)tile * p.nbA);
+            tile_end = (int64_t)(tile + 1) * p.nbA;
+        } else {
+            const int64_t y = x - blocksA;
+            int lo = 0, hi = p.B - 1;                    // the last b with pre[b] * tilesB <= y
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if ((int64_t)pre[mid] * tilesB <= y) lo = mid; else hi = mid - 1;
+            }
+            const int nb = pre[lo + 1] - pre[lo];
+            const int64_t z = y - (int64_t)pre[lo] * tilesB;
+            const int t = (int)(z / nb);
+            tile = tilesA + lo * tilesB + t;
+            w.own_b = lo;
+            w.h = t / p.nrtB;
+            rows_per = p.tb;
+            w.row0 = (t - w.h * p.nrtB) * p.tb;
+            w.kbeg = p.nbA ? p.shared : 0;
+            own_blocks(p, lo, w.kend);
+            w.blk0 = (int)(z - (int64_t)t * nb);
+            tile_end = x - w.blk0 + nb;
+        }
+        const int64_t stop = end < tile_end ? end : tile_end;
+        w.nblk = (int)(stop - x);
+        const bool whole = w.blk0 == 0 && stop == tile_end && p.nbA == 0;
+        w.slot = whole ? -1 : tile + (int)blockIdx.x;
+        if (rows_per == 16) run_piece<I8, 1>(p, w, smem);
+        else if (rows_per == 32) run_piece<I8, 2>(p, w, smem);
+        else run_piece<I8, 4>(p, w, smem);
+        x = stop;
+    }
+}
+
+// Joins the partial results of every row (one warp each): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
+template <bool I8> __global__ void __launch_bounds__(256) k_paged_join(const Params p, int ctas) {
+    const int lane = threadIdx.x & 31;
+    const int64_t items = (int64_t)p.B * p.Lq * p.H;
+    const int tilesA = p.nbA ? p.Hkv * p.nrtA : 0, tilesB = p.Hkv * p.nrtB;
+    const int64_t blocksA = (int64_t)tilesA * p.nbA, total = blocksA + (int64_t)p.sched[p.B] * tilesB;
+    const int64_t quota = quota_of(p, total, ctas);
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
+        const int head = (int)(it % p.H);
+        const int64_t bl = it / p.H;
+        const int l = (int)(bl % p.Lq), b = (int)(bl / p.Lq);
+        const int h = head / p.G, r = l * p.G + head - h * p.G;
+        const int nb = p.sched[b + 1] - p.sched[b];
+        float M = -INFINITY, L = 0.0f;
+        float4 acc = make_float4(0, 0, 0, 0);
+        auto take = [&](int tile, int64_t first, int n, int row) {
+            const int c0 = (int)(first / quota), c1 = (int)((first + n - 1) / quota);
+            for (int c = c0; c <= c1; ++c) {
+                const int64_t at = (int64_t)(tile + c) * p.part_rows + row;
+                const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
+                const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * HD + 4 * lane);
+                const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+                const float f0 = ex2(M - ref), f1 = ex2(ml.x - ref);
+                M = mn;
+                L = fmaf(L, f0, f1 * ml.y);
+                acc.x = fmaf(acc.x, f0, f1 * x.x); acc.y = fmaf(acc.y, f0, f1 * x.y);
+                acc.z = fmaf(acc.z, f0, f1 * x.z); acc.w = fmaf(acc.w, f0, f1 * x.w);
+            }
+        };
+        if (p.nbA) {
+            const int64_t ra = (int64_t)b * p.Lq * p.G + r;
+            const int tile = h * p.nrtA + (int)(ra / p.ta);
+            take(tile, (int64_t)tile * p.nbA, p.nbA, (int)(ra % p.ta));
+        }
+        if (nb > 0) {
+            const int t = h * p.nrtB + r / p.tb;
+            const int64_t first = blocksA + (int64_t)p.sched[b] * tilesB + (int64_t)t * nb;
+            if (p.nbA == 0 && first / quota == (first + nb - 1) / quota) continue;      // the rows ended in their CTA
+            take(tilesA + b * tilesB + t, first, nb, r % p.tb);
+        }
+        const float inv = L > 0.0f ? __frcp_rn(L) : L == 0.0f ? 0.0f : L;
+        uint2 y;
+        y.x = bf16x2_rn(acc.x * inv, acc.y * inv);
+        y.y = bf16x2_rn(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2 *>(p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs + 4 * lane) = y;
+        if (p.lse != nullptr && lane == 0)
+            p.lse[((int64_t)b * p.H + head) * p.Lq + l] = (M + lg2(L) - (I8 ? P_SHIFT : 0.0f)) * 0.6931471805599453f;
+    }
+}
+
+static int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// CTAs of the main kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
+static int ctas_for(bool i8) { return num_sms() * (i8 ? 3 : 2); }
+
+static void plan(const PagedAttnArgs &a, Params &p, int64_t &slots) {
+    p.B = a.B; p.Lq = a.Lq; p.H = a.H; p.Hkv = a.cache.heads; p.G = a.H / a.cache.heads;
+    p.shared = a.shared; p.causal = a.causal;
+    const int64_t r1 = (int64_t)a.Lq * p.G;
+    // one sequence has nothing to share: it walks all of its keys as its own
+    const bool split = a.shared > 0 && a.B > 1;
+    p.nbA = split ? (int)cdiv(a.shared, BK) : 0;
+    p.ta = tile_rows(r1 * a.B); p.tb = tile_rows(r1);
+    p.nrtA = (int)cdiv(r1 * a.B, p.ta); p.nrtB = (int)cdiv(r1, p.tb);
+    p.part_rows = p.ta > p.tb ? p.ta : p.tb;
+    p.min_quota = 4;
+    const int64_t tiles = (split ? (int64_t)p.Hkv * p.nrtA : 0) + (int64_t)a.B * p.Hkv * p.nrtB;
+    slots = tiles + ctas_for(a.cache.ks != nullptr);
+}
+
+} // namespace paged
+
+int64_t paged_attention_ws(const PagedAttnArgs &a) {
+    paged::Params p;
+    int64_t slots;
+    paged::plan(a, p, slots);
+    return slots * p.part_rows * (paged::HD + 2) * 4 + ((int64_t)a.B + 1) * 4;
+}
+
+cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
+    using namespace paged;
+    Params p;
+    int64_t slots;
+    plan(a, p, slots);
+    const bool i8 = a.cache.ks != nullptr;
+    p.q = static_cast<const __nv_bfloat16 *>(a.q); p.q_bs = a.q_bs; p.q_ls = a.q_ls; p.q_hs = a.q_hs;
+    p.out = static_cast<__nv_bfloat16 *>(a.out); p.o_bs = a.o_bs; p.o_ls = a.o_ls; p.o_hs = a.o_hs;
+    p.lse = a.lse;
+    p.k = static_cast<const uint8_t *>(a.cache.k); p.v = static_cast<const uint8_t *>(a.cache.v);
+    p.ks = a.cache.ks; p.vs = a.cache.vs;
+    p.table = a.cache.meta.table; p.lengths = a.cache.meta.lengths; p.rows = a.rows;
+    p.slots = a.cache.meta.slots; p.width = a.cache.meta.width; p.pages = a.cache.meta.pages; p.page = a.cache.meta.page;
+    p.sl2 = a.scale * 1.4426950408889634f;
+    p.part_o = static_cast<float *>(a.ws);
+    p.part_ml = p.part_o + slots * p.part_rows * HD;
+    p.sched = reinterpret_cast<int *>(p.part_ml + slots * p.part_rows * 2);
+    const int ctas = ctas_for(i8);
+    const int smem = (i8 ? smem_bytes<true>() : smem_bytes<false>()) + (a.B + 1) * 4;
+    static bool configured[HN_MAX_DEV];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
+    if (!configured[dev]) {
+        const int extra = (MAX_B + 1) * 4;
+        e = cudaFuncSetAttribute(k_paged_attention<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<true>() + extra);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(k_paged_attention<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     smem_bytes<false>() + extra);
+        if (e != cudaSuccess) return e;
+        configured[dev] = true;
+    }
+    if (i8) k_paged_attention<true><<<ctas, THREADS, smem, st>>>(p);
+    else k_paged_attention<false><<<ctas, THREADS, smem, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const int64_t rows = (int64_t)a.B * a.Lq * a.H;
+    int64_t grid = cdiv(rows, 8);
+    if (grid > (int64_t)num_sms() * 8) grid = (int64_t)num_sms() * 8;
+    if (i8) k_paged_join<true><<<(unsigned)grid, 256, 0, st>>>(p, ctas);
+    else k_paged_join<false><<<(unsigned)grid, 256, 0, st>>>(p, ctas);
+    return cudaGetLastError();
+}
+
+} // namespace hn

@@ -46,6 +46,17 @@ SIGNATURES = {
     "hn_quantize_fp8_block": [_V, _I32, _I64, _I64, _V, _V, _V],
     "hn_rmsnorm_quant": [_V, _I64, _V, _I64, _I64, _F32, _I32, _V, _I64, _V, _I64, _I64, _V],
     "hn_silu_mul_quant": [_V, _I64, _V, _I64, _I64, _I64, _I32, _V, _I64, _V, _I64, _I64, _V],
+    "hn_add_rmsnorm_quant": [_V, _I64, _V, _I64, _V, _I64, _I64, _F32, _I32, _I32, _V, _I64, _V, _I64, _V, _I64, _I64, _V],
+    "hn_cache_workspace": [_V, _I64, ctypes.POINTER(ctypes.c_int64)],
+    "hn_cache_extend": [_V, _V, _I64, _I64, _V, _V],
+    "hn_cache_append": [_V, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _V],
+    "hn_cache_free": [_V, _V, _I64, _V],
+    "hn_cache_fork": [_V, _V, _V, _I64, _V, _V],
+    "hn_cache_compact": [_V, _V, _V],
+    "hn_cache_copy": [_V, _V, _V, _I64, _V],
+    "hn_paged_attention_workspace": [_V, _I64, _I64, _I64, _I64, _I32, ctypes.POINTER(ctypes.c_int64)],
+    "hn_paged_attention": [_V, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I32, _F32, _V, _I64, _I64,
+                           _I64, _V, _V, _I64, _V],
     "hn_attention": [_V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                      _F32, _V, _I64, _I64, _I64, _V, _V, _V],
     "hn_attn_merge": [_V, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _V, _I64, _I64, _I64,

@@ -230,3 +230,45 @@ def silu_mul_quant(gate, up, kind="fp8"):
                                     q.stride(0), _lib.ptr(s), srs, sgs, _lib.stream_of(g))
     _lib.check(rc, "silu_mul_quant")
     return q, s
+
+
+def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False, out=None):
+    """The residual's addition, RMSNorm and the quantizer of the linears that read it, in one pass: x, residual
+    [..., D] bf16 -> (x + residual as bf16, codes [rows, D], fp32 scales [rows, D / 128], or [rows, 1] `per_token`). The
+    norm reads the fp32 sum and its result is quantized in fp32, so nothing is rounded but what is returned; for the
+    reference's RMSNorm with its two bf16 roundings add first and call `rmsnorm_quant`. `out`: a caller-owned bf16
+    tensor of x's shape, last dimension contiguous (x or residual themselves may be given: the stream's update in place)."""
+    _lib.require_cuda(x, residual, weight)
+    _bf16(x, residual, weight)
+    if x.shape != residual.shape or weight.shape != x.shape[-1:]:
+        raise ValueError(f"add_rmsnorm_quant: x {tuple(x.shape)}, residual {tuple(residual.shape)} and weight "
+                         f"{tuple(weight.shape)} do not match")
+    if out is not None and (out.shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device):
+        raise ValueError(f"add_rmsnorm_quant: out must be a bf16 {tuple(x.shape)} tensor on {x.device}")
+    d = x.shape[-1]
+    x2, r2, w = _rows16(x.reshape(-1, d)), _rows16(residual.reshape(-1, d)), _lib.dense(weight)
+    rows = x2.shape[0]
+    total = torch.empty(x.shape, device=x.device, dtype=torch.bfloat16) if out is None else out
+    o2 = total.view(-1, d)
+    if out is not None and not _rows16_ok(o2):
+        raise ValueError("add_rmsnorm_quant: out needs contiguous, 16-byte aligned rows")
+    code, dtype = _KINDS[kind]
+    q = torch.empty((rows, d), device=x.device, dtype=dtype)
+    if per_token:
+        s, srs, sgs = torch.empty((rows, 1), device=x.device, dtype=torch.float32), 1, 1
+    else:
+        s, srs, sgs = _lib.group_scales(rows, d // 128, x.device)
+    rc = _lib.lib.hn_add_rmsnorm_quant(x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), w.data_ptr(), rows, d, eps,
+                                       code, 1 if per_token else 0, o2.data_ptr(), o2.stride(0), q.data_ptr(), d,
+                                       s.data_ptr(), srs, sgs, _lib.stream_of(x2))
+    _lib.check(rc, "add_rmsnorm_quant")
+    return total, q, s
+
+
+def _rows16_ok(t):
+    return t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
+
+
+def _rows16(t):
+    """[rows, D] whose rows start on 16-byte boundaries: t itself, or a dense copy (of an expanded view, too)."""
+    return t if _rows16_ok(t) else _lib.dense(t)

@@ -322,6 +322,75 @@ int hn_peer_push2d(void *dst, int64_t dpitch, const void *src, int64_t spitch, i
 int hn_wait_flags(const int32_t *flags, int64_t groups, int64_t count, int64_t group_stride, int64_t skip,
                   uint32_t value, uint32_t timeout_us, void *stream);
 
+/*
+ * Residual addition + RMSNorm + the 8-bit quantizer of the linears that follow, in one pass:
+ *   h = x + r (fp32), out = bf16(h), y = h / sqrt(mean(h^2) + eps) * weight (fp32, from the unrounded h),
+ *   codes and scales of y as in hn_quant_act (int8 half away from zero, or e4m3), per row and 128 columns or per row
+ *   (flags HN_QUANT_PER_ROW: scale s[row * s_rs]). A NaN in a group gives a NaN scale.
+ * No reference counterpart as one call: the decoder layer's `x = x + sublayer(x)` and its next norm
+ * (hy_nomas/pixelumm.py:246-259, 330-337). hn_rmsnorm_quant rounds the normalized row to bf16 twice as the reference's
+ * RMSNorm does; this one rounds only what it stores. x, r, out [rows, D] bf16 (pitches ldx, ldr, ldo; out may be x
+ * or r), q [rows, D] codes. D % 128 == 0, D <= 16384; 16-byte aligned pointers and row pitches.
+ */
+int hn_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr, const void *weight, int64_t rows,
+                         int64_t D, float eps, int kind, int flags, void *out, int64_t ldo, void *q, int64_t ldq,
+                         float *s, int64_t s_rs, int64_t s_gs, void *stream);
+
+/*
+ * The paged K/V cache of forked sequences. No reference counterpart: the reference keeps one int8 history per run
+ * (hy_nomas/world.py:80-204); this holds many sequences that share pages, in the same two formats.
+ *   k, v [layers][pages][heads][page][128]: bf16, or int8 codes with k_scale, v_scale [layers][pages][heads][page]
+ *   fp32 per (token, head) (both null: bf16). page: tokens per page, a multiple of 16.
+ *   table [slots][width] page ids (-1: none), lengths [slots], refs [pages] (0: free), failed [1]: requests that could
+ *   not be met, added up. All device memory, one page table for all layers.
+ * New pages are the free ids, lowest first, handed out in the order of the requests. A request that cannot be met (no
+ * free page, a full table row, an id out of range, a row listed twice, a child that is not empty) changes nothing but
+ * *failed. `rows`, `parents`, `children`, `src`, `dst` are int32 device arrays. Nothing synchronizes.
+ *
+ * hn_cache_workspace: int32 words of scratch that extend / fork / compact take in `ws` for n requests.
+ * hn_cache_extend: each listed row grows by `tokens`, on new pages where needed.
+ * hn_cache_append: k, v [B, n, heads, 128] bf16 (strides in elements for batch, token, head; multiples of 8; the
+ *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic).
+ * hn_cache_free: the listed rows drop their pages and become empty.
+ * hn_cache_fork: children[i] (empty, listed once) becomes a copy of parents[i]: full pages are shared, the tokens of a
+ *   partial last page are copied to a new page, in every layer.
+ * hn_cache_compact: pages move (in every layer) so that the used ids are 0 .. n_used - 1; the table follows.
+ * hn_cache_copy: page src[i] to page dst[i] in every layer; no page is both in src and in dst, or twice in dst.
+ */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t *table, *lengths, *refs, *failed;
+    int64_t layers, pages, heads, page, slots, width;
+} hn_kv_cache;
+int hn_cache_workspace(const hn_kv_cache *cache, int64_t n, int64_t *words_host);
+int hn_cache_extend(const hn_kv_cache *cache, const int32_t *rows, int64_t n, int64_t tokens, int32_t *ws, void *stream);
+int hn_cache_append(const hn_kv_cache *cache, int64_t layer, const void *k, int64_t k_bs, int64_t k_ts, int64_t k_hs,
+                    const void *v, int64_t v_bs, int64_t v_ts, int64_t v_hs, const int32_t *rows, int64_t B, int64_t n,
+                    void *stream);
+int hn_cache_free(const hn_kv_cache *cache, const int32_t *rows, int64_t n, void *stream);
+int hn_cache_fork(const hn_kv_cache *cache, const int32_t *parents, const int32_t *children, int64_t n, int32_t *ws,
+                  void *stream);
+int hn_cache_compact(const hn_kv_cache *cache, int32_t *ws, void *stream);
+int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+/*
+ * Attention over the paged cache for sequences that share their first `shared` tokens (a multiple of the page; on the
+ * same pages in every listed row; 0: nothing is shared): out = softmax(q k^T * scale) v over each sequence's tokens, or,
+ * `causal`, query i of Lq at position lengths - Lq + i sees the tokens up to its own. The shared tokens are read once
+ * for all sequences. A query that sees nothing gives 0 (lse -inf).
+ * q, out [B, Lq, H, 128] bf16 (element strides for batch, query, head; multiples of 8), H a multiple of the cache's
+ * heads (query heads h * H / heads .. share K/V head h), lse [B, H, Lq] fp32 natural log or NULL. rows [B] int32.
+ * Scales of an int8 cache are positive, as its quantizer gives them. ws: hn_paged_attention_workspace bytes, 16-byte
+ * aligned. B <= 4096.
+ */
+int hn_paged_attention_workspace(const hn_kv_cache *cache, int64_t B, int64_t Lq, int64_t H, int64_t shared, int causal,
+                                 int64_t *bytes_host);
+int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, int64_t q_bs, int64_t q_ls, int64_t q_hs,
+                       const int32_t *rows, int64_t B, int64_t Lq, int64_t H, int64_t D, int64_t shared, int causal,
+                       float scale, void *out, int64_t o_bs, int64_t o_ls, int64_t o_hs, float *lse, void *ws,
+                       int64_t ws_bytes, void *stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
