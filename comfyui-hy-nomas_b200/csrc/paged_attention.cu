@@ -21,33 +21,14 @@
 //    q is brought to fp16 by a power of two per row (exact but for values 2^-24 below the row's largest).
 #include <cuda_fp16.h>
 
-#include "hn_common.cuh"
-#include "hn_kernels.h"
+#include "paged.cuh"
 
 namespace hn {
 namespace paged {
 
-constexpr int HD = 128;
 constexpr int BK = 64;                  // keys per block
 constexpr int THREADS = 128;
-constexpr int MAX_B = 4096;             // sequences (their block counts' prefix sums sit in shared memory)
 constexpr float P_SHIFT = 14.0f;        // int8: P' <= 2^14
-
-struct Params {
-    const __nv_bfloat16 *q; int64_t q_bs, q_ls, q_hs;
-    __nv_bfloat16 *out; int64_t o_bs, o_ls, o_hs;
-    float *lse;
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    const int *table, *lengths, *rows;
-    int slots, width, pages, page;
-    int B, Lq, H, Hkv, G, shared, causal;
-    float sl2;                          // scale * log2 e
-    int nbA, nrtA, ta, nrtB, tb;        // shared part: blocks, row tiles per head, rows per tile; own part
-    float *part_o, *part_ml;            // [slots][rows per slot][128], [slots][rows per slot][2]
-    int *sched;                         // [B + 1] prefix sums of the own blocks, written for the join
-    int part_rows, min_quota;
-};
 
 __device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
@@ -58,16 +39,6 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool valid) {
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -91,14 +62,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t *a, uint32_t b
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two biased code bytes (code + 128) selected from w -> two fp16 integers
-template <uint32_t SEL> __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, SEL);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));       // 1152
-    __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&u), off);
-    return *reinterpret_cast<uint32_t *>(&x);
-}
-
 // Bytes of one stage: K and V blocks, and the int8 scales
 template <bool I8> constexpr int tile_bytes() { return BK * (I8 ? HD : 2 * HD); }
 template <bool I8> constexpr int stage_bytes() { return 2 * tile_bytes<I8>() + (I8 ? 2 * BK * 4 : 0); }
@@ -107,23 +70,6 @@ template <bool I8> constexpr int stages() { return I8 ? 4 : 3; }
 constexpr int END_BYTES = 4 * 16 * HD * 4 + 4 * 16 * 2 * 4;
 template <bool I8> constexpr int smem_bytes() {
     return stages<I8>() * stage_bytes<I8>() > END_BYTES ? stages<I8>() * stage_bytes<I8>() : END_BYTES;
-}
-
-// One piece: rows [row0, row0 + 16 * RG) of a tile, key blocks [blk0, blk0 + nblk) of [kbeg, kend).
-struct Piece {
-    int own_b;          // the sequence, or -1: the shared part, rows over all sequences
-    int h, row0;        // K/V head, first row
-    int kbeg, kend;     // keys of the part
-    int blk0, nblk;
-    int slot;           // of the partial result, or -1: the rows end here
-};
-
-__device__ __forceinline__ void split_row(const Params &p, const Piece &w, int r, int &b, int &l, int &g) {
-    const int r1 = p.Lq * p.G;
-    b = w.own_b;
-    if (b < 0) { b = r / r1; r -= b * r1; }
-    l = r / p.G;
-    g = r - l * p.G;
 }
 
 template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piece &w, uint8_t *smem) {
@@ -148,9 +94,7 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
         if (valid) {
             int b, l, g;
             split_row(p, w, r, b, l, g);
-            const int seq = p.rows[b];
-            const int len = (unsigned)seq < (unsigned)p.slots ? p.lengths[seq] : 0;
-            lim[i] = p.causal ? len - p.Lq + l + 1 : len;
+            lim[i] = row_limit(p, seq_length(p, b), l);
             if (lim[i] > w.kend) lim[i] = w.kend;
             qp += b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + g) * p.q_hs;
         }
@@ -158,8 +102,8 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
         if (!I8) {
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                qf[s][i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 2 * tq) : 0u;
-                qf[s][2 + i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 8 + 2 * tq) : 0u;
+                qf[s][i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 2 * tq) ^ p.flip : 0u;
+                qf[s][2 + i] = valid ? *reinterpret_cast<const uint32_t *>(qp + 16 * s + 8 + 2 * tq) ^ p.flip : 0u;
             }
         } else {
             // k-step s, element j of this lane's four: d = 64 (s / 4) + 16 tq + 4 (s % 4) + j, on both operands
@@ -170,17 +114,15 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
                 for (int u = 0; u < 2; ++u) {
                     uint4 x = make_uint4(0, 0, 0, 0);
                     if (valid) x = *reinterpret_cast<const uint4 *>(qp + 64 * c + 16 * tq + 8 * u);
-                    raw[8 * c + 4 * u] = x.x; raw[8 * c + 4 * u + 1] = x.y;
-                    raw[8 * c + 4 * u + 2] = x.z; raw[8 * c + 4 * u + 3] = x.w;
+                    raw[8 * c + 4 * u] = x.x ^ p.flip; raw[8 * c + 4 * u + 1] = x.y ^ p.flip;
+                    raw[8 * c + 4 * u + 2] = x.z ^ p.flip; raw[8 * c + 4 * u + 3] = x.w ^ p.flip;
                 }
             float top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, fmaxf(fabsf(bf16_lo(raw[j])), fabsf(bf16_hi(raw[j]))));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^-e brings the largest into [1, 2); e in [-126, 126] so that both powers are normal numbers
-            int e = (int)(__float_as_uint(top) >> 23) - 127;
-            e = e < -126 ? -126 : e > 126 ? 126 : e;
+            const int e = row_exponent(top);
             const float down = pow2i(-e);
             rowscale[i] *= pow2i(e);
 #pragma unroll
@@ -432,234 +374,209 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
             int b, ll, g;
             split_row(p, w, r, b, ll, g);
             const int head = w.h * p.G + g;
-            const float inv = L > 0.0f ? __frcp_rn(L) : L == 0.0f ? 0.0f : L;     // a NaN stays one
+            const float inv = inverse(L);
             uint2 y;
             y.x = bf16x2_rn(acc.x * inv, acc.y * inv);
             y.y = bf16x2_rn(acc.z * inv, acc.w * inv);
             *reinterpret_cast<uint2 *>(p.out + b * p.o_bs + ll * p.o_ls + head * p.o_hs + 4 * lane) = y;
             if (p.lse != nullptr && lane == 0)
-                p.lse[((int64_t)b * p.H + head) * p.Lq + ll] = (M + lg2(L) - (I8 ? P_SHIFT : 0.0f)) * 0.6931471805599453f;
+                p.lse[((int64_t)b * p.H + head) * p.Lq + ll] = row_lse(p, M, L);
         }
     }
     __syncthreads();                        // the ring is free for the next piece
 }
 
-__device__ __forceinline__ int own_blocks(const Params &p, int b, int &len) {
-    const int seq = p.rows[b];
-    len = (unsigned)seq < (unsigned)p.slots ? p.lengths[seq] : 0;
-    const int most = p.width * p.page;
-    if (len > most) len = most;
-    const int first = p.nbA ? p.shared : 0;
-    return len > first ? (len - first + BK - 1) / BK : 0;
-}
-
-// pre[b] = own blocks of the sequences before b (every CTA computes it; B <= MAX_B)
-__device__ void prefix_blocks(const Params &p, int *pre) {
-    __shared__ int sums[4];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += THREADS) {
-        int len;
-        const int n = b0 + tid < p.B ? own_blocks(p, b0 + tid, len) : 0;
-        int x = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) sums[warp] = x;
-        __syncthreads();
-        for (int i = 0; i < warp; ++i) x += sums[i];
-        const int total = sums[0] + sums[1] + sums[2] + sums[3];
-        if (b0 + tid < p.B) pre[b0 + tid] = base + x - n;
-        base += total;
-        __syncthreads();
-    }
-    if (tid == 0) pre[p.B] = base;
-    __syncthreads();
-}
-
-__device__ __forceinline__ int64_t quota_of(const Params &p, int64_t total, int ctas) {
-    const int64_t q = (total + ctas - 1) / ctas;
-    return q < p.min_quota ? p.min_quota : q;
-}
-
 template <bool I8> __global__ void __launch_bounds__(THREADS) k_paged_attention(const Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int sums[32];
     int *pre = reinterpret_cast<int *>(smem + smem_bytes<I8>());
-    prefix_blocks(p, pre);
+    prefix_blocks(p, pre, sums, THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += THREADS) p.sched[b] = pre[b];
-    const int tilesA = p.nbA ? p.Hkv * p.nrtA : 0, tilesB = p.Hkv * p.nrtB;      // tilesB: per sequence
-    const int64_t blocksA = (int64_t)tilesA * p.nbA, total = blocksA + (int64_t)pre[p.B] * tilesB;
-    const int64_t quota = quota_of(p, total, gridDim.x);
-    int64_t x = quota * blockIdx.x;
-    const int64_t end = x + quota < total ? x + quota : total;
-    while (x < end) {
-        Piece w;
-        int64_t tile_end;
-        int tile, rows_per;
-        if (x < blocksA) {
-            tile = (int)(x / p.nbA);
-            w.own_b = -1;
-            w.h = tile / p.nrtA;
-            rows_per = p.ta;
-            w.row0 = (tile - w.h * p.nrtA) * p.ta;
-            w.kbeg = 0; w.kend = p.shared;
-            w.blk0 = (int)(x - (int64_t)tile * p.nbA);
-            tile_end = (int64_t)(tile + 1) * p.nbA;
-        } else {
-            const int64_t y = x - blocksA;
-            int lo = 0, hi = p.B - 1;                    // the last b with pre[b] * tilesB <= y
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if ((int64_t)pre[mid] * tilesB <= y) lo = mid; else hi = mid - 1;
-            }
-            const int nb = pre[lo + 1] - pre[lo];
-            const int64_t z = y - (int64_t)pre[lo] * tilesB;
-            const int t = (int)(z / nb);
-            tile = tilesA + lo * tilesB + t;
-            w.own_b = lo;
-            w.h = t / p.nrtB;
-            rows_per = p.tb;
-            w.row0 = (t - w.h * p.nrtB) * p.tb;
-            w.kbeg = p.nbA ? p.shared : 0;
-            own_blocks(p, lo, w.kend);
-            w.blk0 = (int)(z - (int64_t)t * nb);
-            tile_end = x - w.blk0 + nb;
-        }
-        const int64_t stop = end < tile_end ? end : tile_end;
-        w.nblk = (int)(stop - x);
-        const bool whole = w.blk0 == 0 && stop == tile_end && p.nbA == 0;
-        w.slot = whole ? -1 : tile + (int)blockIdx.x;
+    Walker walk(p, pre, blockIdx.x);
+    Piece w;
+    while (walk.next(p, pre, blockIdx.x, w)) {
+        const int rows_per = w.own_b < 0 ? p.ta : p.tb;
         if (rows_per == 16) run_piece<I8, 1>(p, w, smem);
         else if (rows_per == 32) run_piece<I8, 2>(p, w, smem);
         else run_piece<I8, 4>(p, w, smem);
-        x = stop;
     }
 }
 
-// Joins the partial results of every row (one warp each): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
-template <bool I8> __global__ void __launch_bounds__(256) k_paged_join(const Params p, int ctas) {
+// Joins the partial results of every row (one warp each): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. `a` is the
+// line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
+__global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b) {
     const int lane = threadIdx.x & 31;
-    const int64_t items = (int64_t)p.B * p.Lq * p.H;
-    const int tilesA = p.nbA ? p.Hkv * p.nrtA : 0, tilesB = p.Hkv * p.nrtB;
-    const int64_t blocksA = (int64_t)tilesA * p.nbA, total = blocksA + (int64_t)p.sched[p.B] * tilesB;
-    const int64_t quota = quota_of(p, total, ctas);
+    const int64_t items = (int64_t)b.B * b.Lq * b.H;
+    const int64_t blocksA = (int64_t)a.Hkv * a.nrtA * a.nbA, aheadB = (int64_t)b.Hkv * b.nrtA * b.nbA;
+    const int64_t qA = a.nbA ? Walker::quota(a, blocksA + (int64_t)a.sched[a.B] * a.Hkv) : 1;
+    const int64_t qB = Walker::quota(b, aheadB + (int64_t)b.sched[b.B] * b.Hkv);
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
-        const int head = (int)(it % p.H);
-        const int64_t bl = it / p.H;
-        const int l = (int)(bl % p.Lq), b = (int)(bl / p.Lq);
-        const int h = head / p.G, r = l * p.G + head - h * p.G;
-        const int nb = p.sched[b + 1] - p.sched[b];
+        const int64_t bl = div_nonneg(it, b.H);
+        const int head = (int)(it - bl * b.H);
+        const int s = (int)div_nonneg(bl, b.Lq), l = (int)(bl - (int64_t)s * b.Lq);
+        const int h = head / b.G, r = l * b.G + head - h * b.G;
         float M = -INFINITY, L = 0.0f;
         float4 acc = make_float4(0, 0, 0, 0);
-        auto take = [&](int tile, int64_t first, int n, int row) {
-            const int c0 = (int)(first / quota), c1 = (int)((first + n - 1) / quota);
-            for (int c = c0; c <= c1; ++c) {
-                const int64_t at = (int64_t)(tile + c) * p.part_rows + row;
-                const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
-                const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * HD + 4 * lane);
-                const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-                const float f0 = ex2(M - ref), f1 = ex2(ml.x - ref);
-                M = mn;
-                L = fmaf(L, f0, f1 * ml.y);
-                acc.x = fmaf(acc.x, f0, f1 * x.x); acc.y = fmaf(acc.y, f0, f1 * x.y);
-                acc.z = fmaf(acc.z, f0, f1 * x.z); acc.w = fmaf(acc.w, f0, f1 * x.w);
-            }
+        auto add = [&](const Params &p, int64_t at) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
+            const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * HD + 4 * lane);
+            const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f0 = ex2(M - ref), f1 = ex2(ml.x - ref);
+            M = mn;
+            L = fmaf(L, f0, f1 * ml.y);
+            acc.x = fmaf(acc.x, f0, f1 * x.x); acc.y = fmaf(acc.y, f0, f1 * x.y);
+            acc.z = fmaf(acc.z, f0, f1 * x.z); acc.w = fmaf(acc.w, f0, f1 * x.w);
         };
-        if (p.nbA) {
-            const int64_t ra = (int64_t)b * p.Lq * p.G + r;
-            const int tile = h * p.nrtA + (int)(ra / p.ta);
-            take(tile, (int64_t)tile * p.nbA, p.nbA, (int)(ra % p.ta));
+        auto take = [&](const Params &p, int tile, int64_t first, int n, int64_t quota, int row) {
+            const int c0 = (int)(first / quota), c1 = (int)((first + n - 1) / quota);
+            for (int c = c0; c <= c1; ++c)
+                for (int k = 0; k < p.halves; ++k) add(p, (int64_t)(tile + c) * p.part_rows + k * 128 + row);
+        };
+        const int len = seq_length(b, s), rt = r / b.tb, nb = own_blocks(b, len, rt);
+        const int64_t first = aheadB + (int64_t)b.sched[s] * b.Hkv +
+                              (int64_t)h * (b.sched[s + 1] - b.sched[s]) + own_blocks_below(b, len, rt);
+        // the rows ended in their CTA
+        if (b.ends && b.halves == 1 && nb > 0 && first / qB == (first + nb - 1) / qB) continue;
+        if (a.nbA) {
+            const int64_t ra = (int64_t)s * a.Lq * a.G + r;
+            const int tile = h * a.nrtA + (int)(ra / a.ta);
+            take(a, tile, (int64_t)tile * a.nbA, a.nbA, qA, (int)(ra % a.ta));
         }
-        if (nb > 0) {
-            const int t = h * p.nrtB + r / p.tb;
-            const int64_t first = blocksA + (int64_t)p.sched[b] * tilesB + (int64_t)t * nb;
-            if (p.nbA == 0 && first / quota == (first + nb - 1) / quota) continue;      // the rows ended in their CTA
-            take(tilesA + b * tilesB + t, first, nb, r % p.tb);
-        }
-        const float inv = L > 0.0f ? __frcp_rn(L) : L == 0.0f ? 0.0f : L;
+        if (nb > 0) take(b, b.Hkv * b.nrtA + (s * b.Hkv + h) * b.nrtB + rt, first, nb, qB, r % b.tb);
+        const float inv = inverse(L);
         uint2 y;
         y.x = bf16x2_rn(acc.x * inv, acc.y * inv);
         y.y = bf16x2_rn(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2 *>(p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs + 4 * lane) = y;
-        if (p.lse != nullptr && lane == 0)
-            p.lse[((int64_t)b * p.H + head) * p.Lq + l] = (M + lg2(L) - (I8 ? P_SHIFT : 0.0f)) * 0.6931471805599453f;
+        *reinterpret_cast<uint2 *>(b.out + s * b.o_bs + l * b.o_ls + head * b.o_hs + 4 * lane) = y;
+        if (b.lse != nullptr && lane == 0) b.lse[((int64_t)s * b.H + head) * b.Lq + l] = row_lse(b, M, L);
     }
 }
 
 static int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// CTAs of the streaming kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
+static int stream_ctas(bool i8) { return num_sms() * (i8 ? 3 : 2); }
+constexpr int TC_ROWS = 65;             // rows from which a tile goes to the tensor-core line
 
-// CTAs of the main kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
-static int ctas_for(bool i8) { return num_sms() * (i8 ? 3 : 2); }
+struct Plan {
+    bool shared_tc, own_tc;             // which line holds which part
+    int64_t stream_slots, tc_slots;
+    int64_t bytes;
+    size_t tc_at, sched_at;             // byte offsets in the workspace: the second line's partials, the prefix sums
+};
 
-static void plan(const PagedAttnArgs &a, Params &p, int64_t &slots) {
-    p.B = a.B; p.Lq = a.Lq; p.H = a.H; p.Hkv = a.cache.heads; p.G = a.H / a.cache.heads;
-    p.shared = a.shared; p.causal = a.causal;
-    const int64_t r1 = (int64_t)a.Lq * p.G;
-    // one sequence has nothing to share: it walks all of its keys as its own
-    const bool split = a.shared > 0 && a.B > 1;
-    p.nbA = split ? (int)cdiv(a.shared, BK) : 0;
-    p.ta = tile_rows(r1 * a.B); p.tb = tile_rows(r1);
-    p.nrtA = (int)cdiv(r1 * a.B, p.ta); p.nrtB = (int)cdiv(r1, p.tb);
-    p.part_rows = p.ta > p.tb ? p.ta : p.tb;
-    p.min_quota = 4;
-    const int64_t tiles = (split ? (int64_t)p.Hkv * p.nrtA : 0) + (int64_t)a.B * p.Hkv * p.nrtB;
-    slots = tiles + ctas_for(a.cache.ks != nullptr);
+// The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_ROWS rows per K/V head or
+// more walks all of its keys on the tensor-core line; else the rows of all sequences attend to the shared part
+// together, on the tensor cores if there are TC_ROWS of them, and the own parts stream.
+static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
+    Plan pl;
+    const bool i8 = a.cache.ks != nullptr;
+    s.B = a.B; s.Lq = a.Lq; s.H = a.H; s.Hkv = a.cache.heads; s.G = a.H / a.cache.heads;
+    s.shared = a.shared; s.causal = a.causal;
+    s.nbA = s.nrtA = 0; s.ta = 16;
+    s.has_own = 0; s.nrtB = 0; s.tb = 16; s.own_first = 0;
+    s.halves = 1; s.ends = 0; s.min_quota = 4;
+    t = s;
+    const int64_t r1 = (int64_t)a.Lq * s.G, all = r1 * a.B;
+    pl.own_tc = r1 >= TC_ROWS;
+    // one sequence has nothing to share
+    const bool split = a.shared > 0 && a.B > 1 && !pl.own_tc;
+    pl.shared_tc = split && all >= TC_ROWS;
+    s.bk = BK; s.ctas = stream_ctas(i8);
+    t.bk = 128; t.ctas = num_sms();
+    Params &own = pl.own_tc ? t : s;
+    own.has_own = 1;
+    own.own_first = split ? a.shared : 0;
+    own.ends = !split;
+    own.tb = pl.own_tc ? 256 : tile_rows(r1);
+    own.nrtB = (int)cdiv(r1, own.tb);
+    if (split) {
+        Params &sh = pl.shared_tc ? t : s;
+        sh.nbA = (int)cdiv(a.shared, sh.bk);
+        sh.ta = !pl.shared_tc ? tile_rows(all) : all <= 128 ? 128 : 256;
+        sh.nrtA = (int)cdiv(all, sh.ta);
+        if (sh.ta == 128) sh.halves = 2;
+    }
+    auto slots = [&](Params &p) -> int64_t {
+        p.part_rows = p.bk == 128 ? 256 : p.ta > p.tb ? p.ta : p.tb;
+        const int64_t tiles = (int64_t)p.Hkv * p.nrtA + (int64_t)p.B * p.Hkv * p.nrtB;
+        return tiles ? tiles + p.ctas : 0;
+    };
+    pl.stream_slots = slots(s);
+    pl.tc_slots = slots(t);
+    const int64_t row = (HD + 2) * 4;
+    pl.tc_at = (size_t)(pl.stream_slots * s.part_rows * row);
+    pl.sched_at = pl.tc_at + (size_t)(pl.tc_slots * t.part_rows * row);
+    pl.bytes = (int64_t)pl.sched_at + 2 * ((int64_t)a.B + 1) * 4;
+    return pl;
 }
 
 } // namespace paged
 
 int64_t paged_attention_ws(const PagedAttnArgs &a) {
-    paged::Params p;
-    int64_t slots;
-    paged::plan(a, p, slots);
-    return slots * p.part_rows * (paged::HD + 2) * 4 + ((int64_t)a.B + 1) * 4;
+    paged::Params s, t;
+    return paged::plan(a, s, t).bytes;
 }
 
 cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
     using namespace paged;
-    Params p;
-    int64_t slots;
-    plan(a, p, slots);
+    Params s, t;
+    const Plan pl = plan(a, s, t);
     const bool i8 = a.cache.ks != nullptr;
-    p.q = static_cast<const __nv_bfloat16 *>(a.q); p.q_bs = a.q_bs; p.q_ls = a.q_ls; p.q_hs = a.q_hs;
-    p.out = static_cast<__nv_bfloat16 *>(a.out); p.o_bs = a.o_bs; p.o_ls = a.o_ls; p.o_hs = a.o_hs;
-    p.lse = a.lse;
-    p.k = static_cast<const uint8_t *>(a.cache.k); p.v = static_cast<const uint8_t *>(a.cache.v);
-    p.ks = a.cache.ks; p.vs = a.cache.vs;
-    p.table = a.cache.meta.table; p.lengths = a.cache.meta.lengths; p.rows = a.rows;
-    p.slots = a.cache.meta.slots; p.width = a.cache.meta.width; p.pages = a.cache.meta.pages; p.page = a.cache.meta.page;
-    p.sl2 = a.scale * 1.4426950408889634f;
-    p.part_o = static_cast<float *>(a.ws);
-    p.part_ml = p.part_o + slots * p.part_rows * HD;
-    p.sched = reinterpret_cast<int *>(p.part_ml + slots * p.part_rows * 2);
-    const int ctas = ctas_for(i8);
-    const int smem = (i8 ? smem_bytes<true>() : smem_bytes<false>()) + (a.B + 1) * 4;
-    static bool configured[HN_MAX_DEV];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    int *err = nullptr;
+    cudaError_t e = device_error_word(err_slot(st), &err);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
-    if (!configured[dev]) {
-        const int extra = (MAX_B + 1) * 4;
-        e = cudaFuncSetAttribute(k_paged_attention<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<true>() + extra);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(k_paged_attention<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     smem_bytes<false>() + extra);
-        if (e != cudaSuccess) return e;
-        configured[dev] = true;
+    for (Params *p : {&s, &t}) {
+        p->q = static_cast<const __nv_bfloat16 *>(a.q); p->q_bs = a.q_bs; p->q_ls = a.q_ls; p->q_hs = a.q_hs;
+        p->out = static_cast<__nv_bfloat16 *>(a.out); p->o_bs = a.o_bs; p->o_ls = a.o_ls; p->o_hs = a.o_hs;
+        p->lse = a.lse;
+        p->k = static_cast<const uint8_t *>(a.cache.k); p->v = static_cast<const uint8_t *>(a.cache.v);
+        p->ks = a.cache.ks; p->vs = a.cache.vs;
+        p->table = a.cache.meta.table; p->lengths = a.cache.meta.lengths; p->rows = a.rows;
+        p->slots = a.cache.meta.slots; p->width = a.cache.meta.width; p->pages = a.cache.meta.pages;
+        p->page = a.cache.meta.page;
+        p->sl2 = fabsf(a.scale) * 1.4426950408889634f;
+        p->flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        p->lse_shift = i8 ? P_SHIFT : 0.0f;
+        p->err = err;
     }
-    if (i8) k_paged_attention<true><<<ctas, THREADS, smem, st>>>(p);
-    else k_paged_attention<false><<<ctas, THREADS, smem, st>>>(p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    const int64_t rows = (int64_t)a.B * a.Lq * a.H;
-    int64_t grid = cdiv(rows, 8);
+    char *ws = static_cast<char *>(a.ws);
+    s.part_o = reinterpret_cast<float *>(ws);
+    s.part_ml = s.part_o + pl.stream_slots * s.part_rows * HD;
+    t.part_o = reinterpret_cast<float *>(ws + pl.tc_at);
+    t.part_ml = t.part_o + pl.tc_slots * t.part_rows * HD;
+    s.sched = reinterpret_cast<int *>(ws + pl.sched_at);
+    t.sched = s.sched + a.B + 1;
+    if (pl.tc_slots) {
+        e = launch_tc(t, st);
+        if (e != cudaSuccess) return e;
+    }
+    if (pl.stream_slots) {
+        const int smem = (i8 ? smem_bytes<true>() : smem_bytes<false>()) + (a.B + 1) * 4;
+        static bool configured[HN_MAX_DEV];
+        int dev = 0;
+        e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
+        if (!configured[dev]) {
+            const int extra = (MAX_B + 1) * 4;
+            e = cudaFuncSetAttribute(k_paged_attention<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     smem_bytes<true>() + extra);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(k_paged_attention<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         smem_bytes<false>() + extra);
+            if (e != cudaSuccess) return e;
+            configured[dev] = true;
+        }
+        if (i8) k_paged_attention<true><<<s.ctas, THREADS, smem, st>>>(s);
+        else k_paged_attention<false><<<s.ctas, THREADS, smem, st>>>(s);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    int64_t grid = cdiv((int64_t)a.B * a.Lq * a.H, 8);
     if (grid > (int64_t)num_sms() * 8) grid = (int64_t)num_sms() * 8;
-    if (i8) k_paged_join<true><<<(unsigned)grid, 256, 0, st>>>(p, ctas);
-    else k_paged_join<false><<<(unsigned)grid, 256, 0, st>>>(p, ctas);
+    const bool tc_a = pl.shared_tc, tc_b = pl.own_tc;
+    k_paged_join<<<(unsigned)grid, 256, 0, st>>>(tc_a ? t : s, tc_b ? t : s);
     return cudaGetLastError();
 }
 
