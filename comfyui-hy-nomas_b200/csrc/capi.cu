@@ -524,7 +524,7 @@ static int cache_args(const hn_kv_cache *c, const char *what, CacheArgs &a) {
             (long long)c->page);
     const int64_t most = 0x7fffffff;
     REQUIRE(c->layers <= most && c->pages <= most / 4 && c->heads <= 65536 && c->slots <= most / 4 && c->page <= most &&
-                c->width <= most / c->page && c->heads * c->page <= most, HN_ERR_SHAPE, "%s: the cache is too large", what);
+                c->width <= most / c->page && c->heads * c->page <= most / 256 && c->pages <= most / c->heads / (c->page / 16), HN_ERR_SHAPE, "%s: the cache is too large", what);
     REQUIRE(al16(c->k) && al16(c->v) && al16(c->k_scale) && al16(c->v_scale), HN_ERR_ALIGN,
             "%s: the pools must be 16-byte aligned", what);
     a.k = c->k; a.v = c->v; a.ks = c->k_scale; a.vs = c->v_scale;

@@ -535,7 +535,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
         p->table = a.cache.meta.table; p->lengths = a.cache.meta.lengths; p->rows = a.rows;
         p->slots = a.cache.meta.slots; p->width = a.cache.meta.width; p->pages = a.cache.meta.pages;
         p->page = a.cache.meta.page;
-        p->sl2 = fabsf(a.scale) * 1.4426950408889634f;
+        p->sl2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);      // (a zero would make NaN of a masked -inf)
         p->flip = a.scale < 0.0f ? 0x80008000u : 0u;
         p->lse_shift = i8 ? P_SHIFT : 0.0f;
         p->err = err;

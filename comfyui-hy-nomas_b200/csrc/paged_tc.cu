@@ -2,22 +2,36 @@
 // and the shared tokens, or the rows of many sequences over the shared ones). tcgen05 kind::f16 products, S / P and O in
 // tensor memory; the pieces, partial results and formulas are paged.cuh's and paged_attention.cu's.
 //
-// One CTA per SM, 128 keys per block, two softmax groups of 128 rows each. Two row tiles of one K/V head share each K and
-// V block (a tile of 256 rows), or, for tiles of at most 128 rows (`halves` 2), the groups hold the same rows and take the even
-// and the odd blocks. Either way one group's exponentials run beside the other's products:
-//   warps 0-7    softmax: a thread per row (its TMEM lane). Loads q, writes it to shared memory; per block reads S, keeps the
-//                running maximum and sum, writes P over S (S 0-127, 128-255; O 256-383, 384-511), rescales O only when the
-//                maximum grew by more than 2^8.
-//   warp 8       MMA issuer: S_g(i) = Q_g K^T, O_g += P_g(i) V, in the order S0 S1 | PV0 S0' | PV1 S1' | ... S_g(i + 1) overwrites
-//                P_g(i), which the product before it in the pipe has read.
-//   warps 12-15  producer: gathers the pages' rows of K and V into a ring of four 32 KB slots (K, V, K, V), in the
-//                128-byte-swizzled layout of the products (K-major K, MN-major V); rows past the end are zeros. bf16 rows go by cp.async;
-//                int8 codes go through registers and become fp16 integers (exact), with (sk scale log2 e, log2 sv, 1 / sv)
-//                of each key in a second ring of four.
-// The register file is split by setmaxnreg: 2 x 128 x 184 for the softmax, the rest of 512 x 128 for the other two warpgroups.
+// One CTA per SM, blocks of 128 keys, two softmax groups of 128 rows each. Two row tiles of one K/V head share each K and
+// V block (a tile of 256 rows), or, for tiles of at most 128 rows (`halves` 2), the groups hold the same rows and take
+// every other block of the CTA (so each group always meets the same two ring slots, and no phase of theirs is skipped).
+// A block goes through a group in two steps of 64 keys, with S in one of two TMEM buffers: the products of step k + 1 run
+// while step k is in the softmax (with one buffer of 128 keys the softmax waited for S 2250 of every 5100 clocks).
+//   warps 0-7    softmax. q to shared memory (a thread per row), then per step: S from TMEM in the fragment layout (a thread
+//                holds a quarter of the columns of four rows, so the factors of int8 keys come from shared memory once for four
+//                rows, not once per row), running maximum and sum, P over S; O is rescaled only when the maximum grew by more
+//                than 2^STALE. Part of the exponentials are polynomials on the FMA pipe: at 16 a clock and SM, MUFU alone would
+//                take as long as the products. TMEM: S / P of group g at 128 g + 64 (step % 2), O at 256 + 128 g.
+//   warps 8, 9   MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
+//                thread that issues blocks until its products have read their operands, so each group has a thread of its own:
+//                the tensor pipe runs one's products while the other waits.
+//   warp 10      walks the line: the CTA's pieces into a ring of four
+//   warp 11      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
+//   warps 12-15  producers: the pages' rows of K and V into a ring of four 32 KB slots (K, V, K, V), in the 128-byte-swizzled
+//                layout of the products (K-major K, MN-major V). bf16: one warp, a TMA box per page (or its part in the block) and half
+//                of the head dim; V rows past the end become zeros (K's are masked). int8: four warps; codes go through
+//                registers and become fp16 integers (exact).
+//
+// int8: t_j = (q . ck_j) * sk_j scale log2 e, x_j = t_j 2^e (2^e: the row's power of two), P'_j = 2^(x_j - m + 12) sv_j. m is the
+// running maximum of x plus that of ceil(log2 sv), so P' <= 2^12 (fp16) and the normaliser's terms 2^(x_j - m + 12) are at hand.
+// The register file is split by setmaxnreg: what each role needs without spills (with shared memory taking all of L1, a spilled
+// register comes back from L2).
 // Every mbarrier wait is bounded; on expiry the kernel records HN_DEVERR_TIMEOUT, the roles leave their loops, copies and MMAs in
 // flight are drained (bounded) and TMEM is freed.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
+#include <string.h>
 
 #include "hn_tc.cuh"
 #include "paged.cuh"
@@ -34,56 +48,96 @@ constexpr int NSC = 4;                      // scale ring
 constexpr int TC_THREADS = 512;
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = 2 * TILE;
-constexpr int OFF_SC = OFF_KV + NS * TILE;  // per block: [64 key pairs]{a0, a1, l0, l1}, then [128] 1 / sv
-constexpr int SC_BYTES = BKT * 12;
+constexpr int OFF_SC = OFF_KV + NS * TILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
+                                            // the largest sv (16 B); where the 8 groups of 16 keys are (32 B)
+constexpr int SC_BYTES = BKT * 8 + 16 + 32;
 constexpr int OFF_BAR = OFF_SC + NSC * SC_BYTES;
-// full[NS], empty[NS], s[2], p[2], q[2], o[2], scales[NSC], end
-constexpr int NBARS = 2 * NS + 8 + NSC + 1;
-constexpr int OFF_MISC = OFF_BAR + NBARS * 8;
+constexpr int NP = 4;                       // pieces
+// full[NS], empty[NS], s[2][2], p[2][2], q[2], v[2][2] (of a group's steps in turn: two of them may be on their way, and a parity
+// tells a phase from its neighbours only), scales full[NSC], scales empty[NSC], piece full[NP], piece empty[NP], end[2], tail
+constexpr int NBARS = 2 * NS + 14 + 2 * NSC + 2 * NP + 3;
+constexpr int OFF_PIECE = OFF_BAR + NBARS * 8;
+constexpr int OFF_MISC = OFF_PIECE + NP * 32;
 constexpr int OFF_PRE = OFF_MISC + 16 + 32 * 4;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;     // 2 s
-// int8: P' <= 2^7 at the running maximum, so <= 2^15 at one stale by 2^8; the partial results are brought to the
-// streaming kernel's 2^14
-constexpr float TC_SHIFT = 7.0f, STREAM_SHIFT = 14.0f;
+// O is rescaled when the maximum grew by more than 2^STALE. int8: P' <= 2^12 at the running maximum, so <= 2^15 at one stale by 2^3
+// (fp16 ends at 65504; what is lost below its smallest step is 2^-37 of the largest). A bound of 2^1 rescaled every few blocks:
+// 10200 clocks of softmax per block against FILL. Partial results are brought to the streaming kernel's 2^14.
+constexpr float TC_SHIFT = 12.0f, STREAM_SHIFT = 14.0f;
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float nan_max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 32 lanes x 32 columns into registers, not waited for
-__device__ __forceinline__ void ld32_async(uint32_t taddr, uint32_t *r) {
+__device__ __forceinline__ float nan_max(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// 2^a of a pair on the FMA pipe: a = n + f, n the nearest integer (a magic addition), 2^f by a degree-4 polynomial fitted here to
+// the least largest relative error on [-1/2, 1/2] with the constant term 1 (2.9e-6 in fp32; P is rounded to 2^-9 or 2^-12), and
+// n added to the exponent field. From -127 down (a masked logit's -inf): exactly 0. a <= 127.
+__device__ __forceinline__ uint64_t exp2_fma(uint64_t a) {
+    float a0, a1;
+    x2_split(a, a0, a1);
+    a = x2(fmaxf(a0, -127.0f), fmaxf(a1, -127.0f));
+    const uint64_t t = x2_add(a, x2_splat(12582912.0f));
+    const uint64_t f = x2_fma(x2_add(t, x2_splat(-12582912.0f)), x2_splat(-1.0f), a);
+    uint64_t y = x2_fma(x2_splat(0x1.3a02ccp-7f), f, x2_splat(0x1.c9fc46p-5f));
+    y = x2_fma(y, f, x2_splat(0x1.ec0378p-3f));
+    y = x2_fma(y, f, x2_splat(0x1.62e12cp-1f));
+    y = x2_fma(y, f, x2_splat(1.0f));
+    float y0, y1, t0, t1;
+    x2_split(y, y0, y1);
+    x2_split(t, t0, t1);
+    return x2(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)),
+              __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)));
+}
+
+// The fragment layout of 16 TMEM lanes: lane l of the warp holds row l / 4 (and, in the second pair of registers, row l / 4 + 8),
+// columns 8 c + 2 (l % 4) and the next. 32 columns into registers, not waited for:
+__device__ __forceinline__ void ld_frag(uint32_t taddr, uint32_t *r) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
 }
-// orders the registers' uses after the loads: the first call waits for all of them
-__device__ __forceinline__ void ld_fence32(uint32_t *r, bool wait) {
-    if (wait) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    asm volatile(""
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
+// the registers' uses stay behind this (and a wait::ld before it)
+__device__ __forceinline__ void frag_fence(uint32_t *r) {
+#pragma unroll
+    for (int i = 0; i < 64; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                          "+r"(r[i + 6]), "+r"(r[i + 7]) :: "memory");
 }
-// 32 lanes x 16 columns from registers, not waited for
-__device__ __forceinline__ void st16_async(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
+// 16-bit pairs of 32 columns (16 TMEM columns): lane l holds pair 4 c + l % 4 of rows l / 4 and l / 4 + 8
+__device__ __forceinline__ void st_frag(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
+}
+// 32 columns of 16 lanes in the fragment layout, times f0 (rows l / 4) and f1 (rows l / 4 + 8)
+__device__ __forceinline__ void scale_frag(uint32_t taddr, float f0, float f1) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * (i & 2 ? f1 : f0));
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {"
+        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
 }
 // D (TMEM, fp32) (+)= A (TMEM, 16-bit pairs per column, one row per lane) x B (smem), K = 16
 __device__ __forceinline__ void mma_pv(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
@@ -98,13 +152,23 @@ __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32
 // 16-byte chunk c (of 16) of row r of a [128][128 elements] operand tile
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
-template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(const Params p) {
+// box of 64 elements x rows at (0, token, half, page and head) of a bf16 pool
+__device__ __forceinline__ void tma_rows(const CUtensorMap *map, uint32_t dst, uint32_t bar, int token, int half, int page) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(bar), "r"(0), "r"(token), "r"(half), "r"(page) : "memory");
+}
+
+// `box`: tokens per TMA box (bf16), a divisor of the page and of 128
+template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
+    k_paged_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int box) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr int R_SOFTMAX = 184, R_MMA = I8 ? 40 : 48, R_LOAD = I8 ? 104 : 96;
+    constexpr float STALE = I8 ? 3.0f : 8.0f;
+    constexpr int POLY = I8 ? 2 : 3;            // of 8 pairs: what balances the FMA pipe and MUFU
+    constexpr int R_SOFTMAX = I8 ? 176 : 192, R_MMA = 56, R_LOAD = I8 ? 104 : 72;     // what each role needs without spills
     static_assert(2 * R_SOFTMAX + R_MMA + R_LOAD == 512, "the registers that the block was launched with");
     const uint32_t sb = smem_u32(smem);
-    const uint32_t b_full = sb + OFF_BAR, b_empty = b_full + 8 * NS, b_s = b_empty + 8 * NS, b_p = b_s + 16, b_q = b_p + 16,
-                   b_o = b_q + 16, b_sc = b_o + 16, b_end = b_sc + 8 * NSC;
+    const uint32_t b_full = sb + OFF_BAR, b_empty = b_full + 8 * NS, b_s = b_empty + 8 * NS, b_p = b_s + 32, b_q = b_p + 32,
+                   b_v = b_q + 16, b_sc = b_v + 32, b_se = b_sc + 8 * NSC, b_pf = b_se + 8 * NSC, b_pe = b_pf + 8 * NP, b_end = b_pe + 8 * NP, b_tail = b_end + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + OFF_MISC + 4);
     int *sums = reinterpret_cast<int *>(smem + OFF_MISC + 16), *pre = reinterpret_cast<int *>(smem + OFF_PRE);
@@ -115,15 +179,15 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
     }
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, 128); mbar_init(b_empty + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(b_s + 8 * i, 1);
-            mbar_init(b_p + 8 * i, 4);
-            mbar_init(b_q + 8 * i, 128);
-            mbar_init(b_o + 8 * i, 1);
-        }
-        for (int i = 0; i < NSC; ++i) mbar_init(b_sc + 8 * i, 128);
+        // a block of two row tiles is given back by both groups' issuers, else by the one that takes it
+        for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, I8 ? 128 : 1); mbar_init(b_empty + 8 * i, p.halves == 2 ? 1 : 2); }
+        for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, 10 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
+        for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 4); mbar_init(b_v + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 128);
+        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, p.halves == 2 ? 8 : 12); }   // softmax, producers
         mbar_init(b_end, 1);
+        mbar_init(b_end + 8, 1);
+        mbar_init(b_tail, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
@@ -143,29 +207,44 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
     const uint32_t tmem = *tmem_slot;
     const bool split = p.halves == 2;           // the groups share the rows and take every other block
     const int rows_all = p.nbA ? p.B * p.Lq * p.G : p.Lq * p.G;
-    Walker walk(p, pre, blockIdx.x);
-    Piece w;
     bool ok = true;
+    // the next piece of the ring, for every warp that reads pieces; nblk 0: there are no more
+    const Piece *ring = reinterpret_cast<const Piece *>(smem + OFF_PIECE);
+    int n_piece = 0;
+    auto next_piece = [&]() -> const Piece * {
+        ok = warp_wait(lane, b_pf + 8 * (n_piece % NP), (n_piece / NP) & 1, abort_flag, WAIT_NS, p.err);
+        __syncwarp();
+        const Piece *w = ring + n_piece % NP;
+        return ok && w->nblk > 0 ? w : nullptr;
+    };
+    auto done_piece = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_pe + 8 * (n_piece % NP));
+        ++n_piece;
+    };
 
     if (warp < 8) {
         // ------------------------------------------------------------------ softmax and the results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R_SOFTMAX));
         const int g = warp >> 2, wq = warp & 3, rr = 32 * wq + lane;
         const uint32_t tl = tmem + ((uint32_t)(32 * wq) << 16), ts = tl + 128 * g, to = tl + 256 + 128 * g;
-        int n_s = 0, n_piece = 0, n_tile = 0;   // phases: blocks this group has seen, pieces, blocks of the CTA
-        while (ok && walk.next(p, pre, blockIdx.x, w)) {
+        int n_s = 0, n_tile = 0;                // steps of this group, blocks of the CTA
+        while (const Piece *pc = next_piece()) {
+            const Piece &w = *pc;
             const int r = w.row0 + (split ? 0 : 128 * g) + rr;
             const bool valid = r < rows_all;
-            int b = 0, l = 0, gm = 0, lim = w.kend;       // a row past the tile's end: computed and dropped
+            int lim = w.kend;                   // a row past the tile's end: computed and dropped
+            const __nv_bfloat16 *qp = p.q;
             if (valid) {
+                int b, l, gm;
                 split_row(p, w, r, b, l, gm);
+                qp += b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + gm) * p.q_hs;
                 lim = row_limit(p, seq_length(p, b), l);
                 lim = lim > w.kend ? w.kend : lim;
             }
             // --- q to shared memory (a row past the tile's end: zeros)
             float rs = I8 ? 1.0f : p.sl2;       // int8: the keys' factors carry scale * log2 e
             {
-                const __nv_bfloat16 *qp = p.q + b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + gm) * p.q_hs;
                 uint32_t x[64];
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
@@ -191,128 +270,185 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
             fence_async();
             mbar_arrive(b_q + 8 * g);
 
-            float m = -INFINITY, sum = 0.0f;
-            const int count = split ? (w.nblk + 1 - g) >> 1 : w.nblk;
-            for (int i = 0; i < count; ++i) {
-                const int j = split ? 2 * i + g : i;
-                ok = warp_wait(lane, b_s + 8 * g, n_s & 1, abort_flag, WAIT_NS, p.err);
-                ++n_s;
-                if (!ok) break;
-                tc_fence_after();
-                uint32_t x[128];
+            // --- from here on a thread works on rows 16 hf + 8 u + lane / 4 of its warp's 32
+            const int nblk = w.nblk, j0 = split ? (n_tile ^ g) & 1 : 0;          // the group's first block
+            const int count = split ? (nblk + 1 - j0) >> 1 : nblk;
+            int seen[4];                                                        // keys of the block that the row sees
+            float m[4], sum[4], rsf[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) ld32_async(ts + 32 * c, x + 32 * c);
-                const float4 *al = nullptr, *iv = nullptr;
-                if (I8) {
-                    const int t = n_tile + j;
+            for (int u = 0; u < 4; ++u) {
+                seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + (w.blk0 + j0) * BKT);
+                rsf[u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
+                m[u] = -INFINITY;
+                sum[u] = 0.0f;
+            }
+            float ev = -1000.0f;                // int8: running maximum of ceil(log2 sv), at least
+            for (int k = 0; k < 2 * count; ++k, ++n_s) {        // steps of 64 keys
+                const int sub = k & 1, t = n_tile + (split ? 2 * (k >> 1) + j0 : k >> 1);
+                const uint32_t tsb = ts + 64 * sub;
+                const ulonglong2 *factors = reinterpret_cast<const ulonglong2 *>(smem + OFF_SC + (t % NSC) * SC_BYTES) +
+                                            16 * sub + (lane & 3);
+                if (I8 && sub == 0) {
                     ok = warp_wait(lane, b_sc + 8 * (t % NSC), (t / NSC) & 1, abort_flag, WAIT_NS, p.err);
                     if (!ok) break;
                     __syncwarp();
-                    al = reinterpret_cast<const float4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES);
-                    iv = al + 64;
                 }
-                ld_fence32(x, true);
-                ld_fence32(x + 32, false);
-                ld_fence32(x + 64, false);
-                ld_fence32(x + 96, false);
-                const uint64_t rs2 = x2_splat(rs);
-                if (I8) {           // base-2 logits + log2 sv
+                ok = warp_wait(lane, b_s + 16 * g + 8 * sub, (n_s >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t x[64];                 // [16-lane half][8 column groups][row l / 4, l / 4 + 8][2 columns]
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        const float4 f = al[c];
-                        float y0, y1;
-                        x2_split(x2_fma(x2_mul(x2(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), x2(f.x, f.y)), rs2,
-                                        x2(f.z, f.w)), y0, y1);
-                        x[2 * c] = __float_as_uint(y0);
-                        x[2 * c + 1] = __float_as_uint(y1);
+                for (int c = 0; c < 4; ++c) ld_frag(tsb + ((uint32_t)(16 * (c >> 1)) << 16) + 32 * (c & 1), x + 16 * c);
+                bool rescale = false;
+                float f = 1.0f;
+                if (I8 && sub == 0) {
+                    const float top = *reinterpret_cast<const float *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 2 * BKT * 4);
+                    // 2^e > sv: the exponent field, plus one; not below -60, so that 2^(12 - e) stays in range
+                    const float e = fmaxf((float)((int)(__float_as_uint(top) >> 23) - 126), -60.0f);
+                    if (e > ev) {               // all rows' references grow with it
+                        f = ex2(ev - e);
+                        rescale = true;
+                        ev = e;
                     }
                 }
-                const int k0 = w.kbeg + (w.blk0 + j) * BKT;
-                if (__any_sync(0xffffffffu, k0 + BKT > lim)) {
-                    const int seen = lim - k0;
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                frag_fence(x);
+                if (I8) {
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c >= seen) x[c] = __float_as_uint(-INFINITY);
+                    for (int c = 0; c < 8; c += 2) {
+                        const ulonglong2 kf = factors[2 * c];
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) {           // 2 column groups x 4 rows
+                            uint32_t *y = x + 32 * (v >> 2) + 4 * (c + (v & 1)) + (v & 2);
+                            float y0, y1;
+                            x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
+                            y[0] = __float_as_uint(y0);
+                            y[1] = __float_as_uint(y1);
+                        }
+                    }
                 }
-                float mx[8];
+                if (__any_sync(0xffffffffu, min(min(seen[0], seen[1]), min(seen[2], seen[3])) < 64)) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) mx[c] = max3(__uint_as_float(x[c]), __uint_as_float(x[8 + c]), __uint_as_float(x[16 + c]));
+                    for (int c = 0; c < 64; ++c)
+                        if (8 * ((c & 31) >> 2) + 2 * (lane & 3) + (c & 1) >= seen[2 * (c >> 5) + ((c >> 1) & 1)])
+                            x[c] = __float_as_uint(-INFINITY);
+                }
+                float mn[4];
 #pragma unroll
-                for (int c = 24; c < 120; c += 16)
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t *y = x + 32 * (u >> 1) + 2 * (u & 1);
+                    float mx[4];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        mx[u] = max3(mx[u], __uint_as_float(x[c + u]), __uint_as_float(x[c + 8 + u]));
+                    for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
 #pragma unroll
-                for (int u = 0; u < 8; ++u) mx[u] = fmaxf(mx[u], __uint_as_float(x[120 + u]));
-                float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-                if (!I8) top *= rs;
-                const float mn = fmaxf(m, top);
-                if (i == 0) {
-                    m = mn;
-                } else {
-                    const bool need = mn > m + 8.0f;
-                    if (__any_sync(0xffffffffu, need)) {
-                        // O holds this group's products up to the block before (S's commit came after them)
-                        const float alpha = need ? ex2(m - mn) : 1.0f;
-                        if (need) { sum *= alpha; m = mn; }
+                    for (int c = 0; c < 4; ++c)
+                        mx[c] = nan_max3(mx[c], __uint_as_float(y[16 + 4 * c]), __uint_as_float(y[16 + 4 * c + 1]));
+                    mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
+                bool need = rescale;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
+                    mn[u] = nan_max(m[u], mn[u] * rsf[u]);      // a NaN stays in the row
+                    need |= !(mn[u] <= m[u] + STALE);
+                }
+                if (k == 0) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) m[u] = mn[u];
+                } else if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const bool grow = !(mn[u] <= m[u] + STALE);
+                        const float al = (grow ? ex2(m[u] - mn[u]) : 1.0f) * f;
+                        m[u] = grow ? mn[u] : m[u];
+                        mn[u] = al;
+                        sum[u] *= al;
+                    }
+                    // the product before this step's is the last one given to the pipe
+                    ok = warp_wait(lane, b_v + 16 * g + 8 * (sub ^ 1), ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
-                            uint32_t o[16];
-                            asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                                         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-                                         "tcgen05.wait::ld.sync.aligned;"
-                                         : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]),
-                                           "=r"(o[6]), "=r"(o[7]), "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]),
-                                           "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                                         : "r"(to + c)
-                                         : "memory");
-#pragma unroll
-                            for (int u = 0; u < 16; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
-                            st16_async(to + c, o);
-                        }
+                    for (int c = 0; c < HD; c += 32) {
+                        scale_frag(to + c, mn[0], mn[1]);
+                        scale_frag(to + (16u << 16) + c, mn[2], mn[3]);
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const uint64_t nref = x2_splat(I8 ? TC_SHIFT - ref : -ref);
-                uint64_t acc = 0ull;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint64_t nref[2], acc[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        const int k = 32 * c + 2 * u;
-                        const uint64_t s2 = x2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                        float a0, a1;
-                        x2_split(I8 ? x2_add(s2, nref) : x2_fma(s2, rs2, nref), a0, a1);
-                        const float e0 = ex2(a0), e1 = ex2(a1);
+                    for (int u = 0; u < 2; ++u) {
+                        const float ref = m[2 * hf + u] == -INFINITY ? 0.0f : m[2 * hf + u];
+                        nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4) {            // 4 column groups: a store of 8 registers
+                        uint64_t v[4];
                         if (I8) {
-                            const float2 v = reinterpret_cast<const float2 *>(iv)[16 * c + u];
-                            acc = x2_fma(x2(e0, e1), x2(v.x, v.y), acc);
-                            pk[u] = pack_f16_rn(e0, e1);
-                        } else {
-                            acc = x2_add(acc, x2(e0, e1));
-                            pk[u] = bf16x2_rn(e0, e1);
+                            const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
+                            v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
                         }
+                        uint32_t pk[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {           // column group c + q / 2, row q % 2
+                            const int u = q & 1;
+                            const uint32_t *y = x + 32 * hf + 4 * c + 2 * q;
+                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), x2_splat(rsf[2 * hf + u]), nref[u]);
+                            uint64_t e;
+                            if (q < POLY) {
+                                e = exp2_fma(a);
+                            } else {
+                                float a0, a1;
+                                x2_split(a, a0, a1);
+                                e = x2(ex2(a0), ex2(a1));
+                            }
+                            acc[u] = x2_add(acc[u], e);
+                            if (I8) e = x2_mul(e, v[q >> 1]);
+                            float e0, e1;
+                            x2_split(e, e0, e1);
+                            pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
+                        }
+                        st_frag(tsb + ((uint32_t)(16 * hf) << 16) + 4 * c, pk);
                     }
-                    st16_async(ts + 16 * c, pk);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float a0, a1;
+                        x2_split(acc[u], a0, a1);
+                        sum[2 * hf + u] += a0 + a1;
+                    }
                 }
-                float a0, a1;
-                x2_split(acc, a0, a1);
-                sum += a0 + a1;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) seen[u] -= sub && split ? 64 + BKT : 64;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b_p + 8 * g);
+                if (lane == 0) {
+                    mbar_arrive(b_p + 16 * g + 8 * sub);
+                    if (I8 && sub == 1) mbar_arrive(b_se + 8 * (t % NSC));
+                }
+            }
+            // back to a thread per row: row `lane` is 8 u + lane / 4 in the quad 4 (lane % 8)
+            float mrow = 0.0f, srow = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
+                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
+                const float a = __shfl_sync(0xffffffffu, m[u], 4 * (lane & 7)), c = __shfl_sync(0xffffffffu, sum[u], 4 * (lane & 7));
+                if ((lane >> 3) == u) { mrow = I8 ? a + ev + (STREAM_SHIFT - TC_SHIFT) : a; srow = c; }
             }
             if (!ok) break;
-            n_tile += w.nblk;
+            n_tile += nblk;
             // --- O: to the output, or to the piece's slot
-            ok = warp_wait(lane, b_o + 8 * g, n_piece & 1, abort_flag, WAIT_NS, p.err);
-            ++n_piece;
+            if (count > 0) ok = warp_wait(lane, b_v + 16 * g + 8, ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
             if (!ok) break;
             tc_fence_after();
             const bool ends = w.slot < 0;
-            const float inv = ends ? inverse(sum) : 1.0f;
+            const float inv = ends ? inverse(srow) : 1.0f;
+            int b = 0, l = 0, gm = 0;
+            if (valid) split_row(p, w, r, b, l, gm);
             const int head = w.h * p.G + gm;
             const int64_t at = (int64_t)(ends ? 0 : w.slot) * p.part_rows + 128 * g + rr;
             __nv_bfloat16 *op = p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs;
@@ -344,147 +480,228 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
                 __syncwarp();
             }
             if (valid) {
-                const float M = I8 ? m + (STREAM_SHIFT - TC_SHIFT) : m;
-                if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(M, sum);
-                else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, M, sum);
+                if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mrow, srow);
+                else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, mrow, srow);
             }
             tc_fence_before();          // O is read before the next piece's products, which wait for this group's P
+            done_piece();
         }
     } else if (warp < 12) {
-        // ------------------------------------------------------------------ MMA issuer (warp 8)
+        // ------------------------------------------------------------------ MMA issuers, walker
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_MMA));
-        if (warp == 8) {
+        if (warp < 10) {
             // kind::f16: fp32 D (bit 4), A and B bf16 (bits 7, 10) or f16 (0), N / 8 at bit 17, M / 16 at bit 24; V is MN-major (bit 16)
-            const uint32_t types = (1u << 4) | (I8 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKT >> 3) << 17) | (8u << 24);
-            const uint32_t idesc_s = types, idesc_o = types | (1u << 16);
-            uint32_t half0 = 0;                 // ring index of the piece's first K block
-            int n_p[2] = {0, 0}, n_piece = 0;
-            while (ok && walk.next(p, pre, blockIdx.x, w)) {
-                const int tasks = split ? w.nblk : 2 * w.nblk;
-                for (int g = 0; g < 2 && ok; ++g)
-                    ok = warp_wait(lane, b_q + 8 * g, n_piece & 1, abort_flag, WAIT_NS, p.err);
-                ++n_piece;
-                if (!ok) break;
-                auto issue_s = [&](int t) -> bool {
-                    const int g = t & 1, j = split ? t : t >> 1;
-                    const uint32_t h = half0 + 2 * j, slot = h % NS;
-                    if (!warp_wait(lane, b_full + 8 * slot, (h / NS) & 1, abort_flag, WAIT_NS, p.err)) return false;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t qa = sb + OFF_Q + g * TILE, ka = sb + OFF_KV + slot * TILE;
-#pragma unroll
-                        for (int i = 0; i < HD / 16; ++i)
-                            mma_f16(tmem + 128 * g, sdesc(qa + (i >> 2) * HALF) + 2 * (i & 3), sdesc(ka + (i >> 2) * HALF) + 2 * (i & 3),
-                                    idesc_s, (uint32_t)(i > 0));
-                        mma_commit(b_s + 8 * g);
-                        if (split || g == 1) mma_commit(b_empty + 8 * slot);
-                    }
-                    __syncwarp();
-                    return true;
+            constexpr uint32_t types = (1u << 4) | (I8 ? 0u : (1u << 7) | (1u << 10)) | (8u << 24);
+            constexpr uint32_t idesc_s = types | (8u << 17), idesc_o = types | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
+            const int g = warp - 8, step = split ? 2 : 1;
+            const uint32_t ds = tmem + 128 * g, dout = tmem + 256 + 128 * g;
+            uint32_t h = 0;                         // ring index of this group's next K block; V follows it
+            uint32_t n_p = 0;
+            while (const Piece *pc = next_piece()) {
+                const int nblk = pc->nblk;
+                ok = warp_wait(lane, b_q + 8 * g, n_piece & 1, abort_flag, WAIT_NS, p.err);
+                const uint32_t h_next = h + 2 * nblk;
+                const int j0 = split ? (int)(h >> 1 ^ g) & 1 : 0;
+                const int count = split ? (nblk + 1 - j0) >> 1 : nblk;
+                h += 2 * j0;
+                auto wait_full = [&](uint32_t x) {
+                    return warp_wait(lane, b_full + 8 * (x % NS), (x / NS) & 1, abort_flag, WAIT_NS, p.err);
                 };
-                for (int t = 0; t < 2 && t < tasks && ok; ++t) ok = issue_s(t);
-                for (int t = 0; t < tasks && ok; ++t) {
-                    const int g = t & 1, j = split ? t : t >> 1, i = t >> 1;
-                    const uint32_t h = half0 + 2 * j + 1, slot = h % NS;
-                    ok = warp_wait(lane, b_full + 8 * slot, (h / NS) & 1, abort_flag, WAIT_NS, p.err);
-                    if (ok) ok = warp_wait(lane, b_p + 8 * g, n_p[g] & 1, abort_flag, WAIT_NS, p.err);
-                    if (!ok) break;
-                    ++n_p[g];
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t va = sb + OFF_KV + slot * TILE;
+                // step `sub` of the block at ring index x; the second gives K back
+                auto issue_s = [&](uint32_t x, uint32_t sub) {
+                    const uint64_t qd = sdesc(sb + OFF_Q + g * TILE), kd = sdesc(sb + OFF_KV + (x % NS) * TILE + sub * 8192);
 #pragma unroll
-                        for (int u = 0; u < BKT / 16; ++u)      // 16 keys: 8 columns of P, two 8-row groups of V
-                            mma_pv(tmem + 256 + 128 * g, tmem + 128 * g + 8 * u, sdesc_mn(va, HALF) + (uint64_t)(2048 >> 4) * u, idesc_o,
-                                   (uint32_t)(i > 0 || u > 0));
-                        if (split || g == 1) mma_commit(b_empty + 8 * slot);
-                        if (t + 2 >= tasks) mma_commit(b_o + 8 * g);
+                    for (int i = 0; i < HD / 16; ++i)
+                        mma_f16(ds + 64 * sub, qd + (HALF >> 4) * (i >> 2) + 2 * (i & 3), kd + (HALF >> 4) * (i >> 2) + 2 * (i & 3),
+                                idesc_s, (uint32_t)(i > 0));
+                    mma_commit(b_s + 16 * g + 8 * sub);
+                    if (sub) mma_commit(b_empty + 8 * (x % NS));
+                };
+                if (ok && count > 0) {
+                    ok = wait_full(h);
+                    tc_fence_after();
+                    if (ok && lane == 0) {
+                        issue_s(h, 0);
+                        issue_s(h, 1);
                     }
                     __syncwarp();
-                    if (t + 2 < tasks) ok = issue_s(t + 2);
                 }
-                // a group without a block has its phase completed all the same
-                if (ok && tasks == 1 && lane == 0) mbar_arrive(b_o + 8);
-                __syncwarp();
-                half0 += 2 * w.nblk;
+                for (int k = 0; k < 2 * count && ok; ++k, ++n_p) {
+                    const uint32_t sub = k & 1;
+                    if (sub == 0) ok = wait_full(h + 1);
+                    if (ok) ok = warp_wait(lane, b_p + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint64_t vd = sdesc_mn(sb + OFF_KV + ((h + 1) % NS) * TILE + sub * 8192, HALF);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)             // 16 keys: 8 columns of P, two 8-row groups of V
+                            mma_pv(dout, ds + 64 * sub + 8 * u, vd + (uint64_t)(2048 >> 4) * u, idesc_o, (uint32_t)(k > 0 || u > 0));
+                        mma_commit(b_v + 16 * g + 8 * sub);
+                        if (sub) mma_commit(b_empty + 8 * ((h + 1) % NS));
+                    }
+                    __syncwarp();
+                    if (k + 2 < 2 * count) {
+                        // S(k + 2) goes over P(k): products on different accumulators are not ordered, so P V has to be done
+                        // (it is, long before the softmax of step k + 1 asks for S(k + 2))
+                        if (sub == 0) ok = wait_full(h + 2 * step);
+                        if (ok) ok = warp_wait(lane, b_v + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                        tc_fence_after();
+                        if (ok && lane == 0) issue_s(h + 2 * step, sub);
+                        __syncwarp();
+                    }
+                    if (sub) h += 2 * step;
+                }
+                if (!ok) break;
+                h = h_next;
+                done_piece();
             }
             // every MMA issued has completed before TMEM is freed
             if (lane == 0) {
-                mma_commit(b_end);
+                mma_commit(b_end + 8 * g);
                 volatile int never = 0;
-                mbar_wait(b_end, 0, &never, 100000000ull, p.err);
+                mbar_wait(b_end + 8 * g, 0, &never, 100000000ull, p.err);
             }
             __syncwarp();
+        } else if (warp == 10 && lane == 0) {
+            Walker walk(p, pre, blockIdx.x);
+            Piece w;
+            for (bool more = true; more; ++n_piece) {
+                if (!mbar_wait(b_pe + 8 * (n_piece % NP), ((n_piece / NP) & 1) ^ 1, abort_flag, WAIT_NS, p.err)) break;
+                more = walk.next(p, pre, blockIdx.x, w);
+                if (!more) w.nblk = 0;
+                const_cast<Piece *>(ring)[n_piece % NP] = w;
+                mbar_arrive(b_pf + 8 * (n_piece % NP));
+            }
+        } else if (I8 && warp == 11) {
+            int n_tile = 0;
+            while (const Piece *pc = next_piece()) {
+                const int own_b = pc->own_b, head = pc->h, kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
+                const int seq = p.rows[own_b < 0 ? 0 : own_b];
+                const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
+                auto page_of = [&](int j, int &off) -> int {        // lane s < 8 (and its copies): the page of key 16 s of block j
+                    const int kk = key0 + j * BKT + 16 * (lane & 7), pg = kk / p.page;
+                    off = kk - pg * p.page;
+                    return j < nblk && kk < kend && pg < p.width ? tab[pg] : -1;
+                };
+                // in flight: the pages of block j + 2 and the factors of block j + 1, while block j is written
+                int off, id = page_of(0, off), at, at_next;
+                float sk[4], sv[4], sk_next[4], sv_next[4];
+                auto gather = [&](int j, int &where, float (&k)[4], float (&v)[4]) {
+                    // where key 16 s is in the pool, in units of 16 tokens (pages are multiples of 16), -1: not there
+                    where = (unsigned)id < (unsigned)p.pages ? (id * p.Hkv + head) * (p.page >> 4) + (off >> 4) : -1;
+                    int x[4];                                       // key 32 u + lane; the shuffles before any load: one behind
+#pragma unroll                                                              // a load waits some 290 clocks (measured)
+                    for (int u = 0; u < 4; ++u) x[u] = __shfl_sync(0xffffffffu, where, 2 * u + (lane >> 4));
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        k[u] = v[u] = 0.0f;
+                        if (x[u] >= 0 && 32 * u + lane < kend - (key0 + j * BKT)) {
+                            k[u] = p.ks[(int64_t)x[u] * 16 + (lane & 15)];
+                            v[u] = p.vs[(int64_t)x[u] * 16 + (lane & 15)];
+                        }
+                    }
+                    id = page_of(j + 1, off);
+                };
+                gather(0, at_next, sk_next, sv_next);
+                for (int j = 0; j < nblk && ok; ++j, ++n_tile) {
+                    at = at_next;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) { sk[u] = sk_next[u]; sv[u] = sv_next[u]; }
+                    if (j + 1 < nblk) gather(j + 1, at_next, sk_next, sv_next);
+                    ok = warp_wait(lane, b_se + 8 * (n_tile % NSC), ((n_tile / NSC) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
+                    if (!ok) break;
+                    float *sc = reinterpret_cast<float *>(smem + OFF_SC + (n_tile % NSC) * SC_BYTES);
+                    float top = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        // key 8 c + 2 q + e goes to the quad's lane q, place 2 c + e of 32; four places of the four lanes in turn, so
+                        // that the lanes' 16-byte loads meet different banks
+                        const int key = 32 * u + lane, place = 2 * (key >> 3) + (key & 1);
+                        const int to = 16 * (place >> 2) + 4 * ((key >> 1) & 3) + (place & 3);
+                        sc[to] = sk[u] * p.sl2;
+                        sc[BKT + to] = sv[u];
+                        top = fmaxf(top, sv[u]);
+                    }
+                    top = warp_max_xor(top, 32);
+                    if (lane == 0) sc[2 * BKT] = top;
+                    if (lane < 8) reinterpret_cast<int *>(sc)[2 * BKT + 4 + lane] = at;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_sc + 8 * (n_tile % NSC));
+                }
+                done_piece();
+            }
         }
     } else {
-        // ------------------------------------------------------------------ producer
+        // ------------------------------------------------------------------ producers
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_LOAD));
         const int tid = threadIdx.x - 384;
-        constexpr int ROW = I8 ? HD : 2 * HD;
         uint32_t half = 0;                      // ring index
+        uint32_t tails = 0;
         int n_tile = 0;
-        while (ok && walk.next(p, pre, blockIdx.x, w)) {
-            const int seq = p.rows[w.own_b < 0 ? 0 : w.own_b];
-            const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
-            // lane s < 8: the token index of key 16 s of block j in the pool, or -1; the 16 keys are in one page
-            auto place = [&](int j) -> int64_t {
-                const int kk = w.kbeg + (w.blk0 + j) * BKT + 16 * (lane & 7), pg = kk / p.page;
-                const int id = kk < w.kend && pg < p.width ? tab[pg] : -1;
-                return (unsigned)id < (unsigned)p.pages ? ((int64_t)id * p.Hkv + w.h) * p.page + (kk - pg * p.page) : -1;
-            };
+        while (I8 || warp == 12) {
+            const Piece *pc = next_piece();
+            if (pc == nullptr) break;
+            const int kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
             if (!I8) {
-                const int c = tid & 15, r8 = tid >> 4;
-                int64_t at = place(0);
-                for (int j = 0; j < w.nblk && ok; ++j) {
-                    const int64_t next = j + 1 < w.nblk ? place(j + 1) : -1;
-                    const int k0 = w.kbeg + (w.blk0 + j) * BKT;
-#pragma unroll
-                    for (int kv = 0; kv < 2; ++kv) {
+                const int own_b = pc->own_b, head = pc->h, seq = p.rows[own_b < 0 ? 0 : own_b];
+                const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
+                const int groups = BKT / box;                   // a lane each
+                for (int j = 0; j < nblk && ok; ++j) {
+                    const int k0 = key0 + j * BKT, kk = k0 + box * lane, pg = kk / p.page;
+                    const int id = lane < groups && kk < kend && pg < p.width ? tab[pg] : -1;
+                    const bool here = (unsigned)id < (unsigned)p.pages;
+                    const uint32_t bytes = 256u * box * __popc(__ballot_sync(0xffffffffu, here));
+                    const int left = kend - k0;                 // rows of the block that are there
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv, ++half) {
                         const uint32_t slot = half % NS;
                         ok = warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
                         if (!ok) break;
-                        const uint8_t *pool = kv ? p.v : p.k;
-                        const uint32_t dst = sb + OFF_KV + slot * TILE;
-#pragma unroll
-                        for (int it = 0; it < 16; ++it) {
-                            const int64_t base = __shfl_sync(0xffffffffu, at, it >> 1);
-                            const int row = 8 * it + r8;
-                            const bool here = base >= 0 && k0 + row < w.kend;
-                            const uint8_t *src = here ? pool + (base + (row & 15)) * ROW + 16 * c : pool;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                                         ::"r"(dst + chunk_at(row, c)), "l"(src), "r"(here ? 16 : 0) : "memory");
+                        const bool tail = kv == 1 && left < BKT;
+                        const uint32_t bar = tail ? b_tail : b_full + 8 * slot, dst = sb + OFF_KV + slot * TILE;
+                        if (lane == 0) mbar_arrive_tx(bar, bytes);
+                        __syncwarp();
+                        if (here)
+                            for (int u = 0; u < 2; ++u)
+                                tma_rows(kv ? &tm_v : &tm_k, dst + u * HALF + lane * box * 128, bar, kk - pg * p.page, u,
+                                         id * p.Hkv + head);
+                        __syncwarp();
+                        if (tail) {                             // rows past the end: zeros, whatever the page holds there
+                            ok = warp_wait(lane, b_tail, tails & 1, abort_flag, WAIT_NS, p.err);
+                            ++tails;
+                            if (!ok) break;
+                            for (int r = left; r < BKT; ++r)
+                                if (lane < 16) sts16(dst + chunk_at(r, lane), 0, 0, 0, 0);
+                            fence_async();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(b_full + 8 * slot);
                         }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        // the block two before has landed: hand it over
-                        asm volatile("cp.async.wait_group 2;" ::: "memory");
-                        fence_async();
-                        if (half >= 2) mbar_arrive(b_full + 8 * ((half - 2) % NS));
-                        ++half;
                     }
-                    at = next;
                 }
             } else {
                 // a quarter of a warp holds 64 B of two neighbouring rows, so that its 16-byte stores use every bank once
-                const int row16 = 2 * (tid >> 4) + ((tid >> 2) & 1), c = ((tid >> 3) & 1) * 4 + (tid & 3);
+                const int row16 = 2 * (tid >> 4) + ((tid >> 2) & 1), c = ((tid >> 3) & 1) * 4 + (tid & 3), mine = row16 * HD + 16 * c;
                 uint4 kreg[8], vreg[8];
-                float sk = 0.0f, sv = 1.0f;
-                auto fetch = [&](uint4 (&reg)[8], const uint8_t *pool, int64_t at, int j) {
-                    const int k0 = w.kbeg + (w.blk0 + j) * BKT;
+                auto fetch = [&](uint4 (&reg)[8], const uint8_t *pool, int j, int t) {
+                    const int left = kend - (key0 + j * BKT) - row16;
+                    const int4 *at4 = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16);
 #pragma unroll
-                    for (int it = 0; it < 8; ++it) {
-                        const int64_t base = __shfl_sync(0xffffffffu, at, it);
-                        reg[it] = make_uint4(0, 0, 0, 0);
-                        if (base >= 0 && k0 + 16 * it + row16 < w.kend)
-                            reg[it] = ldg_stream(pool + (base + row16) * ROW + 16 * c);
+                    for (int v = 0; v < 2; ++v) {
+                        const int4 a = at4[v];
+                        const int at[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                        for (int it = 0; it < 4; ++it) {
+                            reg[4 * v + it] = make_uint4(0, 0, 0, 0);
+                            if (at[it] >= 0 && 16 * (4 * v + it) < left)
+                                reg[4 * v + it] = ldg_stream(pool + (int64_t)at[it] * (16 * HD) + mine);
+                        }
                     }
                 };
-                auto fetch_scales = [&](int64_t at, int j) {
-                    const int64_t base = __shfl_sync(0xffffffffu, at, tid >> 4);
-                    sk = 0.0f; sv = 1.0f;
-                    if (base >= 0 && w.kbeg + (w.blk0 + j) * BKT + tid < w.kend) {
-                        sk = p.ks[base + (tid & 15)];
-                        sv = p.vs[base + (tid & 15)];
-                    }
+                auto wait_index = [&](int t) {
+                    const bool r = warp_wait(lane, b_sc + 8 * (t % NSC), (t / NSC) & 1, abort_flag, WAIT_NS, p.err);
+                    __syncwarp();
+                    return r;
                 };
                 auto store = [&](const uint4 (&reg)[8], uint32_t slot) {
                     const uint32_t dst = sb + OFF_KV + slot * TILE;
@@ -499,47 +716,50 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
                               codes_f16<0x4140>(x[3]), codes_f16<0x4342>(x[3]));
                     }
                 };
-                int64_t at = place(0);
-                fetch(kreg, p.k, at, 0);
-                fetch_scales(at, 0);
-                fetch(vreg, p.v, at, 0);
-                at = w.nblk > 1 ? place(1) : -1;
-                for (int j = 0; j < w.nblk && ok; ++j, ++n_tile) {
-                    uint32_t slot = half % NS;
-                    ok = warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
+                auto hand_over = [&](const uint4 (&reg)[8]) {
+                    const uint32_t slot = half % NS;
+                    if (!warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err)) return false;
+                    store(reg, slot);
+                    fence_async();
+                    mbar_arrive(b_full + 8 * slot);
+                    ++half;
+                    return true;
+                };
+                ok = wait_index(n_tile);
+                if (ok) {
+                    fetch(kreg, p.k, 0, n_tile);
+                    fetch(vreg, p.v, 0, n_tile);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_se + 8 * (n_tile % NSC));
+                }
+                for (int j = 0; j < nblk && ok; ++j) {
+                    const int t = ++n_tile;
+                    ok = hand_over(kreg);
                     if (!ok) break;
-                    store(kreg, slot);
-                    {
-                        float *sc = reinterpret_cast<float *>(smem + OFF_SC + (n_tile % NSC) * SC_BYTES);
-                        // a scale below 2^-100 (an all but zero row) counts as 2^-100: its values then are below 2^-93
-                        const float s1 = sv < 0x1p-100f ? 0x1p-100f : sv;
-                        sc[4 * (tid >> 1) + (tid & 1)] = sk * p.sl2;
-                        sc[4 * (tid >> 1) + 2 + (tid & 1)] = lg2(s1);
-                        sc[2 * BKT + tid] = __frcp_rn(s1);
-                        mbar_arrive(b_sc + 8 * (n_tile % NSC));
+                    if (j + 1 < nblk) {
+                        ok = wait_index(t);
+                        if (!ok) break;
+                        fetch(kreg, p.k, j + 1, t);
                     }
-                    fence_async();
-                    mbar_arrive(b_full + 8 * slot);
-                    ++half;
-                    const int64_t next = j + 2 < w.nblk ? place(j + 2) : -1;
-                    if (j + 1 < w.nblk) { fetch(kreg, p.k, at, j + 1); fetch_scales(at, j + 1); }
-                    slot = half % NS;
-                    ok = warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
+                    ok = hand_over(vreg);
                     if (!ok) break;
-                    store(vreg, slot);
-                    fence_async();
-                    mbar_arrive(b_full + 8 * slot);
-                    ++half;
-                    if (j + 1 < w.nblk) fetch(vreg, p.v, at, j + 1);
-                    at = next;
+                    if (j + 1 < nblk) {
+                        fetch(vreg, p.v, j + 1, t);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b_se + 8 * (t % NSC));
+                    }
                 }
             }
+            if (ok) done_piece();
         }
-        if (!I8) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            fence_async();
-            for (uint32_t h = half >= 2 ? half - 2 : 0; h < half && ok; ++h) mbar_arrive(b_full + 8 * (h % NS));
+        // every copy issued has landed before the CTA may exit (immediate on the normal path)
+        if (!I8 && warp == 12 && lane == 0) {
+            volatile int never = 0;
+            for (uint32_t h = half >= NS ? half - NS : 0; h < half; ++h)
+                mbar_wait(b_full + 8 * (h % NS), (h / NS) & 1, &never, 100000000ull, p.err);
+            if (!ok && tails) mbar_wait(b_tail, (tails - 1) & 1, &never, 100000000ull, p.err);
         }
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -547,6 +767,25 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1) k_paged_tc(c
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
+}
+
+// 4-D map {64 elements, tokens of a page, 2 halves of the head dim, pages x heads} over one layer's bf16 pool
+static bool make_map(CUtensorMap *map, const void *pool, const Params &p, int box) {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (fn == nullptr) {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return false;
+        fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    }
+    cuuint64_t dims[4] = {64, (cuuint64_t)p.page, 2, (cuuint64_t)p.pages * p.Hkv};
+    cuuint64_t strides[3] = {2 * HD, HD, (cuuint64_t)p.page * 2 * HD};
+    cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(pool), dims, strides, boxes, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 cudaError_t launch_tc(const Params &p, cudaStream_t st) {
@@ -565,8 +804,14 @@ cudaError_t launch_tc(const Params &p, cudaStream_t st) {
         configured[dev] = true;
     }
     const int smem = OFF_PRE + (p.B + 1) * 4;
-    if (i8) k_paged_tc<true><<<p.ctas, TC_THREADS, smem, st>>>(p);
-    else k_paged_tc<false><<<p.ctas, TC_THREADS, smem, st>>>(p);
+    int box = BKT;                              // the largest power of two up to 128 that divides the page
+    while (p.page % box) box >>= 1;
+    CUtensorMap tk, tv;
+    memset(&tk, 0, sizeof(tk));
+    memset(&tv, 0, sizeof(tv));
+    if (!i8 && !(make_map(&tk, p.k, p, box) && make_map(&tv, p.v, p, box))) return cudaErrorInvalidValue;
+    if (i8) k_paged_tc<true><<<p.ctas, TC_THREADS, smem, st>>>(tk, tv, p, box);
+    else k_paged_tc<false><<<p.ctas, TC_THREADS, smem, st>>>(tk, tv, p, box);
     return cudaGetLastError();
 }
 

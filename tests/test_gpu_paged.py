@@ -128,6 +128,11 @@ CASES = [
     (130, 2, 1, 16, 0, [130, 131, 64], True),
     (200, 4, 4, 64, 192, [200, 257], False),
     (333, 2, 2, 16, 16, [40, 333], True),                    # more queries than tokens
+    (1, 32, 8, 32, 1600, [9] * 20 + [0, 33, 200], True),     # 92 rows of all sequences on the shared part
+    (2, 16, 2, 16, 112, [2, 30, 65, 9, 2, 100, 7], True),    # ... 112, and one block
+    (1, 8, 1, 16, 0, [300] * 3, False),
+    (16, 64, 8, 16, 0, [16, 77, 900], True),                 # 128 rows of one sequence
+    (3, 32, 1, 48, 48 * 40, [3, 500], True),                 # 192 rows on the shared part, one head
 ]
 
 
