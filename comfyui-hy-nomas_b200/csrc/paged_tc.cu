@@ -10,8 +10,7 @@
 //   warps 0-7    softmax. q to shared memory (a thread per row), then per step: S from TMEM in the fragment layout (a thread
 //                holds a quarter of the columns of four rows, so the factors of int8 keys come from shared memory once for four
 //                rows, not once per row), running maximum and sum, P over S; O is rescaled only when the maximum grew by more
-//                than 2^STALE. Part of the exponentials are polynomials on the FMA pipe: at 16 a clock and SM, MUFU alone would
-//                take as long as the products. TMEM: S / P of group g at 128 g + 64 (step % 2), O at 256 + 128 g.
+//                than 2^STALE. (Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%: issue is what is short, not MUFU.) TMEM: S / P of group g at 128 g + 64 (step % 2), O at 256 + 128 g.
 //   warps 8, 9   MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
 //                thread that issues blocks until its products have read their operands, so each group has a thread of its own:
 //                the tensor pipe runs one's products while the other waits.
@@ -61,9 +60,10 @@ constexpr int OFF_MISC = OFF_PIECE + NP * 32;
 constexpr int OFF_PRE = OFF_MISC + 16 + 32 * 4;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;     // 2 s
-// O is rescaled when the maximum grew by more than 2^STALE. int8: P' <= 2^12 at the running maximum, so <= 2^15 at one stale by 2^3
-// (fp16 ends at 65504; what is lost below its smallest step is 2^-37 of the largest). A bound of 2^1 rescaled every few blocks:
-// 10200 clocks of softmax per block against FILL. Partial results are brought to the streaming kernel's 2^14.
+// A row's reference m is the maximum it was set at plus AHEAD, and is moved (and O rescaled) when a logit passes it by STALE.
+// int8: P' <= 2^12 at the reference, so <= 2^15 (fp16 ends at 65504); what is lost below fp16's smallest step is 2^-35 of the
+// largest. AHEAD spares most of the moves that come as the maximum of more and more keys grows. Partial results are
+// brought to the streaming kernel's 2^14.
 constexpr float TC_SHIFT = 12.0f, STREAM_SHIFT = 14.0f;
 
 __device__ __forceinline__ float nan_max3(float a, float b, float c) {
@@ -76,26 +76,6 @@ __device__ __forceinline__ float nan_max(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// 2^a of a pair on the FMA pipe: a = n + f, n the nearest integer (a magic addition), 2^f by a degree-4 polynomial fitted here to
-// the least largest relative error on [-1/2, 1/2] with the constant term 1 (2.9e-6 in fp32; P is rounded to 2^-9 or 2^-12), and
-// n added to the exponent field. From -127 down (a masked logit's -inf): exactly 0. a <= 127.
-__device__ __forceinline__ uint64_t exp2_fma(uint64_t a) {
-    float a0, a1;
-    x2_split(a, a0, a1);
-    a = x2(fmaxf(a0, -127.0f), fmaxf(a1, -127.0f));
-    const uint64_t t = x2_add(a, x2_splat(12582912.0f));
-    const uint64_t f = x2_fma(x2_add(t, x2_splat(-12582912.0f)), x2_splat(-1.0f), a);
-    uint64_t y = x2_fma(x2_splat(0x1.3a02ccp-7f), f, x2_splat(0x1.c9fc46p-5f));
-    y = x2_fma(y, f, x2_splat(0x1.ec0378p-3f));
-    y = x2_fma(y, f, x2_splat(0x1.62e12cp-1f));
-    y = x2_fma(y, f, x2_splat(1.0f));
-    float y0, y1, t0, t1;
-    x2_split(y, y0, y1);
-    x2_split(t, t0, t1);
-    return x2(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)),
-              __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)));
-}
-
 // The fragment layout of 16 TMEM lanes: lane l of the warp holds row l / 4 (and, in the second pair of registers, row l / 4 + 8),
 // columns 8 c + 2 (l % 4) and the next. 32 columns into registers, not waited for:
 __device__ __forceinline__ void ld_frag(uint32_t taddr, uint32_t *r) {
@@ -162,8 +142,7 @@ __device__ __forceinline__ void tma_rows(const CUtensorMap *map, uint32_t dst, u
 template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     k_paged_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int box) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr float STALE = I8 ? 3.0f : 8.0f;
-    constexpr int POLY = I8 ? 2 : 3;            // of 8 pairs: what balances the FMA pipe and MUFU
+    constexpr float STALE = I8 ? 3.0f : 8.0f, AHEAD = I8 ? 2.0f : 0.0f;
     constexpr int R_SOFTMAX = I8 ? 176 : 192, R_MMA = 56, R_LOAD = I8 ? 104 : 72;     // what each role needs without spills
     static_assert(2 * R_SOFTMAX + R_MMA + R_LOAD == 512, "the registers that the block was launched with");
     const uint32_t sb = smem_u32(smem);
@@ -351,18 +330,18 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
-                    mn[u] = nan_max(m[u], mn[u] * rsf[u]);      // a NaN stays in the row
-                    need |= !(mn[u] <= m[u] + STALE);
+                    mn[u] *= rsf[u];
+                    need |= !(mn[u] <= m[u] + STALE);           // or a NaN, which stays in the row
                 }
                 if (k == 0) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) m[u] = mn[u];
+                    for (int u = 0; u < 4; ++u) m[u] = mn[u] + AHEAD;
                 } else if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const bool grow = !(mn[u] <= m[u] + STALE);
-                        const float al = (grow ? ex2(m[u] - mn[u]) : 1.0f) * f;
-                        m[u] = grow ? mn[u] : m[u];
+                        const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
+                        m[u] = grow ? mn[u] + AHEAD : m[u];
                         mn[u] = al;
                         sum[u] *= al;
                     }
@@ -397,14 +376,9 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                             const int u = q & 1;
                             const uint32_t *y = x + 32 * hf + 4 * c + 2 * q;
                             const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), x2_splat(rsf[2 * hf + u]), nref[u]);
-                            uint64_t e;
-                            if (q < POLY) {
-                                e = exp2_fma(a);
-                            } else {
-                                float a0, a1;
-                                x2_split(a, a0, a1);
-                                e = x2(ex2(a0), ex2(a1));
-                            }
+                            float a0, a1;
+                            x2_split(a, a0, a1);
+                            uint64_t e = x2(ex2(a0), ex2(a1));
                             acc[u] = x2_add(acc[u], e);
                             if (I8) e = x2_mul(e, v[q >> 1]);
                             float e0, e1;
