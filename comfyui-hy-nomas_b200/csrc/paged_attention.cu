@@ -436,20 +436,40 @@ __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params
         const int h = head / b.G, r = l * b.G + head - h * b.G;
         float M = -INFINITY, L = 0.0f;
         float4 acc = make_float4(0, 0, 0, 0);
-        auto add = [&](const Params &p, int64_t at) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at);
-            const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * HD + 4 * lane);
-            const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f0 = ex2(M - ref), f1 = ex2(ml.x - ref);
-            M = mn;
-            L = fmaf(L, f0, f1 * ml.y);
-            acc.x = fmaf(acc.x, f0, f1 * x.x); acc.y = fmaf(acc.y, f0, f1 * x.y);
-            acc.z = fmaf(acc.z, f0, f1 * x.z); acc.w = fmaf(acc.w, f0, f1 * x.w);
+        // n pieces `step` rows apart from `at`, eight at a time: their loads go out together
+        auto add = [&](const Params &p, int64_t at, int64_t step, int n) {
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                float2 ml[8];
+                float4 x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ml[i] = make_float2(-INFINITY, 0.0f);
+                    x[i] = make_float4(0, 0, 0, 0);
+                    if (i0 + i < n) {
+                        ml[i] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (at + (i0 + i) * step));
+                        x[i] = *reinterpret_cast<const float4 *>(p.part_o + (at + (i0 + i) * step) * HD + 4 * lane);
+                    }
+                }
+                float mn = M;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+                const float ref = mn == -INFINITY ? 0.0f : mn, f0 = ex2(M - ref);
+                M = mn;
+                L *= f0;
+                acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float f = ex2(ml[i].x - ref);
+                    L = fmaf(f, ml[i].y, L);
+                    acc.x = fmaf(f, x[i].x, acc.x); acc.y = fmaf(f, x[i].y, acc.y);
+                    acc.z = fmaf(f, x[i].z, acc.z); acc.w = fmaf(f, x[i].w, acc.w);
+                }
+            }
         };
         auto take = [&](const Params &p, int tile, int64_t first, int n, int64_t quota, int row) {
             const int c0 = (int)(first / quota), c1 = (int)((first + n - 1) / quota);
-            for (int c = c0; c <= c1; ++c)
-                for (int k = 0; k < p.halves; ++k) add(p, (int64_t)(tile + c) * p.part_rows + k * 128 + row);
+            for (int k = 0; k < p.halves; ++k)
+                add(p, (int64_t)(tile + c0) * p.part_rows + k * 128 + row, p.part_rows, c1 - c0 + 1);
         };
         const int len = seq_length(b, s), rt = r / b.tb, nb = own_blocks(b, len, rt);
         const int64_t first = aheadB + (int64_t)b.sched[s] * b.Hkv +

@@ -114,6 +114,23 @@ def _load():
 lib = _load()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_DIRECT = {}
+
+
+def launch(name, device, *args):
+    """Call entry point `name` with `args` and torch's current stream on `device` (a torch.device) as its last argument,
+    that device current. The short way for calls whose host time counts: no stream object, no per-call lookup."""
+    fn = _DIRECT.get(name)
+    if fn is None:
+        fn = _DIRECT[name] = getattr(lib._cdll, name)
+    index = device.index
+    if _raw_stream is not None and index == torch._C._cuda_getDevice():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
 def last_error():
     return lib.hn_last_error().decode(errors="replace")
 

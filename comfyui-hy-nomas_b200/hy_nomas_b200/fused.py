@@ -238,29 +238,41 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False
     norm reads the fp32 sum and its result is quantized in fp32, so nothing is rounded but what is returned; for the
     reference's RMSNorm with its two bf16 roundings add first and call `rmsnorm_quant`. `out`: a caller-owned bf16
     tensor of x's shape, last dimension contiguous (x or residual themselves may be given: the stream's update in place)."""
-    _lib.require_cuda(x, residual, weight)
-    _bf16(x, residual, weight)
-    if x.shape != residual.shape or weight.shape != x.shape[-1:]:
-        raise ValueError(f"add_rmsnorm_quant: x {tuple(x.shape)}, residual {tuple(residual.shape)} and weight "
+    if not (x.is_cuda and residual.is_cuda and weight.is_cuda):
+        _lib.require_cuda(x, residual, weight)
+    bf16, device, shape = torch.bfloat16, x.device, x.shape
+    if x.dtype != bf16 or residual.dtype != bf16 or weight.dtype != bf16:
+        _bf16(x, residual, weight)
+    d = shape[-1]
+    if shape != residual.shape or weight.dim() != 1 or weight.shape[0] != d:
+        raise ValueError(f"add_rmsnorm_quant: x {tuple(shape)}, residual {tuple(residual.shape)} and weight "
                          f"{tuple(weight.shape)} do not match")
-    if out is not None and (out.shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device):
-        raise ValueError(f"add_rmsnorm_quant: out must be a bf16 {tuple(x.shape)} tensor on {x.device}")
-    d = x.shape[-1]
-    x2, r2, w = _rows16(x.reshape(-1, d)), _rows16(residual.reshape(-1, d)), _lib.dense(weight)
+    if kind not in _KINDS:
+        raise ValueError(f"add_rmsnorm_quant: kind {kind!r} (int8 or fp8)")
+    flat = x.dim() == 2
+    x2, r2 = (x, residual) if flat else (x.reshape(-1, d), residual.reshape(-1, d))
+    x2, r2 = _rows16(x2), _rows16(r2)
+    w = weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else _lib.dense(weight)
     rows = x2.shape[0]
-    total = torch.empty(x.shape, device=x.device, dtype=torch.bfloat16) if out is None else out
-    o2 = total.view(-1, d)
-    if out is not None and not _rows16_ok(o2):
-        raise ValueError("add_rmsnorm_quant: out needs contiguous, 16-byte aligned rows")
-    code, dtype = _KINDS[kind]
-    q = torch.empty((rows, d), device=x.device, dtype=dtype)
-    if per_token:
-        s, srs, sgs = torch.empty((rows, 1), device=x.device, dtype=torch.float32), 1, 1
+    if out is None:
+        total = torch.empty(shape, dtype=bf16, device=device)
+        o2, ldo = total, d
     else:
-        s, srs, sgs = _lib.group_scales(rows, d // 128, x.device)
-    rc = _lib.lib.hn_add_rmsnorm_quant(x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), w.data_ptr(), rows, d, eps,
-                                       code, 1 if per_token else 0, o2.data_ptr(), o2.stride(0), q.data_ptr(), d,
-                                       s.data_ptr(), srs, sgs, _lib.stream_of(x2))
+        if out.shape != shape or out.dtype != bf16 or out.device != device:
+            raise ValueError(f"add_rmsnorm_quant: out must be a bf16 {tuple(shape)} tensor on {device}")
+        total, o2 = out, out.view(-1, d)
+        if not _rows16_ok(o2):
+            raise ValueError("add_rmsnorm_quant: out needs contiguous, 16-byte aligned rows")
+        ldo = o2.stride(0)
+    code, dtype = _KINDS[kind]
+    q = torch.empty((rows, d), dtype=dtype, device=device)
+    if per_token:
+        s, srs, sgs = torch.empty((rows, 1), dtype=torch.float32, device=device), 1, 1
+    else:
+        sgs = (rows + 3) // 4 * 4                # group-major, as _lib.group_scales lays them out
+        s, srs = torch.empty_strided((rows, d // 128), (1, sgs), dtype=torch.float32, device=device), 1
+    rc = _lib.launch("hn_add_rmsnorm_quant", device, x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), w.data_ptr(),
+                     rows, d, eps, code, 1 if per_token else 0, o2.data_ptr(), ldo, q.data_ptr(), d, s.data_ptr(), srs, sgs)
     _lib.check(rc, "add_rmsnorm_quant")
     return total, q, s
 

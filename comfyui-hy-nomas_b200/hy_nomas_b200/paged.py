@@ -83,6 +83,7 @@ class KVCache:
         self._struct = _Struct(p(k), p(v), p(ks), p(vs), p(self.table), p(self.lengths), p(self.refs), p(self.failed),
                                layers, pages, heads, page, slots, width)
         self._ref = ctypes.addressof(self._struct)
+        self._ws_bytes = {}
 
     def _ids(self, x, what):
         """A list of row or page ids as a contiguous int32 tensor on the cache's device."""
@@ -108,8 +109,8 @@ class KVCache:
         if tokens < 0:
             raise ValueError(f"extend: {tokens} tokens")
         ws = self._scratch(rows.numel())
-        _lib.check(_lib.lib.hn_cache_extend(self._ref, rows.data_ptr(), rows.numel(), tokens, ws.data_ptr(),
-                                            _lib.stream_of(self.k)), "cache.extend")
+        _lib.check(_lib.launch("hn_cache_extend", self.device, self._ref, rows.data_ptr(), rows.numel(), tokens,
+                               ws.data_ptr()), "cache.extend")
 
     def append(self, layer, k, v, rows):
         """k, v [B, n, heads, 128] bf16 (any strides in whole 16-byte steps, the last dimension contiguous) into the last n
@@ -125,15 +126,17 @@ class KVCache:
         if not 0 <= layer < self.layers:
             raise ValueError(f"append: layer {layer} of {self.layers}")
         k, v = _operand(k), _operand(v)
+        if k.device != self.device or v.device != self.device:
+            raise RuntimeError(f"append: k on {k.device} and v on {v.device}, the cache is on {self.device}")
         kb, kt, kh, _ = k.stride()
         vb, vt, vh, _ = v.stride()
-        _lib.check(_lib.lib.hn_cache_append(self._ref, layer, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh,
-                                            rows.data_ptr(), k.shape[0], k.shape[1], _lib.stream_of(k)), "cache.append")
+        _lib.check(_lib.launch("hn_cache_append", self.device, self._ref, layer, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt,
+                               vh, rows.data_ptr(), k.shape[0], k.shape[1]), "cache.append")
 
     def free(self, rows):
         """The listed rows drop their pages and become empty. A page is free again when its last row drops it."""
         rows = self._ids(rows, "free")
-        _lib.check(_lib.lib.hn_cache_free(self._ref, rows.data_ptr(), rows.numel(), _lib.stream_of(self.k)), "cache.free")
+        _lib.check(_lib.launch("hn_cache_free", self.device, self._ref, rows.data_ptr(), rows.numel()), "cache.free")
 
     def fork(self, parents, children):
         """children[i], an empty row, becomes a branch of parents[i]: it shares the full pages, and the tokens of a
@@ -143,21 +146,21 @@ class KVCache:
         if children.numel() != n:
             raise ValueError(f"fork: {n} parents for {children.numel()} children")
         ws = self._scratch(n)
-        _lib.check(_lib.lib.hn_cache_fork(self._ref, parents.data_ptr(), children.data_ptr(), n, ws.data_ptr(),
-                                          _lib.stream_of(self.k)), "cache.fork", 2)
+        _lib.check(_lib.launch("hn_cache_fork", self.device, self._ref, parents.data_ptr(), children.data_ptr(), n,
+                               ws.data_ptr()), "cache.fork", 2)
 
     def compact(self):
         """The pages in use move to the lowest ids: the k-th used page above the number in use goes to the k-th free
         id below it, in every layer, and the table follows."""
         ws = self._scratch(0)
-        _lib.check(_lib.lib.hn_cache_compact(self._ref, ws.data_ptr(), _lib.stream_of(self.k)), "cache.compact", 2)
+        _lib.check(_lib.launch("hn_cache_compact", self.device, self._ref, ws.data_ptr()), "cache.compact", 2)
 
     def copy_pages(self, src, dst):
         """Page src[i] to page dst[i] in every layer. No page may be both a source and a target, or twice a target."""
         src, dst = self._ids(src, "copy_pages"), self._ids(dst, "copy_pages")
         if src.numel() != dst.numel():
             raise ValueError(f"copy_pages: {src.numel()} sources for {dst.numel()} targets")
-        _lib.check(_lib.lib.hn_cache_copy(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), _lib.stream_of(self.k)),
+        _lib.check(_lib.launch("hn_cache_copy", self.device, self._ref, src.data_ptr(), dst.data_ptr(), src.numel()),
                    "cache.copy_pages")
 
     def save(self):
@@ -195,8 +198,11 @@ def attention(q, cache, layer, rows, shared=0, causal=True, scale=None, out=None
 
     `shared`: the rows' first `shared` tokens, a multiple of the page, are on the same pages, as `fork` leaves them;
     those are read once for all rows. The result is the same as with shared=0 up to rounding."""
+    device = cache.device
     if not q.is_cuda:
         _lib.require_cuda(q)
+    if q.device != device:
+        raise RuntimeError(f"attention: q on {q.device}, the cache is on {device}")
     if q.dtype != torch.bfloat16:
         raise TypeError(f"attention: q must be bf16, got {q.dtype}")
     if q.dim() != 4 or q.shape[3] != HEAD_DIM:
@@ -205,22 +211,25 @@ def attention(q, cache, layer, rows, shared=0, causal=True, scale=None, out=None
     b, lq, h, d = q.shape
     if rows.numel() != b:
         raise ValueError(f"attention: {rows.numel()} rows for {b} sequences")
-    if q.device != cache.device:
-        raise RuntimeError(f"attention: q on {q.device}, the cache is on {cache.device}")
     q = _operand(q)
     if out is None:
-        out = torch.empty((b, lq, h, d), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != q.device or _operand(out) is not out:
+        out = torch.empty((b, lq, h, d), dtype=torch.bfloat16, device=device)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != device or _operand(out) is not out:
         raise ValueError(f"attention: out must be bf16 {tuple(q.shape)} with contiguous, 16-byte aligned rows of {d}")
-    lse = torch.empty((b, h, lq), dtype=torch.float32, device=q.device) if return_lse else None
-    size = ctypes.c_int64()
-    _lib.check(_lib.lib.hn_paged_attention_workspace(cache._ref, b, lq, h, shared, int(causal), ctypes.byref(size)),
-               "paged.attention", 0)
-    ws = torch.empty(max(size.value, 16), dtype=torch.uint8, device=q.device)
+    lse = torch.empty((b, h, lq), dtype=torch.float32, device=device) if return_lse else None
+    causal = 1 if causal else 0
+    plan = (b, lq, h, shared, causal)
+    size = cache._ws_bytes.get(plan)            # the workspace's size goes by these numbers alone
+    if size is None:
+        n = ctypes.c_int64()
+        _lib.check(_lib.lib.hn_paged_attention_workspace(cache._ref, b, lq, h, shared, causal, ctypes.byref(n)),
+                   "paged.attention", 0)
+        size = cache._ws_bytes[plan] = max(n.value, 16)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
     qb, ql, qh, _ = q.stride()
     ob, ol, oh, _ = out.stride()
-    _lib.check(_lib.lib.hn_paged_attention(
-        cache._ref, layer, q.data_ptr(), qb, ql, qh, rows.data_ptr(), b, lq, h, d, shared, int(causal),
+    _lib.check(_lib.launch(
+        "hn_paged_attention", device, cache._ref, layer, q.data_ptr(), qb, ql, qh, rows.data_ptr(), b, lq, h, d, shared, causal,
         1.0 / math.sqrt(d) if scale is None else float(scale), out.data_ptr(), ob, ol, oh,
-        None if lse is None else lse.data_ptr(), ws.data_ptr(), size.value, _lib.stream_of(q)), "paged.attention", 2)
+        None if lse is None else lse.data_ptr(), ws.data_ptr(), size), "paged.attention", 2)
     return (out, lse) if return_lse else out
