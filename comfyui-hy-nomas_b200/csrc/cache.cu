@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(256) k_free(Meta m, const int *rows, int n) {
 // fork, plan: request i gets a new page for its parent's partial last page. moves: src, dst, tokens of request i
 // (dst -1: nothing to copy), and ok[i] whether the child's row is to be written.
 __global__ void __launch_bounds__(PLAN) k_fork_plan(Meta m, const int *parents, const int *children, int n, int *ws) {
+    dep_launch();
     __shared__ int sums[32];
     int *claim = ws, *list = claim + m.slots, *src = list + m.pages, *dst = src + n, *ntok = dst + n, *ok = ntok + n;
     for (int i = threadIdx.x; i < n; i += PLAN)
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(PLAN) k_fork_plan(Meta m, const int *parents, 
 // compact, plan: with n live pages, the k-th live page at or above n moves to the k-th free id below n. move_to[p]
 // (p >= n) is where page p goes; src, dst list the moves, count[0] is their number.
 __global__ void __launch_bounds__(PLAN) k_compact_plan(Meta m, int *ws) {
+    dep_launch();
     __shared__ int sums[32];
     int *count = ws, *to = ws + 4, *src = to + m.pages, *dst = src + m.pages;
     int live = 0;
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(256) k_copy_pages(CopyParams p) { copy_units(p
 // fork, pass: the children's rows (full pages shared, the new tail page), then the tails' data
 __global__ void __launch_bounds__(256) k_fork_pass(CopyParams p, Meta m, const int *parents, const int *children, int n,
                                                    const int *ok) {
+    dep_wait();
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
         if (!ok[i]) continue;
         const int a = parents[i], c = children[i], len = m.lengths[a], full = len / m.page;
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(256) k_fork_pass(CopyParams p, Meta m, const i
 
 // compact, pass: table entries at or above the live count follow their pages, then the pages' data
 __global__ void __launch_bounds__(256) k_compact_pass(CopyParams p, Meta m, const int *ws) {
+    dep_wait();
     const int live = ws[1];
     const int *to = ws + 4;
     const int64_t n = (int64_t)m.slots * m.width;
@@ -418,8 +422,8 @@ cudaError_t launch_cache_fork(const CacheArgs &a, const int *parents, const int 
     CopyParams p = copy_params(a);
     const int *src = ws + a.meta.slots + a.meta.pages;
     p.src = src; p.dst = src + n; p.ntok = src + 2 * n; p.n = n;
-    k_fork_pass<<<copy_grid((int64_t)n * a.layers * 2 * a.heads), 256, 0, st>>>(p, a.meta, parents, children, n, src + 3 * n);
-    return cudaGetLastError();
+    return launch_after(k_fork_pass, copy_grid((int64_t)n * a.layers * 2 * a.heads), 256, 0, st, p, a.meta, parents, children, n,
+                        src + 3 * n);
 }
 cudaError_t launch_cache_compact(const CacheArgs &a, int *ws, cudaStream_t st) {
     k_compact_plan<<<1, PLAN, 0, st>>>(a.meta, ws);
@@ -428,8 +432,7 @@ cudaError_t launch_cache_compact(const CacheArgs &a, int *ws, cudaStream_t st) {
     CopyParams p = copy_params(a);
     p.count = ws; p.src = ws + 4 + a.meta.pages; p.dst = p.src + a.meta.pages;
     // at most half of the pages move
-    k_compact_pass<<<copy_grid((int64_t)(a.meta.pages / 2) * a.layers * 2 * a.heads), 256, 0, st>>>(p, a.meta, ws);
-    return cudaGetLastError();
+    return launch_after(k_compact_pass, copy_grid((int64_t)(a.meta.pages / 2) * a.layers * 2 * a.heads), 256, 0, st, p, a.meta, ws);
 }
 cudaError_t launch_cache_copy(const CacheArgs &a, const int *src, const int *dst, int n, cudaStream_t st) {
     CopyParams p = copy_params(a);

@@ -401,4 +401,27 @@ __device__ __forceinline__ int64_t div_nonneg(int64_t a, int64_t d) {
     return a / d;
 }
 
+// ---------------------------------------------------------------------------------------------------
+// A kernel that follows another of the same call on its stream: it may start while the one before it drains
+// (programmatic stream serialization). The first kernel of a call is launched plainly, so nothing of a call starts
+// before what was on the stream; every other one waits (dep_wait) before it reads what the one before wrote, and at the
+// latest before it ends, so that its end is the end of all of them.
+__device__ __forceinline__ void dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+inline cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 } // namespace hn

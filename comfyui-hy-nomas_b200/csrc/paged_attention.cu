@@ -86,6 +86,56 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
     const uint32_t sb = saddr(smem);
     const int rows = w.own_b < 0 ? p.B * p.Lq * p.G : p.Lq * p.G;
 
+    // --- loader: block i of the piece into stage i % ST. A thread's chunks of step `it` are all in 16-key group
+    // it * (128 / CPR) / 16, which lies in one page (pages and the parts' first keys are multiples of 16 tokens).
+    const int seq = p.rows[w.own_b < 0 ? 0 : w.own_b];
+    const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
+    constexpr int RPI = THREADS / CPR;                           // rows per step: 8 (bf16), 16 (int8)
+    // The page and the place in it of the next block's four groups. The table is read a block ahead, so that no warp waits
+    // for it, and the place moves on by addition (a division per group took a fifth of the loader's instructions).
+    int id[4], off[4], pg = (w.kbeg + w.blk0 * BK) / p.page, at = w.kbeg + w.blk0 * BK - pg * p.page, key = w.kbeg + w.blk0 * BK;
+    auto look_up = [&]() {
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) {
+            id[sub] = key < w.kend && pg < p.width ? tab[pg] : -1;
+            off[sub] = at;
+            key += 16;
+            at += 16;
+            if (at == p.page) { at = 0; ++pg; }
+        }
+    };
+    look_up();
+    auto load = [&](int i) {
+        if (i < w.nblk) {
+            const uint32_t st = sb + (uint32_t)(i % ST) * STAGE;
+            const int left = w.kend - (w.kbeg + (w.blk0 + i) * BK);     // keys of the block that are there
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub) {
+                const bool there = (unsigned)id[sub] < (unsigned)p.pages;
+                const int64_t tok = there ? ((int64_t)id[sub] * p.Hkv + w.h) * p.page + off[sub] : 0;
+#pragma unroll
+                for (int it = 0; it < 16 / RPI; ++it) {
+                    const int r = it * RPI + tid / CPR, c = tid % CPR, row = 16 * sub + r;
+                    const bool ok = there && row < left;
+                    const int64_t src = ok ? (tok + r) * (CPR * 16) + c * 16 : 0;
+                    const int ck = I8 ? c ^ ((row & 1) << 2) : c ^ (row & 7);
+                    const int cv = I8 ? c ^ (((row >> 1) & 3) << 1) : c ^ (row & 7);
+                    cp16(st + row * (CPR * 16) + ck * 16, p.k + src, ok);
+                    cp16(st + TILE + row * (CPR * 16) + cv * 16, p.v + src, ok);
+                }
+                if (I8 && tid < 32) {
+                    const int r = tid & 15;
+                    const bool ok = there && 16 * sub + r < left;
+                    const float *sc = tid < 16 ? p.ks : p.vs;
+                    cp4(st + 2 * TILE + (tid < 16 ? 0 : BK * 4) + (16 * sub + r) * 4, sc + (ok ? tok + r : 0), ok);
+                }
+            }
+            look_up();
+        }
+        cp_commit();
+    };
+    for (int i = 0; i < ST - 1; ++i) load(i);       // on their way while q is read
+
     // --- the two rows of this lane: their key limits and q
     int lim[2];
     float rowscale[2];
@@ -145,61 +195,11 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
         minlim = y < minlim ? y : minlim;
     }
 
-    // --- loader: block i of the piece into stage i % ST. A thread's chunks of step `it` are all in 16-key group
-    // it * (128 / CPR) / 16, which lies in one page (pages and the parts' first keys are multiples of 16 tokens).
-    const int seq = p.rows[w.own_b < 0 ? 0 : w.own_b];
-    const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
-    constexpr int RPI = THREADS / CPR;                           // rows per step: 8 (bf16), 16 (int8)
-    // The page and the place in it of the next block's four groups. The table is read a block ahead, so that no warp waits
-    // for it, and the place moves on by addition (a division per group took a fifth of the loader's instructions).
-    int id[4], off[4], pg = (w.kbeg + w.blk0 * BK) / p.page, at = w.kbeg + w.blk0 * BK - pg * p.page, key = w.kbeg + w.blk0 * BK;
-    auto look_up = [&]() {
-#pragma unroll
-        for (int sub = 0; sub < 4; ++sub) {
-            id[sub] = key < w.kend && pg < p.width ? tab[pg] : -1;
-            off[sub] = at;
-            key += 16;
-            at += 16;
-            if (at == p.page) { at = 0; ++pg; }
-        }
-    };
-    look_up();
-    auto load = [&](int i) {
-        if (i < w.nblk) {
-            const uint32_t st = sb + (uint32_t)(i % ST) * STAGE;
-            const int left = w.kend - (w.kbeg + (w.blk0 + i) * BK);     // keys of the block that are there
-#pragma unroll
-            for (int sub = 0; sub < 4; ++sub) {
-                const bool there = (unsigned)id[sub] < (unsigned)p.pages;
-                const int64_t tok = there ? ((int64_t)id[sub] * p.Hkv + w.h) * p.page + off[sub] : 0;
-#pragma unroll
-                for (int it = 0; it < 16 / RPI; ++it) {
-                    const int r = it * RPI + tid / CPR, c = tid % CPR, row = 16 * sub + r;
-                    const bool ok = there && row < left;
-                    const int64_t src = ok ? (tok + r) * (CPR * 16) + c * 16 : 0;
-                    const int ck = I8 ? c ^ ((row & 1) << 2) : c ^ (row & 7);
-                    const int cv = I8 ? c ^ (((row >> 1) & 3) << 1) : c ^ (row & 7);
-                    cp16(st + row * (CPR * 16) + ck * 16, p.k + src, ok);
-                    cp16(st + TILE + row * (CPR * 16) + cv * 16, p.v + src, ok);
-                }
-                if (I8 && tid < 32) {
-                    const int r = tid & 15;
-                    const bool ok = there && 16 * sub + r < left;
-                    const float *sc = tid < 16 ? p.ks : p.vs;
-                    cp4(st + 2 * TILE + (tid < 16 ? 0 : BK * 4) + (16 * sub + r) * 4, sc + (ok ? tok + r : 0), ok);
-                }
-            }
-            look_up();
-        }
-        cp_commit();
-    };
-
     float o[16][4];
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-    for (int i = 0; i < ST - 1; ++i) load(i);
     for (int i = 0; i < w.nblk; ++i) {
         cp_wait<ST - 2>();
         __syncthreads();                        // block i is here, and every warp is done with block i - 1
@@ -408,6 +408,7 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sums[32];
     int *pre = reinterpret_cast<int *>(smem + smem_bytes<I8>());
+    dep_launch();
     prefix_blocks(p, pre, sums, THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += THREADS) p.sched[b] = pre[b];
@@ -419,11 +420,13 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
         else if (rows_per == 32) run_piece<I8, 2>(p, w, smem);
         else run_piece<I8, 4>(p, w, smem);
     }
+    dep_wait();             // nothing here reads what the other line writes, but the join waits for this kernel only
 }
 
 // Joins the partial results of every row (one warp each): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. `a` is the
 // line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
 __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b) {
+    dep_wait();
     const int lane = threadIdx.x & 31;
     const int64_t items = (int64_t)b.B * b.Lq * b.H;
     const int64_t blocksA = (int64_t)a.Hkv * a.nrtA * a.nbA, aheadB = (int64_t)b.Hkv * b.nrtA * b.nbA;
@@ -606,16 +609,19 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
             if (e != cudaSuccess) return e;
             configured[dev] = true;
         }
-        if (i8) k_paged_attention<true><<<s.ctas, THREADS, smem, st>>>(s);
-        else k_paged_attention<false><<<s.ctas, THREADS, smem, st>>>(s);
-        e = cudaGetLastError();
+        const auto kernel = i8 ? k_paged_attention<true> : k_paged_attention<false>;
+        if (pl.tc_slots) {
+            e = launch_after(kernel, s.ctas, THREADS, smem, st, s);
+        } else {
+            kernel<<<s.ctas, THREADS, smem, st>>>(s);
+            e = cudaGetLastError();
+        }
         if (e != cudaSuccess) return e;
     }
     int64_t grid = cdiv((int64_t)a.B * a.Lq * a.H, 8);
     if (grid > (int64_t)num_sms() * 8) grid = (int64_t)num_sms() * 8;
     const bool tc_a = pl.shared_tc, tc_b = pl.own_tc;
-    k_paged_join<<<(unsigned)grid, 256, 0, st>>>(tc_a ? t : s, tc_b ? t : s);
-    return cudaGetLastError();
+    return launch_after(k_paged_join, (unsigned)grid, 256, 0, st, tc_a ? t : s, tc_b ? t : s);
 }
 
 } // namespace hn

@@ -177,6 +177,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    dep_launch();
     prefix_blocks(p, pre, sums, TC_THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += TC_THREADS) p.sched[b] = pre[b];
