@@ -342,16 +342,29 @@ struct AppendParams {
     int B, n, heads;
 };
 
-// append: the last n tokens of each listed row. One warp per (sequence, token, head): lanes 0-15 hold the K row, 16-31
-// the V row, 8 elements each. bf16 is copied; int8 takes the absmax over the 16 lanes, hn_quantize_kv's scale and codes.
+// append: the last n tokens of each listed row. A warp takes the heads of one token, four K and V rows of 128 at a time
+// (lanes 0-15 a K row, 16-31 the V row, 8 elements each), so that eight rows are in flight. bf16 is copied; int8 takes the
+// absmax over the 16 lanes, hn_quantize_kv's scale and codes.
 template <bool I8>
 __global__ void __launch_bounds__(256) k_append(AppendParams p, Meta m) {
-    const int lane = threadIdx.x & 31, sub = lane & 15, kv = lane >> 4;
-    const int64_t units = (int64_t)p.B * p.n * p.heads, step = (int64_t)gridDim.x * 8;
+    const int lane = threadIdx.x & 31, sub = lane & 15;
+    const bool isv = lane >= 16;
+    const __nv_bfloat16 *x = (isv ? p.x[1] : p.x[0]) + 8 * sub;
+    const int64_t bs = isv ? p.bs[1] : p.bs[0], ts = isv ? p.ts[1] : p.ts[0], hs = isv ? p.hs[1] : p.hs[0];
+    uint8_t *pool = isv ? p.pool[1] : p.pool[0];
+    float *scale = isv ? p.scale[1] : p.scale[0];
+    constexpr int U = 4;
+    const int groups = (p.heads + U - 1) / U;               // a warp's share of a token: U heads
+    const int64_t units = (int64_t)p.B * p.n * groups, step = (int64_t)gridDim.x * 8;
     for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += step) {
-        const int64_t bt = div_nonneg(u, p.heads);
-        const int h = (int)(u - bt * p.heads);
+        const int64_t bt = div_nonneg(u, groups);
+        const int h0 = (int)(u - bt * groups) * U;
         const int b = (int)div_nonneg(bt, p.n), t = (int)(bt - (int64_t)b * p.n);
+        const __nv_bfloat16 *src = x + b * bs + t * ts + h0 * hs;
+        uint4 raw[U];                                       // before the table is known: the loads do not depend on it
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (h0 + i < p.heads) raw[i] = ldg_stream(src + i * hs);
         const int row = p.rows[b];
         int page = -1, at = 0;
         if (in_range(row, m.slots)) {
@@ -361,28 +374,32 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p, Meta m) {
             at -= j * m.page;
         }
         if (!in_range(page, m.pages)) {          // the token has no place: extend did not (or could not) make one
-            if (lane == 0) atomicAdd(m.failed, 1);
+            if (lane == 0 && h0 == 0) atomicAdd(m.failed, p.heads);
             continue;
         }
-        const uint4 raw = ldg_stream(p.x[kv] + b * p.bs[kv] + t * p.ts[kv] + h * p.hs[kv] + 8 * sub);
-        const int64_t token = ((int64_t)page * p.heads + h) * m.page + at;
-        if (!I8) {
-            *reinterpret_cast<uint4 *>(p.pool[kv] + token * (2 * HD) + 16 * sub) = raw;
-        } else {
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-            float v[8], peak = 0.0f;
+        const int64_t token = ((int64_t)page * p.heads + h0) * m.page + at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = bf16_lo(w[i]);
-                v[2 * i + 1] = bf16_hi(w[i]);
-                peak = absmax3(peak, v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < U; ++i) {
+            if (h0 + i >= p.heads) break;
+            const int64_t to = token + (int64_t)i * m.page;
+            if (!I8) {
+                *reinterpret_cast<uint4 *>(pool + to * (2 * HD) + 16 * sub) = raw[i];
+            } else {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                float v[8], peak = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[2 * j] = bf16_lo(w[j]);
+                    v[2 * j + 1] = bf16_hi(w[j]);
+                    peak = absmax3(peak, v[2 * j], v[2 * j + 1]);
+                }
+                peak = warp_max_xor(peak, 16);
+                const float sc = i8_scale_bf16(peak);
+                const bool fast = sc >= 0x1p-90f;
+                *reinterpret_cast<uint2 *>(pool + to * HD + 8 * sub) =
+                    quant_chunk8<0, false>(v, sc, fast, x2_splat(-sc), x2_splat(__frcp_rn(sc)));
+                if (sub == 0) scale[to] = sc;
             }
-            peak = warp_max_xor(peak, 16);
-            const float sc = i8_scale_bf16(peak);
-            const bool fast = sc >= 0x1p-90f;
-            *reinterpret_cast<uint2 *>(p.pool[kv] + token * HD + 8 * sub) =
-                quant_chunk8<0, false>(v, sc, fast, x2_splat(-sc), x2_splat(__frcp_rn(sc)));
-            if (sub == 0) p.scale[kv][token] = sc;
         }
     }
 }
@@ -454,7 +471,7 @@ cudaError_t launch_cache_append(const CacheArgs &a, int layer, const void *k, in
     p.scale[0] = a.ks ? a.ks + tokens : nullptr;
     p.scale[1] = a.ks ? a.vs + tokens : nullptr;
     p.rows = rows; p.B = B; p.n = n; p.heads = a.heads;
-    int64_t grid = cdiv((int64_t)B * n * a.heads, 8);
+    int64_t grid = cdiv((int64_t)B * n * cdiv(a.heads, 4), 8);
     const int64_t most = (int64_t)num_sms() * 8;
     if (grid > most) grid = most;
     if (a.ks) k_append<true><<<(unsigned)grid, 256, 0, st>>>(p, a.meta);

@@ -36,7 +36,6 @@ struct Params {
     int nbA, nrtA, ta;                  // shared tiles: blocks, row tiles per head, rows per tile (nbA 0: not on this line)
     int has_own, nrtB, tb, own_first;   // own tiles
     int ends;                           // a whole own tile ends its rows
-    int halves;                         // 2: a tile's even and odd blocks are summed apart, rows [0, ta) and [ta, 2 ta) of a slot
     int part_rows;                      // rows per slot
     float *part_o, *part_ml;            // [slots][part_rows][128], [slots][part_rows][2]
     int *sched;                         // [B + 1] prefix sums of the own blocks (of one head), written for the join
@@ -159,7 +158,7 @@ struct Walker {
         }
         const int64_t stop = end < tile_end ? end : tile_end;
         w.nblk = (int)(stop - x);
-        const bool whole = w.blk0 == 0 && stop == tile_end && w.own_b >= 0 && p.ends && p.halves == 1;
+        const bool whole = w.blk0 == 0 && stop == tile_end && w.own_b >= 0 && p.ends;
         w.slot = whole ? -1 : tile + cta;
         x = stop;
         return true;

@@ -471,14 +471,13 @@ __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params
         };
         auto take = [&](const Params &p, int tile, int64_t first, int n, int64_t quota, int row) {
             const int c0 = (int)(first / quota), c1 = (int)((first + n - 1) / quota);
-            for (int k = 0; k < p.halves; ++k)
-                add(p, (int64_t)(tile + c0) * p.part_rows + k * 128 + row, p.part_rows, c1 - c0 + 1);
+            add(p, (int64_t)(tile + c0) * p.part_rows + row, p.part_rows, c1 - c0 + 1);
         };
         const int len = seq_length(b, s), rt = r / b.tb, nb = own_blocks(b, len, rt);
         const int64_t first = aheadB + (int64_t)b.sched[s] * b.Hkv +
                               (int64_t)h * (b.sched[s + 1] - b.sched[s]) + own_blocks_below(b, len, rt);
         // the rows ended in their CTA
-        if (b.ends && b.halves == 1 && nb > 0 && first / qB == (first + nb - 1) / qB) continue;
+        if (b.ends && nb > 0 && first / qB == (first + nb - 1) / qB) continue;
         if (a.nbA) {
             const int64_t ra = (int64_t)s * a.Lq * a.G + r;
             const int tile = h * a.nrtA + (int)(ra / a.ta);
@@ -497,7 +496,10 @@ __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params
 static int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 // CTAs of the streaming kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
 static int stream_ctas(bool i8) { return num_sms() * (i8 ? 3 : 2); }
-constexpr int TC_ROWS = 65;             // rows from which a tile goes to the tensor-core line
+// Rows from which a part goes to the tensor-core line. A tile there is two groups of 128 rows over the same keys; measured, us, on
+// this line / the tensor cores: shared part of 15840 tokens, 8 heads, bf16: 128 rows 67 / 76, 256 rows 107 / 91, 512 rows 270 /
+// 92; int8 81 / 90, 141 / 105, 268 / 138. Own parts of 2000 tokens, 8 sequences, 16 heads, 100 rows: 97 / 79 and 122 / 119.
+constexpr int TC_SHARED = 129, TC_OWN = 65;
 
 struct Plan {
     bool shared_tc, own_tc;             // which line holds which part
@@ -506,9 +508,10 @@ struct Plan {
     size_t tc_at, sched_at;             // byte offsets in the workspace: the second line's partials, the prefix sums
 };
 
-// The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_ROWS rows per K/V head or
-// more walks all of its keys on the tensor-core line; else the rows of all sequences attend to the shared part
-// together, on the tensor cores if there are TC_ROWS of them, and the own parts stream.
+// The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_OWN rows per K/V head or
+// more walks all of its keys on the tensor-core line (it is bound by the products, and the shared pages come from L2); else
+// the rows of all sequences attend to the shared part together, on the tensor cores if there are TC_SHARED of them, and the
+// own parts stream.
 static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     Plan pl;
     const bool i8 = a.cache.ks != nullptr;
@@ -516,13 +519,14 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     s.shared = a.shared; s.causal = a.causal;
     s.nbA = s.nrtA = 0; s.ta = 16;
     s.has_own = 0; s.nrtB = 0; s.tb = 16; s.own_first = 0;
-    s.halves = 1; s.ends = 0; s.min_quota = 4;
+    // two blocks a CTA at least (four: 31.7 -> 35.7 us for 256 rows over 4096 keys, 8 heads; the rest within 2%)
+    s.ends = 0; s.min_quota = 2;
     t = s;
     const int64_t r1 = (int64_t)a.Lq * s.G, all = r1 * a.B;
-    pl.own_tc = r1 >= TC_ROWS;
+    pl.own_tc = r1 >= TC_OWN;
     // one sequence has nothing to share
     const bool split = a.shared > 0 && a.B > 1 && !pl.own_tc;
-    pl.shared_tc = split && all >= TC_ROWS;
+    pl.shared_tc = split && all >= TC_SHARED;
     s.bk = BK; s.ctas = stream_ctas(i8);
     t.bk = 128; t.ctas = num_sms();
     Params &own = pl.own_tc ? t : s;
@@ -534,9 +538,8 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     if (split) {
         Params &sh = pl.shared_tc ? t : s;
         sh.nbA = (int)cdiv(a.shared, sh.bk);
-        sh.ta = !pl.shared_tc ? tile_rows(all) : all <= 128 ? 128 : 256;
+        sh.ta = pl.shared_tc ? 256 : tile_rows(all);
         sh.nrtA = (int)cdiv(all, sh.ta);
-        if (sh.ta == 128) sh.halves = 2;
     }
     auto slots = [&](Params &p) -> int64_t {
         p.part_rows = p.bk == 128 ? 256 : p.ta > p.tb ? p.ta : p.tb;

@@ -1,10 +1,8 @@
-// paged_tc.cu - the tensor-core line of the paged attention: tiles of 65 rows and more (a segment's queries over its own
-// and the shared tokens, or the rows of many sequences over the shared ones). tcgen05 kind::f16 products, S / P and O in
+// paged_tc.cu - the tensor-core line of the paged attention: many rows (a segment's queries over its own and the shared
+// tokens, or the rows of many sequences over the shared ones). tcgen05 kind::f16 products, S / P and O in
 // tensor memory; the pieces, partial results and formulas are paged.cuh's and paged_attention.cu's.
 //
-// One CTA per SM, blocks of 128 keys, two softmax groups of 128 rows each. Two row tiles of one K/V head share each K and
-// V block (a tile of 256 rows), or, for tiles of at most 128 rows (`halves` 2), the groups hold the same rows and take
-// every other block of the CTA (so each group always meets the same two ring slots, and no phase of theirs is skipped).
+// One CTA per SM, tiles of 256 rows: two softmax groups of 128 rows each share the K and V blocks of 128 keys.
 // A block goes through a group in two steps of 64 keys, with S in one of two TMEM buffers: the products of step k + 1 run
 // while step k is in the softmax (with one buffer of 128 keys the softmax waited for S 2250 of every 5100 clocks).
 //   warps 0-7    softmax. q to shared memory (a thread per row), then per step: S from TMEM in the fragment layout (a thread
@@ -158,12 +156,12 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     }
 
     if (threadIdx.x == 0) {
-        // a block of two row tiles is given back by both groups' issuers, else by the one that takes it
-        for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, I8 ? 128 : 1); mbar_init(b_empty + 8 * i, p.halves == 2 ? 1 : 2); }
+        // a block is given back by both groups' issuers
+        for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, I8 ? 128 : 1); mbar_init(b_empty + 8 * i, 2); }
         for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, 10 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
         for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 4); mbar_init(b_v + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 128);
-        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, p.halves == 2 ? 8 : 12); }   // softmax, producers
+        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, 12); }   // softmax, producers
         mbar_init(b_end, 1);
         mbar_init(b_end + 8, 1);
         mbar_init(b_tail, 1);
@@ -185,7 +183,6 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const bool split = p.halves == 2;           // the groups share the rows and take every other block
     const int rows_all = p.nbA ? p.B * p.Lq * p.G : p.Lq * p.G;
     bool ok = true;
     // the next piece of the ring, for every warp that reads pieces; nblk 0: there are no more
@@ -211,7 +208,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         int n_s = 0, n_tile = 0;                // steps of this group, blocks of the CTA
         while (const Piece *pc = next_piece()) {
             const Piece &w = *pc;
-            const int r = w.row0 + (split ? 0 : 128 * g) + rr;
+            const int r = w.row0 + 128 * g + rr;
             const bool valid = r < rows_all;
             int lim = w.kend;                   // a row past the tile's end: computed and dropped
             const __nv_bfloat16 *qp = p.q;
@@ -251,20 +248,19 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             mbar_arrive(b_q + 8 * g);
 
             // --- from here on a thread works on rows 16 hf + 8 u + lane / 4 of its warp's 32
-            const int nblk = w.nblk, j0 = split ? (n_tile ^ g) & 1 : 0;          // the group's first block
-            const int count = split ? (nblk + 1 - j0) >> 1 : nblk;
+            const int nblk = w.nblk;
             int seen[4];                                                        // keys of the block that the row sees
             float m[4], sum[4], rsf[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + (w.blk0 + j0) * BKT);
+                seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + w.blk0 * BKT);
                 rsf[u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
                 m[u] = -INFINITY;
                 sum[u] = 0.0f;
             }
             float ev = -1000.0f;                // int8: running maximum of ceil(log2 sv), at least
-            for (int k = 0; k < 2 * count; ++k, ++n_s) {        // steps of 64 keys
-                const int sub = k & 1, t = n_tile + (split ? 2 * (k >> 1) + j0 : k >> 1);
+            for (int k = 0; k < 2 * nblk; ++k, ++n_s) {         // steps of 64 keys
+                const int sub = k & 1, t = n_tile + (k >> 1);
                 const uint32_t tsb = ts + 64 * sub;
                 const ulonglong2 *factors = reinterpret_cast<const ulonglong2 *>(smem + OFF_SC + (t % NSC) * SC_BYTES) +
                                             16 * sub + (lane & 3);
@@ -396,7 +392,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) seen[u] -= sub && split ? 64 + BKT : 64;
+                for (int u = 0; u < 4; ++u) seen[u] -= 64;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -417,7 +413,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (!ok) break;
             n_tile += nblk;
             // --- O: to the output, or to the piece's slot
-            if (count > 0) ok = warp_wait(lane, b_v + 16 * g + 8, ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
+            ok = warp_wait(lane, b_v + 16 * g + 8, ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
             if (!ok) break;
             tc_fence_after();
             const bool ends = w.slot < 0;
@@ -430,12 +426,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
-                if (count > 0) {
-                    tmem_ld32(to + c, o);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = 0u;
-                }
+                tmem_ld32(to + c, o);
                 if (valid && ends) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
@@ -468,17 +459,13 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             // kind::f16: fp32 D (bit 4), A and B bf16 (bits 7, 10) or f16 (0), N / 8 at bit 17, M / 16 at bit 24; V is MN-major (bit 16)
             constexpr uint32_t types = (1u << 4) | (I8 ? 0u : (1u << 7) | (1u << 10)) | (8u << 24);
             constexpr uint32_t idesc_s = types | (8u << 17), idesc_o = types | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
-            const int g = warp - 8, step = split ? 2 : 1;
+            const int g = warp - 8;
             const uint32_t ds = tmem + 128 * g, dout = tmem + 256 + 128 * g;
             uint32_t h = 0;                         // ring index of this group's next K block; V follows it
             uint32_t n_p = 0;
             while (const Piece *pc = next_piece()) {
                 const int nblk = pc->nblk;
                 ok = warp_wait(lane, b_q + 8 * g, n_piece & 1, abort_flag, WAIT_NS, p.err);
-                const uint32_t h_next = h + 2 * nblk;
-                const int j0 = split ? (int)(h >> 1 ^ g) & 1 : 0;
-                const int count = split ? (nblk + 1 - j0) >> 1 : nblk;
-                h += 2 * j0;
                 auto wait_full = [&](uint32_t x) {
                     return warp_wait(lane, b_full + 8 * (x % NS), (x / NS) & 1, abort_flag, WAIT_NS, p.err);
                 };
@@ -492,7 +479,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     mma_commit(b_s + 16 * g + 8 * sub);
                     if (sub) mma_commit(b_empty + 8 * (x % NS));
                 };
-                if (ok && count > 0) {
+                if (ok) {
                     ok = wait_full(h);
                     tc_fence_after();
                     if (ok && lane == 0) {
@@ -501,7 +488,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     }
                     __syncwarp();
                 }
-                for (int k = 0; k < 2 * count && ok; ++k, ++n_p) {
+                for (int k = 0; k < 2 * nblk && ok; ++k, ++n_p) {
                     const uint32_t sub = k & 1;
                     if (sub == 0) ok = wait_full(h + 1);
                     if (ok) ok = warp_wait(lane, b_p + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
@@ -516,19 +503,18 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                         if (sub) mma_commit(b_empty + 8 * ((h + 1) % NS));
                     }
                     __syncwarp();
-                    if (k + 2 < 2 * count) {
+                    if (k + 2 < 2 * nblk) {
                         // S(k + 2) goes over P(k): products on different accumulators are not ordered, so P V has to be done
                         // (it is, long before the softmax of step k + 1 asks for S(k + 2))
-                        if (sub == 0) ok = wait_full(h + 2 * step);
+                        if (sub == 0) ok = wait_full(h + 2);
                         if (ok) ok = warp_wait(lane, b_v + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
                         tc_fence_after();
-                        if (ok && lane == 0) issue_s(h + 2 * step, sub);
+                        if (ok && lane == 0) issue_s(h + 2, sub);
                         __syncwarp();
                     }
-                    if (sub) h += 2 * step;
+                    if (sub) h += 2;
                 }
                 if (!ok) break;
-                h = h_next;
                 done_piece();
             }
             // every MMA issued has completed before TMEM is freed
