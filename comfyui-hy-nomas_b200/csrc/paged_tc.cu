@@ -14,8 +14,8 @@
 //                the tensor pipe runs one's products while the other waits.
 //   warp 10      walks the line: the CTA's pieces into a ring of four
 //   warp 11      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
-//   warps 12-15  producers: the pages' rows of K and V into a ring of four 32 KB slots (K, V, K, V), in the 128-byte-swizzled
-//                layout of the products (K-major K, MN-major V). bf16: one warp, a TMA box per page (or its part in the block) and half
+//   warps 12-15  producers: the pages' rows of K and V into a ring of eight 16 KB slots (K and V of a step in turn: given
+//                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout of the products (K-major K, MN-major V). bf16: one warp, a TMA box per page (or its part in the block) and half
 //                of the head dim; V rows past the end become zeros (K's are masked). int8: four warps; codes go through
 //                registers and become fp16 integers (exact).
 //
@@ -38,14 +38,17 @@ namespace paged {
 using namespace tc;
 
 constexpr int BKT = 128;                    // keys per block
-constexpr int HALF = 128 * 128;             // [128 rows][128 B]: one half (64 elements) of the head dim
+constexpr int HALF = 128 * 128;             // q: [128 rows][128 B], one half (64 elements) of the head dim
 constexpr int TILE = 2 * HALF;
-constexpr int NS = 4;                       // ring slots (K and V blocks in turn)
+constexpr int STEP = 64;                    // keys of a step
+constexpr int KHALF = STEP * 128;           // K, V of a step: [64 rows][128 B] twice
+constexpr int KTILE = 2 * KHALF;
+constexpr int NS = 8;                       // ring slots (K and V of the steps in turn)
 constexpr int NSC = 4;                      // scale ring
 constexpr int TC_THREADS = 512;
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = 2 * TILE;
-constexpr int OFF_SC = OFF_KV + NS * TILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
+constexpr int OFF_SC = OFF_KV + NS * KTILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
                                             // the largest sv (16 B); where the 8 groups of 16 keys are (32 B)
 constexpr int SC_BYTES = BKT * 8 + 16 + 32;
 constexpr int OFF_BAR = OFF_SC + NSC * SC_BYTES;
@@ -127,8 +130,10 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// 16-byte chunk c (of 16) of row r of a [128][128 elements] operand tile
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+// 16-byte chunk c (of 16) of row r of an operand tile whose halves are `half` bytes
+template <int half> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return (c >> 3) * half + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
 
 // box of 64 elements x rows at (0, token, half, page and head) of a bf16 pool
 __device__ __forceinline__ void tma_rows(const CUtensorMap *map, uint32_t dst, uint32_t bar, int token, int half, int page) {
@@ -242,7 +247,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 }
 #pragma unroll
                 for (int c = 0; c < 16; ++c)
-                    sts16(sb + OFF_Q + g * TILE + chunk_at(rr, c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+                    sts16(sb + OFF_Q + g * TILE + chunk_at<HALF>(rr, c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
             }
             fence_async();
             mbar_arrive(b_q + 8 * g);
@@ -461,7 +466,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             constexpr uint32_t idesc_s = types | (8u << 17), idesc_o = types | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
             const int g = warp - 8;
             const uint32_t ds = tmem + 128 * g, dout = tmem + 256 + 128 * g;
-            uint32_t h = 0;                         // ring index of this group's next K block; V follows it
+            uint32_t h = 0;                         // ring index of the next step's K; V follows it
             uint32_t n_p = 0;
             while (const Piece *pc = next_piece()) {
                 const int nblk = pc->nblk;
@@ -469,50 +474,46 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 auto wait_full = [&](uint32_t x) {
                     return warp_wait(lane, b_full + 8 * (x % NS), (x / NS) & 1, abort_flag, WAIT_NS, p.err);
                 };
-                // step `sub` of the block at ring index x; the second gives K back
+                // the step whose K is at ring index x
                 auto issue_s = [&](uint32_t x, uint32_t sub) {
-                    const uint64_t qd = sdesc(sb + OFF_Q + g * TILE), kd = sdesc(sb + OFF_KV + (x % NS) * TILE + sub * 8192);
+                    const uint64_t qd = sdesc(sb + OFF_Q + g * TILE), kd = sdesc(sb + OFF_KV + (x % NS) * KTILE);
 #pragma unroll
                     for (int i = 0; i < HD / 16; ++i)
-                        mma_f16(ds + 64 * sub, qd + (HALF >> 4) * (i >> 2) + 2 * (i & 3), kd + (HALF >> 4) * (i >> 2) + 2 * (i & 3),
+                        mma_f16(ds + 64 * sub, qd + (HALF >> 4) * (i >> 2) + 2 * (i & 3), kd + (KHALF >> 4) * (i >> 2) + 2 * (i & 3),
                                 idesc_s, (uint32_t)(i > 0));
                     mma_commit(b_s + 16 * g + 8 * sub);
-                    if (sub) mma_commit(b_empty + 8 * (x % NS));
+                    mma_commit(b_empty + 8 * (x % NS));
                 };
-                if (ok) {
-                    ok = wait_full(h);
+                for (uint32_t k = 0; k < 2 && ok; ++k) {
+                    ok = wait_full(h + 2 * k);
                     tc_fence_after();
-                    if (ok && lane == 0) {
-                        issue_s(h, 0);
-                        issue_s(h, 1);
-                    }
+                    if (ok && lane == 0) issue_s(h + 2 * k, k);
                     __syncwarp();
                 }
-                for (int k = 0; k < 2 * nblk && ok; ++k, ++n_p) {
+                for (int k = 0; k < 2 * nblk && ok; ++k, ++n_p, h += 2) {
                     const uint32_t sub = k & 1;
-                    if (sub == 0) ok = wait_full(h + 1);
+                    ok = wait_full(h + 1);
                     if (ok) ok = warp_wait(lane, b_p + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        const uint64_t vd = sdesc_mn(sb + OFF_KV + ((h + 1) % NS) * TILE + sub * 8192, HALF);
+                        const uint64_t vd = sdesc_mn(sb + OFF_KV + ((h + 1) % NS) * KTILE, KHALF);
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)             // 16 keys: 8 columns of P, two 8-row groups of V
+                        for (int u = 0; u < STEP / 16; ++u)     // 16 keys: 8 columns of P, two 8-row groups of V
                             mma_pv(dout, ds + 64 * sub + 8 * u, vd + (uint64_t)(2048 >> 4) * u, idesc_o, (uint32_t)(k > 0 || u > 0));
                         mma_commit(b_v + 16 * g + 8 * sub);
-                        if (sub) mma_commit(b_empty + 8 * ((h + 1) % NS));
+                        mma_commit(b_empty + 8 * ((h + 1) % NS));
                     }
                     __syncwarp();
                     if (k + 2 < 2 * nblk) {
                         // S(k + 2) goes over P(k): products on different accumulators are not ordered, so P V has to be done
                         // (it is, long before the softmax of step k + 1 asks for S(k + 2))
-                        if (sub == 0) ok = wait_full(h + 2);
+                        ok = wait_full(h + 4);
                         if (ok) ok = warp_wait(lane, b_v + 16 * g + 8 * sub, (n_p >> 1) & 1, abort_flag, WAIT_NS, p.err);
                         tc_fence_after();
-                        if (ok && lane == 0) issue_s(h + 2, sub);
+                        if (ok && lane == 0) issue_s(h + 4, sub);
                         __syncwarp();
                     }
-                    if (sub) h += 2;
                 }
                 if (!ok) break;
                 done_piece();
@@ -607,33 +608,33 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (!I8) {
                 const int own_b = pc->own_b, head = pc->h, seq = p.rows[own_b < 0 ? 0 : own_b];
                 const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
-                const int groups = BKT / box;                   // a lane each
-                for (int j = 0; j < nblk && ok; ++j) {
-                    const int k0 = key0 + j * BKT, kk = k0 + box * lane, pg = kk / p.page;
+                const int groups = STEP / box;                  // a lane each
+                for (int k = 0; k < 2 * nblk && ok; ++k) {
+                    const int k0 = key0 + k * STEP, kk = k0 + box * lane, pg = kk / p.page;
                     const int id = lane < groups && kk < kend && pg < p.width ? tab[pg] : -1;
                     const bool here = (unsigned)id < (unsigned)p.pages;
                     const uint32_t bytes = 256u * box * __popc(__ballot_sync(0xffffffffu, here));
-                    const int left = kend - k0;                 // rows of the block that are there
+                    const int left = max(kend - k0, 0);         // rows of the step that are there
 #pragma unroll 1
                     for (int kv = 0; kv < 2; ++kv, ++half) {
                         const uint32_t slot = half % NS;
                         ok = warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
                         if (!ok) break;
-                        const bool tail = kv == 1 && left < BKT;
-                        const uint32_t bar = tail ? b_tail : b_full + 8 * slot, dst = sb + OFF_KV + slot * TILE;
+                        const bool tail = kv == 1 && left < STEP;
+                        const uint32_t bar = tail ? b_tail : b_full + 8 * slot, dst = sb + OFF_KV + slot * KTILE;
                         if (lane == 0) mbar_arrive_tx(bar, bytes);
                         __syncwarp();
                         if (here)
                             for (int u = 0; u < 2; ++u)
-                                tma_rows(kv ? &tm_v : &tm_k, dst + u * HALF + lane * box * 128, bar, kk - pg * p.page, u,
+                                tma_rows(kv ? &tm_v : &tm_k, dst + u * KHALF + lane * box * 128, bar, kk - pg * p.page, u,
                                          id * p.Hkv + head);
                         __syncwarp();
                         if (tail) {                             // rows past the end: zeros, whatever the page holds there
                             ok = warp_wait(lane, b_tail, tails & 1, abort_flag, WAIT_NS, p.err);
                             ++tails;
                             if (!ok) break;
-                            for (int r = left; r < BKT; ++r)
-                                if (lane < 16) sts16(dst + chunk_at(r, lane), 0, 0, 0, 0);
+                            for (int r = left; r < STEP; ++r)
+                                if (lane < 16) sts16(dst + chunk_at<KHALF>(r, lane), 0, 0, 0, 0);
                             fence_async();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(b_full + 8 * slot);
@@ -643,20 +644,16 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             } else {
                 // a quarter of a warp holds 64 B of two neighbouring rows, so that its 16-byte stores use every bank once
                 const int row16 = 2 * (tid >> 4) + ((tid >> 2) & 1), c = ((tid >> 3) & 1) * 4 + (tid & 3), mine = row16 * HD + 16 * c;
-                uint4 kreg[8], vreg[8];
-                auto fetch = [&](uint4 (&reg)[8], const uint8_t *pool, int j, int t) {
-                    const int left = kend - (key0 + j * BKT) - row16;
-                    const int4 *at4 = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16);
+                // half a block (a step) of K or V per thread: 4 chunks; the registers hold both steps of the block ahead
+                uint4 kreg[2][4], vreg[2][4];
+                auto fetch = [&](uint4 (&reg)[4], const uint8_t *pool, int j, int st, int t) {
+                    const int left = kend - (key0 + j * BKT + st * STEP) - row16;
+                    const int4 a = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16)[st];
+                    const int at[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                    for (int v = 0; v < 2; ++v) {
-                        const int4 a = at4[v];
-                        const int at[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                        for (int it = 0; it < 4; ++it) {
-                            reg[4 * v + it] = make_uint4(0, 0, 0, 0);
-                            if (at[it] >= 0 && 16 * (4 * v + it) < left)
-                                reg[4 * v + it] = ldg_stream(pool + (int64_t)at[it] * (16 * HD) + mine);
-                        }
+                    for (int it = 0; it < 4; ++it) {
+                        reg[it] = make_uint4(0, 0, 0, 0);
+                        if (at[it] >= 0 && 16 * it < left) reg[it] = ldg_stream(pool + (int64_t)at[it] * (16 * HD) + mine);
                     }
                 };
                 auto wait_index = [&](int t) {
@@ -664,23 +661,19 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     __syncwarp();
                     return r;
                 };
-                auto store = [&](const uint4 (&reg)[8], uint32_t slot) {
-                    const uint32_t dst = sb + OFF_KV + slot * TILE;
+                auto hand_over = [&](const uint4 (&reg)[4]) {
+                    const uint32_t slot = half % NS, dst = sb + OFF_KV + slot * KTILE;
+                    if (!warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err)) return false;
 #pragma unroll
-                    for (int it = 0; it < 8; ++it) {
+                    for (int it = 0; it < 4; ++it) {
                         const int row = 16 * it + row16;
                         const uint32_t x[4] = {reg[it].x ^ 0x80808080u, reg[it].y ^ 0x80808080u, reg[it].z ^ 0x80808080u,
                                                reg[it].w ^ 0x80808080u};
-                        sts16(dst + chunk_at(row, 2 * c), codes_f16<0x4140>(x[0]), codes_f16<0x4342>(x[0]),
+                        sts16(dst + chunk_at<KHALF>(row, 2 * c), codes_f16<0x4140>(x[0]), codes_f16<0x4342>(x[0]),
                               codes_f16<0x4140>(x[1]), codes_f16<0x4342>(x[1]));
-                        sts16(dst + chunk_at(row, 2 * c + 1), codes_f16<0x4140>(x[2]), codes_f16<0x4342>(x[2]),
+                        sts16(dst + chunk_at<KHALF>(row, 2 * c + 1), codes_f16<0x4140>(x[2]), codes_f16<0x4342>(x[2]),
                               codes_f16<0x4140>(x[3]), codes_f16<0x4342>(x[3]));
                     }
-                };
-                auto hand_over = [&](const uint4 (&reg)[8]) {
-                    const uint32_t slot = half % NS;
-                    if (!warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err)) return false;
-                    store(reg, slot);
                     fence_async();
                     mbar_arrive(b_full + 8 * slot);
                     ++half;
@@ -688,27 +681,27 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 };
                 ok = wait_index(n_tile);
                 if (ok) {
-                    fetch(kreg, p.k, 0, n_tile);
-                    fetch(vreg, p.v, 0, n_tile);
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        fetch(kreg[st], p.k, 0, st, n_tile);
+                        fetch(vreg[st], p.v, 0, st, n_tile);
+                    }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(b_se + 8 * (n_tile % NSC));
                 }
                 for (int j = 0; j < nblk && ok; ++j) {
                     const int t = ++n_tile;
-                    ok = hand_over(kreg);
-                    if (!ok) break;
-                    if (j + 1 < nblk) {
-                        ok = wait_index(t);
-                        if (!ok) break;
-                        fetch(kreg, p.k, j + 1, t);
+                    const bool more = j + 1 < nblk;
+                    if (more) ok = wait_index(t);
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        if (ok) ok = hand_over(kreg[st]);
+                        if (ok && more) fetch(kreg[st], p.k, j + 1, st, t);
+                        if (ok) ok = hand_over(vreg[st]);
+                        if (ok && more) fetch(vreg[st], p.v, j + 1, st, t);
                     }
-                    ok = hand_over(vreg);
-                    if (!ok) break;
-                    if (j + 1 < nblk) {
-                        fetch(vreg, p.v, j + 1, t);
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(b_se + 8 * (t % NSC));
-                    }
+                    __syncwarp();
+                    if (ok && more && lane == 0) mbar_arrive(b_se + 8 * (t % NSC));
                 }
             }
             if (ok) done_piece();
@@ -765,7 +758,7 @@ cudaError_t launch_tc(const Params &p, cudaStream_t st) {
         configured[dev] = true;
     }
     const int smem = OFF_PRE + (p.B + 1) * 4;
-    int box = BKT;                              // the largest power of two up to 128 that divides the page
+    int box = STEP;                             // the largest power of two up to 64 that divides the page
     while (p.page % box) box >>= 1;
     CUtensorMap tk, tv;
     memset(&tk, 0, sizeof(tk));

@@ -249,13 +249,18 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False
                          f"{tuple(weight.shape)} do not match")
     if kind not in _KINDS:
         raise ValueError(f"add_rmsnorm_quant: kind {kind!r} (int8 or fp8)")
-    flat = x.dim() == 2
-    x2, r2 = (x, residual) if flat else (x.reshape(-1, d), residual.reshape(-1, d))
-    x2, r2 = _rows16(x2), _rows16(r2)
-    w = weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else _lib.dense(weight)
+    if x.dim() == 2:
+        x2, r2 = x, residual
+    else:
+        x2, r2 = x.reshape(-1, d), residual.reshape(-1, d)
+    # whole rows, one after the other, from a 16-byte boundary: the usual case, without a look at each stride
+    plain = x2.is_contiguous() and r2.is_contiguous() and not (x2.data_ptr() | r2.data_ptr()) % 16
+    if not plain:
+        x2, r2 = _rows16(x2), _rows16(r2)
+    w = weight if weight.is_contiguous() and not weight.data_ptr() % 16 else _lib.dense(weight)
     rows = x2.shape[0]
     if out is None:
-        total = torch.empty(shape, dtype=bf16, device=device)
+        total = torch.empty_like(x) if plain else torch.empty(shape, dtype=bf16, device=device)
         o2, ldo = total, d
     else:
         if out.shape != shape or out.dtype != bf16 or out.device != device:
@@ -265,14 +270,14 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False
             raise ValueError("add_rmsnorm_quant: out needs contiguous, 16-byte aligned rows")
         ldo = o2.stride(0)
     code, dtype = _KINDS[kind]
-    q = torch.empty((rows, d), dtype=dtype, device=device)
+    q = torch.empty_like(x2, dtype=dtype) if plain else torch.empty((rows, d), dtype=dtype, device=device)
     if per_token:
         s, srs, sgs = torch.empty((rows, 1), dtype=torch.float32, device=device), 1, 1
     else:
         sgs = (rows + 3) // 4 * 4                # group-major, as _lib.group_scales lays them out
         s, srs = torch.empty_strided((rows, d // 128), (1, sgs), dtype=torch.float32, device=device), 1
-    rc = _lib.launch("hn_add_rmsnorm_quant", device, x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), w.data_ptr(),
-                     rows, d, eps, code, 1 if per_token else 0, o2.data_ptr(), ldo, q.data_ptr(), d, s.data_ptr(), srs, sgs)
+    rc = _lib.launch("hn_add_rmsnorm_quant", device, x2.data_ptr(), d if plain else x2.stride(0), r2.data_ptr(),
+                     d if plain else r2.stride(0), w.data_ptr(), rows, d, eps, code, 1 if per_token else 0, o2.data_ptr(), ldo, q.data_ptr(), d, s.data_ptr(), srs, sgs)
     _lib.check(rc, "add_rmsnorm_quant")
     return total, q, s
 
