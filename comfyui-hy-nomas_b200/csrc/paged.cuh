@@ -202,6 +202,7 @@ __device__ __forceinline__ int row_exponent(float top) {
 }
 
 cudaError_t launch_tc(const Params &p, cudaStream_t st);       // the tensor-core line (paged_tc.cu); bk = 128
+int tc_most_sequences();                                       // ... takes at most so many sequences
 
 } // namespace paged
 } // namespace hn

@@ -523,10 +523,11 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     s.ends = 0; s.min_quota = 2;
     t = s;
     const int64_t r1 = (int64_t)a.Lq * s.G, all = r1 * a.B;
-    pl.own_tc = r1 >= TC_OWN;
+    const bool fits = a.B <= tc_most_sequences();
+    pl.own_tc = fits && r1 >= TC_OWN;
     // one sequence has nothing to share
     const bool split = a.shared > 0 && a.B > 1 && !pl.own_tc;
-    pl.shared_tc = split && all >= TC_SHARED;
+    pl.shared_tc = fits && split && all >= TC_SHARED;
     s.bk = BK; s.ctas = stream_ctas(i8);
     t.bk = 128; t.ctas = num_sms();
     Params &own = pl.own_tc ? t : s;

@@ -14,7 +14,7 @@
 //                the tensor pipe runs one's products while the other waits.
 //   warp 10      walks the line: the CTA's pieces into a ring of four
 //   warp 11      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
-//   warps 12-15  producers: the pages' rows of K and V into a ring of eight 16 KB slots (K and V of a step in turn: given
+//   warps 12-15  producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
 //                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout of the products (K-major K, MN-major V). bf16: one warp, a TMA box per page (or its part in the block) and half
 //                of the head dim; V rows past the end become zeros (K's are masked). int8: four warps; codes go through
 //                registers and become fp16 integers (exact).
@@ -43,7 +43,7 @@ constexpr int TILE = 2 * HALF;
 constexpr int STEP = 64;                    // keys of a step
 constexpr int KHALF = STEP * 128;           // K, V of a step: [64 rows][128 B] twice
 constexpr int KTILE = 2 * KHALF;
-constexpr int NS = 8;                       // ring slots (K and V of the steps in turn)
+constexpr int NS = 9;                       // ring slots (K and V of the steps in turn); int8 with 8: 2.99 ms, with 9: 2.80
 constexpr int NSC = 4;                      // scale ring
 constexpr int TC_THREADS = 512;
 constexpr int OFF_Q = 0;
@@ -59,6 +59,8 @@ constexpr int NBARS = 2 * NS + 14 + 2 * NSC + 2 * NP + 3;
 constexpr int OFF_PIECE = OFF_BAR + NBARS * 8;
 constexpr int OFF_MISC = OFF_PIECE + NP * 32;
 constexpr int OFF_PRE = OFF_MISC + 16 + 32 * 4;
+constexpr int SMEM_MOST = 232448;
+constexpr int TC_MAX_B = (SMEM_MOST - OFF_PRE) / 4 - 1;        // sequences whose prefix sums fit
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;     // 2 s
 // A row's reference m is the maximum it was set at plus AHEAD, and is moved (and O rescaled) when a logit passes it by STALE.
@@ -742,6 +744,8 @@ static bool make_map(CUtensorMap *map, const void *pool, const Params &p, int bo
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int tc_most_sequences() { return TC_MAX_B; }
+
 cudaError_t launch_tc(const Params &p, cudaStream_t st) {
     const bool i8 = p.ks != nullptr;
     static bool configured[HN_MAX_DEV];
@@ -750,8 +754,8 @@ cudaError_t launch_tc(const Params &p, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
     if (!configured[dev]) {
-        const int most = OFF_PRE + (MAX_B + 1) * 4;
-        static_assert(OFF_PRE + (MAX_B + 1) * 4 <= 232448, "shared memory budget");
+        const int most = OFF_PRE + (TC_MAX_B + 1) * 4;
+        static_assert(TC_MAX_B >= 1024, "shared memory budget");
         e = cudaFuncSetAttribute(k_paged_tc<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_tc<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return e;
