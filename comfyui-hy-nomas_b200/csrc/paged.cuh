@@ -76,12 +76,19 @@ __device__ __forceinline__ int own_blocks_below(const Params &p, int len, int n_
     return n;
 }
 
-// pre[b] = own blocks (of one head) of the sequences before b. `threads` threads, a multiple of 32; sums: [32] ints.
-__device__ __forceinline__ void prefix_blocks(const Params &p, int *pre, int *sums, int threads) {
+// pre[b] = own blocks (of one head) of the sequences before b. *lead = the sequence whose table the shared pages are looked
+// up in: the first of those that hold the most of them (a listed row may be short or empty: it sees what it holds).
+// `threads` threads, a multiple of 32; sums: [32] ints; lead: 8-byte aligned.
+__device__ __forceinline__ void prefix_blocks(const Params &p, int *pre, int *sums, unsigned long long *lead, int threads) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int base = 0;
+    if (tid == 0) *lead = 0;
+    __syncthreads();
     for (int b0 = 0; b0 < p.B; b0 += threads) {
-        const int n = b0 + tid < p.B && p.has_own ? own_blocks_below(p, seq_length(p, b0 + tid), p.nrtB) : 0;
+        const int len = b0 + tid < p.B ? seq_length(p, b0 + tid) : 0;
+        const int n = b0 + tid < p.B && p.has_own ? own_blocks_below(p, len, p.nrtB) : 0;
+        if (p.nbA && b0 + tid < p.B)
+            atomicMax(lead, (unsigned long long)(len < p.shared ? len : p.shared) << 13 | (unsigned)(MAX_B - (b0 + tid)));
         int x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -99,7 +106,10 @@ __device__ __forceinline__ void prefix_blocks(const Params &p, int *pre, int *su
         base += total;
         __syncthreads();
     }
-    if (tid == 0) pre[p.B] = base;
+    if (tid == 0) {
+        pre[p.B] = base;
+        *lead = MAX_B - (int)(*lead & 8191);
+    }
     __syncthreads();
 }
 

@@ -77,7 +77,7 @@ template <bool I8> constexpr int smem_bytes() {
     return stages<I8>() * stage_bytes<I8>() > END_BYTES ? stages<I8>() * stage_bytes<I8>() : END_BYTES;
 }
 
-template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piece &w, uint8_t *smem) {
+template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piece &w, int lead, uint8_t *smem) {
     constexpr int KG = 4 / RG, KW = BK / KG, NT = KW / 8;        // key groups, keys and 8-key tiles per warp and block
     constexpr int ST = stages<I8>(), TILE = tile_bytes<I8>(), STAGE = stage_bytes<I8>();
     constexpr int CPR = I8 ? 8 : 16;                             // 16-byte chunks per row
@@ -88,7 +88,7 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
 
     // --- loader: block i of the piece into stage i % ST. A thread's chunks of step `it` are all in 16-key group
     // it * (128 / CPR) / 16, which lies in one page (pages and the parts' first keys are multiples of 16 tokens).
-    const int seq = p.rows[w.own_b < 0 ? 0 : w.own_b];
+    const int seq = p.rows[w.own_b < 0 ? lead : w.own_b];
     const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
     constexpr int RPI = THREADS / CPR;                           // rows per step: 8 (bf16), 16 (int8)
     // The page and the place in it of the next block's four groups. The table is read a block ahead, so that no warp waits
@@ -407,18 +407,19 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
 template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_paged_attention(const Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sums[32];
+    __shared__ unsigned long long lead;
     int *pre = reinterpret_cast<int *>(smem + smem_bytes<I8>());
     dep_launch();
-    prefix_blocks(p, pre, sums, THREADS);
+    prefix_blocks(p, pre, sums, &lead, THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += THREADS) p.sched[b] = pre[b];
     Walker walk(p, pre, blockIdx.x);
     Piece w;
     while (walk.next(p, pre, blockIdx.x, w)) {
         const int rows_per = w.own_b < 0 ? p.ta : p.tb;
-        if (rows_per == 16) run_piece<I8, 1>(p, w, smem);
-        else if (rows_per == 32) run_piece<I8, 2>(p, w, smem);
-        else run_piece<I8, 4>(p, w, smem);
+        if (rows_per == 16) run_piece<I8, 1>(p, w, (int)lead, smem);
+        else if (rows_per == 32) run_piece<I8, 2>(p, w, (int)lead, smem);
+        else run_piece<I8, 4>(p, w, (int)lead, smem);
     }
     dep_wait();             // nothing here reads what the other line writes, but the join waits for this kernel only
 }

@@ -58,7 +58,7 @@ constexpr int NP = 4;                       // pieces
 constexpr int NBARS = 2 * NS + 14 + 2 * NSC + 2 * NP + 3;
 constexpr int OFF_PIECE = OFF_BAR + NBARS * 8;
 constexpr int OFF_MISC = OFF_PIECE + NP * 32;
-constexpr int OFF_PRE = OFF_MISC + 16 + 32 * 4;
+constexpr int OFF_PRE = OFF_MISC + 16 + 32 * 4;        // misc: TMEM address, abort flag, the leading sequence; 32 sums
 constexpr int SMEM_MOST = 232448;
 constexpr int TC_MAX_B = (SMEM_MOST - OFF_PRE) / 4 - 1;        // sequences whose prefix sums fit
 constexpr uint32_t TMEM_COLS = 512;
@@ -155,6 +155,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                    b_v = b_q + 16, b_sc = b_v + 32, b_se = b_sc + 8 * NSC, b_pf = b_se + 8 * NSC, b_pe = b_pf + 8 * NP, b_end = b_pe + 8 * NP, b_tail = b_end + 16;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + OFF_MISC + 4);
+    unsigned long long *lead = reinterpret_cast<unsigned long long *>(smem + OFF_MISC + 8);
     int *sums = reinterpret_cast<int *>(smem + OFF_MISC + 16), *pre = reinterpret_cast<int *>(smem + OFF_PRE);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (sb & 1023) {                            // the swizzled tiles need it; shared memory starts on such a boundary
@@ -183,7 +184,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     dep_launch();
-    prefix_blocks(p, pre, sums, TC_THREADS);
+    prefix_blocks(p, pre, sums, lead, TC_THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += TC_THREADS) p.sched[b] = pre[b];
     tc_fence_before();
@@ -541,7 +542,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             int n_tile = 0;
             while (const Piece *pc = next_piece()) {
                 const int own_b = pc->own_b, head = pc->h, kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
-                const int seq = p.rows[own_b < 0 ? 0 : own_b];
+                const int seq = p.rows[own_b < 0 ? (int)*lead : own_b];
                 const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
                 auto page_of = [&](int j, int &off) -> int {        // lane s < 8 (and its copies): the page of key 16 s of block j
                     const int kk = key0 + j * BKT + 16 * (lane & 7), pg = kk / p.page;
@@ -608,7 +609,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (pc == nullptr) break;
             const int kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
             if (!I8) {
-                const int own_b = pc->own_b, head = pc->h, seq = p.rows[own_b < 0 ? 0 : own_b];
+                const int own_b = pc->own_b, head = pc->h, seq = p.rows[own_b < 0 ? (int)*lead : own_b];
                 const int *tab = p.table + (int64_t)((unsigned)seq < (unsigned)p.slots ? seq : 0) * p.width;
                 const int groups = STEP / box;                  // a lane each
                 for (int k = 0; k < 2 * nblk && ok; ++k) {

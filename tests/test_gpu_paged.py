@@ -170,6 +170,28 @@ def test_attention_many_sequences(paged, cuda, kind):
     check_attention(c, 0, q, rows, out, lse, True, 1 / math.sqrt(D))
 
 
+@pytest.mark.parametrize("heads", [4, 64])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_attention_with_freed_and_short_rows(paged, cuda, kind, heads):
+    """Rows that were freed or hold less than the shared part, the first one listed too: the others are not touched by it (64
+    heads on one K/V head: the shared part's rows fill a tensor-core tile)."""
+    c = filled(paged, 1, 40, 1, 16, 6, 12, kind, seed=11)
+    c.extend([0], 130)
+    c.fork([0, 0, 0], [1, 2, 3])
+    c.extend([1, 2, 3], 7)
+    c.free([0])
+    c.extend([0], 20)
+    c.fork([0], [4])                                     # holds less than the shared part, on pages of its own
+    c.free([0])
+    c.table[4, :2] = c.table[1, :2]                      # ... or rather on the first of the shared ones
+    q = torch.randn((6, 1, heads, D), device=cuda).to(torch.bfloat16)
+    for rows in ([5, 0, 1, 2, 3, 4], [0, 5, 4, 3, 2, 1]):
+        out, lse = paged.attention(q, c, 0, rows, shared=128, return_lse=True)
+        check_attention(c, 0, q, rows, out, lse, True, 1 / math.sqrt(D))
+    out, lse = paged.attention(q[:3], c, 0, [5, 4, 0], shared=128, return_lse=True)      # none holds it all
+    check_attention(c, 0, q[:3], [5, 4, 0], out, lse, True, 1 / math.sqrt(D))
+
+
 @pytest.mark.parametrize("lq", [1, 300])
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 def test_attention_ignores_what_no_query_may_see(paged, cuda, kind, lq):
