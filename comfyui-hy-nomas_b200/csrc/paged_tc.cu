@@ -93,7 +93,7 @@ __device__ __forceinline__ void ld_frag(uint32_t taddr, uint32_t *r) {
 // the registers' uses stay behind this (and a wait::ld before it)
 __device__ __forceinline__ void frag_fence(uint32_t *r) {
 #pragma unroll
-    for (int i = 0; i < 64; i += 8)
+    for (int i = 0; i < 32; i += 8)
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                           "+r"(r[i + 6]), "+r"(r[i + 7]) :: "memory");
 }
@@ -280,10 +280,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 ok = warp_wait(lane, b_s + 16 * g + 8 * sub, (n_s >> 1) & 1, abort_flag, WAIT_NS, p.err);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t x[64];                 // [16-lane half][8 column groups][row l / 4, l / 4 + 8][2 columns]
-#pragma unroll
-                for (int c = 0; c < 4; ++c) ld_frag(tsb + ((uint32_t)(16 * (c >> 1)) << 16) + 32 * (c & 1), x + 16 * c);
-                bool rescale = false;
+                bool grown = false;
                 float f = 1.0f;
                 if (I8 && sub == 0) {
                     const float top = *reinterpret_cast<const float *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 2 * BKT * 4);
@@ -291,81 +288,82 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     const float e = fmaxf((float)((int)(__float_as_uint(top) >> 23) - 126), -60.0f);
                     if (e > ev) {               // all rows' references grow with it
                         f = ex2(ev - e);
-                        rescale = true;
+                        grown = true;
                         ev = e;
                     }
                 }
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                frag_fence(x);
-                if (I8) {
+                // 16 of the warp's 32 rows, then the others, by the same instructions (HF_WHY)
+                #pragma unroll 1
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint32_t lanes = (uint32_t)(16 * hf) << 16;
+                    uint32_t x[32];             // [8 column groups][row l / 4, l / 4 + 8][2 columns]
+                    ld_frag(tsb + lanes, x);
+                    ld_frag(tsb + lanes + 32, x + 16);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    frag_fence(x);
+                    if (I8) {
 #pragma unroll
-                    for (int c = 0; c < 8; c += 2) {
-                        const ulonglong2 kf = factors[2 * c];
+                        for (int c = 0; c < 8; c += 2) {
+                            const ulonglong2 kf = factors[2 * c];
 #pragma unroll
-                        for (int v = 0; v < 8; ++v) {           // 2 column groups x 4 rows
-                            uint32_t *y = x + 32 * (v >> 2) + 4 * (c + (v & 1)) + (v & 2);
-                            float y0, y1;
-                            x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
-                            y[0] = __float_as_uint(y0);
-                            y[1] = __float_as_uint(y1);
+                            for (int v = 0; v < 4; ++v) {       // 2 column groups x 2 rows
+                                uint32_t *y = x + 4 * (c + (v & 1)) + (v & 2);
+                                float y0, y1;
+                                x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
+                                y[0] = __float_as_uint(y0);
+                                y[1] = __float_as_uint(y1);
+                            }
                         }
                     }
-                }
-                if (__any_sync(0xffffffffu, min(min(seen[0], seen[1]), min(seen[2], seen[3])) < 64)) {
+                    if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < 64)) {
 #pragma unroll
-                    for (int c = 0; c < 64; ++c)
-                        if (8 * ((c & 31) >> 2) + 2 * (lane & 3) + (c & 1) >= seen[2 * (c >> 5) + ((c >> 1) & 1)])
-                            x[c] = __float_as_uint(-INFINITY);
-                }
-                float mn[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const uint32_t *y = x + 32 * (u >> 1) + 2 * (u & 1);
-                    float mx[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        mx[c] = nan_max3(mx[c], __uint_as_float(y[16 + 4 * c]), __uint_as_float(y[16 + 4 * c + 1]));
-                    mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
-                bool need = rescale;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
-                    mn[u] *= rsf[u];
-                    need |= !(mn[u] <= m[u] + STALE);           // or a NaN, which stays in the row
-                }
-                if (k == 0) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) m[u] = mn[u] + AHEAD;
-                } else if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const bool grow = !(mn[u] <= m[u] + STALE);
-                        const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
-                        m[u] = grow ? mn[u] + AHEAD : m[u];
-                        mn[u] = al;
-                        sum[u] *= al;
+                        for (int c = 0; c < 32; ++c)
+                            if (8 * (c >> 2) + 2 * (lane & 3) + (c & 1) >= seen[(c >> 1) & 1]) x[c] = __float_as_uint(-INFINITY);
                     }
-                    // the product before this step's is the last one given to the pipe
-                    ok = warp_wait(lane, b_v + 16 * g + 8 * (sub ^ 1), ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
-                    if (!ok) break;
-                    tc_fence_after();
+                    float mn[2];
+                    bool need = grown;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t *y = x + 2 * u;
+                        float mx[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            mx[c] = nan_max3(mx[c], __uint_as_float(y[16 + 4 * c]), __uint_as_float(y[16 + 4 * c + 1]));
+                        mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
+                        mn[u] *= rsf[u];
+                        need |= !(mn[u] <= m[u] + STALE);       // or a NaN, which stays in the row
+                    }
+                    if (k == 0) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) m[u] = mn[u] + AHEAD;
+                    } else if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const bool grow = !(mn[u] <= m[u] + STALE);
+                            const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
+                            m[u] = grow ? mn[u] + AHEAD : m[u];
+                            mn[u] = al;
+                            sum[u] *= al;
+                        }
+                        // the product before this step's is the last one given to the pipe
+                        ok = warp_wait(lane, b_v + 16 * g + 8 * (sub ^ 1), ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        scale_frag(to + c, mn[0], mn[1]);
-                        scale_frag(to + (16u << 16) + c, mn[2], mn[3]);
+                        for (int c = 0; c < HD; c += 32) scale_frag(to + lanes + c, mn[0], mn[1]);
                     }
-                }
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
                     uint64_t nref[2], acc[2] = {0ull, 0ull};
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const float ref = m[2 * hf + u] == -INFINITY ? 0.0f : m[2 * hf + u];
+                        const float ref = m[u] == -INFINITY ? 0.0f : m[u];
                         nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
                     }
 #pragma unroll
@@ -379,8 +377,8 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
 #pragma unroll
                         for (int q = 0; q < 8; ++q) {           // column group c + q / 2, row q % 2
                             const int u = q & 1;
-                            const uint32_t *y = x + 32 * hf + 4 * c + 2 * q;
-                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), x2_splat(rsf[2 * hf + u]), nref[u]);
+                            const uint32_t *y = x + 4 * c + 2 * q;
+                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), x2_splat(rsf[u]), nref[u]);
                             float a0, a1;
                             x2_split(a, a0, a1);
                             uint64_t e = x2(ex2(a0), ex2(a1));
@@ -390,17 +388,21 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                             x2_split(e, e0, e1);
                             pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
                         }
-                        st_frag(tsb + ((uint32_t)(16 * hf) << 16) + 4 * c, pk);
+                        st_frag(tsb + lanes + 4 * c, pk);
                     }
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         float a0, a1;
                         x2_split(acc[u], a0, a1);
-                        sum[2 * hf + u] += a0 + a1;
+                        // the other rows' state comes to the front
+                        float y = sum[u] + (a0 + a1);
+                        sum[u] = sum[u + 2]; sum[u + 2] = y;
+                        y = m[u]; m[u] = m[u + 2]; m[u + 2] = y;
+                        y = rsf[u]; rsf[u] = rsf[u + 2]; rsf[u + 2] = y;
+                        const int z = seen[u] - 64; seen[u] = seen[u + 2]; seen[u + 2] = z;
                     }
                 }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) seen[u] -= 64;
+                if (!ok) break;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -647,11 +649,11 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             } else {
                 // a quarter of a warp holds 64 B of two neighbouring rows, so that its 16-byte stores use every bank once
                 const int row16 = 2 * (tid >> 4) + ((tid >> 2) & 1), c = ((tid >> 3) & 1) * 4 + (tid & 3), mine = row16 * HD + 16 * c;
-                // half a block (a step) of K or V per thread: 4 chunks; the registers hold both steps of the block ahead
-                uint4 kreg[2][4], vreg[2][4];
-                auto fetch = [&](uint4 (&reg)[4], const uint8_t *pool, int j, int st, int t) {
-                    const int left = kend - (key0 + j * BKT + st * STEP) - row16;
-                    const int4 a = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16)[st];
+                // a step of K or V per thread: 4 chunks; the registers hold the step ahead
+                uint4 kreg[4], vreg[4];
+                auto fetch = [&](uint4 (&reg)[4], const uint8_t *pool, int k, int t) {
+                    const int left = kend - (key0 + k * STEP) - row16;
+                    const int4 a = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16)[k & 1];
                     const int at[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                     for (int it = 0; it < 4; ++it) {
@@ -684,27 +686,22 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 };
                 ok = wait_index(n_tile);
                 if (ok) {
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        fetch(kreg[st], p.k, 0, st, n_tile);
-                        fetch(vreg[st], p.v, 0, st, n_tile);
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(b_se + 8 * (n_tile % NSC));
+                    fetch(kreg, p.k, 0, n_tile);
+                    fetch(vreg, p.v, 0, n_tile);
                 }
-                for (int j = 0; j < nblk && ok; ++j) {
-                    const int t = ++n_tile;
-                    const bool more = j + 1 < nblk;
-                    if (more) ok = wait_index(t);
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        if (ok) ok = hand_over(kreg[st]);
-                        if (ok && more) fetch(kreg[st], p.k, j + 1, st, t);
-                        if (ok) ok = hand_over(vreg[st]);
-                        if (ok && more) fetch(vreg[st], p.v, j + 1, st, t);
+#pragma unroll 1
+                for (int k = 0; k < 2 * nblk && ok; ++k) {
+                    const bool more = k + 1 < 2 * nblk;
+                    if (k & 1) {                                // the block's index has been read
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b_se + 8 * (n_tile % NSC));
+                        ++n_tile;
+                        if (more) ok = wait_index(n_tile);
                     }
-                    __syncwarp();
-                    if (ok && more && lane == 0) mbar_arrive(b_se + 8 * (t % NSC));
+                    if (ok) ok = hand_over(kreg);
+                    if (ok && more) fetch(kreg, p.k, k + 1, n_tile);
+                    if (ok) ok = hand_over(vreg);
+                    if (ok && more) fetch(vreg, p.v, k + 1, n_tile);
                 }
             }
             if (ok) done_piece();

@@ -249,6 +249,8 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False
                          f"{tuple(weight.shape)} do not match")
     if kind not in _KINDS:
         raise ValueError(f"add_rmsnorm_quant: kind {kind!r} (int8 or fp8)")
+    if residual.device != device or weight.device != device:
+        raise RuntimeError(f"add_rmsnorm_quant: tensors on {device}, {residual.device} and {weight.device}")
     if x.dim() == 2:
         x2, r2 = x, residual
     else:

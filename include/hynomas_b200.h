@@ -6,6 +6,9 @@
  * (hy_nomas/kernels.py, hy_nomas/fused.py, hy_nomas/ops.py, hy_nomas/model.py, hy_nomas/pixelumm.py,
  * hy_nomas/world.py).
  *
+ * The serving operators (a paged K/V cache with its attention, residual + RMSNorm + quantizer) have no counterpart
+ * there as one call; what they stand beside is cited in the same way.
+ *
  * Conventions
  *  - All pointers are DEVICE pointers unless the name ends in `_host`. Nothing here allocates device
  *    memory; outputs are caller-owned buffers of the documented shape. Inputs are never written.
