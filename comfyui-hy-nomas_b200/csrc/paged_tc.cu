@@ -5,19 +5,23 @@
 // One CTA per SM, tiles of 256 rows: two softmax groups of 128 rows each share the K and V blocks of 128 keys.
 // A block goes through a group in two steps of 64 keys, with S in one of two TMEM buffers: the products of step k + 1 run
 // while step k is in the softmax (with one buffer of 128 keys the softmax waited for S 2250 of every 5100 clocks).
-//   warps 0-7    softmax. q to shared memory (a thread per row), then per step: S from TMEM in the fragment layout (a thread
-//                holds a quarter of the columns of four rows, so the factors of int8 keys come from shared memory once for four
-//                rows, not once per row), running maximum and sum, P over S; O is rescaled only when the maximum grew by more
-//                than 2^STALE. (Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%: issue is what is short, not MUFU.) TMEM: S / P of group g at 128 g + 64 (step % 2), O at 256 + 128 g.
-//   warps 8, 9   MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
+//   warps 0-15   softmax, 16 rows of a group each. q to shared memory (half a row a thread), then per step: S from TMEM in the
+//                fragment layout (a thread holds a quarter of the columns of two rows), running maximum and sum, P over S; O is
+//                rescaled only when the maximum grew by more than 2^STALE. TMEM: S / P of group g and step k at
+//                128 g + 64 (k % 2), O at 256 + 128 g. Sixteen warps of 16 rows, not eight of 32: a warp's chain of load,
+//                maximum, exponentials and store is latency, and a body of 32 rows did not fit the instruction caches (int8:
+//                2 stalls on instructions an issue). int8 2.91 ms with eight, 2.45 with their rows in two turns of one body and
+//                the producers' loop by a step, 2.16 with sixteen; bf16 1.73 with eight, 1.81 with sixteen (2 x 4400 queries over
+//                20240 keys, 16 heads). Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%.
+//   warps 16, 17 MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
 //                thread that issues blocks until its products have read their operands, so each group has a thread of its own:
 //                the tensor pipe runs one's products while the other waits.
-//   warp 10      walks the line: the CTA's pieces into a ring of four
-//   warp 11      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
-//   warps 12-15  producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
-//                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout of the products (K-major K, MN-major V). bf16: one warp, a TMA box per page (or its part in the block) and half
-//                of the head dim; V rows past the end become zeros (K's are masked). int8: four warps; codes go through
-//                registers and become fp16 integers (exact).
+//   warp 18      walks the line: the CTA's pieces into a ring of four
+//   warp 19      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
+//   warps 20-23  producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
+//                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout
+//                of the products (K-major K, MN-major V; V rows past the end become zeros, K's are masked). bf16: TMA, one warp.
+//                int8: four warps; codes go through registers, a step ahead, and become fp16 integers (exact).
 //
 // int8: t_j = (q . ck_j) * sk_j scale log2 e, x_j = t_j 2^e (2^e: the row's power of two), P'_j = 2^(x_j - m + 12) sv_j. m is the
 // running maximum of x plus that of ceil(log2 sv), so P' <= 2^12 (fp16) and the normaliser's terms 2^(x_j - m + 12) are at hand.
@@ -45,7 +49,7 @@ constexpr int KHALF = STEP * 128;           // K, V of a step: [64 rows][128 B] 
 constexpr int KTILE = 2 * KHALF;
 constexpr int NS = 9;                       // ring slots (K and V of the steps in turn); int8 with 8: 2.99 ms, with 9: 2.80
 constexpr int NSC = 4;                      // scale ring
-constexpr int TC_THREADS = 512;
+constexpr int TC_THREADS = 768;
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = 2 * TILE;
 constexpr int OFF_SC = OFF_KV + NS * KTILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
@@ -91,9 +95,9 @@ __device__ __forceinline__ void ld_frag(uint32_t taddr, uint32_t *r) {
         : "memory");
 }
 // the registers' uses stay behind this (and a wait::ld before it)
-__device__ __forceinline__ void frag_fence(uint32_t *r) {
+template <int N> __device__ __forceinline__ void frag_fence(uint32_t (&r)[N]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
+    for (int i = 0; i < N; i += 8)
         asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
                           "+r"(r[i + 6]), "+r"(r[i + 7]) :: "memory");
 }
@@ -148,8 +152,8 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     k_paged_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int box) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr float STALE = I8 ? 3.0f : 8.0f, AHEAD = I8 ? 2.0f : 0.0f;
-    constexpr int R_SOFTMAX = I8 ? 176 : 192, R_MMA = 56, R_LOAD = I8 ? 104 : 72;     // what each role needs without spills
-    static_assert(2 * R_SOFTMAX + R_MMA + R_LOAD == 512, "the registers that the block was launched with");
+    constexpr int R_SOFTMAX = 88, R_MMA = 48, R_LOAD = 80;      // what each role needs without spills
+    static_assert(4 * R_SOFTMAX + R_MMA + R_LOAD <= 6 * 80, "the registers that the block was launched with");
     const uint32_t sb = smem_u32(smem);
     const uint32_t b_full = sb + OFF_BAR, b_empty = b_full + 8 * NS, b_s = b_empty + 8 * NS, b_p = b_s + 32, b_q = b_p + 32,
                    b_v = b_q + 16, b_sc = b_v + 32, b_se = b_sc + 8 * NSC, b_pf = b_se + 8 * NSC, b_pe = b_pf + 8 * NP, b_end = b_pe + 8 * NP, b_tail = b_end + 16;
@@ -166,10 +170,10 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     if (threadIdx.x == 0) {
         // a block is given back by both groups' issuers
         for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, I8 ? 128 : 1); mbar_init(b_empty + 8 * i, 2); }
-        for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, 10 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
-        for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 4); mbar_init(b_v + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 128);
-        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, 12); }   // softmax, producers
+        for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, 18 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
+        for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 8); mbar_init(b_v + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 256);
+        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, 20); }   // softmax, producers
         mbar_init(b_end, 1);
         mbar_init(b_end + 8, 1);
         mbar_init(b_tail, 1);
@@ -177,7 +181,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(TMEM_COLS)
                      : "memory");
@@ -208,64 +212,62 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         ++n_piece;
     };
 
-    if (warp < 8) {
+    if (warp < 16) {
         // ------------------------------------------------------------------ softmax and the results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R_SOFTMAX));
-        const int g = warp >> 2, wq = warp & 3, rr = 32 * wq + lane;
-        const uint32_t tl = tmem + ((uint32_t)(32 * wq) << 16), ts = tl + 128 * g, to = tl + 256 + 128 * g;
+        const int g = warp >> 3, row16 = 32 * (warp & 3) + 16 * ((warp >> 2) & 1);     // of the group's 128 rows
+        const uint32_t tl = tmem + ((uint32_t)row16 << 16), ts = tl + 128 * g, to = tl + 256 + 128 * g;
         int n_s = 0, n_tile = 0;                // steps of this group, blocks of the CTA
         while (const Piece *pc = next_piece()) {
             const Piece &w = *pc;
-            const int r = w.row0 + 128 * g + rr;
-            const bool valid = r < rows_all;
-            int lim = w.kend;                   // a row past the tile's end: computed and dropped
-            const __nv_bfloat16 *qp = p.q;
-            if (valid) {
-                int b, l, gm;
-                split_row(p, w, r, b, l, gm);
-                qp += b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + gm) * p.q_hs;
-                lim = row_limit(p, seq_length(p, b), l);
-                lim = lim > w.kend ? w.kend : lim;
-            }
-            // --- q to shared memory (a row past the tile's end: zeros)
-            float rs = I8 ? 1.0f : p.sl2;       // int8: the keys' factors carry scale * log2 e
+            int seen[2];                        // keys, from the piece's first, that rows lane / 4 and lane / 4 + 8 see
+            float m[2], sum[2], rsf[2];
             {
-                uint32_t x[64];
+                // --- q to shared memory, half a row a thread (a row past the tile's end: zeros)
+                const int rr = row16 + (lane & 15), r = w.row0 + 128 * g + rr, c0 = 8 * (lane >> 4);
+                int lim = w.kend;               // a row past the tile's end: computed and dropped
+                float rs = I8 ? 1.0f : p.sl2;   // int8: the keys' factors carry scale * log2 e
+                uint32_t x[32];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    uint4 y = make_uint4(0, 0, 0, 0);
-                    if (valid) y = *reinterpret_cast<const uint4 *>(qp + 8 * c);
-                    x[4 * c] = y.x ^ p.flip; x[4 * c + 1] = y.y ^ p.flip;
-                    x[4 * c + 2] = y.z ^ p.flip; x[4 * c + 3] = y.w ^ p.flip;
+                for (int i = 0; i < 32; ++i) x[i] = 0;
+                if (r < rows_all) {
+                    int b, l, gm;
+                    split_row(p, w, r, b, l, gm);
+                    const __nv_bfloat16 *qp = p.q + b * p.q_bs + l * p.q_ls + (int64_t)(w.h * p.G + gm) * p.q_hs + 8 * c0;
+                    lim = row_limit(p, seq_length(p, b), l);
+                    lim = lim > w.kend ? w.kend : lim;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 y = *reinterpret_cast<const uint4 *>(qp + 8 * c);
+                        x[4 * c] = y.x ^ p.flip; x[4 * c + 1] = y.y ^ p.flip;
+                        x[4 * c + 2] = y.z ^ p.flip; x[4 * c + 3] = y.w ^ p.flip;
+                    }
                 }
                 if (I8) {
                     float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(x[i])), fabsf(bf16_hi(x[i]))));
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(x[i])), fabsf(bf16_hi(x[i]))));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     const int e = row_exponent(top);
                     const float down = pow2i(-e);
                     rs = pow2i(e);
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) x[i] = pack_f16_rn(bf16_lo(x[i]) * down, bf16_hi(x[i]) * down);
+                    for (int i = 0; i < 32; ++i) x[i] = pack_f16_rn(bf16_lo(x[i]) * down, bf16_hi(x[i]) * down);
                 }
 #pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    sts16(sb + OFF_Q + g * TILE + chunk_at<HALF>(rr, c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+                for (int c = 0; c < 8; ++c)
+                    sts16(sb + OFF_Q + g * TILE + chunk_at<HALF>(rr, c0 + c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + w.blk0 * BKT);
+                    rsf[u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
+                    m[u] = -INFINITY;
+                    sum[u] = 0.0f;
+                }
             }
             fence_async();
             mbar_arrive(b_q + 8 * g);
-
-            // --- from here on a thread works on rows 16 hf + 8 u + lane / 4 of its warp's 32
             const int nblk = w.nblk;
-            int seen[4];                                                        // keys of the block that the row sees
-            float m[4], sum[4], rsf[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + w.blk0 * BKT);
-                rsf[u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
-                m[u] = -INFINITY;
-                sum[u] = 0.0f;
-            }
             float ev = -1000.0f;                // int8: running maximum of ceil(log2 sv), at least
             for (int k = 0; k < 2 * nblk; ++k, ++n_s) {         // steps of 64 keys
                 const int sub = k & 1, t = n_tile + (k >> 1);
@@ -292,116 +294,110 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                         ev = e;
                     }
                 }
-                // 16 of the warp's 32 rows, then the others, by the same instructions (HF_WHY)
-                #pragma unroll 1
-                for (int hf = 0; hf < 2; ++hf) {
-                    const uint32_t lanes = (uint32_t)(16 * hf) << 16;
-                    uint32_t x[32];             // [8 column groups][row l / 4, l / 4 + 8][2 columns]
-                    ld_frag(tsb + lanes, x);
-                    ld_frag(tsb + lanes + 32, x + 16);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    frag_fence(x);
-                    if (I8) {
+                uint32_t x[32];                 // [8 column groups][row l / 4, l / 4 + 8][2 columns]
 #pragma unroll
-                        for (int c = 0; c < 8; c += 2) {
-                            const ulonglong2 kf = factors[2 * c];
+                for (int c = 0; c < 2; ++c) ld_frag(tsb + 32 * c, x + 16 * c);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                frag_fence(x);
+                if (I8) {
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) {       // 2 column groups x 2 rows
-                                uint32_t *y = x + 4 * (c + (v & 1)) + (v & 2);
-                                float y0, y1;
-                                x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
-                                y[0] = __float_as_uint(y0);
-                                y[1] = __float_as_uint(y1);
-                            }
+                    for (int c = 0; c < 8; c += 2) {
+                        const ulonglong2 kf = factors[2 * c];
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {           // 2 column groups x the rows
+                            uint32_t *y = x + 4 * (c + (v & 1)) + (v & 2);
+                            float y0, y1;
+                            x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
+                            y[0] = __float_as_uint(y0);
+                            y[1] = __float_as_uint(y1);
                         }
-                    }
-                    if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < 64)) {
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (8 * (c >> 2) + 2 * (lane & 3) + (c & 1) >= seen[(c >> 1) & 1]) x[c] = __float_as_uint(-INFINITY);
-                    }
-                    float mn[2];
-                    bool need = grown;
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t *y = x + 2 * u;
-                        float mx[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            mx[c] = nan_max3(mx[c], __uint_as_float(y[16 + 4 * c]), __uint_as_float(y[16 + 4 * c + 1]));
-                        mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
-                        mn[u] *= rsf[u];
-                        need |= !(mn[u] <= m[u] + STALE);       // or a NaN, which stays in the row
-                    }
-                    if (k == 0) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) m[u] = mn[u] + AHEAD;
-                    } else if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const bool grow = !(mn[u] <= m[u] + STALE);
-                            const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
-                            m[u] = grow ? mn[u] + AHEAD : m[u];
-                            mn[u] = al;
-                            sum[u] *= al;
-                        }
-                        // the product before this step's is the last one given to the pipe
-                        ok = warp_wait(lane, b_v + 16 * g + 8 * (sub ^ 1), ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < HD; c += 32) scale_frag(to + lanes + c, mn[0], mn[1]);
-                    }
-                    uint64_t nref[2], acc[2] = {0ull, 0ull};
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float ref = m[u] == -INFINITY ? 0.0f : m[u];
-                        nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
-                    }
-#pragma unroll
-                    for (int c = 0; c < 8; c += 4) {            // 4 column groups: a store of 8 registers
-                        uint64_t v[4];
-                        if (I8) {
-                            const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
-                            v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
-                        }
-                        uint32_t pk[8];
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) {           // column group c + q / 2, row q % 2
-                            const int u = q & 1;
-                            const uint32_t *y = x + 4 * c + 2 * q;
-                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), x2_splat(rsf[u]), nref[u]);
-                            float a0, a1;
-                            x2_split(a, a0, a1);
-                            uint64_t e = x2(ex2(a0), ex2(a1));
-                            acc[u] = x2_add(acc[u], e);
-                            if (I8) e = x2_mul(e, v[q >> 1]);
-                            float e0, e1;
-                            x2_split(e, e0, e1);
-                            pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
-                        }
-                        st_frag(tsb + lanes + 4 * c, pk);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float a0, a1;
-                        x2_split(acc[u], a0, a1);
-                        // the other rows' state comes to the front
-                        float y = sum[u] + (a0 + a1);
-                        sum[u] = sum[u + 2]; sum[u + 2] = y;
-                        y = m[u]; m[u] = m[u + 2]; m[u + 2] = y;
-                        y = rsf[u]; rsf[u] = rsf[u + 2]; rsf[u + 2] = y;
-                        const int z = seen[u] - 64; seen[u] = seen[u + 2]; seen[u + 2] = z;
                     }
                 }
+                if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < 64)) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (8 * (c >> 2) + 2 * (lane & 3) + (c & 1) >= seen[(c >> 1) & 1])
+                            x[c] = __float_as_uint(-INFINITY);
+                }
+                float mn[2];
+                bool need = grown;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t *y = x + 2 * u;
+                    float mx[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        mx[c] = nan_max3(mx[c], __uint_as_float(y[16 + 4 * c]), __uint_as_float(y[16 + 4 * c + 1]));
+                    mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
+                    mn[u] *= rsf[u];
+                    need |= !(mn[u] <= m[u] + STALE);           // or a NaN, which stays in the row
+                }
+                if (k == 0) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) m[u] = mn[u] + AHEAD;
+                } else if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const bool grow = !(mn[u] <= m[u] + STALE);
+                        const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
+                        m[u] = grow ? mn[u] + AHEAD : m[u];
+                        mn[u] = al;
+                        sum[u] *= al;
+                    }
+                    // the product before this step's is the last one given to the pipe
+                    ok = warp_wait(lane, b_v + 16 * g + 8 * (sub ^ 1), ((n_s - 1) >> 1) & 1, abort_flag, WAIT_NS, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) scale_frag(to + c, mn[0], mn[1]);
+                }
+                uint64_t nref[2], acc[2] = {0ull, 0ull};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float ref = m[u] == -INFINITY ? 0.0f : m[u];
+                    nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
+                }
+#pragma unroll
+                for (int c = 0; c < 8; c += 4) {                // 4 column groups: a store of 8 registers
+                    uint64_t v[4];
+                    if (I8) {
+                        const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
+                        v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
+                    }
+                    uint32_t pk[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {               // column group c + q / 2, row q % 2
+                        const int u = q & 1;
+                        const uint32_t *y = x + 4 * c + 2 * q;
+                        const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])),
+                                                  x2_splat(rsf[u]), nref[u]);
+                        float a0, a1;
+                        x2_split(a, a0, a1);
+                        uint64_t e = x2(ex2(a0), ex2(a1));
+                        acc[u] = x2_add(acc[u], e);
+                        if (I8) e = x2_mul(e, v[q >> 1]);
+                        float e0, e1;
+                        x2_split(e, e0, e1);
+                        pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
+                    }
+                    st_frag(tsb + 4 * c, pk);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float a0, a1;
+                    x2_split(acc[u], a0, a1);
+                    sum[u] += a0 + a1;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) seen[u] -= 64;
                 if (!ok) break;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
@@ -411,15 +407,6 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     if (I8 && sub == 1) mbar_arrive(b_se + 8 * (t % NSC));
                 }
             }
-            // back to a thread per row: row `lane` is 8 u + lane / 4 in the quad 4 (lane % 8)
-            float mrow = 0.0f, srow = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
-                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
-                const float a = __shfl_sync(0xffffffffu, m[u], 4 * (lane & 7)), c = __shfl_sync(0xffffffffu, sum[u], 4 * (lane & 7));
-                if ((lane >> 3) == u) { mrow = I8 ? a + ev + (STREAM_SHIFT - TC_SHIFT) : a; srow = c; }
-            }
             if (!ok) break;
             n_tile += nblk;
             // --- O: to the output, or to the piece's slot
@@ -427,49 +414,56 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (!ok) break;
             tc_fence_after();
             const bool ends = w.slot < 0;
-            const float inv = ends ? inverse(srow) : 1.0f;
-            int b = 0, l = 0, gm = 0;
-            if (valid) split_row(p, w, r, b, l, gm);
-            const int head = w.h * p.G + gm;
-            const int64_t at = (int64_t)(ends ? 0 : w.slot) * p.part_rows + 128 * g + rr;
-            __nv_bfloat16 *op = p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs;
+            float inv[2];
+            bool valid[2];
+            __nv_bfloat16 *op[2];
+            float *part[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
+                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
+                const float ref = I8 ? m[u] + ev + (STREAM_SHIFT - TC_SHIFT) : m[u];
+                const int rr = row16 + 8 * u + (lane >> 2), r = w.row0 + 128 * g + rr;
+                valid[u] = r < rows_all;
+                int b = 0, l = 0, gm = 0;
+                if (valid[u]) split_row(p, w, r, b, l, gm);
+                const int head = w.h * p.G + gm;
+                const int64_t at = (int64_t)(ends ? 0 : w.slot) * p.part_rows + 128 * g + rr;
+                inv[u] = inverse(sum[u]);
+                op[u] = p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs + 2 * (lane & 3);
+                part[u] = p.part_o + at * HD + 2 * (lane & 3);
+                if (valid[u] && (lane & 3) == 0) {
+                    if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(ref, sum[u]);
+                    else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, ref, sum[u]);
+                }
+            }
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
-                if (valid && ends) {
+                uint32_t o[16];                 // [4 column groups][2 rows][2 columns]
+                ld_frag(to + c, o);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                frag_fence(o);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        uint4 y;
-                        uint32_t *z = &y.x;
-#pragma unroll
-                        for (int v = 0; v < 4; ++v)
-                            z[v] = bf16x2_rn(__uint_as_float(o[8 * u + 2 * v]) * inv, __uint_as_float(o[8 * u + 2 * v + 1]) * inv);
-                        *reinterpret_cast<uint4 *>(op + c + 8 * u) = y;
-                    }
-                } else if (valid) {
-#pragma unroll
-                    for (int u = 0; u < 8; ++u)
-                        *reinterpret_cast<uint4 *>(p.part_o + at * HD + c + 4 * u) =
-                            make_uint4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                for (int v = 0; v < 8; ++v) {
+                    const int u = v & 1, at = c + 8 * (v >> 1);
+                    if (!valid[u]) continue;
+                    const float a0 = __uint_as_float(o[2 * v]), a1 = __uint_as_float(o[2 * v + 1]);
+                    if (ends) *reinterpret_cast<uint32_t *>(op[u] + at) = bf16x2_rn(a0 * inv[u], a1 * inv[u]);
+                    else *reinterpret_cast<float2 *>(part[u] + at) = make_float2(a0, a1);
                 }
                 __syncwarp();
-            }
-            if (valid) {
-                if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(mrow, srow);
-                else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, mrow, srow);
             }
             tc_fence_before();          // O is read before the next piece's products, which wait for this group's P
             done_piece();
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ------------------------------------------------------------------ MMA issuers, walker
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_MMA));
-        if (warp < 10) {
+        if (warp < 18) {
             // kind::f16: fp32 D (bit 4), A and B bf16 (bits 7, 10) or f16 (0), N / 8 at bit 17, M / 16 at bit 24; V is MN-major (bit 16)
             constexpr uint32_t types = (1u << 4) | (I8 ? 0u : (1u << 7) | (1u << 10)) | (8u << 24);
             constexpr uint32_t idesc_s = types | (8u << 17), idesc_o = types | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
-            const int g = warp - 8;
+            const int g = warp - 16;
             const uint32_t ds = tmem + 128 * g, dout = tmem + 256 + 128 * g;
             uint32_t h = 0;                         // ring index of the next step's K; V follows it
             uint32_t n_p = 0;
@@ -530,7 +524,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 mbar_wait(b_end + 8 * g, 0, &never, 100000000ull, p.err);
             }
             __syncwarp();
-        } else if (warp == 10 && lane == 0) {
+        } else if (warp == 18 && lane == 0) {
             Walker walk(p, pre, blockIdx.x);
             Piece w;
             for (bool more = true; more; ++n_piece) {
@@ -540,7 +534,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 const_cast<Piece *>(ring)[n_piece % NP] = w;
                 mbar_arrive(b_pf + 8 * (n_piece % NP));
             }
-        } else if (I8 && warp == 11) {
+        } else if (I8 && warp == 19) {
             int n_tile = 0;
             while (const Piece *pc = next_piece()) {
                 const int own_b = pc->own_b, head = pc->h, kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
@@ -602,11 +596,11 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     } else {
         // ------------------------------------------------------------------ producers
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_LOAD));
-        const int tid = threadIdx.x - 384;
+        const int tid = threadIdx.x - 640;
         uint32_t half = 0;                      // ring index
         uint32_t tails = 0;
         int n_tile = 0;
-        while (I8 || warp == 12) {
+        while (I8 || warp == 20) {
             const Piece *pc = next_piece();
             if (pc == nullptr) break;
             const int kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
@@ -707,7 +701,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (ok) done_piece();
         }
         // every copy issued has landed before the CTA may exit (immediate on the normal path)
-        if (!I8 && warp == 12 && lane == 0) {
+        if (!I8 && warp == 20 && lane == 0) {
             volatile int never = 0;
             for (uint32_t h = half >= NS ? half - NS : 0; h < half; ++h)
                 mbar_wait(b_full + 8 * (h % NS), (h / NS) & 1, &never, 100000000ull, p.err);
@@ -717,7 +711,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
