@@ -6,7 +6,7 @@
 //
 // Bound by HBM: 4 B read and 3 B written per element (+ scales). T threads hold a row in registers, NCH chunks of 8
 // elements each (chunk i * T + t at elements [8c, 8c + 8)), so that x and r are read once; a 128-column group is 16
-// neighbouring lanes of one i.
+// neighbouring lanes of one i. Measured (kernel alone): 20240 x 4096, e4m3: 89 us, 6.5 TB/s; 1 x 4096: 4.2 us, a launch.
 #include "hn_common.cuh"
 #include "hn_kernels.h"
 

@@ -11,7 +11,10 @@
 // computes the cut itself from the lengths on the device). A tile that spans CTAs leaves a partial result per CTA
 // (fp32 sums, maximum, normaliser), joined by k_paged_join.
 //
-// Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head).
+// Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head): 64 sequences of about 2500
+// tokens, 8 K/V heads: bf16 126 us (5.9 TB/s), int8 118 us (3.3 TB/s: the conversion of the codes issues as much as the products).
+// With 64-row tiles by the shared-memory reads of the fragments: 32 sequences on 15840 shared tokens, 32 / 8 heads, int8: 75 us
+// and the join's 11.
 // Per warp: 16 rows; m16n8k16 products, S and O in registers. The four warps split a block's keys (16-row tiles), its
 // rows (64), or both (32). Blocks arrive by cp.async, STAGES deep; the smem chunks are permuted so that no read conflicts.
 //  - bf16 cache: K by ldmatrix, V by its transposing form, P rounded to bf16.

@@ -5,20 +5,21 @@
 // One CTA per SM, tiles of 256 rows: two softmax groups of 128 rows each share the K and V blocks of 128 keys.
 // A block goes through a group in two steps of 64 keys, with S in one of two TMEM buffers: the products of step k + 1 run
 // while step k is in the softmax (with one buffer of 128 keys the softmax waited for S 2250 of every 5100 clocks).
-//   warps 0-15   softmax, 16 rows of a group each. q to shared memory (half a row a thread), then per step: S from TMEM in the
-//                fragment layout (a thread holds a quarter of the columns of two rows), running maximum and sum, P over S; O is
-//                rescaled only when the maximum grew by more than 2^STALE. TMEM: S / P of group g and step k at
-//                128 g + 64 (k % 2), O at 256 + 128 g. Sixteen warps of 16 rows, not eight of 32: a warp's chain of load,
-//                maximum, exponentials and store is latency, and a body of 32 rows did not fit the instruction caches (int8:
-//                2 stalls on instructions an issue). int8 2.91 ms with eight, 2.45 with their rows in two turns of one body and
-//                the producers' loop by a step, 2.16 with sixteen; bf16 1.73 with eight, 1.81 with sixteen (2 x 4400 queries over
-//                20240 keys, 16 heads). Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%.
-//   warps 16, 17 MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
+//   NW warps     softmax. q to shared memory (half a row a thread), then per step: S from TMEM in the fragment layout (a thread
+//                holds a quarter of the columns of every eighth row), running maximum and sum, P over S; O is rescaled only when
+//                the maximum grew by more than 2^STALE. TMEM: S / P of group g and step k at 128 g + 64 (k % 2), O at
+//                256 + 128 g. int8: sixteen warps of 16 rows. A warp's chain of load, factors, maximum, exponentials and store is
+//                latency, and with 32 rows its body, beside the producers', did not fit the instruction caches (2 stalls on
+//                instructions an issue): 2.91 ms with eight warps, 2.45 with their rows in two turns of one body and the
+//                producers' loop by a step, 2.17 with sixteen. bf16: eight of 32 rows, whose body is shorter and whose
+//                handovers are what counts: causal 1.68-1.71 ms, sixteen 1.85 (2 x 4400 queries over 20240 keys, 16 heads).
+//                Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%.
+//   2 warps      MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
 //                thread that issues blocks until its products have read their operands, so each group has a thread of its own:
 //                the tensor pipe runs one's products while the other waits.
-//   warp 18      walks the line: the CTA's pieces into a ring of four
-//   warp 19      int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
-//   warps 20-23  producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
+//   1 warp       walks the line: the CTA's pieces into a ring of four
+//   1 warp       int8: looks the block's pages up and gathers its keys' factors, into a second ring of four
+//   4 warps      producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
 //                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout
 //                of the products (K-major K, MN-major V; V rows past the end become zeros, K's are masked). bf16: TMA, one warp.
 //                int8: four warps; codes go through registers, a step ahead, and become fp16 integers (exact).
@@ -49,7 +50,10 @@ constexpr int KHALF = STEP * 128;           // K, V of a step: [64 rows][128 B] 
 constexpr int KTILE = 2 * KHALF;
 constexpr int NS = 9;                       // ring slots (K and V of the steps in turn); int8 with 8: 2.99 ms, with 9: 2.80
 constexpr int NSC = 4;                      // scale ring
-constexpr int TC_THREADS = 768;
+// 16-row parts of a group that a softmax warp takes, and the softmax warps (of both groups); four issuers and helpers, four producers
+template <bool I8> constexpr int PARTS = I8 ? 1 : 2;
+template <bool I8> constexpr int SOFTMAX_WARPS = 16 / PARTS<I8>;
+template <bool I8> constexpr int TC_THREADS = 32 * (SOFTMAX_WARPS<I8> + 8);
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = 2 * TILE;
 constexpr int OFF_SC = OFF_KV + NS * KTILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
@@ -148,12 +152,13 @@ __device__ __forceinline__ void tma_rows(const CUtensorMap *map, uint32_t dst, u
 }
 
 // `box`: tokens per TMA box (bf16), a divisor of the page and of 128
-template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
+template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
     k_paged_tc(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p, int box) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr float STALE = I8 ? 3.0f : 8.0f, AHEAD = I8 ? 2.0f : 0.0f;
-    constexpr int R_SOFTMAX = 88, R_MMA = 48, R_LOAD = 80;      // what each role needs without spills
-    static_assert(4 * R_SOFTMAX + R_MMA + R_LOAD <= 6 * 80, "the registers that the block was launched with");
+    constexpr int H = PARTS<I8>, NW = SOFTMAX_WARPS<I8>;
+    constexpr int R_SOFTMAX = I8 ? 88 : 192, R_MMA = I8 ? 48 : 56, R_LOAD = I8 ? 80 : 72;      // what each role needs without spills
+    static_assert(NW / 4 * R_SOFTMAX + R_MMA + R_LOAD <= (I8 ? 6 * 80 : 4 * 128), "the registers that the block was launched with");
     const uint32_t sb = smem_u32(smem);
     const uint32_t b_full = sb + OFF_BAR, b_empty = b_full + 8 * NS, b_s = b_empty + 8 * NS, b_p = b_s + 32, b_q = b_p + 32,
                    b_v = b_q + 16, b_sc = b_v + 32, b_se = b_sc + 8 * NSC, b_pf = b_se + 8 * NSC, b_pe = b_pf + 8 * NP, b_end = b_pe + 8 * NP, b_tail = b_end + 16;
@@ -170,10 +175,10 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     if (threadIdx.x == 0) {
         // a block is given back by both groups' issuers
         for (int i = 0; i < NS; ++i) { mbar_init(b_full + 8 * i, I8 ? 128 : 1); mbar_init(b_empty + 8 * i, 2); }
-        for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, 18 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
-        for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 8); mbar_init(b_v + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 256);
-        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, 20); }   // softmax, producers
+        for (int i = 0; i < NP; ++i) { mbar_init(b_pf + 8 * i, 1); mbar_init(b_pe + 8 * i, NW + 2 + (I8 ? 5 : 1)); }   // softmax, issuers, producers
+        for (int i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, NW / 2); mbar_init(b_v + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) mbar_init(b_q + 8 * i, 16 * NW);
+        for (int i = 0; i < NSC; ++i) { mbar_init(b_sc + 8 * i, 1); mbar_init(b_se + 8 * i, NW + 4); }   // softmax, producers
         mbar_init(b_end, 1);
         mbar_init(b_end + 8, 1);
         mbar_init(b_tail, 1);
@@ -181,16 +186,16 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
-    if (warp == 16) {
+    if (warp == NW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     dep_launch();
-    prefix_blocks(p, pre, sums, lead, TC_THREADS);
+    prefix_blocks(p, pre, sums, lead, TC_THREADS<I8>);
     if (blockIdx.x == 0)
-        for (int b = threadIdx.x; b <= p.B; b += TC_THREADS) p.sched[b] = pre[b];
+        for (int b = threadIdx.x; b <= p.B; b += TC_THREADS<I8>) p.sched[b] = pre[b];
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -212,19 +217,20 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
         ++n_piece;
     };
 
-    if (warp < 16) {
+    if (warp < NW) {
         // ------------------------------------------------------------------ softmax and the results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R_SOFTMAX));
-        const int g = warp >> 3, row16 = 32 * (warp & 3) + 16 * ((warp >> 2) & 1);     // of the group's 128 rows
-        const uint32_t tl = tmem + ((uint32_t)row16 << 16), ts = tl + 128 * g, to = tl + 256 + 128 * g;
+        const int g = warp / (NW / 2), row0 = 32 * (warp & 3) + (H == 1 ? 16 * ((warp >> 2) & 1) : 0);       // of the group's 128 rows
+        const uint32_t tl = tmem + ((uint32_t)row0 << 16), ts = tl + 128 * g, to = tl + 256 + 128 * g;
         int n_s = 0, n_tile = 0;                // steps of this group, blocks of the CTA
         while (const Piece *pc = next_piece()) {
             const Piece &w = *pc;
-            int seen[2];                        // keys, from the piece's first, that rows lane / 4 and lane / 4 + 8 see
-            float m[2], sum[2], rsf[2];
-            {
+            int seen[2 * H];                    // keys, from the piece's first, that rows 8 u + lane / 4 see
+            float m[2 * H], sum[2 * H], rsf[2 * H];
+#pragma unroll
+            for (int hf = 0; hf < H; ++hf) {
                 // --- q to shared memory, half a row a thread (a row past the tile's end: zeros)
-                const int rr = row16 + (lane & 15), r = w.row0 + 128 * g + rr, c0 = 8 * (lane >> 4);
+                const int rr = row0 + 16 * hf + (lane & 15), r = w.row0 + 128 * g + rr, c0 = 8 * (lane >> 4);
                 int lim = w.kend;               // a row past the tile's end: computed and dropped
                 float rs = I8 ? 1.0f : p.sl2;   // int8: the keys' factors carry scale * log2 e
                 uint32_t x[32];
@@ -259,10 +265,10 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     sts16(sb + OFF_Q + g * TILE + chunk_at<HALF>(rr, c0 + c), x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    seen[u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + w.blk0 * BKT);
-                    rsf[u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
-                    m[u] = -INFINITY;
-                    sum[u] = 0.0f;
+                    seen[2 * hf + u] = __shfl_sync(0xffffffffu, lim, 8 * u + (lane >> 2)) - (w.kbeg + w.blk0 * BKT);
+                    rsf[2 * hf + u] = I8 ? __shfl_sync(0xffffffffu, rs, 8 * u + (lane >> 2)) : rs;
+                    m[2 * hf + u] = -INFINITY;
+                    sum[2 * hf + u] = 0.0f;
                 }
             }
             fence_async();
@@ -294,9 +300,9 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                         ev = e;
                     }
                 }
-                uint32_t x[32];                 // [8 column groups][row l / 4, l / 4 + 8][2 columns]
+                uint32_t x[32 * H];             // [16-row part][8 column groups][row l / 4, l / 4 + 8][2 columns]
 #pragma unroll
-                for (int c = 0; c < 2; ++c) ld_frag(tsb + 32 * c, x + 16 * c);
+                for (int c = 0; c < 2 * H; ++c) ld_frag(tsb + ((uint32_t)(16 * (c >> 1)) << 16) + 32 * (c & 1), x + 16 * c);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 frag_fence(x);
                 if (I8) {
@@ -304,8 +310,8 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     for (int c = 0; c < 8; c += 2) {
                         const ulonglong2 kf = factors[2 * c];
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) {           // 2 column groups x the rows
-                            uint32_t *y = x + 4 * (c + (v & 1)) + (v & 2);
+                        for (int v = 0; v < 4 * H; ++v) {       // 2 column groups x the rows
+                            uint32_t *y = x + 32 * (v >> 2) + 4 * (c + (v & 1)) + (v & 2);
                             float y0, y1;
                             x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
                             y[0] = __float_as_uint(y0);
@@ -313,17 +319,20 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                         }
                     }
                 }
-                if (__any_sync(0xffffffffu, min(seen[0], seen[1]) < 64)) {
+                int least = seen[0];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (8 * (c >> 2) + 2 * (lane & 3) + (c & 1) >= seen[(c >> 1) & 1])
+                for (int u = 1; u < 2 * H; ++u) least = min(least, seen[u]);
+                if (__any_sync(0xffffffffu, least < 64)) {
+#pragma unroll
+                    for (int c = 0; c < 32 * H; ++c)
+                        if (8 * ((c & 31) >> 2) + 2 * (lane & 3) + (c & 1) >= seen[2 * (c >> 5) + ((c >> 1) & 1)])
                             x[c] = __float_as_uint(-INFINITY);
                 }
-                float mn[2];
+                float mn[2 * H];
                 bool need = grown;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t *y = x + 2 * u;
+                for (int u = 0; u < 2 * H; ++u) {
+                    const uint32_t *y = x + 32 * (u >> 1) + 2 * (u & 1);
                     float mx[4];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) mx[c] = nan_max(__uint_as_float(y[4 * c]), __uint_as_float(y[4 * c + 1]));
@@ -333,19 +342,19 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     mn[u] = nan_max(nan_max3(mx[0], mx[1], mx[2]), mx[3]);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
+                for (int u = 0; u < 2 * H; ++u) mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 1));
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < 2 * H; ++u) {
                     mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
                     mn[u] *= rsf[u];
                     need |= !(mn[u] <= m[u] + STALE);           // or a NaN, which stays in the row
                 }
                 if (k == 0) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) m[u] = mn[u] + AHEAD;
+                    for (int u = 0; u < 2 * H; ++u) m[u] = mn[u] + AHEAD;
                 } else if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < 2 * H; ++u) {
                         const bool grow = !(mn[u] <= m[u] + STALE);
                         const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
                         m[u] = grow ? mn[u] + AHEAD : m[u];
@@ -357,47 +366,54 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) scale_frag(to + c, mn[0], mn[1]);
-                }
-                uint64_t nref[2], acc[2] = {0ull, 0ull};
+                    for (int c = 0; c < HD; c += 32) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float ref = m[u] == -INFINITY ? 0.0f : m[u];
-                    nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
-                }
-#pragma unroll
-                for (int c = 0; c < 8; c += 4) {                // 4 column groups: a store of 8 registers
-                    uint64_t v[4];
-                    if (I8) {
-                        const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
-                        v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
+                        for (int hf = 0; hf < H; ++hf)
+                            scale_frag(to + ((uint32_t)(16 * hf) << 16) + c, mn[2 * hf], mn[2 * hf + 1]);
                     }
-                    uint32_t pk[8];
+                }
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {               // column group c + q / 2, row q % 2
-                        const int u = q & 1;
-                        const uint32_t *y = x + 4 * c + 2 * q;
-                        const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])),
-                                                  x2_splat(rsf[u]), nref[u]);
+                for (int hf = 0; hf < H; ++hf) {
+                    uint64_t nref[2], acc[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float ref = m[2 * hf + u] == -INFINITY ? 0.0f : m[2 * hf + u];
+                        nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4) {                // 4 column groups: a store of 8 registers
+                        uint64_t v[4];
+                        if (I8) {
+                            const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
+                            v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
+                        }
+                        uint32_t pk[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) {               // column group c + q / 2, row q % 2
+                            const int u = q & 1;
+                            const uint32_t *y = x + 32 * hf + 4 * c + 2 * q;
+                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])),
+                                                      x2_splat(rsf[2 * hf + u]), nref[u]);
+                            float a0, a1;
+                            x2_split(a, a0, a1);
+                            uint64_t e = x2(ex2(a0), ex2(a1));
+                            acc[u] = x2_add(acc[u], e);
+                            if (I8) e = x2_mul(e, v[q >> 1]);
+                            float e0, e1;
+                            x2_split(e, e0, e1);
+                            pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
+                        }
+                        st_frag(tsb + ((uint32_t)(16 * hf) << 16) + 4 * c, pk);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
                         float a0, a1;
-                        x2_split(a, a0, a1);
-                        uint64_t e = x2(ex2(a0), ex2(a1));
-                        acc[u] = x2_add(acc[u], e);
-                        if (I8) e = x2_mul(e, v[q >> 1]);
-                        float e0, e1;
-                        x2_split(e, e0, e1);
-                        pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
+                        x2_split(acc[u], a0, a1);
+                        sum[2 * hf + u] += a0 + a1;
                     }
-                    st_frag(tsb + 4 * c, pk);
                 }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float a0, a1;
-                    x2_split(acc[u], a0, a1);
-                    sum[u] += a0 + a1;
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) seen[u] -= 64;
+                for (int u = 0; u < 2 * H; ++u) seen[u] -= 64;
                 if (!ok) break;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
@@ -414,56 +430,59 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (!ok) break;
             tc_fence_after();
             const bool ends = w.slot < 0;
-            float inv[2];
-            bool valid[2];
-            __nv_bfloat16 *op[2];
-            float *part[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
-                sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
-                const float ref = I8 ? m[u] + ev + (STREAM_SHIFT - TC_SHIFT) : m[u];
-                const int rr = row16 + 8 * u + (lane >> 2), r = w.row0 + 128 * g + rr;
-                valid[u] = r < rows_all;
-                int b = 0, l = 0, gm = 0;
-                if (valid[u]) split_row(p, w, r, b, l, gm);
-                const int head = w.h * p.G + gm;
-                const int64_t at = (int64_t)(ends ? 0 : w.slot) * p.part_rows + 128 * g + rr;
-                inv[u] = inverse(sum[u]);
-                op[u] = p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs + 2 * (lane & 3);
-                part[u] = p.part_o + at * HD + 2 * (lane & 3);
-                if (valid[u] && (lane & 3) == 0) {
-                    if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(ref, sum[u]);
-                    else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, ref, sum[u]);
+            for (int hf = 0; hf < H; ++hf) {
+                float inv[2];
+                bool valid[2];
+                __nv_bfloat16 *op[2];
+                float *part[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    sum[2 * hf + u] += __shfl_xor_sync(0xffffffffu, sum[2 * hf + u], 1);
+                    sum[2 * hf + u] += __shfl_xor_sync(0xffffffffu, sum[2 * hf + u], 2);
+                    const float ref = I8 ? m[2 * hf + u] + ev + (STREAM_SHIFT - TC_SHIFT) : m[2 * hf + u];
+                    const int rr = row0 + 16 * hf + 8 * u + (lane >> 2), r = w.row0 + 128 * g + rr;
+                    valid[u] = r < rows_all;
+                    int b = 0, l = 0, gm = 0;
+                    if (valid[u]) split_row(p, w, r, b, l, gm);
+                    const int head = w.h * p.G + gm;
+                    const int64_t at = (int64_t)(ends ? 0 : w.slot) * p.part_rows + 128 * g + rr;
+                    inv[u] = inverse(sum[2 * hf + u]);
+                    op[u] = p.out + b * p.o_bs + l * p.o_ls + head * p.o_hs + 2 * (lane & 3);
+                    part[u] = p.part_o + at * HD + 2 * (lane & 3);
+                    if (valid[u] && (lane & 3) == 0) {
+                        if (!ends) *reinterpret_cast<float2 *>(p.part_ml + 2 * at) = make_float2(ref, sum[2 * hf + u]);
+                        else if (p.lse != nullptr) p.lse[((int64_t)b * p.H + head) * p.Lq + l] = row_lse(p, ref, sum[2 * hf + u]);
+                    }
                 }
-            }
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t o[16];                 // [4 column groups][2 rows][2 columns]
-                ld_frag(to + c, o);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                frag_fence(o);
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[16];                 // [4 column groups][2 rows][2 columns]
+                    ld_frag(to + ((uint32_t)(16 * hf) << 16) + c, o);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    frag_fence(o);
 #pragma unroll
-                for (int v = 0; v < 8; ++v) {
-                    const int u = v & 1, at = c + 8 * (v >> 1);
-                    if (!valid[u]) continue;
-                    const float a0 = __uint_as_float(o[2 * v]), a1 = __uint_as_float(o[2 * v + 1]);
-                    if (ends) *reinterpret_cast<uint32_t *>(op[u] + at) = bf16x2_rn(a0 * inv[u], a1 * inv[u]);
-                    else *reinterpret_cast<float2 *>(part[u] + at) = make_float2(a0, a1);
+                    for (int v = 0; v < 8; ++v) {
+                        const int u = v & 1, at = c + 8 * (v >> 1);
+                        if (!valid[u]) continue;
+                        const float a0 = __uint_as_float(o[2 * v]), a1 = __uint_as_float(o[2 * v + 1]);
+                        if (ends) *reinterpret_cast<uint32_t *>(op[u] + at) = bf16x2_rn(a0 * inv[u], a1 * inv[u]);
+                        else *reinterpret_cast<float2 *>(part[u] + at) = make_float2(a0, a1);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             tc_fence_before();          // O is read before the next piece's products, which wait for this group's P
             done_piece();
         }
-    } else if (warp < 20) {
+    } else if (warp < NW + 4) {
         // ------------------------------------------------------------------ MMA issuers, walker
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_MMA));
-        if (warp < 18) {
+        if (warp < NW + 2) {
             // kind::f16: fp32 D (bit 4), A and B bf16 (bits 7, 10) or f16 (0), N / 8 at bit 17, M / 16 at bit 24; V is MN-major (bit 16)
             constexpr uint32_t types = (1u << 4) | (I8 ? 0u : (1u << 7) | (1u << 10)) | (8u << 24);
             constexpr uint32_t idesc_s = types | (8u << 17), idesc_o = types | ((uint32_t)(HD >> 3) << 17) | (1u << 16);
-            const int g = warp - 16;
+            const int g = warp - NW;
             const uint32_t ds = tmem + 128 * g, dout = tmem + 256 + 128 * g;
             uint32_t h = 0;                         // ring index of the next step's K; V follows it
             uint32_t n_p = 0;
@@ -524,7 +543,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 mbar_wait(b_end + 8 * g, 0, &never, 100000000ull, p.err);
             }
             __syncwarp();
-        } else if (warp == 18 && lane == 0) {
+        } else if (warp == NW + 2 && lane == 0) {
             Walker walk(p, pre, blockIdx.x);
             Piece w;
             for (bool more = true; more; ++n_piece) {
@@ -534,7 +553,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
                 const_cast<Piece *>(ring)[n_piece % NP] = w;
                 mbar_arrive(b_pf + 8 * (n_piece % NP));
             }
-        } else if (I8 && warp == 19) {
+        } else if (I8 && warp == NW + 3) {
             int n_tile = 0;
             while (const Piece *pc = next_piece()) {
                 const int own_b = pc->own_b, head = pc->h, kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
@@ -596,11 +615,11 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     } else {
         // ------------------------------------------------------------------ producers
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_LOAD));
-        const int tid = threadIdx.x - 640;
+        const int tid = threadIdx.x - 32 * (NW + 4);
         uint32_t half = 0;                      // ring index
         uint32_t tails = 0;
         int n_tile = 0;
-        while (I8 || warp == 20) {
+        while (I8 || warp == NW + 4) {
             const Piece *pc = next_piece();
             if (pc == nullptr) break;
             const int kend = pc->kend, nblk = pc->nblk, key0 = pc->kbeg + pc->blk0 * BKT;
@@ -701,7 +720,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
             if (ok) done_piece();
         }
         // every copy issued has landed before the CTA may exit (immediate on the normal path)
-        if (!I8 && warp == 20 && lane == 0) {
+        if (!I8 && warp == NW + 4 && lane == 0) {
             volatile int never = 0;
             for (uint32_t h = half >= NS ? half - NS : 0; h < half; ++h)
                 mbar_wait(b_full + 8 * (h % NS), (h / NS) & 1, &never, 100000000ull, p.err);
@@ -711,7 +730,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == NW) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }
@@ -760,8 +779,8 @@ cudaError_t launch_tc(const Params &p, cudaStream_t st) {
     memset(&tk, 0, sizeof(tk));
     memset(&tv, 0, sizeof(tv));
     if (!i8 && !(make_map(&tk, p.k, p, box) && make_map(&tv, p.v, p, box))) return cudaErrorInvalidValue;
-    if (i8) k_paged_tc<true><<<p.ctas, TC_THREADS, smem, st>>>(tk, tv, p, box);
-    else k_paged_tc<false><<<p.ctas, TC_THREADS, smem, st>>>(tk, tv, p, box);
+    if (i8) k_paged_tc<true><<<p.ctas, TC_THREADS<true>, smem, st>>>(tk, tv, p, box);
+    else k_paged_tc<false><<<p.ctas, TC_THREADS<false>, smem, st>>>(tk, tv, p, box);
     return cudaGetLastError();
 }
 
