@@ -427,21 +427,21 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
     dep_wait();             // nothing here reads what the other line writes, but the join waits for this kernel only
 }
 
-// Joins the partial results of every row (a warp takes `run` rows of a tile, one after the other): out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. `a` is the
-// line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts. 140800 rows of which a quarter are
-// cut: 47 us (a row a warp at a time, each looked up in the line: 105); 32 x 32 rows of 13 pieces: 11 us, of latency.
-__global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b, int run) {
+// Joins the partial results of every row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. A warp takes RUN rows of a tile,
+// one after the other. `a` is the line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
+// 140800 rows of which a quarter are cut: 47 us (each row looked up in the line: 105); 32 x 32 rows of 13 pieces: 11-13 us, of latency.
+template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b) {
     dep_wait();
     const int lane = threadIdx.x & 31;
-    const int rows = b.Lq * b.G, runs = (rows + run - 1) / run;      // of a sequence and K/V head
+    const int rows = b.Lq * b.G, runs = (rows + RUN - 1) / RUN;      // of a sequence and K/V head
     const int64_t items = (int64_t)b.B * b.Hkv * runs;
     const int64_t blocksA = (int64_t)a.Hkv * a.nrtA * a.nbA, aheadB = (int64_t)b.Hkv * b.nrtA * b.nbA;
     const int64_t qA = a.nbA ? Walker::quota(a, blocksA + (int64_t)a.sched[a.B] * a.Hkv) : 1;
     const int64_t qB = Walker::quota(b, aheadB + (int64_t)b.sched[b.B] * b.Hkv);
     for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
         const int64_t sh = div_nonneg(it, runs);
-        const int s = (int)div_nonneg(sh, b.Hkv), h = (int)(sh - (int64_t)s * b.Hkv), r0 = (int)(it - sh * runs) * run;
-        const int r1 = r0 + run < rows ? r0 + run : rows;
+        const int s = (int)div_nonneg(sh, b.Hkv), h = (int)(sh - (int64_t)s * b.Hkv), r0 = (int)(it - sh * runs) * RUN;
+        const int r1 = RUN == 1 || r0 + RUN < rows ? r0 + RUN : rows;
         // the own part's pieces, the same for the run's rows
         const int len = seq_length(b, s), rt = r0 / b.tb, nb = own_blocks(b, len, rt);
         const int64_t first = aheadB + (int64_t)b.sched[s] * b.Hkv +
@@ -638,7 +638,7 @@ cudaError_t launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
     int64_t grid = cdiv((int64_t)a.B * s.Hkv * cdiv((int64_t)a.Lq * s.G, run), 8);
     if (grid > (int64_t)num_sms() * 8) grid = (int64_t)num_sms() * 8;
     const bool tc_a = pl.shared_tc, tc_b = pl.own_tc;
-    return launch_after(k_paged_join, (unsigned)grid, 256, 0, st, tc_a ? t : s, tc_b ? t : s, run);
+    return launch_after(run == 1 ? k_paged_join<1> : k_paged_join<8>, (unsigned)grid, 256, 0, st, tc_a ? t : s, tc_b ? t : s);
 }
 
 } // namespace hn
