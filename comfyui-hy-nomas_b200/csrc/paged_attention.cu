@@ -13,8 +13,8 @@
 //
 // Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head): 64 sequences of about 2500
 // tokens, 8 K/V heads: bf16 126 us (5.9 TB/s), int8 118 us (3.3 TB/s: the conversion of the codes issues as much as the products).
-// With 64-row tiles by the shared-memory reads of the fragments: 32 sequences on 15840 shared tokens, 32 / 8 heads, int8: 75 us
-// and the join's 11.
+// With 64-row tiles by the shared-memory reads of the fragments: 16 x 5 queries over 4096 shared and about 1100 own tokens, 16
+// heads, bf16: 54 us and the join's 9.
 // Per warp: 16 rows; m16n8k16 products, S and O in registers. The four warps split a block's keys (16-row tiles), its
 // rows (64), or both (32). Blocks arrive by cp.async, STAGES deep; the smem chunks are permuted so that no read conflicts.
 //  - bf16 cache: K by ldmatrix, V by its transposing form, P rounded to bf16.
@@ -429,7 +429,7 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
 
 // Joins the partial results of every row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. A warp takes RUN rows of a tile,
 // one after the other. `a` is the line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
-// 140800 rows of which a quarter are cut: 47 us (each row looked up in the line: 105); 32 x 32 rows of 13 pieces: 11-13 us, of latency.
+// 140800 rows of which a quarter are cut: 47 us (each row looked up in the line: 105); small calls: 6-9 us, of latency.
 template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b) {
     dep_wait();
     const int lane = threadIdx.x & 31;
@@ -505,10 +505,14 @@ template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Par
 static int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 // CTAs of the streaming kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
 static int stream_ctas(bool i8) { return num_sms() * (i8 ? 3 : 2); }
-// Rows from which a part goes to the tensor-core line. A tile there is two groups of 128 rows over the same keys; measured, us, on
-// this line / the tensor cores: shared part of 15840 tokens, 8 heads, bf16: 128 rows 67 / 76, 256 rows 107 / 91, 512 rows 270 /
-// 92; int8 81 / 90, 141 / 105, 268 / 138. Own parts of 2000 tokens, 8 sequences, 16 heads, 100 rows: 97 / 79 and 122 / 119.
-constexpr int TC_SHARED = 129, TC_OWN = 65;
+// Rows from which a part goes to the tensor-core line. A tile there is two groups of 128 rows over the same keys, and its launch and
+// first blocks are dearer. Measured, us, on this line / the tensor cores, bf16 and int8: a shared part of 15872 tokens, 8 heads, 68
+// rows 71 / 54 and 81 / 69, 128 rows 75 / 56 and 81 / 71, and with own parts of 512 tokens 65 / 65 and 80 / 74; of 4096 tokens, 16
+// heads, 80 rows (own 1101) 58 / 68 and 68 / 69; of 1024 tokens, 96 rows 24 / 30 and 25 / 34. From 129 rows the streaming line reads
+// the keys for a third tile of 64: 256 rows on 15840 tokens 107 / 62 and 141 / 75. Own parts of 2000 tokens, 8 sequences, 16 heads,
+// 100 rows: 97 / 82 and 122 / 94.
+constexpr int TC_LONG = 8192;           // tokens: a long shared part
+constexpr int TC_SHARED = 129, TC_SHARED_LONG = 65, TC_OWN = 65;
 
 struct Plan {
     bool shared_tc, own_tc;             // which line holds which part
@@ -519,8 +523,8 @@ struct Plan {
 
 // The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_OWN rows per K/V head or
 // more walks all of its keys on the tensor-core line (it is bound by the products, and the shared pages come from L2); else
-// the rows of all sequences attend to the shared part together, on the tensor cores if there are TC_SHARED of them, and the
-// own parts stream.
+// the rows of all sequences attend to the shared part together, on the tensor cores if there are TC_SHARED of them
+// (TC_SHARED_LONG over a long part), and the own parts stream.
 static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     Plan pl;
     const bool i8 = a.cache.ks != nullptr;
@@ -536,7 +540,7 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     pl.own_tc = fits && r1 >= TC_OWN;
     // one sequence has nothing to share
     const bool split = a.shared > 0 && a.B > 1 && !pl.own_tc;
-    pl.shared_tc = fits && split && all >= TC_SHARED;
+    pl.shared_tc = fits && split && all >= (a.shared >= TC_LONG ? TC_SHARED_LONG : TC_SHARED);
     s.bk = BK; s.ctas = stream_ctas(i8);
     t.bk = 128; t.ctas = num_sms();
     Params &own = pl.own_tc ? t : s;
