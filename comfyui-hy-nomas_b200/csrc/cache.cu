@@ -6,6 +6,7 @@
 //   table   [slots][width]  page ids in order, -1 where there is none
 //   lengths [slots]         tokens held
 //   refs    [pages]         how many table entries name the page; 0 = free
+//   refused [slots]         `epoch` where the row's last extend could not be met: append leaves such a row as it is
 // New pages are the free ids in ascending order, handed to the requests in the order they are listed, so the
 // result does not depend on timing. A request that cannot be met (no page left, table row full, an id out of
 // range, a row listed twice, a child that is not empty) leaves its row as it was and adds 1 to *failed.
@@ -118,7 +119,9 @@ __global__ void __launch_bounds__(PLAN) k_extend(Meta m, const int *rows, int n,
         const int need = i < n ? needs(i, row, first) : 0;
         const int64_t at = off + block_scan(need > 0 ? need : 0, sums, &total);
         if (i < n) {
-            if (need < 0 || at + need > have) {
+            const bool met = need >= 0 && at + need <= have;
+            if (in_range(row, m.slots) && claim[row] == i) m.refused[row] = met ? 0 : m.epoch;
+            if (!met) {
                 atomicAdd(m.failed, 1);
             } else {
                 for (int j = 0; j < need; ++j) {
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(256) k_free(Meta m, const int *rows, int n) {
         const int p = atomicExch(&entry[j], -1);
         if (in_range(p, m.pages)) atomicSub(&m.refs[p], 1);
     }
-    if (threadIdx.x == 0) m.lengths[row] = 0;
+    if (threadIdx.x == 0) { m.lengths[row] = 0; m.refused[row] = 0; }
 }
 
 // fork, plan: request i gets a new page for its parent's partial last page. moves: src, dst, tokens of request i
@@ -192,6 +195,7 @@ __global__ void __launch_bounds__(PLAN) k_fork_plan(Meta m, const int *parents, 
             else {
                 if (need) m.refs[d] = 1;
                 m.lengths[c] = len;
+                m.refused[c] = 0;
             }
             src[i] = s; dst[i] = need < 0 ? -1 : d; ntok[i] = t; ok[i] = need >= 0;
         }
@@ -344,7 +348,9 @@ struct AppendParams {
     int B, n, heads;
 };
 
-// append: the last n tokens of each listed row. A warp takes the heads of one token, four K and V rows of 128 at a time
+// append: the last n tokens of each listed row. A row that its last extend refused has no room for them (its last tokens are
+// old ones), a page that several rows name is not one row's to write, and a row listed again is written by its first listing
+// alone: such tokens are left out and counted. A warp takes the heads of one token, four K and V rows of 128 at a time
 // (lanes 0-15 a K row, 16-31 the V row, 8 elements each), so that eight rows are in flight. bf16 is copied; int8 takes the
 // absmax over the 16 lanes, hn_quantize_kv's scale and codes. Measured: 2 x 4400 tokens, 16 heads, int8 31 us (3.6 TB/s of
 // reads and writes): the absmax stands between a row's load and its store.
@@ -370,13 +376,17 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p, Meta m) {
             if (h0 + i < p.heads) raw[i] = ldg_stream(src + i * hs);
         const int row = p.rows[b];
         int page = -1, at = 0;
+        bool again = false;
+        for (int i = lane; i < b; i += 32) again |= p.rows[i] == row;
         if (in_range(row, m.slots)) {
+            const int refused = m.refused[row];
             at = m.lengths[row] - p.n + t;
             const int j = at / m.page;
-            if (at >= 0 && j < m.width) page = m.table[(int64_t)row * m.width + j];
+            if (at >= 0 && j < m.width && refused != m.epoch) page = m.table[(int64_t)row * m.width + j];
             at -= j * m.page;
         }
-        if (!in_range(page, m.pages)) {          // the token has no place: extend did not (or could not) make one
+        if (in_range(page, m.pages) && m.refs[page] > 1) page = -1;
+        if (__any_sync(0xffffffffu, again) || !in_range(page, m.pages)) {          // the token has no place of its own
             if (lane == 0 && h0 == 0) atomicAdd(m.failed, p.heads);
             continue;
         }

@@ -530,6 +530,7 @@ static int cache_args(const hn_kv_cache *c, const char *what, CacheArgs &a) {
     a.k = c->k; a.v = c->v; a.ks = c->k_scale; a.vs = c->v_scale;
     a.layers = (int)c->layers; a.heads = (int)c->heads;
     a.meta.table = c->table; a.meta.lengths = c->lengths; a.meta.refs = c->refs; a.meta.failed = c->failed;
+    a.meta.refused = c->refused; a.meta.epoch = c->epoch;
     a.meta.slots = (int)c->slots; a.meta.width = (int)c->width; a.meta.pages = (int)c->pages; a.meta.page = (int)c->page;
     return HN_OK;
 }
@@ -552,7 +553,8 @@ int hn_cache_extend(const hn_kv_cache *cache, const int32_t *rows, int64_t n, in
     REQUIRE(n >= 0 && n <= MAX_REQUESTS && tokens >= 0 && tokens <= 0x3fffffff, HN_ERR_SHAPE,
             "hn_cache_extend: bad count (n=%lld tokens=%lld)", (long long)n, (long long)tokens);
     if (n == 0) return HN_OK;
-    REQUIRE(rows && ws, HN_ERR_ARG, "hn_cache_extend: null pointer");
+    REQUIRE(rows && ws && cache->refused, HN_ERR_ARG, "hn_cache_extend: null pointer");
+    REQUIRE(cache->epoch != 0, HN_ERR_ARG, "hn_cache_extend: the cache's epoch is 0");
     CHECK_DEVICE(cache->k);
     return launched(launch_cache_extend(a.meta, rows, (int)n, (int)tokens, ws, (cudaStream_t)stream), "hn_cache_extend launch");
 }
@@ -569,6 +571,8 @@ int hn_cache_append(const hn_kv_cache *cache, int64_t layer, const void *k, int6
     REQUIRE(k && v && rows, HN_ERR_ARG, "hn_cache_append: null pointer");
     REQUIRE(al16(k) && al16(v) && (k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0, HN_ERR_ALIGN,
             "hn_cache_append: k and v need 16-byte aligned rows of 128");
+    REQUIRE(cache->refused, HN_ERR_ARG, "hn_cache_append: null pointer in the cache");
+    REQUIRE(cache->epoch != 0, HN_ERR_ARG, "hn_cache_append: the cache's epoch is 0");
     CHECK_DEVICE(k);
     return launched(launch_cache_append(a, (int)layer, k, k_bs, k_ts, k_hs, v, v_bs, v_ts, v_hs, rows, (int)B, (int)n,
                                         (cudaStream_t)stream), "hn_cache_append launch");
@@ -579,7 +583,7 @@ int hn_cache_free(const hn_kv_cache *cache, const int32_t *rows, int64_t n, void
     if (int rc = cache_args(cache, "hn_cache_free", a)) return rc;
     REQUIRE(n >= 0 && n <= MAX_REQUESTS, HN_ERR_SHAPE, "hn_cache_free: bad count %lld", (long long)n);
     if (n == 0) return HN_OK;
-    REQUIRE(rows, HN_ERR_ARG, "hn_cache_free: null pointer");
+    REQUIRE(rows && cache->refused, HN_ERR_ARG, "hn_cache_free: null pointer");
     CHECK_DEVICE(cache->k);
     return launched(launch_cache_free(a.meta, rows, (int)n, (cudaStream_t)stream), "hn_cache_free launch");
 }
@@ -590,7 +594,7 @@ int hn_cache_fork(const hn_kv_cache *cache, const int32_t *parents, const int32_
     if (int rc = cache_args(cache, "hn_cache_fork", a)) return rc;
     REQUIRE(n >= 0 && n <= MAX_REQUESTS, HN_ERR_SHAPE, "hn_cache_fork: bad count %lld", (long long)n);
     if (n == 0) return HN_OK;
-    REQUIRE(parents && children && ws, HN_ERR_ARG, "hn_cache_fork: null pointer");
+    REQUIRE(parents && children && ws && cache->refused, HN_ERR_ARG, "hn_cache_fork: null pointer");
     CHECK_DEVICE(cache->k);
     return launched(launch_cache_fork(a, parents, children, (int)n, ws, (cudaStream_t)stream), "hn_cache_fork launch");
 }

@@ -100,10 +100,11 @@ cudaError_t launch_attn_merge(const MergeArgs &a, cudaStream_t st);
 cudaError_t launch_wait_flags(const uint32_t *flags, int groups, int count, int group_stride, int skip,
                               uint32_t value, uint32_t timeout_us, cudaStream_t st);
 
-// the paged K/V cache (cache.cu, paged_attention.cu): page table, lengths, reference counts, failure counter
+// the paged K/V cache (cache.cu, paged_attention.cu): page table, lengths, reference counts, failure counter; a row whose
+// refused[row] is `epoch` was not given what its last extend asked for
 struct Meta {
-    int *table, *lengths, *refs, *failed;
-    int slots, width, pages, page;
+    int *table, *lengths, *refs, *failed, *refused;
+    int slots, width, pages, page, epoch;
 };
 struct CacheArgs {
     void *k, *v;            // [layers][pages][heads][page][128], bf16, or int8 with scales

@@ -15,7 +15,8 @@ and a branch of a sequence shares its parent's full pages instead of copying the
 `rows`, `parents`, `children`, `src` and `dst` are int32 CUDA tensors (or sequences of ints, copied to the device). The
 page table, lengths and reference counts live on the device and every call is asynchronous: a request that cannot be
 met - no free page, a full table row, a row listed twice, a child that is not empty - leaves its row as it was and is counted,
-and `check()` raises if any was. Head dim 128.
+and `check()` raises if any was. `append` leaves out a row whose last `extend` was not met, so a step that found no room
+changes no token; the row goes on with its next `extend`. Head dim 128.
 """
 import ctypes
 import math
@@ -30,7 +31,8 @@ HEAD_DIM = 128
 class _Struct(ctypes.Structure):
     """hn_kv_cache of include/hynomas_b200.h."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table", "lengths", "refs", "failed")] + \
-        [(n, ctypes.c_int64) for n in ("layers", "pages", "heads", "page", "slots", "width")]
+        [(n, ctypes.c_int64) for n in ("layers", "pages", "heads", "page", "slots", "width")] + \
+        [("refused", ctypes.c_void_p), ("epoch", ctypes.c_int32)]
 
 
 class KVCache:
@@ -78,10 +80,10 @@ class KVCache:
         self.device = k.device
         n = slots * width
         self.table, self.lengths, self.refs = meta[:n].view(slots, width), meta[n:n + slots], meta[n + slots:]
-        self.failed = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self.failed, self._refused = torch.zeros(1 + slots, dtype=torch.int32, device=k.device).split([1, slots])
         p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         self._struct = _Struct(p(k), p(v), p(ks), p(vs), p(self.table), p(self.lengths), p(self.refs), p(self.failed),
-                               layers, pages, heads, page, slots, width)
+                               layers, pages, heads, page, slots, width, p(self._refused), 1)
         self._ref = ctypes.addressof(self._struct)
         self._ws_bytes = {}
 
@@ -114,7 +116,8 @@ class KVCache:
 
     def append(self, layer, k, v, rows):
         """k, v [B, n, heads, 128] bf16 (any strides in whole 16-byte steps, the last dimension contiguous) into the last n
-        tokens of the listed rows, which `extend` has made room for; once per layer."""
+        tokens of the listed rows, which `extend` has made room for; once per layer. Rows whose last `extend` was not met,
+        pages that other rows hold too and a row's listings after its first are left out and counted."""
         _lib.require_cuda(k, v)
         rows = self._ids(rows, "append")
         if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
@@ -172,6 +175,7 @@ class KVCache:
         if saved.shape != self.meta.shape or saved.dtype != torch.int32:
             raise ValueError("restore: not a saved table of this cache")
         self.meta.copy_(saved)
+        self._struct.epoch = self._struct.epoch % 0x7fffffff + 1        # what extend refused since is past
 
     def check(self):
         """Waits for the calls so far; raises if a request could not be met, and clears the count."""
@@ -179,7 +183,7 @@ class KVCache:
         if n:
             self.failed.zero_()
             raise RuntimeError(f"KVCache: {n} request(s) could not be met (no free page, a full row, a row listed twice or "
-                               "out of range, a child that is not empty, or a token without a page)")
+                               "out of range, a child that is not empty, or a token without a page of its row's own)")
 
 
 def _operand(t):

@@ -345,16 +345,20 @@ int hn_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr,
  *   k, v [layers][pages][heads][page][128]: bf16, or int8 codes with k_scale, v_scale [layers][pages][heads][page]
  *   fp32 per (token, head) (both null: bf16). page: tokens per page, a multiple of 16.
  *   table [slots][width] page ids (-1: none), lengths [slots], refs [pages] (0: free), failed [1]: requests that could
- *   not be met, added up. All device memory, one page table for all layers.
+ *   not be met, added up; refused [slots], zeros at first: rows whose last extend could not be met hold `epoch` (any number
+ *   but 0; who puts back metadata of before takes another, and those refusals are past). All device memory, one page
+ *   table for all layers.
  * New pages are the free ids, lowest first, handed out in the order of the requests. A request that cannot be met (no
  * free page, a full table row, an id out of range, a row listed twice, a child that is not empty) changes nothing but
- * *failed. `rows`, `parents`, `children`, `src`, `dst` are int32 device arrays. Nothing synchronizes.
+ * *failed and refused. `rows`, `parents`, `children`, `src`, `dst` are int32 device arrays. Nothing synchronizes.
  *
  * hn_cache_workspace: int32 words of scratch that extend / fork / compact take in `ws` for n requests.
  * hn_cache_extend: each listed row grows by `tokens`, on new pages where needed.
  * hn_cache_append: k, v [B, n, heads, 128] bf16 (strides in elements for batch, token, head; multiples of 8; the
- *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic).
- * hn_cache_free: the listed rows drop their pages and become empty.
+ *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic). Left out
+ *   and counted, `heads` for each token: rows whose last extend was refused (until an extend, free or fork into them is
+ *   met), tokens on pages that other rows hold too, tokens without a page, a row's listings after its first.
+ * hn_cache_free: the listed rows drop their pages and become empty (a row listed twice, once).
  * hn_cache_fork: children[i] (empty, listed once) becomes a copy of parents[i]: full pages are shared, the tokens of a
  *   partial last page are copied to a new page, in every layer.
  * hn_cache_compact: pages move (in every layer) so that the used ids are 0 .. n_used - 1; the table follows.
@@ -365,6 +369,8 @@ typedef struct {
     float *k_scale, *v_scale;
     int32_t *table, *lengths, *refs, *failed;
     int64_t layers, pages, heads, page, slots, width;
+    int32_t *refused;
+    int32_t epoch;
 } hn_kv_cache;
 int hn_cache_workspace(const hn_kv_cache *cache, int64_t n, int64_t *words_host);
 int hn_cache_extend(const hn_kv_cache *cache, const int32_t *rows, int64_t n, int64_t tokens, int32_t *ws, void *stream);

@@ -108,3 +108,32 @@ def test_branches_of_one_history(hn, cuda, kind):
         want = plain(hn, dec, x, torch.arange(past + steps, device=cuda))
         assert float((first.double() - want[:past]).norm() / want[:past].norm()) < 0.1
         assert float((got[b].double() - want[past:]).norm() / want[past:].norm()) < 0.1
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_step_without_room_keeps_the_history(hn, cuda, kind):
+    """Two branches of a whole-page history and a pool with one free page: the second branch's step is counted, and the shared
+    pages hold what they held. With room it goes on where it was."""
+    from hy_nomas_b200 import paged
+    from test_gpu_paged import bits
+    dec = build(hn, cuda)
+    cache = paged.KVCache(len(dec.layers), 4, KV, 16, 4, 4, kind)
+    history = torch.randn((1, 48, HIDDEN), device=cuda).to(torch.bfloat16)
+    dec.step(history, *tables(torch.arange(48, device=cuda), cuda), cache, [0])
+    cache.fork([0, 0], [1, 2])
+    pools = [t for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+    before = [t[:, :3].clone() for t in pools]
+    x = torch.randn((2, 1, HIDDEN), device=cuda).to(torch.bfloat16)
+    at = tables(torch.full((2,), 48, device=cuda), cuda)
+    dec.step(x, *at, cache, [1, 2], shared=48)
+    with pytest.raises(RuntimeError, match="could not be met"):
+        cache.check()
+    assert cache.lengths.tolist() == [48, 49, 48, 0]
+    assert all(torch.equal(bits(t[:, :3]), bits(was)) for t, was in zip(pools, before))
+    cache.free([1])
+    got, _, _ = dec.step(x[1:], *(t[1:] for t in at), cache, [2])
+    cache.check()
+    fresh = paged.KVCache(len(dec.layers), 4, KV, 16, 4, 4, kind)
+    dec.step(history, *tables(torch.arange(48, device=cuda), cuda), fresh, [0])
+    want, _, _ = dec.step(x[1:], *(t[1:] for t in at), fresh, [0])
+    assert torch.equal(got, want)

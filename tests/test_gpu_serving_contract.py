@@ -1,0 +1,126 @@
+"""What the paged cache and its attention promise where a call meets a limit: rows without room, rows listed twice, shared parts
+that nobody holds, numbers that are not finite, views that overlap. The bounds of attention are test_gpu_paged's."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import D, Model, bits, check_attention, filled, place
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def paged(hn):
+    from hy_nomas_b200 import paged
+    return paged
+
+
+def tokens(b, n, heads, device, seed=0):
+    g = torch.Generator(device=device).manual_seed(seed)
+    return [torch.randn((b, n, heads, D), generator=g, device=device).to(torch.bfloat16) for _ in range(2)]
+
+
+# ------------------------------------------------------------------------------------- append without room
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_append_after_a_refused_extend_writes_nothing(paged, hn, cuda, kind):
+    """No page is left: two branches of a whole-page history, and a row on pages of its own, keep every byte."""
+    c = filled(paged, 2, 6, 2, 16, 4, 8, kind, seed=1)
+    c.extend([0], 32)
+    c.fork([0, 0], [1, 2])
+    c.extend([3], 64)
+    m = Model(c)
+    c.extend([1, 2], 1)
+    m.extend([1, 2], 1)
+    k, v = tokens(2, 1, 2, cuda)
+    for layer in range(2):
+        c.append(layer, k, v, [1, 2])
+    c.extend([3], 16)
+    m.extend([3], 16)
+    k, v = tokens(1, 16, 2, cuda)
+    c.append(0, k, v, [3])
+    m.failed += 2 * 2 * 2 + 16 * 2
+    assert m.failed == 3 + 40
+    m.same_as(c)
+    with pytest.raises(RuntimeError, match="could not be met"):
+        c.check()
+    # room again: the row that is extended is written, the other still is not
+    c.free([3])
+    c.extend([1], 1)
+    page, before = int(c.table[1, 2]), c.k.clone()
+    k, v = tokens(2, 1, 2, cuda, 1)
+    c.append(1, k, v, [1, 2])
+    assert int(c.failed) == 2
+    if kind == "bf16":
+        before[1, page, :, 0] = k[0, 0]
+    else:
+        before[1, page, :, 0] = hn.world.quantize_kv(k[0])[0][0]
+    assert torch.equal(bits(c.k), bits(before))
+
+
+def test_append_goes_on_after_free_fork_and_restore(paged, cuda):
+    """A refusal ends with the row's next extend, free or fork, and with a table that is put back."""
+    c = filled(paged, 1, 3, 1, 16, 3, 4, "bf16", seed=2)
+    c.extend([0], 20)
+    saved = c.save()
+    k, v = tokens(1, 1, 1, cuda)
+
+    def refuse():
+        c.extend([0], 40)
+        c.append(0, k, v, [0])
+        with pytest.raises(RuntimeError, match="could not be met"):
+            c.check()
+    refuse()
+    c.extend([0], 0)
+    c.append(0, k, v, [0])
+    c.check()
+    refuse()
+    c.restore(saved)
+    c.append(0, k, v, [0])
+    c.check()
+    refuse()
+    c.fork([0], [1])
+    c.append(0, k, v, [1])
+    c.check()
+    c.free([0, 1])
+    c.extend([2], 40)
+    c.extend([1], 16)                                    # refused: row 1 is empty, the pool is not
+    assert int(c.failed) == 1
+    c.failed.zero_()
+    c.free([2])
+    c.extend([0], 5)
+    c.fork([0], [1])                                     # a child that was refused while it was empty
+    c.append(0, k, v, [1])
+    c.check()
+
+
+def test_append_leaves_shared_pages_alone(paged, cuda):
+    """Without an extend the last tokens of a branch of whole pages are its parent's as well."""
+    c = filled(paged, 1, 4, 2, 16, 3, 4, "bf16", seed=3)
+    c.extend([0], 32)
+    c.fork([0], [1])
+    m = Model(c)
+    k, v = tokens(1, 3, 2, cuda)
+    c.append(0, k, v, [1])
+    m.failed = 6
+    m.same_as(c)
+    c.free([1])
+    c.append(0, k, v, [0])                               # its own again
+    assert torch.equal(c.k[0, int(c.table[0, 1]), :, 13:].transpose(0, 1), k[0])
+
+
+@pytest.mark.parametrize("n,b", [(1, 3), (40, 70)])
+def test_append_takes_a_row_once(paged, cuda, n, b):
+    """A row listed again: the first listing is written, the others are counted."""
+    c = filled(paged, 1, 2 * b * -(-n // 16) + 2, 2, 16, b, -(-n // 16) + 1, "bf16", seed=4)
+    rows = list(range(b))
+    c.extend(rows, n)
+    listed = rows + [b - 1, 0]
+    k, v = tokens(b + 2, n, 2, cuda)
+    c.append(0, k, v, listed)
+    assert int(c.failed) == 2 * n * 2
+    c.failed.zero_()
+    for r in rows:
+        pos = torch.arange(n, device=cuda)
+        assert torch.equal(c.v[0, c.table[r][pos // 16].long(), :, pos % 16], v[r])
