@@ -262,8 +262,11 @@ def add_rmsnorm_quant(x, residual, weight, eps=1e-6, kind="fp8", per_token=False
     w = weight if weight.is_contiguous() and not weight.data_ptr() % 16 else _lib.dense(weight)
     rows = x2.shape[0]
     if out is None:
-        total = torch.empty_like(x) if plain else torch.empty(shape, dtype=bf16, device=device)
+        # dense rows in x2's order: x may be a permuted view, whose strides empty_like(x) would keep
+        total = torch.empty_like(x2) if plain else torch.empty((rows, d), dtype=bf16, device=device)
         o2, ldo = total, d
+        if x.dim() != 2:
+            total = total.view(shape)
     else:
         if out.shape != shape or out.dtype != bf16 or out.device != device:
             raise ValueError(f"add_rmsnorm_quant: out must be a bf16 {tuple(shape)} tensor on {device}")

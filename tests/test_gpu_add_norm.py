@@ -80,6 +80,21 @@ def test_views_and_in_place(hn, cuda):
     assert hn.fused.add_rmsnorm_quant(x[:0], r[:0], w)[1].shape == (0, 512)
 
 
+@pytest.mark.parametrize("kind,per_token", [("fp8", False), ("int8", False), ("int8", True)])
+def test_permuted_inputs(hn, cuda, kind, per_token):
+    """Dense tensors whose dimensions are stored in another order (tokens first): the sum's rows are the inputs' rows."""
+    x, r, w = data(30, 256, cuda, 7)
+    x, r = x.view(5, 3, 2, 256), r.view(5, 3, 2, 256)
+    for order in ((1, 0, 2, 3), (2, 1, 0, 3), (1, 2, 0, 3)):
+        a, b = x.permute(order), r.permute(order)
+        want = hn.fused.add_rmsnorm_quant(a.contiguous(), b.contiguous(), w, kind=kind, per_token=per_token)
+        for u, v in ((a, b), (a.contiguous(), b), (a, b.contiguous())):
+            got = hn.fused.add_rmsnorm_quant(u, v, w, kind=kind, per_token=per_token)
+            assert got[0].shape == a.shape and torch.equal(got[0], want[0])
+            assert torch.equal(got[1].view(torch.uint8), want[1].view(torch.uint8)) and torch.equal(got[2], want[2])
+            check(a.reshape(-1, 256), b.reshape(-1, 256), w, 1e-6, kind, per_token, got[0].reshape(-1, 256), *got[1:])
+
+
 def test_zeros_nan_and_infinity(hn, cuda):
     x, r, w = data(4, 256, cuda, 2)
     x[0], r[0] = 0, 0
