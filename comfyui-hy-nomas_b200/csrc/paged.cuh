@@ -113,10 +113,17 @@ __device__ __forceinline__ void prefix_blocks(const Params &p, int *pre, int *su
     __syncthreads();
 }
 
-// Walks the pieces of one CTA. Every warp role of a CTA walks them in step, each with its own walker.
+// Walks the pieces of one CTA. `lead`: the sequence whose table the shared pages are looked up in; where it holds fewer than
+// `shared` tokens nobody holds the rest, and the shared part ends where it does.
 struct Walker {
     int64_t x, end, blocksA;
-    __device__ __forceinline__ Walker(const Params &p, const int *pre, int cta) {
+    int shared;
+    __device__ __forceinline__ Walker(const Params &p, const int *pre, int lead, int cta) {
+        shared = 0;
+        if (p.nbA) {
+            const int len = seq_length(p, lead);
+            shared = len < p.shared ? len : p.shared;
+        }
         blocksA = (int64_t)p.Hkv * p.nrtA * p.nbA;
         const int64_t total = blocksA + (int64_t)pre[p.B] * p.Hkv;
         const int64_t q = quota(p, total);
@@ -136,7 +143,7 @@ struct Walker {
             w.own_b = -1;
             w.h = tile / p.nrtA;
             w.row0 = (tile - w.h * p.nrtA) * p.ta;
-            w.kbeg = 0; w.kend = p.shared;
+            w.kbeg = 0; w.kend = shared;
             w.blk0 = (int)(x - (int64_t)tile * p.nbA);
             tile_end = (int64_t)(tile + 1) * p.nbA;
         } else {

@@ -416,7 +416,7 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
     prefix_blocks(p, pre, sums, &lead, THREADS);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= p.B; b += THREADS) p.sched[b] = pre[b];
-    Walker walk(p, pre, blockIdx.x);
+    Walker walk(p, pre, (int)lead, blockIdx.x);
     Piece w;
     while (walk.next(p, pre, blockIdx.x, w)) {
         const int rows_per = w.own_b < 0 ? p.ta : p.tb;

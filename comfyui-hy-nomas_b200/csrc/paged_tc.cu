@@ -545,7 +545,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
             }
             __syncwarp();
         } else if (warp == NW + 2 && lane == 0) {
-            Walker walk(p, pre, blockIdx.x);
+            Walker walk(p, pre, (int)*lead, blockIdx.x);
             Piece w;
             for (bool more = true; more; ++n_piece) {
                 if (!mbar_wait(b_pe + 8 * (n_piece % NP), ((n_piece / NP) & 1) ^ 1, abort_flag, WAIT_NS, p.err)) break;
@@ -638,13 +638,15 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                     const int id = lane < groups && kk < kend && pg < p.width ? tab[pg] : -1;
                     const bool here = (unsigned)id < (unsigned)p.pages;
                     const uint32_t bytes = 256u * box * __popc(__ballot_sync(0xffffffffu, here));
+                    // groups of the step before the end whose page id is none: zeros, as on the streaming line
+                    const uint32_t gone = __ballot_sync(0xffffffffu, lane < groups && kk < kend && !here);
                     const int left = max(kend - k0, 0);         // rows of the step that are there
 #pragma unroll 1
                     for (int kv = 0; kv < 2; ++kv, ++half) {
                         const uint32_t slot = half % NS;
                         ok = warp_wait(lane, b_empty + 8 * slot, ((half / NS) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
                         if (!ok) break;
-                        const bool tail = kv == 1 && left < STEP;
+                        const bool tail = (kv == 1 && left < STEP) || gone;
                         const uint32_t bar = tail ? b_tail : b_full + 8 * slot, dst = sb + OFF_KV + slot * KTILE;
                         if (lane == 0) mbar_arrive_tx(bar, bytes);
                         __syncwarp();
@@ -657,8 +659,9 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                             ok = warp_wait(lane, b_tail, tails & 1, abort_flag, WAIT_NS, p.err);
                             ++tails;
                             if (!ok) break;
-                            for (int r = left; r < STEP; ++r)
-                                if (lane < 16) sts16(dst + chunk_at<KHALF>(r, lane), 0, 0, 0, 0);
+                            for (int r = gone ? 0 : left; r < STEP; ++r)
+                                if (lane < 16 && ((kv == 1 && r >= left) || (gone >> (r / box) & 1)))
+                                    sts16(dst + chunk_at<KHALF>(r, lane), 0, 0, 0, 0);
                             fence_async();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(b_full + 8 * slot);

@@ -124,3 +124,64 @@ def test_append_takes_a_row_once(paged, cuda, n, b):
     for r in rows:
         pos = torch.arange(n, device=cuda)
         assert torch.equal(c.v[0, c.table[r][pos // 16].long(), :, pos % 16], v[r])
+
+
+# ------------------------------------------------------------------------------------------- shared parts
+
+@pytest.mark.parametrize("heads", [4, 64])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_shared_part_that_nobody_holds_in_full(paged, cuda, kind, heads):
+    """Three rows of 0, 20 and 37 tokens with 128 declared as shared: NaN past their ends, in every free page and in what an
+    earlier call left in shared memory reaches nobody (64 heads on one: the tensor cores)."""
+    c = filled(paged, 1, 40, 1, 16, 6, 12, kind, seed=8)
+    q = torch.randn((3, 1, heads, D), device=cuda).to(torch.bfloat16)
+    pools = [c.k, c.v] if kind == "bf16" else [c.k_scale, c.v_scale]
+    kept = [t.clone() for t in pools]
+    c.extend([0], 160)
+    for t in pools:
+        t.fill_(math.nan)
+    paged.attention(q, c, 0, [0, 0, 0], shared=128)
+    for t, was in zip(pools, kept):
+        t.copy_(was)
+    c.free([0])
+    c.extend([1], 37)
+    c.table[2, :2] = c.table[1, :2]
+    c.lengths[2] = 20
+    hidden = torch.ones(c.pages, c.page, dtype=torch.bool, device=cuda)
+    pos = torch.arange(37, device=cuda)
+    hidden[c.table[1][pos // 16].long(), pos % 16] = False
+    for t in pools:
+        t[hidden[None, :, None, :].expand(1, c.pages, 1, 16)] = math.nan
+    for rows in ([1, 2, 3], [3, 2, 1]):
+        for causal in (True, False):
+            out, lse = paged.attention(q, c, 0, rows, shared=128, causal=causal, return_lse=True)
+            check_attention(c, 0, q, rows, out, lse, causal, 1 / math.sqrt(D))
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+@pytest.mark.parametrize("shared", [0, 64])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_tokens_without_a_page_are_zeros(paged, cuda, kind, heads, shared):
+    """Ids out of range in a table, on both lines: as if the page held zeros, whatever shared memory held before."""
+    c = filled(paged, 1, 40, 1, 16, 3, 12, kind, seed=31)
+    place(c, [150, 131], seed=32, shared=shared)
+    q = torch.randn((2, 1, heads, D), device=cuda).to(torch.bfloat16)
+    pools = [c.k, c.v] if kind == "bf16" else [c.k_scale, c.v_scale]
+    kept = [t.clone() for t in pools]
+    for t in pools:
+        t.fill_(math.nan)
+    paged.attention(q, c, 0, [0, 1], shared=shared)
+    for t, was in zip(pools, kept):
+        t.copy_(was)
+    zero = next(p for p in range(c.pages) if int(c.refs[p]) == 0)
+    c.k[:, zero], c.v[:, zero] = 0, 0
+    if kind == "int8":
+        c.k_scale[:, zero], c.v_scale[:, zero] = 0, 0
+    gone = ((0, 1, -1), (0, 6, 1 << 30), (1, 1, -1), (1, 8, c.pages))
+    for r, j, bad in gone:
+        c.table[r, j] = zero
+    want = paged.attention(q, c, 0, [0, 1], shared=shared)
+    for r, j, bad in gone:
+        c.table[r, j] = bad
+    got = paged.attention(q, c, 0, [0, 1], shared=shared)
+    assert torch.equal(bits(got), bits(want))
