@@ -158,6 +158,20 @@ def test_shared_part_that_nobody_holds_in_full(paged, cuda, kind, heads):
             check_attention(c, 0, q, rows, out, lse, causal, 1 / math.sqrt(D))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("rows,shared,own", [(72, 8192, [5, 0, 40]), (100, 8256, [64, 1, 130, 0]), (128, 8704, [9] * 4)])
+def test_long_shared_part_of_half_a_tile(paged, cuda, kind, rows, shared, own):
+    """65 to 128 rows over 8192 shared tokens and more."""
+    b = len(own)
+    heads, kv = rows // b, 1
+    lens = [shared + n for n in own]
+    c = filled(paged, 1, shared // 64 + sum(-(-n // 64) for n in own) + 2, kv, 64, b, -(-max(lens) // 64) + 1, kind, seed=9)
+    place(c, lens, seed=10, shared=shared)
+    q = torch.randn((b, 1, heads, D), device=cuda).to(torch.bfloat16)
+    out, lse = paged.attention(q, c, 0, list(range(b)), shared=shared, return_lse=True)
+    check_attention(c, 0, q, list(range(b)), out, lse, True, 1 / math.sqrt(D))
+
+
 @pytest.mark.parametrize("heads", [4, 64])
 @pytest.mark.parametrize("shared", [0, 64])
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
