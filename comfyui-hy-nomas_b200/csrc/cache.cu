@@ -28,27 +28,27 @@ constexpr int HD = 128;
 __device__ __forceinline__ bool in_range(int x, int n) { return (unsigned)x < (unsigned)n; }
 
 // exclusive prefix sum of one value per thread over the planning CTA; *total gets the sum
-__device__ __forceinline__ int block_scan(int v, int *warp_sums, int *total) {
+template <typename T> __device__ __forceinline__ T block_scan(T v, T *warp_sums, T *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    T x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int w = warp_sums[lane];
+        T w = warp_sums[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            const T y = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += y;
         }
         warp_sums[lane] = w;
     }
     __syncthreads();
-    const int base = warp ? warp_sums[warp - 1] : 0;
+    const T base = warp ? warp_sums[warp - 1] : 0;
     *total = warp_sums[31];
     __syncthreads();
     return base + x - v;
@@ -91,6 +91,7 @@ __device__ void claim_rows(const int *rows, int n, int slots, int *claim) {
 // extend: every listed row grows by `tokens`, on new pages where its last one is full
 __global__ void __launch_bounds__(PLAN) k_extend(Meta m, const int *rows, int n, int tokens, int *ws) {
     __shared__ int sums[32];
+    __shared__ int64_t wide[32];            // 1024 requests may want more than 2^31 pages, though there are not so many
     int *claim = ws, *list = ws + m.slots;
     claim_rows(rows, n, m.slots, claim);
     // the pages that all requests need; a request without a row, or past the row's end, needs none and fails
@@ -105,19 +106,21 @@ __global__ void __launch_bounds__(PLAN) k_extend(Meta m, const int *rows, int n,
     int want = 0;
     for (int base = 0; base < n; base += PLAN) {
         const int i = base + threadIdx.x;
-        int row, first, total;
+        int row, first;
+        int64_t total;
         const int need = i < n ? needs(i, row, first) : 0;
-        block_scan(need > 0 ? need : 0, sums, &total);
-        want = total > m.pages - want ? m.pages : want + total;     // no more than there are
+        block_scan<int64_t>(need > 0 ? need : 0, wide, &total);
+        want = total > m.pages - want ? m.pages : want + (int)total;     // no more than there are
     }
     const int have = free_pages(m.refs, m.pages, want, list, sums);
     __syncthreads();
     int64_t off = 0;
     for (int base = 0; base < n; base += PLAN) {
         const int i = base + threadIdx.x;
-        int row = 0, first = 0, total;
+        int row = 0, first = 0;
+        int64_t total;
         const int need = i < n ? needs(i, row, first) : 0;
-        const int64_t at = off + block_scan(need > 0 ? need : 0, sums, &total);
+        const int64_t at = off + block_scan<int64_t>(need > 0 ? need : 0, wide, &total);
         if (i < n) {
             const bool met = need >= 0 && at + need <= have;
             if (in_range(row, m.slots) && claim[row] == i) m.refused[row] = met ? 0 : m.epoch;

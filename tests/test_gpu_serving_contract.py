@@ -126,6 +126,16 @@ def test_append_takes_a_row_once(paged, cuda, n, b):
         assert torch.equal(c.v[0, c.table[r][pos // 16].long(), :, pos % 16], v[r])
 
 
+# ------------------------------------------------------------------------------------------- what extend and fork hand out
+
+def test_extend_counts_pages_past_31_bits(paged, cuda):
+    """1024 rows that want 2^22 pages each, of a pool of four."""
+    c = paged.KVCache(1, 4, 1, 16, 1024, 1 << 22)
+    c.extend(torch.arange(1024, dtype=torch.int32, device=cuda), 1 << 26)
+    assert int(c.failed) == 1024 and int(c.refs.sum()) == 0 and int(c.lengths.abs().sum()) == 0
+    assert int(c.table[:, :4].max()) == -1
+
+
 # ------------------------------------------------------------------------------------------- shared parts
 
 @pytest.mark.parametrize("heads", [4, 64])
