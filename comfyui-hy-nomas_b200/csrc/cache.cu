@@ -172,7 +172,9 @@ __global__ void __launch_bounds__(PLAN) k_fork_plan(Meta m, const int *parents, 
         if (m.lengths[c] != 0 || m.table[(int64_t)c * m.width] >= 0) return -1;
         len = m.lengths[a];
         if (len < 0 || (int64_t)len > (int64_t)m.width * m.page) return -1;
-        return len % m.page ? 1 : 0;
+        if (len % m.page == 0) return 0;
+        // a tail without a page cannot be copied: the request takes none of the free ones
+        return in_range(m.table[(int64_t)a * m.width + len / m.page], m.pages) ? 1 : -1;
     };
     const int have = free_pages(m.refs, m.pages, n < m.pages ? n : m.pages, list, sums);
     __syncthreads();
@@ -189,7 +191,6 @@ __global__ void __launch_bounds__(PLAN) k_fork_plan(Meta m, const int *parents, 
                     d = list[at];
                     s = m.table[(int64_t)a * m.width + len / m.page];
                     t = len % m.page;
-                    if (!in_range(s, m.pages)) need = -1;
                 } else {
                     need = -1;
                 }

@@ -136,6 +136,17 @@ def test_extend_counts_pages_past_31_bits(paged, cuda):
     assert int(c.table[:, :4].max()) == -1
 
 
+def test_fork_of_a_broken_parent_takes_no_page(paged, cuda):
+    """A parent whose last page is not there is refused; the page it would have taken goes to the next request."""
+    c = filled(paged, 1, 3, 1, 16, 4, 2, "bf16", seed=6)
+    c.extend([0], 5)
+    c.extend([1], 5)
+    c.table[0, 0] = -1
+    c.fork([0, 1], [2, 3])
+    assert int(c.failed) == 1 and c.lengths.tolist() == [5, 5, 0, 5]
+    assert int(c.table[3, 0]) == 2
+
+
 # ------------------------------------------------------------------------------------------- shared parts
 
 @pytest.mark.parametrize("heads", [4, 64])
