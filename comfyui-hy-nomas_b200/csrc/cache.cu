@@ -88,7 +88,8 @@ __device__ void claim_rows(const int *rows, int n, int slots, int *claim) {
     __syncthreads();
 }
 
-// extend: every listed row grows by `tokens`, on new pages where its last one is full
+// extend: every listed row grows by `tokens`, on new pages where its last one is full. Served in the order listed, up to the
+// first request that there are not enough pages for: `at` counts that one too, so all after it are refused
 __global__ void __launch_bounds__(PLAN) k_extend(Meta m, const int *rows, int n, int tokens, int *ws) {
     __shared__ int sums[32];
     __shared__ int64_t wide[32];            // 1024 requests may want more than 2^31 pages, though there are not so many

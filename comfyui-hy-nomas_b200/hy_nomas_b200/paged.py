@@ -106,7 +106,8 @@ class KVCache:
         return torch.empty(words, dtype=torch.int32, device=self.device)
 
     def extend(self, rows, tokens):
-        """Every listed row grows by `tokens` tokens, on new pages (lowest free ids first, in the order listed)."""
+        """Every listed row grows by `tokens` tokens, on new pages (lowest free ids first, in the order listed). The first row
+        that there are not enough pages for is refused, and so is every row listed after it."""
         rows = self._ids(rows, "extend")
         if tokens < 0:
             raise ValueError(f"extend: {tokens} tokens")

@@ -353,7 +353,9 @@ int hn_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr,
  * *failed and refused. `rows`, `parents`, `children`, `src`, `dst` are int32 device arrays. Nothing synchronizes.
  *
  * hn_cache_workspace: int32 words of scratch that extend / fork / compact take in `ws` for n requests.
- * hn_cache_extend: each listed row grows by `tokens`, on new pages where needed.
+ * hn_cache_extend: each listed row grows by `tokens`, on new pages where needed. Requests are served in the order listed, up to
+ *   the first that there are not enough free pages for: it and every request after it in the call (one that needs no page,
+ *   too) are refused, so a later row never takes the pages that an earlier one waits for.
  * hn_cache_append: k, v [B, n, heads, 128] bf16 (strides in elements for batch, token, head; multiples of 8; the
  *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic). Left out
  *   and counted, `heads` for each token: rows whose last extend was refused (until an extend, free or fork into them is

@@ -128,6 +128,25 @@ def test_append_takes_a_row_once(paged, cuda, n, b):
 
 # ------------------------------------------------------------------------------------------- what extend and fork hand out
 
+def test_extend_serves_in_order_up_to_the_first_shortage(paged, cuda):
+    """A request that does not find its pages ends the call for those after it, whatever they need; listed first, they are met."""
+    c = filled(paged, 1, 4, 1, 16, 4, 8, "bf16", seed=5)
+    for row, n in ((1, 15), (2, 1), (3, 16)):
+        c.extend([row], n)
+
+    def state(failed, lengths):
+        assert int(c.failed) == failed and c.lengths.tolist() == lengths
+        c.failed.zero_()
+    c.extend([0, 1], 17)                                 # two pages and one, of one
+    state(2, [0, 15, 1, 16])
+    c.extend([1, 0], 17)
+    state(1, [0, 32, 1, 16])
+    c.extend([3, 2], 15)                                 # one page and none, of none
+    state(2, [0, 32, 1, 16])
+    c.extend([2, 3], 15)
+    state(1, [0, 32, 16, 16])
+
+
 def test_extend_counts_pages_past_31_bits(paged, cuda):
     """1024 rows that want 2^22 pages each, of a pool of four."""
     c = paged.KVCache(1, 4, 1, 16, 1024, 1 << 22)
