@@ -13,21 +13,6 @@
 namespace hn {
 namespace addnorm {
 
-__device__ __forceinline__ float nanmax_abs3(float m, float a, float b) {
-    float r;
-    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float nanmax(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-template <int W> __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-    for (int o = 1; o < W; o <<= 1) v = nanmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 // absmax -> scale; a zero group has scale 1 (int8), a NaN stays a NaN
 template <int KIND> __device__ __forceinline__ float scale_of(float peak) {
     if (KIND == 0) return peak == 0.0f ? 1.0f : __fdiv_rn(peak, 127.0f);

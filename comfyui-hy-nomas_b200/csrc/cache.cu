@@ -409,10 +409,11 @@ __global__ void __launch_bounds__(256) k_append(AppendParams p, Meta m) {
                 for (int j = 0; j < 4; ++j) {
                     v[2 * j] = bf16_lo(w[j]);
                     v[2 * j + 1] = bf16_hi(w[j]);
-                    peak = absmax3(peak, v[2 * j], v[2 * j + 1]);
+                    peak = nanmax_abs3(peak, v[2 * j], v[2 * j + 1]);
                 }
-                peak = warp_max_xor(peak, 16);
-                const float sc = i8_scale_bf16(peak);
+                peak = lanes_max<16>(peak);
+                // a NaN or an infinity in the row: its scale is NaN, so that what reads it gives NaN
+                const float sc = peak < INFINITY ? i8_scale_bf16(peak) : __int_as_float(0x7fffffff);
                 const bool fast = sc >= 0x1p-90f;
                 *reinterpret_cast<uint2 *>(pool + to * HD + 8 * sub) =
                     quant_chunk8<0, false>(v, sc, fast, x2_splat(-sc), x2_splat(__frcp_rn(sc)));

@@ -356,6 +356,22 @@ __device__ __forceinline__ float absmax3(float m, float a, float b) {
     asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
     return r;
 }
+// ... and maxima that a NaN stays in; lanes_max: over W neighbouring lanes
+__device__ __forceinline__ float nanmax_abs3(float m, float a, float b) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float nanmax(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+template <int W> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v = nanmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
 
 // ---------------------------------------------------------------------------------------------------
 // warp reductions

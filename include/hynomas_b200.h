@@ -357,7 +357,8 @@ int hn_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, int64_t ldr,
  *   the first that there are not enough free pages for: it and every request after it in the call (one that needs no page,
  *   too) are refused, so a later row never takes the pages that an earlier one waits for.
  * hn_cache_append: k, v [B, n, heads, 128] bf16 (strides in elements for batch, token, head; multiples of 8; the
- *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic). Left out
+ *   last dimension contiguous) become the last n tokens of rows[b] in `layer` (int8: hn_quantize_kv's arithmetic; a row of 128
+ *   with a NaN or an infinity gets a NaN scale, where hn_quantize_kv passes over a NaN). Left out
  *   and counted, `heads` for each token: rows whose last extend was refused (until an extend, free or fork into them is
  *   met), tokens on pages that other rows hold too, tokens without a page, a row's listings after its first.
  * hn_cache_free: the listed rows drop their pages and become empty (a row listed twice, once).

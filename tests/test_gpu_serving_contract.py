@@ -239,3 +239,29 @@ def test_tokens_without_a_page_are_zeros(paged, cuda, kind, heads, shared):
         c.table[r, j] = bad
     got = paged.attention(q, c, 0, [0, 1], shared=shared)
     assert torch.equal(bits(got), bits(want))
+
+
+# ------------------------------------------------------------------------------------------- scales, NaN, infinity
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_appended_nan_and_infinity_are_seen(paged, cuda, kind, bad):
+    """One such number among a token's K or V: the queries that see the token give NaN, those of other sequences do not."""
+    for which in (0, 1):
+        c = filled(paged, 1, 8, 1, 16, 2, 4, kind, seed=14)
+        c.extend([0, 1], 20)
+        kv = tokens(2, 20, 1, cuda)
+        kv[which][0, 7, 0, 33] = bad
+        c.append(0, *kv, [0, 1])
+        if kind == "int8":
+            scale = (c.k_scale, c.v_scale)[which][0, int(c.table[0, 0]), 0, 7]
+            assert not torch.isfinite(scale)
+        for lq in (1, 3, 70):
+            q = torch.ones((2, lq, 1, D), dtype=torch.bfloat16, device=cuda)
+            out = paged.attention(q, c, 0, [0, 1], causal=False)
+            if which == 0 and not (kind == "int8" or math.isnan(bad)):
+                # an infinite logit: the softmax is that token's (+) or leaves it out (-)
+                assert torch.isnan(out[0]).all() if bad > 0 else torch.isfinite(out[0]).all()
+            else:
+                assert torch.isnan(out[0]).any(-1).all() or (torch.isinf(out[0]).any(-1).all() and which == 1)
+            assert torch.isfinite(out[1]).all()
