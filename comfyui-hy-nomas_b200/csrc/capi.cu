@@ -652,6 +652,7 @@ int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, i
     REQUIRE(layer >= 0 && layer < cache->layers, HN_ERR_SHAPE, "hn_paged_attention: layer %lld of %lld", (long long)layer,
             (long long)cache->layers);
     if (B == 0 || Lq == 0) return HN_OK;
+    REQUIRE(std::isfinite(scale), HN_ERR_ARG, "hn_paged_attention: the scale is not a finite number");
     REQUIRE(q && rows && out && ws, HN_ERR_ARG, "hn_paged_attention: null pointer");
     REQUIRE(al16(q) && al16(out) && al16(ws) && (q_bs | q_ls | q_hs | o_bs | o_ls | o_hs) % 8 == 0, HN_ERR_ALIGN,
             "hn_paged_attention: q, out and ws must be 16-byte aligned, strides multiples of 8 elements");

@@ -394,8 +394,8 @@ int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *d
  * holds. A token on a page id out of range counts as one of zeros.
  * q, out [B, Lq, H, 128] bf16 (element strides for batch, query, head; multiples of 8), H a multiple of the cache's
  * heads (query heads h * H / heads .. share K/V head h), lse [B, H, Lq] fp32 natural log or NULL. rows [B] int32.
- * Scales of an int8 cache are positive, as its quantizer gives them. ws: hn_paged_attention_workspace bytes, 16-byte
- * aligned. B <= 4096.
+ * `scale` is any finite number. Scales of an int8 cache are positive, as its quantizer gives them. ws:
+ * hn_paged_attention_workspace bytes, 16-byte aligned. B <= 4096.
  */
 int hn_paged_attention_workspace(const hn_kv_cache *cache, int64_t B, int64_t Lq, int64_t H, int64_t shared, int causal,
                                  int64_t *bytes_host);

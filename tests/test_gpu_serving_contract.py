@@ -243,6 +243,26 @@ def test_tokens_without_a_page_are_zeros(paged, cuda, kind, heads, shared):
 
 # ------------------------------------------------------------------------------------------- scales, NaN, infinity
 
+@pytest.mark.parametrize("lq", [1, 130])
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_negative_scale(paged, cuda, kind, lq):
+    c = filled(paged, 1, 40, 2, 16, 2, 12, kind, seed=11)
+    place(c, [150, 131], seed=12)
+    q = torch.randn((2, lq, 4, D), device=cuda).to(torch.bfloat16)
+    for scale in (-0.2, -1e-3, 0.0):
+        out, lse = paged.attention(q, c, 0, [0, 1], scale=scale, return_lse=True)
+        check_attention(c, 0, q, [0, 1], out, lse, True, scale)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_a_scale_that_is_no_number_is_refused(paged, cuda, scale):
+    c = filled(paged, 1, 4, 1, 16, 1, 2, "bf16", seed=13)
+    c.extend([0], 5)
+    q = torch.zeros((1, 1, 2, D), dtype=torch.bfloat16, device=cuda)
+    with pytest.raises((ValueError, RuntimeError), match="scale"):
+        paged.attention(q, c, 0, [0], scale=scale)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 def test_appended_nan_and_infinity_are_seen(paged, cuda, kind, bad):
