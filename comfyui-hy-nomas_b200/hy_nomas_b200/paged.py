@@ -94,6 +94,8 @@ class KVCache:
         elif x.dtype != torch.int32:
             if x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
                 raise TypeError(f"{what}: ids must be integers, got {x.dtype}")
+            if x.element_size() >= 4:               # not modulo 2^32: what does not fit stays out of range
+                x = x.to(torch.int64).clamp(-1, 0x7fffffff)
             x = x.to(torch.int32)
         if x.device != self.device:
             raise RuntimeError(f"{what}: ids on {x.device}, the cache is on {self.device}")

@@ -166,6 +166,16 @@ def test_fork_of_a_broken_parent_takes_no_page(paged, cuda):
     assert int(c.table[3, 0]) == 2
 
 
+def test_ids_past_32_bits_are_out_of_range(paged, cuda):
+    """64-bit ids are not taken modulo 2^32: row 2^32 is not row 0."""
+    c = filled(paged, 1, 4, 1, 16, 2, 2, "bf16", seed=7)
+    c.extend([0], 20)
+    m = Model(c)
+    c.free(torch.tensor([1 << 32, -(1 << 32), (1 << 40) + 1], device=cuda))
+    m.failed = 3
+    m.same_as(c)
+
+
 # ------------------------------------------------------------------------------------------- shared parts
 
 @pytest.mark.parametrize("heads", [4, 64])
