@@ -11,6 +11,7 @@
 #include <atomic>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include <cmath>
 #include <cuda.h>
@@ -617,6 +618,22 @@ int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *d
     return launched(launch_cache_copy(a, src, dst, (int)n, (cudaStream_t)stream), "hn_cache_copy launch");
 }
 
+// rows of 128 elements at b * bs + l * ls + h * hs that do not overlap: each stride is past what the smaller ones reach (a
+// dimension of one has none)
+static bool rows_apart(int64_t B, int64_t bs, int64_t Lq, int64_t ls, int64_t H, int64_t hs) {
+    int64_t n[3] = {B, Lq, H}, s[3] = {bs < 0 ? -bs : bs, ls < 0 ? -ls : ls, hs < 0 ? -hs : hs};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2 - i; ++j)
+            if (s[j] > s[j + 1]) { std::swap(s[j], s[j + 1]); std::swap(n[j], n[j + 1]); }
+    int64_t reach = 128;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        if (s[i] < reach) return false;
+        reach += s[i] * (n[i] - 1);
+    }
+    return true;
+}
+
 // the shape checks of hn_paged_attention and of its workspace
 static int paged_args(const hn_kv_cache *cache, const char *what, int64_t B, int64_t Lq, int64_t H, int64_t shared, int causal,
                       PagedAttnArgs &a) {
@@ -656,6 +673,7 @@ int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, i
     REQUIRE(q && rows && out && ws, HN_ERR_ARG, "hn_paged_attention: null pointer");
     REQUIRE(al16(q) && al16(out) && al16(ws) && (q_bs | q_ls | q_hs | o_bs | o_ls | o_hs) % 8 == 0, HN_ERR_ALIGN,
             "hn_paged_attention: q, out and ws must be 16-byte aligned, strides multiples of 8 elements");
+    REQUIRE(rows_apart(B, o_bs, Lq, o_ls, H, o_hs), HN_ERR_SHAPE, "hn_paged_attention: the rows of out overlap");
     CHECK_DEVICE(q);
     const int64_t tokens = layer * cache->pages * cache->heads * cache->page;
     const int64_t row_bytes = cache->k_scale ? 128 : 256;

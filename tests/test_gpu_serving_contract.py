@@ -295,3 +295,22 @@ def test_appended_nan_and_infinity_are_seen(paged, cuda, kind, bad):
             else:
                 assert torch.isnan(out[0]).any(-1).all() or (torch.isinf(out[0]).any(-1).all() and which == 1)
             assert torch.isfinite(out[1]).all()
+
+
+# ------------------------------------------------------------------------------------------- outputs, errors
+
+def test_an_output_that_overlaps_itself_is_refused(paged, cuda):
+    c = filled(paged, 1, 4, 2, 16, 2, 2, "bf16", seed=17)
+    c.extend([0, 1], 20)
+    q = torch.randn((2, 3, 2, D), device=cuda).to(torch.bfloat16)
+    store = torch.zeros(4096, dtype=torch.bfloat16, device=cuda)
+    for shape, stride in (((2, 3, 2, D), (0, 256, 128)), ((2, 3, 2, D), (768, 128, 128)), ((2, 3, 2, D), (128, 256, 128)),
+                          ((2, 3, 2, D), (768, 256, 8))):
+        with pytest.raises(RuntimeError, match="out"):
+            paged.attention(q, c, 0, [0, 1], out=store.as_strided(shape, stride + (1,)))
+    want = paged.attention(q, c, 0, [0, 1])
+    for stride in ((128, 512, 256), (128, 256, 1536)):
+        got = paged.attention(q, c, 0, [0, 1], out=store.as_strided((2, 3, 2, D), stride + (1,)))
+        assert torch.equal(bits(got), bits(want))
+    one = paged.attention(q[:1, 2:], c, 0, [0], out=store.as_strided((1, 1, 2, D), (0, 0, 128, 1)))
+    assert torch.equal(bits(one), bits(want[:1, 2:]))
