@@ -181,7 +181,11 @@ class KVCache:
         self._struct.epoch = self._struct.epoch % 0x7fffffff + 1        # what extend refused since is past
 
     def check(self):
-        """Waits for the calls so far; raises if a request could not be met, and clears the count."""
+        """Waits for the calls so far on the current stream; raises if a request could not be met, and clears the count, or if
+        a kernel on this stream gave up a bounded wait (`attention` then left rows unwritten)."""
+        rc, code = _lib.device_error(torch.cuda.current_stream(self.device))
+        if rc != _lib.HN_OK or code:
+            raise RuntimeError(f"KVCache: {_lib.STATUS.get(rc, rc)}, device error word {code:#x}: {_lib.last_error()}")
         n = int(self.failed.item())
         if n:
             self.failed.zero_()

@@ -314,3 +314,14 @@ def test_an_output_that_overlaps_itself_is_refused(paged, cuda):
         assert torch.equal(bits(got), bits(want))
     one = paged.attention(q[:1, 2:], c, 0, [0], out=store.as_strided((1, 1, 2, D), (0, 0, 128, 1)))
     assert torch.equal(bits(one), bits(want[:1, 2:]))
+
+
+def test_check_reports_a_wait_that_ran_out(paged, hn, cuda):
+    """The bounded waits of the tensor-core line record where they gave up; check() tells."""
+    c = filled(paged, 1, 4, 1, 16, 1, 2, "bf16", seed=18)
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            assert hn.lib.lib.hn_selftest_wait_timeout(1000, hn.lib.stream_of(c.k)) == 0
+            with pytest.raises(RuntimeError, match="wait"):
+                c.check()
+            c.check()
