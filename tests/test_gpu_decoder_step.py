@@ -137,3 +137,27 @@ def test_step_without_room_keeps_the_history(hn, cuda, kind):
     dec.step(history, *tables(torch.arange(48, device=cuda), cuda), fresh, [0])
     want, _, _ = dec.step(x[1:], *(t[1:] for t in at), fresh, [0])
     assert torch.equal(got, want)
+
+
+def test_step_refuses_before_it_touches_the_cache(hn, cuda):
+    """A cache or inputs of another shape than the layers': an error, and the rows are as they were."""
+    from hy_nomas_b200 import paged
+    dec = build(hn, cuda)
+    x = torch.randn((2, 3, HIDDEN), device=cuda).to(torch.bfloat16)
+    cos, sin = tables(torch.arange(3, device=cuda).repeat(2), cuda)
+    for kw in (dict(layers=1), dict(heads=KV + 1)):
+        a = dict(layers=2, heads=KV)
+        a.update(kw)
+        cache = paged.KVCache(a["layers"], 8, a["heads"], 16, 4, 4)
+        with pytest.raises(ValueError):
+            dec.step(x, cos, sin, cache, [0, 1])
+        assert cache.lengths.tolist() == [0] * 4
+    cache = paged.KVCache(2, 8, KV, 16, 4, 4)
+    for args in ((x[:, :, :128], cos, sin), (x[0], cos, sin), (x.float(), cos, sin), (x, cos[:5], sin), (x, cos, sin[:, :64]),
+                 (x[:1], cos[:3], sin[:3])):
+        with pytest.raises((ValueError, TypeError)):
+            dec.step(*args, cache, [0, 1])
+    with pytest.raises(ValueError):
+        dec.step(x, cos, sin, cache, [0, 1], shared=8)
+    assert cache.lengths.tolist() == [0] * 4
+    cache.check()
