@@ -25,8 +25,9 @@
 //                of the products (K-major K, MN-major V; V rows past the end become zeros, K's are masked). bf16: TMA, one warp.
 //                int8: four warps; codes go through registers, a step ahead, and become fp16 integers (exact).
 //
-// int8: t_j = (q . ck_j) * sk_j scale log2 e, x_j = t_j 2^e (2^e: the row's power of two), P'_j = 2^(x_j - m + 12) sv_j. m is the
-// running maximum of x plus that of ceil(log2 sv), so P' <= 2^12 (fp16) and the normaliser's terms 2^(x_j - m + 12) are at hand.
+// int8, as on the streaming line: x_j = (q . ck_j) sk_j scale log2 e 2^e + log2 sv_j (2^e: the row's power of two), m the running
+// maximum of x over what the row sees, P'_j = 2^(x_j - m + 12), and the normaliser sums P'_j / sv_j: however far apart V's scales
+// are, a P' is small only where p sv is. The factor warp takes the logarithm and the reciprocal, once per key.
 // The register file is split by setmaxnreg: what each role needs without spills (with shared memory taking all of L1, a spilled
 // register comes back from L2).
 // Every mbarrier wait is bounded; on expiry the kernel records HN_DEVERR_TIMEOUT, the roles leave their loops, copies and MMAs in
@@ -57,9 +58,9 @@ template <bool I8> constexpr int SOFTMAX_WARPS = 16 / PARTS<I8>;
 template <bool I8> constexpr int TC_THREADS = 32 * (SOFTMAX_WARPS<I8> + 8);
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = 2 * TILE;
-constexpr int OFF_SC = OFF_KV + NS * KTILE;  // per block: sk scale log2 e [128], sv [128], in the fragments' order;
-                                            // the largest sv (16 B); where the 8 groups of 16 keys are (32 B)
-constexpr int SC_BYTES = BKT * 8 + 16 + 32;
+constexpr int OFF_SC = OFF_KV + NS * KTILE;  // per block: sk scale log2 e, log2 sv, 1 / sv [128] each, in the fragments' order;
+                                            // where the 8 groups of 16 keys are (32 B)
+constexpr int SC_BYTES = BKT * 12 + 32;
 constexpr int OFF_BAR = OFF_SC + NSC * SC_BYTES;
 constexpr int NP = 4;                       // pieces
 // full[NS], empty[NS], s[2][2], p[2][2], q[2], v[2][2] (of a group's steps in turn: two of them may be on their way, and a parity
@@ -275,7 +276,6 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
             fence_async();
             mbar_arrive(b_q + 8 * g);
             const int nblk = w.nblk;
-            float ev = -1000.0f;                // int8: running maximum of ceil(log2 sv), at least
             for (int k = 0; k < 2 * nblk; ++k, ++n_s) {         // steps of 64 keys
                 const int sub = k & 1, t = n_tile + (k >> 1);
                 const uint32_t tsb = ts + 64 * sub;
@@ -289,18 +289,6 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                 ok = warp_wait(lane, b_s + 16 * g + 8 * sub, (n_s >> 1) & 1, abort_flag, WAIT_NS, p.err);
                 if (!ok) break;
                 tc_fence_after();
-                bool grown = false;
-                float f = 1.0f;
-                if (I8 && sub == 0) {
-                    const float top = *reinterpret_cast<const float *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 2 * BKT * 4);
-                    // 2^e > sv: the exponent field, plus one; not below -60, so that 2^(12 - e) stays in range
-                    const float e = fmaxf((float)((int)(__float_as_uint(top) >> 23) - 126), -60.0f);
-                    if (e > ev) {               // all rows' references grow with it
-                        f = ex2(ev - e);
-                        grown = true;
-                        ev = e;
-                    }
-                }
                 uint32_t x[32 * H];             // [16-row part][8 column groups][row l / 4, l / 4 + 8][2 columns]
 #pragma unroll
                 for (int c = 0; c < 2 * H; ++c) ld_frag(tsb + ((uint32_t)(16 * (c >> 1)) << 16) + 32 * (c & 1), x + 16 * c);
@@ -309,12 +297,13 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                 if (I8) {
 #pragma unroll
                     for (int c = 0; c < 8; c += 2) {
-                        const ulonglong2 kf = factors[2 * c];
+                        const ulonglong2 kf = factors[2 * c], lv = factors[32 + 2 * c];
 #pragma unroll
                         for (int v = 0; v < 4 * H; ++v) {       // 2 column groups x the rows
                             uint32_t *y = x + 32 * (v >> 2) + 4 * (c + (v & 1)) + (v & 2);
                             float y0, y1;
-                            x2_split(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x), y0, y1);
+                            x2_split(x2_fma(x2_mul(x2(__uint_as_float(y[0]), __uint_as_float(y[1])), v & 1 ? kf.y : kf.x),
+                                            x2_splat(rsf[2 * (v >> 2) + ((v >> 1) & 1)]), v & 1 ? lv.y : lv.x), y0, y1);
                             y[0] = __float_as_uint(y0);
                             y[1] = __float_as_uint(y1);
                         }
@@ -330,7 +319,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                             x[c] = __float_as_uint(-INFINITY);
                 }
                 float mn[2 * H];
-                bool need = grown;
+                bool need = false;
 #pragma unroll
                 for (int u = 0; u < 2 * H; ++u) {
                     const uint32_t *y = x + 32 * (u >> 1) + 2 * (u & 1);
@@ -347,7 +336,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
 #pragma unroll
                 for (int u = 0; u < 2 * H; ++u) {
                     mn[u] = nan_max(mn[u], __shfl_xor_sync(0xffffffffu, mn[u], 2));
-                    mn[u] *= rsf[u];
+                    if (!I8) mn[u] *= rsf[u];
                     need |= !(mn[u] <= m[u] + STALE);           // or a NaN, which stays in the row
                 }
                 if (k == 0) {
@@ -357,7 +346,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
 #pragma unroll
                     for (int u = 0; u < 2 * H; ++u) {
                         const bool grow = !(mn[u] <= m[u] + STALE);
-                        const float al = (grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f) * f;
+                        const float al = grow ? ex2(m[u] - (mn[u] + AHEAD)) : 1.0f;
                         m[u] = grow ? mn[u] + AHEAD : m[u];
                         mn[u] = al;
                         sum[u] *= al;
@@ -379,13 +368,13 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const float ref = m[2 * hf + u] == -INFINITY ? 0.0f : m[2 * hf + u];
-                        nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ev - ref : -ref));   // an infinite maximum: NaN
+                        nref[u] = x2_splat(fmaf(ref, 0.0f, I8 ? TC_SHIFT - ref : -ref));        // an infinite maximum: NaN
                     }
 #pragma unroll
                     for (int c = 0; c < 8; c += 4) {                // 4 column groups: a store of 8 registers
                         uint64_t v[4];
                         if (I8) {
-                            const ulonglong2 f0 = factors[32 + 2 * c], f1 = factors[32 + 2 * c + 4];
+                            const ulonglong2 f0 = factors[64 + 2 * c], f1 = factors[64 + 2 * c + 4];
                             v[0] = f0.x; v[1] = f0.y; v[2] = f1.x; v[3] = f1.y;
                         }
                         uint32_t pk[8];
@@ -393,15 +382,12 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                         for (int q = 0; q < 8; ++q) {               // column group c + q / 2, row q % 2
                             const int u = q & 1;
                             const uint32_t *y = x + 32 * hf + 4 * c + 2 * q;
-                            const uint64_t a = x2_fma(x2(__uint_as_float(y[0]), __uint_as_float(y[1])),
-                                                      x2_splat(rsf[2 * hf + u]), nref[u]);
+                            const uint64_t z = x2(__uint_as_float(y[0]), __uint_as_float(y[1]));
+                            const uint64_t a = I8 ? x2_add(z, nref[u]) : x2_fma(z, x2_splat(rsf[2 * hf + u]), nref[u]);
                             float a0, a1;
                             x2_split(a, a0, a1);
-                            uint64_t e = x2(ex2(a0), ex2(a1));
-                            acc[u] = x2_add(acc[u], e);
-                            if (I8) e = x2_mul(e, v[q >> 1]);
-                            float e0, e1;
-                            x2_split(e, e0, e1);
+                            const float e0 = ex2(a0), e1 = ex2(a1);
+                            acc[u] = I8 ? x2_fma(x2(e0, e1), v[q >> 1], acc[u]) : x2_add(acc[u], x2(e0, e1));
                             pk[q] = I8 ? pack_f16_rn(e0, e1) : bf16x2_rn(e0, e1);
                         }
                         st_frag(tsb + ((uint32_t)(16 * hf) << 16) + 4 * c, pk);
@@ -441,7 +427,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                 for (int u = 0; u < 2; ++u) {
                     sum[2 * hf + u] += __shfl_xor_sync(0xffffffffu, sum[2 * hf + u], 1);
                     sum[2 * hf + u] += __shfl_xor_sync(0xffffffffu, sum[2 * hf + u], 2);
-                    const float ref = I8 ? m[2 * hf + u] + ev + (STREAM_SHIFT - TC_SHIFT) : m[2 * hf + u];
+                    const float ref = I8 ? m[2 * hf + u] + (STREAM_SHIFT - TC_SHIFT) : m[2 * hf + u];
                     const int rr = row0 + 16 * hf + 8 * u + (lane >> 2), r = w.row0 + 128 * g + rr;
                     valid[u] = r < rows_all;
                     int b = 0, l = 0, gm = 0;
@@ -598,7 +584,6 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                     ok = warp_wait(lane, b_se + 8 * (n_tile % NSC), ((n_tile / NSC) & 1) ^ 1, abort_flag, WAIT_NS, p.err);
                     if (!ok) break;
                     float *sc = reinterpret_cast<float *>(smem + OFF_SC + (n_tile % NSC) * SC_BYTES);
-                    float top = 0.0f;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         // key 8 c + 2 q + e goes to the quad's lane q, place 2 c + e of 32; four places of the four lanes in turn, so
@@ -606,12 +591,11 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                         const int key = 32 * u + lane, place = 2 * (key >> 3) + (key & 1);
                         const int to = 16 * (place >> 2) + 4 * ((key >> 1) & 3) + (place & 3);
                         sc[to] = sk[u] * p.sl2;
-                        sc[BKT + to] = sv[u];
-                        top = fmaxf(top, sv[u]);
+                        // below 2^-100 as on the other line; the reciprocal of a NaN stays a number, for the rows that do not see it
+                        sc[BKT + to] = lg2(sv[u] < 0x1p-100f ? 0x1p-100f : sv[u]);
+                        sc[2 * BKT + to] = __frcp_rn(fmaxf(sv[u], 0x1p-100f));
                     }
-                    top = warp_max_xor(top, 32);
-                    if (lane == 0) sc[2 * BKT] = top;
-                    if (lane < 8) reinterpret_cast<int *>(sc)[2 * BKT + 4 + lane] = at;
+                    if (lane < 8) reinterpret_cast<int *>(sc)[3 * BKT + lane] = at;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(b_sc + 8 * (n_tile % NSC));
                 }
@@ -675,7 +659,7 @@ template <bool I8> __global__ void __launch_bounds__(TC_THREADS<I8>, 1)
                 uint4 kreg[4], vreg[4];
                 auto fetch = [&](uint4 (&reg)[4], const uint8_t *pool, int k, int t) {
                     const int left = kend - (key0 + k * STEP) - row16;
-                    const int4 a = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 8 * BKT + 16)[k & 1];
+                    const int4 a = reinterpret_cast<const int4 *>(smem + OFF_SC + (t % NSC) * SC_BYTES + 12 * BKT)[k & 1];
                     const int at[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                     for (int it = 0; it < 4; ++it) {

@@ -297,6 +297,25 @@ def test_appended_nan_and_infinity_are_seen(paged, cuda, kind, bad):
             assert torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("spread", [20, 40])
+@pytest.mark.parametrize("lq", [3, 70, 300])
+def test_v_scales_far_apart(paged, cuda, lq, spread):
+    """int8 V scales 2^20 and 2^40 apart: large ones under keys of no weight, and in tokens that only the last query sees, take
+    nothing from the other tokens' precision."""
+    c = filled(paged, 1, 60, 1, 16, 1, 60, "int8", seed=15)
+    n = 500
+    place(c, [n], seed=16)
+    q = torch.randn((1, lq, 2, D), device=cuda).to(torch.bfloat16)
+    q[..., 0] = 20
+    at = torch.tensor([3, 200, 201, 333, n - lq // 2, n - 1], device=cuda)
+    ids = c.table[0][at // 16].long()
+    c.k[0, ids, 0, at % 16, 0] = -127
+    c.k_scale[0, ids, 0, at % 16] = 0.5
+    c.v_scale[0, ids, 0, at % 16] *= 2.0 ** spread
+    out, lse = paged.attention(q, c, 0, [0], return_lse=True)
+    check_attention(c, 0, q, [0], out, lse, True, 1 / math.sqrt(D))
+
+
 # ------------------------------------------------------------------------------------------- outputs, errors
 
 def test_an_output_that_overlaps_itself_is_refused(paged, cuda):
