@@ -251,8 +251,9 @@ template <bool I8, int RG> __device__ void run_piece(const Params &p, const Piec
                 // a scale below 2^-100 (an all but zero row) counts as 2^-100: its values then are below 2^-93
                 sv.x = sv.x < 0x1p-100f ? 0x1p-100f : sv.x;
                 sv.y = sv.y < 0x1p-100f ? 0x1p-100f : sv.y;
-                inv[n][0] = rcp(sv.x);
-                inv[n][1] = rcp(sv.y);
+                // (the reciprocal of a NaN is one of a number: the rows that see the key have the NaN in their logit, the others none)
+                inv[n][0] = rcp(fmaxf(sv.x, 0x1p-100f));
+                inv[n][1] = rcp(fmaxf(sv.y, 0x1p-100f));
                 const float l0 = lg2(sv.x), l1 = lg2(sv.y);
                 s[n][0] = fmaf(s[n][0], sk.x * rowscale[0], l0);
                 s[n][1] = fmaf(s[n][1], sk.y * rowscale[0], l1);

@@ -316,6 +316,23 @@ def test_v_scales_far_apart(paged, cuda, lq, spread):
     check_attention(c, 0, q, [0], out, lse, True, 1 / math.sqrt(D))
 
 
+@pytest.mark.parametrize("lq", [3, 20, 60, 70, 300])
+@pytest.mark.parametrize("kind,which", [("bf16", "k"), ("int8", "k"), ("int8", "v")])
+def test_nan_stays_with_the_queries_that_see_it(paged, cuda, kind, which, lq):
+    """NaN in a token's K, or in its int8 V scale, that only the last queries see: theirs is NaN, the earlier ones' bits are as without."""
+    c = filled(paged, 1, 60, 1, 16, 1, 60, kind, seed=19)
+    place(c, [500], seed=20)
+    q = torch.randn((1, lq, 1, D), device=cuda).to(torch.bfloat16)
+    clean = paged.attention(q, c, 0, [0])
+    at = 500 - 1 - lq // 3
+    pool = getattr(c, which) if kind == "bf16" else getattr(c, which + "_scale")
+    pool[0, int(c.table[0, at // 16]), 0, at % 16] = math.nan
+    out = paged.attention(q, c, 0, [0])
+    first = lq - 1 - lq // 3
+    assert torch.equal(bits(out[:, :first]), bits(clean[:, :first]))
+    assert torch.isnan(out[:, first:]).all()
+
+
 # ------------------------------------------------------------------------------------------- outputs, errors
 
 def test_an_output_that_overlaps_itself_is_refused(paged, cuda):
