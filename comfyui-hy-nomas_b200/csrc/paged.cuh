@@ -6,8 +6,9 @@
 // The tiles' blocks follow one another: shared tiles by head and row tile, then for each sequence by head and row
 // tile. CTA c of n takes blocks [c q, (c + 1) q), q = ceil(total / n): the lengths are on the device, so every CTA
 // computes the cut from them, and the join computes it again. A tile inside one CTA ends there when nothing else adds to
-// its rows; else each CTA's piece leaves fp32 sums, maximum and normaliser in slot tile + CTA (two pieces never share
-// one: along the line each cut raises the tile, the CTA, or both).
+// its rows; else each CTA's piece leaves fp32 sums, maximum and normaliser in a slot. Where whole tiles end their rows, a CTA has
+// two such pieces at most, the end of a tile in slot 2 CTA and the beginning of one in 2 CTA + 1; else every piece has one,
+// tile + CTA (two pieces never share it: along the line each cut raises the tile, the CTA, or both).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -176,7 +177,7 @@ struct Walker {
         const int64_t stop = end < tile_end ? end : tile_end;
         w.nblk = (int)(stop - x);
         const bool whole = w.blk0 == 0 && stop == tile_end && w.own_b >= 0 && p.ends;
-        w.slot = whole ? -1 : tile + cta;
+        w.slot = whole ? -1 : p.ends ? 2 * cta + (w.blk0 == 0) : tile + cta;
         x = stop;
         return true;
     }

@@ -431,7 +431,7 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
 // Joins the partial results of every row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. A warp takes RUN rows of a tile,
 // one after the other. `a` is the line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
 // 140800 rows of which a quarter are cut: 47 us (each row looked up in the line: 105); small calls: 6-9 us, of latency.
-template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Params a, const Params b) {
+template <int RUN> __global__ void __launch_bounds__(256, 2) k_paged_join(const Params a, const Params b) {
     dep_wait();
     const int lane = threadIdx.x & 31;
     const int rows = b.Lq * b.G, runs = (rows + RUN - 1) / RUN;      // of a sequence and K/V head
@@ -452,8 +452,8 @@ template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Par
         for (int r = r0; r < r1; ++r) {
             float M = -INFINITY, L = 0.0f;
             float4 acc = make_float4(0, 0, 0, 0);
-            // n pieces `step` rows apart from `at`, eight at a time: their loads go out together
-            auto add = [&](const Params &p, int64_t at, int64_t step, int n) {
+            // n pieces `step` rows apart from `at` (the first `off` further), eight at a time: their loads go out together
+            auto add = [&](const Params &p, int64_t at, int64_t step, int n, int64_t off) {
                 for (int i0 = 0; i0 < n; i0 += 8) {
                     float2 ml[8];
                     float4 x[8];
@@ -462,8 +462,9 @@ template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Par
                         ml[i] = make_float2(-INFINITY, 0.0f);
                         x[i] = make_float4(0, 0, 0, 0);
                         if (i0 + i < n) {
-                            ml[i] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (at + (i0 + i) * step));
-                            x[i] = *reinterpret_cast<const float4 *>(p.part_o + (at + (i0 + i) * step) * HD + 4 * lane);
+                            const int64_t row = at + (i0 + i) * step + (i == 0 && i0 == 0 ? off : 0);
+                            ml[i] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * row);
+                            x[i] = *reinterpret_cast<const float4 *>(p.part_o + row * HD + 4 * lane);
                         }
                     }
                     float mn = M;
@@ -487,11 +488,13 @@ template <int RUN> __global__ void __launch_bounds__(256) k_paged_join(const Par
                 const int tile = h * a.nrtA + (int)(ra / a.ta);
                 const int64_t at = (int64_t)tile * a.nbA;
                 const int c0 = (int)(at / qA), c1 = (int)((at + a.nbA - 1) / qA);
-                add(a, (int64_t)(tile + c0) * a.part_rows + (ra - (int64_t)(tile - h * a.nrtA) * a.ta), a.part_rows, c1 - c0 + 1);
+                add(a, (int64_t)(tile + c0) * a.part_rows + (ra - (int64_t)(tile - h * a.nrtA) * a.ta), a.part_rows, c1 - c0 + 1, 0);
             }
-            if (nb > 0)
-                add(b, (int64_t)(b.Hkv * b.nrtA + (s * b.Hkv + h) * b.nrtB + rt + own0) * b.part_rows + (r - rt * b.tb), b.part_rows,
-                    own1 - own0 + 1);
+            if (nb > 0) {
+                const int slot = b.ends ? 2 * own0 : b.Hkv * b.nrtA + (s * b.Hkv + h) * b.nrtB + rt + own0;
+                add(b, (int64_t)slot * b.part_rows + (r - rt * b.tb), b.ends ? 2 * b.part_rows : b.part_rows, own1 - own0 + 1,
+                    b.ends ? b.part_rows : 0);
+            }
             const int l = r / b.G, head = h * b.G + r - l * b.G;
             const float inv = inverse(L);
             uint2 y;
@@ -559,7 +562,7 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     auto slots = [&](Params &p) -> int64_t {
         p.part_rows = p.bk == 128 ? 256 : p.ta > p.tb ? p.ta : p.tb;
         const int64_t tiles = (int64_t)p.Hkv * p.nrtA + (int64_t)p.B * p.Hkv * p.nrtB;
-        return tiles ? tiles + p.ctas : 0;
+        return !tiles ? 0 : p.ends ? 2 * p.ctas : tiles + p.ctas;
     };
     pl.stream_slots = slots(s);
     pl.tc_slots = slots(t);

@@ -79,6 +79,16 @@ def test_attention_checks(hn, paged):
     assert attend(b=0) == 0 and attend(lq=0) == 0
 
 
+def test_workspace_of_calls_without_a_shared_part(hn, paged):
+    """What is left in the workspace are the tiles that the cuts between CTAs fall into: it does not grow with the queries."""
+    L = hn.lib.lib
+    n = ctypes.c_int64()
+    big = struct(paged, pages=1 << 16, page=64, width=1 << 13, slots=4096, heads=8)
+    for b, lq, h in ((2, 4400, 16), (1, 1 << 15, 64), (64, 8192, 8), (1, 1 << 16, 1 << 13), (3, 64, 8), (1000, 1, 64)):
+        assert L.hn_paged_attention_workspace(ref(big), b, lq, h, 0, 1, ctypes.byref(n)) == 0
+        assert n.value <= 2 * 148 * 256 * 130 * 4 + 2 * 4 * (b + 1), (b, lq, h, n.value)
+
+
 def test_norm_checks(hn):
     L = hn.lib.lib
 
