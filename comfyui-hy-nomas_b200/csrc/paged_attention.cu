@@ -509,14 +509,20 @@ template <int RUN> __global__ void __launch_bounds__(256, 2) k_paged_join(const 
 static int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 // CTAs of the streaming kernel: what fits an SM by shared memory (bf16 98 KB -> 2, int8 70 KB -> 3), times the SMs
 static int stream_ctas(bool i8) { return num_sms() * (i8 ? 3 : 2); }
-// Rows from which a part goes to the tensor-core line. A tile there is two groups of 128 rows over the same keys, and its launch and
-// first blocks are dearer. Measured, us, on this line / the tensor cores, bf16 and int8: a shared part of 15872 tokens, 8 heads, 68
-// rows 71 / 54 and 81 / 69, 128 rows 75 / 56 and 81 / 71, and with own parts of 512 tokens 65 / 65 and 80 / 74; of 4096 tokens, 16
-// heads, 80 rows (own 1101) 58 / 68 and 68 / 69; of 1024 tokens, 96 rows 24 / 30 and 25 / 34. From 129 rows the streaming line reads
-// the keys for a third tile of 64: 256 rows on 15840 tokens 107 / 62 and 141 / 75. Own parts of 2000 tokens, 8 sequences, 16 heads,
-// 100 rows: 97 / 82 and 122 / 94.
-constexpr int TC_LONG = 8192;           // tokens: a long shared part
-constexpr int TC_SHARED = 129, TC_SHARED_LONG = 65, TC_OWN = 65;
+// Which line takes a part. A tile of the tensor cores is two groups of 128 rows over the same keys, and its launch and first blocks
+// are dearer; a tile of this line is 64 rows, and every tile reads the keys' fragments again. What counts for a shared part is
+// therefore K/V heads x tokens x tiles of 64 rows, from 65 rows on (up to 64 the keys go by once, at HBM's rate). Measured, us, here /
+// tensor cores, bf16 and int8, own parts of 33 to 64 tokens (of 257 to 512):
+//   64K   8 heads x  4096, 128 rows    35 / 42 (41 / 47)   40 / 54 (50 / 57)      8 x 1024, 512 rows   48 / 57 (85 / 93)    56 / 67 (98 / 101)
+//   128K  8 heads x  8192, 128 rows    46 / 48 (50 / 55)   56 / 60 (61 / 64)      8 x 4096, 256 rows   50 / 46 (62 / 70)    57 / 57 (76 / 72)
+//   192K  8 heads x 12288, 128 rows    63 / 52 (60 / 62)   68 / 67 (71 / 70)     16 x 6144,  68 rows   60 / 50 (56 / 64)    67 / 65 (71 / 69)
+//   256K  8 heads x 16384, 128 rows    81 / 56 (67 / 69)   81 / 71 (85 / 77)      8 x 4096, 512 rows   93 / 63 (106 / 99)   98 / 75 (128 / 110)
+//         1 head x 131072, 128 rows    84 / 68 (64 / 71)   95 / 83 (85 / 83)      4 x 32768, 68 rows   77 / 55 (55 / 56)    83 / 70 (73 / 68)
+//   and far below: 1 head x 512, 136 rows 18 / 28, 19 / 34. Longer own parts move the balance to this line: they run beside the shared
+//   part here, after it there.
+// Own parts from 65 rows on: 2000 tokens, 8 sequences, 16 heads, 100 rows 97 / 82 and 122 / 94.
+constexpr int64_t TC_SHARED_WORK = 3 << 16;
+constexpr int TC_ROWS = 65;
 
 struct Plan {
     bool shared_tc, own_tc;             // which line holds which part
@@ -525,10 +531,10 @@ struct Plan {
     size_t tc_at, sched_at;             // byte offsets in the workspace: the second line's partials, the prefix sums
 };
 
-// The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_OWN rows per K/V head or
-// more walks all of its keys on the tensor-core line (it is bound by the products, and the shared pages come from L2); else
-// the rows of all sequences attend to the shared part together, on the tensor cores if there are TC_SHARED of them
-// (TC_SHARED_LONG over a long part), and the own parts stream.
+// The two lines of a call: `s` (this file's kernel) and `t` (paged_tc.cu). A sequence with TC_ROWS rows per K/V head or
+// more walks all of its keys on the tensor-core line, the shared ones too, in tiles of its own (a tile of 256 rows is bound by its
+// products, and the shared pages come from L2; with fewer rows a tile is that much emptier). Else the rows of all sequences attend
+// to the shared part together, on the tensor cores if it is TC_SHARED_WORK, and the own parts stream.
 static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     Plan pl;
     const bool i8 = a.cache.ks != nullptr;
@@ -541,10 +547,10 @@ static Plan plan(const PagedAttnArgs &a, Params &s, Params &t) {
     t = s;
     const int64_t r1 = (int64_t)a.Lq * s.G, all = r1 * a.B;
     const bool fits = a.B <= tc_most_sequences();
-    pl.own_tc = fits && r1 >= TC_OWN;
+    pl.own_tc = fits && r1 >= TC_ROWS;
     // one sequence has nothing to share
     const bool split = a.shared > 0 && a.B > 1 && !pl.own_tc;
-    pl.shared_tc = fits && split && all >= (a.shared >= TC_LONG ? TC_SHARED_LONG : TC_SHARED);
+    pl.shared_tc = fits && split && all >= TC_ROWS && s.Hkv * (int64_t)a.shared * cdiv(all, 64) >= TC_SHARED_WORK;
     s.bk = BK; s.ctas = stream_ctas(i8);
     t.bk = 128; t.ctas = num_sms();
     Params &own = pl.own_tc ? t : s;

@@ -1,5 +1,6 @@
 """What the paged cache and its attention promise where a call meets a limit: rows without room, rows listed twice, shared parts
 that nobody holds, numbers that are not finite, views that overlap. The bounds of attention are test_gpu_paged's."""
+import ctypes
 import math
 
 import pytest
@@ -182,7 +183,7 @@ def test_ids_past_32_bits_are_out_of_range(paged, cuda):
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 def test_shared_part_that_nobody_holds_in_full(paged, cuda, kind, heads):
     """Three rows of 0, 20 and 37 tokens with 128 declared as shared: NaN past their ends, in every free page and in what an
-    earlier call left in shared memory reaches nobody (64 heads on one: the tensor cores)."""
+    earlier call left in shared memory reaches nobody (64 heads on one: three tiles of 64 rows)."""
     c = filled(paged, 1, 40, 1, 16, 6, 12, kind, seed=8)
     q = torch.randn((3, 1, heads, D), device=cuda).to(torch.bfloat16)
     pools = [c.k, c.v] if kind == "bf16" else [c.k_scale, c.v_scale]
@@ -226,7 +227,7 @@ def test_long_shared_part_of_half_a_tile(paged, cuda, kind, rows, shared, own):
 @pytest.mark.parametrize("shared", [0, 64])
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 def test_tokens_without_a_page_are_zeros(paged, cuda, kind, heads, shared):
-    """Ids out of range in a table, on both lines: as if the page held zeros, whatever shared memory held before."""
+    """Ids out of range in a table: as if the page held zeros, whatever shared memory held before."""
     c = filled(paged, 1, 40, 1, 16, 3, 12, kind, seed=31)
     place(c, [150, 131], seed=32, shared=shared)
     q = torch.randn((2, 1, heads, D), device=cuda).to(torch.bfloat16)
@@ -249,6 +250,73 @@ def test_tokens_without_a_page_are_zeros(paged, cuda, kind, heads, shared):
         c.table[r, j] = bad
     got = paged.attention(q, c, 0, [0, 1], shared=shared)
     assert torch.equal(bits(got), bits(want))
+
+
+# ... and on the tensor cores, which a shared part reaches by K/V heads x tokens x tiles of 64 rows
+
+def on_tensor_cores(hn, c, b, lq, heads, shared):
+    """By the call's workspace: a partial result of 256 rows for every SM and tile of the shared part."""
+    n = ctypes.c_int64()
+    assert hn.lib.lib.hn_paged_attention_workspace(c._ref, b, lq, heads, shared, 1, ctypes.byref(n)) == 0
+    return n.value >= (hn.lib.lib.hn_num_sms() + c.heads * -(-b * lq * heads // c.heads // 256)) * 256 * 130 * 4
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("kv,group,lq,shared,page,own", [
+    (16, 24, 1, 6144, 64, [5, 0, 40]),                   # 72 rows: a tile a quarter full
+    (16, 32, 1, 6144, 128, [64, 1, 130, 7]),             # 128
+    (8, 32, 2, 2048, 16, [2, 0, 1, 77] * 3 + [130]),     # 832 rows in four tiles
+    (4, 7, 9, 4096, 32, [9, 500, 3, 31] * 3),            # 756, not whole groups
+])
+def test_shared_part_on_the_tensor_cores(paged, hn, cuda, kind, kv, group, lq, shared, page, own):
+    b, lens = len(own), [shared + n for n in own]
+    c = filled(paged, 1, shared // page + sum(-(-n // page) for n in own) + 2, kv, page, b, -(-max(lens) // page) + 1, kind, seed=22)
+    place(c, lens, seed=23, shared=shared)
+    assert on_tensor_cores(hn, c, b, lq, kv * group, shared)
+    q = torch.randn((b, lq, kv * group, D), device=cuda).to(torch.bfloat16)
+    rows = list(range(b))[::-1]
+    for causal in (True, False):
+        out, lse = paged.attention(q, c, 0, rows, shared=shared, causal=causal, return_lse=True)
+        check_attention(c, 0, q, rows, out, lse, causal, 1 / math.sqrt(D))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+def test_shared_part_on_the_tensor_cores_that_nobody_holds(paged, hn, cuda, kind):
+    """As above: 13 sequences of 0 to 333 tokens with 2048 declared as shared, NaN wherever no row has a token."""
+    b, kv, group, shared = 13, 8, 64, 2048
+    c = filled(paged, 1, 150, kv, 16, b + 1, 130, kind, seed=24)
+    assert on_tensor_cores(hn, c, b, 1, kv * group, shared)
+    q = torch.randn((b, 1, kv * group, D), device=cuda).to(torch.bfloat16)
+    pools = [c.k, c.v] if kind == "bf16" else [c.k_scale, c.v_scale]
+    kept = [t.clone() for t in pools]
+    c.extend([0], 2048)
+    for t in pools:
+        t.fill_(math.nan)
+    paged.attention(q, c, 0, [0] * b, shared=shared)     # what is left in shared memory
+    for t, was in zip(pools, kept):
+        t.copy_(was)
+    c.free([0])
+    c.extend([4], 333)
+    for i in range(1, b):
+        if i != 4:
+            c.table[i] = c.table[4]
+            c.lengths[i] = 27 * (i - 1)
+    hidden = torch.ones(c.pages, c.page, dtype=torch.bool, device=cuda)
+    pos = torch.arange(333, device=cuda)
+    hidden[c.table[4][pos // 16].long(), pos % 16] = False
+    for t in pools:
+        t[hidden[None, :, None, :].expand(1, c.pages, kv, 16)] = math.nan
+    for rows in (list(range(b)), list(range(b))[::-1]):
+        out, lse = paged.attention(q, c, 0, rows, shared=shared, return_lse=True)
+        check_attention(c, 0, q, rows, out, lse, True, 1 / math.sqrt(D))
+    c.table[4, 3], c.table[4, 18] = -1, 1 << 30          # ids out of range: zeros
+    got = paged.attention(q, c, 0, [4] * b, shared=shared)
+    zero = int((c.refs == 0).nonzero()[0])
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        if t is not None:
+            t[:, zero] = 0
+    c.table[4, 3], c.table[4, 18] = zero, zero
+    assert torch.equal(bits(got), bits(paged.attention(q, c, 0, [4] * b, shared=shared)))
 
 
 # ------------------------------------------------------------------------------------------- scales, NaN, infinity
