@@ -14,8 +14,8 @@
 // A page operation is a plan - one CTA, which reads the reference counts and the requests and writes who gets which
 // page - and a pass of many CTAs that moves the data and the table rows. The plan is O(pages + requests) on metadata of
 // a few KB; the pass is one read and one write of the moved bytes, which is what bounds it. Measured (kernel alone): 8 tails of
-// 33 tokens to 64 rows, 36 layers, 8 heads, int8: plan 7.4 us, pass 49 us (316 MB, 6.4 TB/s); 240 pages of 32 tokens,
-// 16 layers, 8 heads, bf16: plan 5.4 us, pass 157 us (1.0 GB, 6.4 TB/s). A small fork is the two launches, 14 us.
+// 33 tokens to 64 rows, 36 layers, 8 heads, int8: plan 8.1 us, pass 50 us (316 MB, 6.3 TB/s); 240 pages of 32 tokens,
+// 16 layers, 8 heads, bf16: plan 5.5 us, pass 155 us (1.0 GB, 6.5 TB/s). A small fork is the two launches, 13 us.
 #include "hn_common.cuh"
 #include "hn_kernels.h"
 
@@ -357,7 +357,7 @@ struct AppendParams {
 // old ones), a page that several rows name is not one row's to write, and a row listed again is written by its first listing
 // alone: such tokens are left out and counted. A warp takes the heads of one token, four K and V rows of 128 at a time
 // (lanes 0-15 a K row, 16-31 the V row, 8 elements each), so that eight rows are in flight. bf16 is copied; int8 takes the
-// absmax over the 16 lanes, hn_quantize_kv's scale and codes. Measured: 2 x 4400 tokens, 16 heads, int8 31 us (3.6 TB/s of
+// absmax over the 16 lanes, hn_quantize_kv's scale and codes. Measured: 2 x 4400 tokens, 16 heads, int8 33 us (3.4 TB/s of
 // reads and writes): the absmax stands between a row's load and its store.
 template <bool I8>
 __global__ void __launch_bounds__(256) k_append(AppendParams p, Meta m) {

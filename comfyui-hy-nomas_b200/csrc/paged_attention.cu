@@ -11,13 +11,14 @@
 // computes the cut itself from the lengths on the device). A tile that spans CTAs leaves a partial result per CTA
 // (fp32 sums, maximum, normaliser), joined by k_paged_join.
 //
-// Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head): 64 sequences of about 2500
-// tokens, 8 K/V heads: bf16 126 us (5.9 TB/s), int8 118 us (3.3 TB/s: the conversion of the codes issues as much as the products).
-// With 64-row tiles by the shared-memory reads of the fragments: 16 x 5 queries over 4096 shared and about 1100 own tokens, 16
-// heads, bf16: 54 us and the join's 9.
+// Bound by HBM for a token per sequence (K and V once: 2 x 256 B, int8 2 x 132 B, per key and head): 64 sequences of 1669 to 4000
+// tokens (181408 in all), 8 K/V heads: bf16 126 us (743 MB, 5.9 TB/s), int8 119 us (383 MB, 3.2 TB/s: the conversion of the codes
+// issues as much as the products). With 64-row tiles by the shared-memory reads of the fragments: 16 x 5 queries over 4096 shared
+// and 546 to 1101 own tokens, 16 heads, bf16: 54 us and the join's 8.
 // Per warp: 16 rows; m16n8k16 products, S and O in registers. The four warps split a block's keys (16-row tiles), its
 // rows (64), or both (32). Blocks arrive by cp.async, STAGES deep; the smem chunks are permuted so that no read conflicts.
-//  - bf16 cache: K by ldmatrix, V by its transposing form, P rounded to bf16.
+//  - bf16 cache: K by ldmatrix, V by its transposing form, P rounded to bf16 (both operands of a product have one type, and V's range
+//    is bf16's): at most 2^-8 of the mean |v|, with the output's own rounding after it.
 //  - int8 cache: codes become fp16 integers (exact: 0x6400 | (code + 128) is 1152 + code), so the scales stay outside the
 //    products: x_j = (q . ck_j) * sk_j * scale + log2 sv_j (base 2), P'_j = 2^(x_j - m + 14) multiplies cv_j, and the
 //    normaliser sums P'_j / sv_j. Taking the maximum over x_j keeps P' in fp16's range whatever the scales are.
@@ -430,7 +431,8 @@ template <bool I8> __global__ void __launch_bounds__(THREADS, I8 ? 3 : 2) k_page
 
 // Joins the partial results of every row: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i. A warp takes RUN rows of a tile,
 // one after the other. `a` is the line that holds the shared part (nbA 0: there is none), `b` the one that holds the own parts.
-// 140800 rows of which a quarter are cut: 47 us (each row looked up in the line: 105); small calls: 6-9 us, of latency.
+// 140800 rows of which a quarter are cut: 46 us (each row looked up in the line: 105); small calls: 5-10 us, of latency. Two CTAs an
+// SM: for three ptxas spills.
 template <int RUN> __global__ void __launch_bounds__(256, 2) k_paged_join(const Params a, const Params b) {
     dep_wait();
     const int lane = threadIdx.x & 31;

@@ -11,14 +11,14 @@
 //                256 + 128 g. int8: sixteen warps of 16 rows. A warp's chain of load, factors, maximum, exponentials and store is
 //                latency, and with 32 rows its body, beside the producers', did not fit the instruction caches (2 stalls on
 //                instructions an issue): 2.91 ms with eight warps, 2.45 with their rows in two turns of one body and the
-//                producers' loop by a step, 2.17 with sixteen. bf16: eight of 32 rows, whose body is shorter and whose
+//                producers' loop by a step, 2.17 with sixteen (2.21 since V's scales are in the exponent). bf16: eight of 32 rows, whose body is shorter and whose
 //                handovers are what counts: causal 1.68-1.71 ms, sixteen 1.85 (2 x 4400 queries over 20240 keys, 16 heads).
 //                Polynomials on the FMA pipe for 3 of 8 exponentials cost 8%.
 //   2 warps      MMA issuers, one per group: O_g += P(k) V, and, when that is done, S(k + 2) = Q_g K^T over P(k). A wait on the
 //                thread that issues blocks until its products have read their operands, so each group has a thread of its own:
 //                the tensor pipe runs one's products while the other waits.
 //   1 warp       walks the line: the CTA's pieces into a ring of four
-//   1 warp       int8: looks the block's pages up, sends for their codes (to L2; from a cold L2 2.41 ms without, 2.26 with) and
+//   1 warp       int8: looks the block's pages up, sends for their codes (to L2; from a cold L2 2.41 ms without, 2.26 with; now 2.31) and
 //                gathers its keys' factors, into a second ring of four
 //   4 warps      producers: the pages' rows of K and V into a ring of nine 16 KB slots (K and V of a step in turn: given
 //                back a step at a time, blocks in slots of 32 KB came late by a third of a step), in the 128-byte-swizzled layout

@@ -140,7 +140,8 @@ class KVCache:
                                vh, rows.data_ptr(), k.shape[0], k.shape[1]), "cache.append")
 
     def free(self, rows):
-        """The listed rows drop their pages and become empty. A page is free again when its last row drops it."""
+        """The listed rows drop their pages and become empty (a row listed twice, once). A page is free again when its last row
+        drops it."""
         rows = self._ids(rows, "free")
         _lib.check(_lib.launch("hn_cache_free", self.device, self._ref, rows.data_ptr(), rows.numel()), "cache.free")
 
@@ -208,7 +209,8 @@ def attention(q, cache, layer, rows, shared=0, causal=True, scale=None, out=None
     each sees the tokens up to itself; otherwise all of them. A query that sees no token gives 0 (lse -inf).
 
     `shared`: the rows' first `shared` tokens, a multiple of the page, are on the same pages, as `fork` leaves them;
-    those are read once for all rows. The result is the same as with shared=0 up to rounding."""
+    those are read together for all rows, where each has up to 64 queries times query heads per K/V head (with more, each walks
+    all of its keys itself). The result is the same as with shared=0 up to rounding. A row may hold fewer: it sees what it holds."""
     device = cache.device
     if not q.is_cuda:
         _lib.require_cuda(q)

@@ -389,11 +389,13 @@ int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *d
 /*
  * Attention over the paged cache for sequences that share their first `shared` tokens (a multiple of the page; on the
  * same pages in every listed row; 0: nothing is shared): out = softmax(q k^T * scale) v over each sequence's tokens, or,
- * `causal`, query i of Lq at position lengths - Lq + i sees the tokens up to its own. The shared tokens are read once
- * for all sequences. A query that sees nothing gives 0 (lse -inf). A row may hold fewer than `shared` tokens: it sees what it
+ * `causal`, query i of Lq at position lengths - Lq + i sees the tokens up to its own. The shared tokens are read together
+ * for all sequences, where each has up to 64 rows (Lq * H / heads) per K/V head; with more, each sequence walks all of its
+ * keys itself. A query that sees nothing gives 0 (lse -inf). A row may hold fewer than `shared` tokens: it sees what it
  * holds. A token on a page id out of range counts as one of zeros.
- * q, out [B, Lq, H, 128] bf16 (element strides for batch, query, head; multiples of 8; out's rows do not overlap), H a multiple of the cache's
- * heads (query heads h * H / heads .. share K/V head h), lse [B, H, Lq] fp32 natural log or NULL. rows [B] int32.
+ * q, out [B, Lq, H, 128] bf16 (element strides for batch, query, head; multiples of 8; out's rows do not overlap), H a
+ * multiple of the cache's heads (query heads h * H / heads .. share K/V head h), lse [B, H, Lq] fp32 natural log or NULL,
+ * rows [B] int32.
  * `scale` is any finite number. Scales of an int8 cache are positive, as its quantizer gives them. ws:
  * hn_paged_attention_workspace bytes, 16-byte aligned. B <= 4096.
  */
