@@ -777,6 +777,148 @@ int hn_attn_merge(const void *const *parts, const float *const *lses, int64_t n,
 } // extern "C"
 
 // ---------------------------------------------------------------------------------------------------
+// 4-bit linears, rotations
+
+extern "C" {
+
+static bool fp4_kind(int kind) { return kind == HN_KIND_MXFP4 || kind == HN_KIND_NVFP4; }
+static bool float_dtype(int dt) { return dt == HN_DTYPE_BF16 || dt == HN_DTYPE_FP16 || dt == HN_DTYPE_FP32; }
+static bool al4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+int hn_quantize_fp4(const void *x, int64_t ldx, int x_dtype, int64_t M, int64_t K, int kind, void *q, int64_t ldq, void *s,
+                    float *r, void *stream) {
+    REQUIRE(fp4_kind(kind), HN_ERR_ARG, "hn_quantize_fp4: unknown kind %d", kind);
+    REQUIRE(float_dtype(x_dtype), HN_ERR_ARG, "hn_quantize_fp4: bad x_dtype %d", x_dtype);
+    REQUIRE(M >= 0 && M <= 0x7fffff00LL && K > 0 && K <= (1LL << 30), HN_ERR_SHAPE,
+            "hn_quantize_fp4: bad shape (M=%lld K=%lld)", (long long)M, (long long)K);
+    if (M == 0) return HN_OK;
+    REQUIRE(x && q && s && (kind == HN_KIND_MXFP4 || r), HN_ERR_ARG, "hn_quantize_fp4: null pointer");
+    REQUIRE(ldx >= K && ldq >= cdiv(K, 32) * 16, HN_ERR_SHAPE, "hn_quantize_fp4: leading dimension too small");
+    REQUIRE(reinterpret_cast<uintptr_t>(x) % dsize(x_dtype) == 0 && al16(q) && ldq % 16 == 0 && al16(s) && al4(r), HN_ERR_ALIGN,
+            "hn_quantize_fp4: q and s need 16-byte aligned rows, x its type's alignment");
+    CHECK_DEVICE(x);
+    return launched(launch_quant_fp4(x, ldx, x_dtype, M, K, kind - HN_KIND_MXFP4, q, ldq, s, r, (cudaStream_t)stream),
+                    "hn_quantize_fp4 launch");
+}
+
+int hn_dequantize_fp4(const void *q, int64_t ldq, const void *s, const float *r, int64_t M, int64_t K, int64_t Kp, int kind,
+                      void *out, int64_t ldo, int out_dtype, void *stream) {
+    REQUIRE(fp4_kind(kind), HN_ERR_ARG, "hn_dequantize_fp4: unknown kind %d", kind);
+    REQUIRE(float_dtype(out_dtype), HN_ERR_ARG, "hn_dequantize_fp4: bad out_dtype %d", out_dtype);
+    REQUIRE(M >= 0 && M <= 0x7fffff00LL && K > 0 && K <= Kp && Kp <= (1LL << 30) && Kp % 32 == 0, HN_ERR_SHAPE,
+            "hn_dequantize_fp4: bad shape (M=%lld K=%lld of %lld)", (long long)M, (long long)K, (long long)Kp);
+    if (M == 0) return HN_OK;
+    REQUIRE(q && s && out && (kind == HN_KIND_MXFP4 || r), HN_ERR_ARG, "hn_dequantize_fp4: null pointer");
+    REQUIRE(ldo >= K && ldq >= Kp / 2, HN_ERR_SHAPE, "hn_dequantize_fp4: leading dimension too small");
+    REQUIRE(al16(q) && ldq % 16 == 0 && al16(s) && al4(r) && reinterpret_cast<uintptr_t>(out) % dsize(out_dtype) == 0, HN_ERR_ALIGN,
+            "hn_dequantize_fp4: q and s need 16-byte aligned rows, out its type's alignment");
+    CHECK_DEVICE(q);
+    return launched(launch_dequant_fp4(q, ldq, s, r, M, K, Kp, kind - HN_KIND_MXFP4, out, ldo, out_dtype, (cudaStream_t)stream),
+                    "hn_dequantize_fp4 launch");
+}
+
+int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, const void *qw, int64_t ldw, const void *sw,
+                const float *rw, const void *bias, int bias_dtype, void *out, int64_t ldo, int out_dtype, int64_t M, int64_t N,
+                int64_t K, int kind, void *stream) {
+    REQUIRE(fp4_kind(kind), HN_ERR_ARG, "hn_fp4_gemm: unknown kind %d", kind);
+    REQUIRE(float_dtype(out_dtype), HN_ERR_ARG, "hn_fp4_gemm: bad out_dtype %d", out_dtype);
+    REQUIRE(M >= 0 && M <= 0x7fffff00LL && N > 0 && N <= 0x7fffff00LL && K > 0 && K <= (1LL << 30) && K % 32 == 0, HN_ERR_SHAPE,
+            "hn_fp4_gemm: need N > 0 and K %% 32 == 0 (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
+    REQUIRE(cdiv(M, 128) * cdiv(N, 128) <= 0x7fffffffLL / 16, HN_ERR_SHAPE, "hn_fp4_gemm: too many outputs");
+    REQUIRE(kind == HN_KIND_NVFP4 || (ra == nullptr && rw == nullptr), HN_ERR_ARG, "hn_fp4_gemm: row scales are for HN_KIND_NVFP4");
+    REQUIRE(bias == nullptr || float_dtype(bias_dtype), HN_ERR_ARG, "hn_fp4_gemm: bad bias dtype %d", bias_dtype);
+    if (M == 0) return HN_OK;
+    REQUIRE(qa && sa && qw && sw && out, HN_ERR_ARG, "hn_fp4_gemm: null pointer");
+    REQUIRE(lda >= K / 2 && ldw >= K / 2 && ldo >= N, HN_ERR_SHAPE, "hn_fp4_gemm: leading dimension too small");
+    REQUIRE(lda < (1LL << 40) && ldw < (1LL << 40), HN_ERR_SHAPE, "hn_fp4_gemm: leading dimension too large");
+    REQUIRE(al16(qa) && al16(qw) && al16(sa) && al16(sw) && lda % 16 == 0 && ldw % 16 == 0, HN_ERR_ALIGN,
+            "hn_fp4_gemm: codes and scales need 16-byte aligned rows");
+    REQUIRE(al4(ra) && al4(rw) && reinterpret_cast<uintptr_t>(out) % dsize(out_dtype) == 0 &&
+                (bias == nullptr || reinterpret_cast<uintptr_t>(bias) % dsize(bias_dtype) == 0), HN_ERR_ALIGN,
+            "hn_fp4_gemm: out, bias and row scales need their type's alignment");
+    CHECK_DEVICE(qa);
+    Fp4GemmArgs a;
+    a.qa = qa; a.lda = lda; a.sa = sa; a.ra = ra;
+    a.qw = qw; a.ldw = ldw; a.sw = sw; a.rw = rw;
+    a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.ldo = ldo; a.out_dtype = out_dtype;
+    a.M = M; a.N = N; a.K = K; a.kind = kind - HN_KIND_MXFP4;
+    const char *msg = nullptr;
+    cudaError_t e = launch_fp4_gemm(a, (cudaStream_t)stream, &msg);
+    if (e != cudaSuccess && msg) return fail(HN_ERR_ALIGN, "hn_fp4_gemm: %s", msg);
+    return launched(e, "hn_fp4_gemm launch");
+}
+
+// what the rotations have in common
+static int rotation_args(const char *what, const void *pos, int wide, const int64_t *freq, int64_t rot, int layout, float factor,
+                         const void *w0, const void *w1, float eps, int64_t D) {
+    REQUIRE(D >= 8 && D <= 256 && D % 8 == 0 && rot >= 8 && rot <= D && rot % 8 == 0, HN_ERR_SHAPE,
+            "%s: need rot <= D <= 256, both multiples of 8 (rot=%lld D=%lld)", what, (long long)rot, (long long)D);
+    REQUIRE(layout == HN_ROPE_HALF || layout == HN_ROPE_INTERLEAVED, HN_ERR_ARG, "%s: unknown layout %d", what, layout);
+    REQUIRE(wide == 0 || wide == 1, HN_ERR_ARG, "%s: pos_wide is 0 or 1", what);
+    REQUIRE(std::isfinite(factor) && std::isfinite(eps) && eps >= 0.0f, HN_ERR_ARG, "%s: factor and eps must be finite, eps >= 0", what);
+    REQUIRE(freq, HN_ERR_ARG, "%s: null pointer", what);
+    REQUIRE(al8(freq) && al16(w0) && al16(w1) && reinterpret_cast<uintptr_t>(pos) % (wide ? 8 : 4) == 0, HN_ERR_ALIGN,
+            "%s: weights must be 16-byte aligned, positions and frequencies as their types", what);
+    return HN_OK;
+}
+
+int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype, const void *pos, int64_t p_bs, int64_t p_ls,
+              int pos_wide, const int64_t *freq, int64_t rot, int layout, float factor, const void *weight, float eps, int64_t B,
+              int64_t L, int64_t H, int64_t D, void *out, int64_t o_bs, int64_t o_ls, int64_t o_hs, void *stream) {
+    REQUIRE(float_dtype(dtype), HN_ERR_ARG, "hn_rotate: bad dtype %d", dtype);
+    REQUIRE(B >= 0 && L >= 0 && H >= 0 && B <= 0x7fffffff && L <= 0x7fffffff && H <= 65536, HN_ERR_SHAPE,
+            "hn_rotate: bad shape (B=%lld L=%lld H=%lld)", (long long)B, (long long)L, (long long)H);
+    if (int rc = rotation_args("hn_rotate", pos, pos_wide, freq, rot, layout, factor, weight, nullptr, eps, D)) return rc;
+    if (B == 0 || L == 0 || H == 0) return HN_OK;
+    REQUIRE(B * L <= (1LL << 40) / H, HN_ERR_SHAPE, "hn_rotate: too many heads");
+    REQUIRE(x && pos && out, HN_ERR_ARG, "hn_rotate: null pointer");
+    REQUIRE(al16(x) && al16(out) && (x_bs | x_ls | x_hs | o_bs | o_ls | o_hs) % 8 == 0, HN_ERR_ALIGN,
+            "hn_rotate: x and out must be 16-byte aligned, strides multiples of 8 elements");
+    CHECK_DEVICE(x);
+    RotateArgs a;
+    a.x = x; a.x_bs = x_bs; a.x_ls = x_ls; a.x_hs = x_hs;
+    a.out = out; a.o_bs = o_bs; a.o_ls = o_ls; a.o_hs = o_hs; a.dtype = dtype;
+    a.pos = pos; a.p_bs = p_bs; a.p_ls = p_ls; a.wide = pos_wide; a.w = weight;
+    a.freq = freq; a.rot = (int)rot; a.layout = layout; a.factor = factor; a.eps = eps;
+    a.B = (int)B; a.L = (int)L; a.H = (int)H; a.D = (int)D;
+    return launched(launch_rotate(a, (cudaStream_t)stream), "hn_rotate launch");
+}
+
+int hn_cache_append_rotated(const hn_kv_cache *cache, int64_t layer, const void *q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
+                            int64_t H, const void *k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void *v, int64_t v_bs,
+                            int64_t v_ts, int64_t v_hs, const int32_t *rows, int64_t B, int64_t n, const void *pos, int64_t p_bs,
+                            int64_t p_ts, int pos_wide, const int64_t *freq, int64_t rot, int layout, float factor,
+                            const void *q_weight, const void *k_weight, float eps, void *out, void *stream) {
+    CacheArgs c;
+    if (int rc = cache_args(cache, "hn_cache_append_rotated", c)) return rc;
+    REQUIRE(layer >= 0 && layer < cache->layers, HN_ERR_SHAPE, "hn_cache_append_rotated: layer %lld of %lld", (long long)layer,
+            (long long)cache->layers);
+    REQUIRE(B >= 0 && n >= 0 && B <= MAX_REQUESTS && n <= 0x3fffffff && H >= 1 && H <= 65536, HN_ERR_SHAPE,
+            "hn_cache_append_rotated: bad count");
+    if (int rc = rotation_args("hn_cache_append_rotated", pos, pos_wide, freq, rot, layout, factor, q_weight, k_weight, eps, 128))
+        return rc;
+    if (B == 0 || n == 0) return HN_OK;
+    REQUIRE(q && k && v && rows && out, HN_ERR_ARG, "hn_cache_append_rotated: null pointer");
+    REQUIRE(al16(q) && al16(k) && al16(v) && al16(out) &&
+                (q_bs | q_ts | q_hs | k_bs | k_ts | k_hs | v_bs | v_ts | v_hs) % 8 == 0, HN_ERR_ALIGN,
+            "hn_cache_append_rotated: q, k, v and out need 16-byte aligned rows of 128");
+    REQUIRE(cache->refused, HN_ERR_ARG, "hn_cache_append_rotated: null pointer in the cache");
+    REQUIRE(cache->epoch != 0, HN_ERR_ARG, "hn_cache_append_rotated: the cache's epoch is 0");
+    CHECK_DEVICE(k);
+    AppendRotatedArgs a;
+    a.x[0] = q; a.bs[0] = q_bs; a.ts[0] = q_ts; a.hs[0] = q_hs;
+    a.x[1] = k; a.bs[1] = k_bs; a.ts[1] = k_ts; a.hs[1] = k_hs;
+    a.x[2] = v; a.bs[2] = v_bs; a.ts[2] = v_ts; a.hs[2] = v_hs;
+    a.out = out; a.rows = rows; a.pos = pos; a.p_bs = p_bs; a.p_ts = p_ts; a.wide = pos_wide;
+    a.w[0] = q_weight; a.w[1] = k_weight;
+    a.freq = freq; a.rot = (int)rot; a.layout = layout; a.factor = factor; a.eps = eps;
+    a.B = (int)B; a.n = (int)n; a.H = (int)H;
+    return launched(launch_append_rotated(c, (int)layer, a, (cudaStream_t)stream), "hn_cache_append_rotated launch");
+}
+
+} // extern "C"
+
+// ---------------------------------------------------------------------------------------------------
 // Sequence-parallel K/V exchange over NVLink by the copy engines (host-side only: CUDA IPC mappings, an
 // asynchronous peer copy, a 32-bit flag write the GPU's front end executes after the copy - no SM involved - and a
 // one-warp bounded wait for the peers' flags). No reference counterpart: the reference runs one GPU.

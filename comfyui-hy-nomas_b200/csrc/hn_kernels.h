@@ -138,4 +138,48 @@ cudaError_t launch_add_rmsnorm_quant(const void *x, int64_t ldx, const void *r, 
                                      int64_t rows, int64_t D, float eps, int kind, bool per_row, void *out, int64_t ldo,
                                      void *q, int64_t ldq, float *s, int64_t s_rs, int64_t s_gs, cudaStream_t st);
 
+// 4-bit codes with block scales (fp4_quant.cu, fp4_gemm.cu; the formats: fp4.cuh). kind 0: 2^e per 32 columns, 1: e4m3 per 16
+// and fp32 per row; ldq, lda and ldw in bytes
+cudaError_t launch_quant_fp4(const void *x, int64_t ldx, int x_dtype, int64_t M, int64_t K, int kind, void *q, int64_t ldq,
+                             void *s, float *r, cudaStream_t st);
+cudaError_t launch_dequant_fp4(const void *q, int64_t ldq, const void *s, const float *r, int64_t M, int64_t K, int64_t Kp,
+                               int kind, void *out, int64_t ldo, int out_dtype, cudaStream_t st);
+struct Fp4GemmArgs {
+    const void *qa; int64_t lda; const void *sa; const float *ra;
+    const void *qw; int64_t ldw; const void *sw; const float *rw;
+    const void *bias; int bias_dtype;
+    void *out; int64_t ldo; int out_dtype;
+    int64_t M, N, K;        // K: of the padded codes, a multiple of 32
+    int kind;
+};
+constexpr int FP4_GEMV_MAX_M = 4;       // rows that run as a GEMV (fp4_gemv.cu)
+bool fp4_gemv_applies(const Fp4GemmArgs &a);
+cudaError_t launch_fp4_gemv(const Fp4GemmArgs &a, cudaStream_t st);
+cudaError_t launch_fp4_gemm(const Fp4GemmArgs &a, cudaStream_t st, const char **msg);
+
+// rotation by position (rotary.cu); layout 1: interleaved pairs. freq [rot / 2]: fractions of a turn, times 2^64; pos int32, or
+// int64 where wide
+struct RotateArgs {
+    const void *x; int64_t x_bs, x_ls, x_hs;
+    void *out; int64_t o_bs, o_ls, o_hs;
+    int dtype;
+    const void *pos; int64_t p_bs, p_ls; int wide;
+    const void *w;          // bf16 [D], or null: no norm
+    const int64_t *freq; int rot, layout; float factor;
+    float eps;
+    int B, L, H, D;
+};
+cudaError_t launch_rotate(const RotateArgs &a, cudaStream_t st);
+struct AppendRotatedArgs {
+    const void *x[3]; int64_t bs[3], ts[3], hs[3];      // q, k, v
+    void *out;                                          // [B, n, H, 128]
+    const int *rows;
+    const void *pos; int64_t p_bs, p_ts; int wide;      // pos null: a token's place in its row
+    const void *w[2];                                   // bf16 [128] of q and k, or null
+    const int64_t *freq; int rot, layout; float factor;
+    float eps;
+    int B, n, H;
+};
+cudaError_t launch_append_rotated(const CacheArgs &c, int layer, const AppendRotatedArgs &a, cudaStream_t st);
+
 } // namespace hn

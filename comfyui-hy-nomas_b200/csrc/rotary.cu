@@ -1,0 +1,246 @@
+// rotary.cu - per-head RMSNorm and the rotation by position: in one pass over the heads, and on the way into the paged cache.
+//
+//   y = R(t) (x / sqrt(mean x^2 + eps) * w),  R(t): pairs of columns turned by t f_i, times the scaling's attention factor
+//
+// in fp32 from the loads to the one rounding. The first `rot` columns of a head are rotated, the others pass.
+//
+// Bound by HBM: each head read once and written once. A warp takes one token and several of its heads: cos and sin of the
+// token's pairs are computed once, by all lanes, and shared through shared memory; P lanes hold a head, eight columns each. In
+// the half layout a column's partner stands in another lane: it is loaded again (from L1), which costs less than an exchange
+// that the part-rotated heads, whose halves begin inside a lane, would need in several forms.
+#include "hn_kernels.h"
+#include "rotary.cuh"
+
+namespace hn {
+namespace rotary {
+
+constexpr int WARPS = 8;
+
+struct Params {
+    const void *x;
+    int64_t x_bs, x_ls, x_hs;
+    void *out;
+    int64_t o_bs, o_ls, o_hs;
+    const void *pos;                    // int32 or int64
+    int64_t p_bs, p_ls;
+    int wide;
+    const __nv_bfloat16 *w;             // or null
+    Rotation r;
+    float eps;
+    int B, L, H, D, per, groups;        // per: heads of a unit, a multiple of 32 / P; groups: units of a token
+};
+
+template <typename E, int P> __global__ void __launch_bounds__(32 * WARPS) k_rotate(Params p) {
+    __shared__ float tables[WARPS][2 * MAX_PAIRS];
+    constexpr int HEADS = 32 / P, U = 2;
+    const int lane = threadIdx.x & 31, sub = lane % P;
+    float *table = tables[threadIdx.x >> 5];
+    const bool in = 8 * sub < p.D;
+    Turn t;
+    partners(p.r, sub, t);
+    Weights w;
+    if (p.w != nullptr && in) load_weights(p.w + 8 * sub, t, w);
+    const int64_t units = (int64_t)p.B * p.L * p.groups, step = (int64_t)gridDim.x * WARPS;
+    for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
+        const int64_t token = div_nonneg(u, p.groups);
+        const int first = (int)(u - token * p.groups) * p.per, last = first + p.per < p.H ? first + p.per : p.H;
+        const int64_t b = div_nonneg(token, p.L), l = token - b * p.L;
+        const E *x = static_cast<const E *>(p.x) + b * p.x_bs + l * p.x_ls + 8 * sub;
+        E *out = static_cast<E *>(p.out) + b * p.o_bs + l * p.o_ls + 8 * sub;
+        const int64_t at = b * p.p_bs + l * p.p_ls;
+        turn_table(p.r, p.wide ? static_cast<const int64_t *>(p.pos)[at] : static_cast<const int32_t *>(p.pos)[at], table, lane);
+        turn_of(p.r, sub, table, t);
+        for (int h0 = first + lane / P; h0 - lane / P < last; h0 += U * HEADS) {
+            float v[U][8], o[U][8];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int h = h0 + i * HEADS;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+                if (in && h < last) {
+                    load8(x + h * p.x_hs, v[i]);
+                    load_partners(x + h * p.x_hs, t, o[i]);
+                }
+            }
+            __syncwarp();               // out may be x: the partners are read before they are written
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int h = h0 + i * HEADS;
+                if (p.w != nullptr) head_norm<P>(v[i], o[i], w, t, p.D, p.eps);
+                turn(t, v[i], o[i]);
+                if (in && h < last) store8(out + h * p.o_hs, v[i]);
+            }
+        }
+    }
+}
+
+template <typename E, int P> cudaError_t go(Params p, cudaStream_t st) {
+    constexpr int HEADS = 32 / P;
+    // a unit takes all heads of its token where there are tokens enough for all SMs, fewer where there are not
+    const int64_t tokens = (int64_t)p.B * p.L, passes = cdiv(p.H, HEADS), want = (int64_t)num_sms() * 32;
+    int64_t each = cdiv(tokens * passes, want);
+    if (each > passes) each = passes;
+    p.per = (int)(each * HEADS);
+    p.groups = (int)cdiv(p.H, p.per);
+    const int64_t grid = cdiv(tokens * p.groups, WARPS), most = (int64_t)num_sms() * 8;
+    k_rotate<E, P><<<(unsigned)(grid < most ? grid : most), 32 * WARPS, 0, st>>>(p);
+    return cudaGetLastError();
+}
+template <typename E> cudaError_t pick(const Params &p, cudaStream_t st) {
+    if (p.D <= 16) return go<E, 2>(p, st);
+    if (p.D <= 32) return go<E, 4>(p, st);
+    if (p.D <= 64) return go<E, 8>(p, st);
+    if (p.D <= 128) return go<E, 16>(p, st);
+    return go<E, 32>(p, st);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// the append
+
+struct AppendParams {
+    const __nv_bfloat16 *x[3];          // q [B, n, H, 128], k and v [B, n, heads, 128]
+    int64_t bs[3], ts[3], hs[3];
+    __nv_bfloat16 *out;                 // rotated q, dense
+    uint8_t *pool[2];                   // this layer's k and v
+    float *scale[2];
+    const int *rows;
+    const void *pos;                    // [B, n] int32 or int64, or null: a token's place in its row
+    int64_t p_bs, p_ts;
+    int wide;
+    const __nv_bfloat16 *w[2];          // norm weights of q and of k, or null
+    Rotation r;
+    float eps;
+    int B, n, H, heads, per, groups;    // per: heads of a unit, of the token's H + 2 heads
+};
+
+// The rules of the plain append: a row whose last extend was refused, a page that several rows name, a row's listings after the
+// first keep what they hold, counted. q is rotated whatever becomes of the row. A unit is a warp's share of a token: some of
+// its q, k and v heads, in that order, two at a time (16 lanes each).
+template <bool I8> __global__ void __launch_bounds__(32 * WARPS) k_append_rotated(AppendParams p, Meta m) {
+    __shared__ float tables[WARPS][2 * MAX_PAIRS];
+    const int lane = threadIdx.x & 31, sub = lane & 15, side = lane >> 4;
+    float *table = tables[threadIdx.x >> 5];
+    Turn t;
+    partners(p.r, sub, t);
+    const int all = p.H + 2 * p.heads;
+    const int64_t units = (int64_t)p.B * p.n * p.groups, step = (int64_t)gridDim.x * WARPS;
+    for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
+        const int64_t bt = div_nonneg(u, p.groups);
+        const int first = (int)(u - bt * p.groups) * p.per, last = first + p.per < all ? first + p.per : all;
+        const int b = (int)div_nonneg(bt, p.n), i = (int)(bt - (int64_t)b * p.n);
+        const int row = p.rows[b];
+        int page = -1, place = 0;
+        int64_t at = i - p.n;
+        bool again = false;
+        if (last > p.H)
+            for (int j = lane; j < b; j += 32) again |= p.rows[j] == row;
+        if ((unsigned)row < (unsigned)m.slots) {
+            at += m.lengths[row];
+            const int64_t j = at / m.page;
+            if (last > p.H && at >= 0 && j < m.width && m.refused[row] != m.epoch) page = m.table[(int64_t)row * m.width + j];
+            place = (int)(at - j * m.page);
+        }
+        if ((unsigned)page < (unsigned)m.pages && m.refs[page] > 1) page = -1;
+        const bool put = !__any_sync(0xffffffffu, again) && (unsigned)page < (unsigned)m.pages;
+        // the token has no place of its own: counted where its k heads begin
+        if (!put && lane == 0 && first <= p.H && p.H < last) atomicAdd(m.failed, p.heads);
+        if (first < p.H + p.heads) {
+            if (p.pos != nullptr) {
+                const int64_t o = b * p.p_bs + i * p.p_ts;
+                at = p.wide ? static_cast<const int64_t *>(p.pos)[o] : static_cast<const int32_t *>(p.pos)[o];
+            }
+            turn_table(p.r, at, table, lane);
+            turn_of(p.r, sub, table, t);
+        }
+        for (int h0 = first; h0 < last; h0 += 2) {
+            const int h = h0 + side;
+            const int which = h < p.H ? 0 : h < p.H + p.heads ? 1 : 2;
+            const int head = which == 0 ? h : which == 1 ? h - p.H : h - p.H - p.heads;
+            const bool in = h < last && (which == 0 || put);
+            float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, o[8];
+            if (in) {
+                const __nv_bfloat16 *x = p.x[which] + b * p.bs[which] + i * p.ts[which] + head * p.hs[which] + 8 * sub;
+                load8(x, v);
+                if (which < 2) load_partners(x, t, o);
+            }
+            const __nv_bfloat16 *w = which < 2 ? p.w[which] : nullptr;
+            if (p.w[0] != nullptr || p.w[1] != nullptr) {
+                float n[8], no[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { n[j] = v[j]; no[j] = o[j]; }
+                Weights ww;
+                if (w != nullptr) load_weights(w + 8 * sub, t, ww);
+                head_norm<16>(n, no, ww, t, 128, p.eps);
+                if (w != nullptr)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { v[j] = n[j]; o[j] = no[j]; }
+            }
+            if (which < 2) turn(t, v, o);
+            const int64_t to = ((int64_t)page * p.heads + head) * m.page + place;
+            if (which == 0) {
+                if (in) store8(p.out + (bt * p.H + head) * 128 + 8 * sub, v);
+            } else if (!I8) {
+                if (in) store8(reinterpret_cast<__nv_bfloat16 *>(p.pool[which - 1]) + to * 128 + 8 * sub, v);
+            }
+            if (I8 && h0 + 1 >= p.H) {          // the pair has a k or v head
+                float peak = nanmax_abs3(0.0f, v[0], v[1]);
+#pragma unroll
+                for (int j = 2; j < 8; j += 2) peak = nanmax_abs3(peak, v[j], v[j + 1]);
+                peak = lanes_max<16>(peak);
+                // a NaN or an infinity in the row: its scale is NaN, so that what reads it gives NaN
+                const float sc = peak < INFINITY ? i8_scale(peak) : __int_as_float(0x7fffffff);
+                if (in && which > 0) {
+                    *reinterpret_cast<uint2 *>(p.pool[which - 1] + to * 128 + 8 * sub) =
+                        quant_chunk8<0, false>(v, sc, sc >= 0x1p-90f, x2_splat(-sc), x2_splat(__frcp_rn(sc)));
+                    if (sub == 0) p.scale[which - 1][to] = sc;
+                }
+            }
+        }
+    }
+}
+
+} // namespace rotary
+
+cudaError_t launch_rotate(const RotateArgs &a, cudaStream_t st) {
+    rotary::Params p;
+    p.x = a.x; p.x_bs = a.x_bs; p.x_ls = a.x_ls; p.x_hs = a.x_hs;
+    p.out = a.out; p.o_bs = a.o_bs; p.o_ls = a.o_ls; p.o_hs = a.o_hs;
+    p.pos = a.pos; p.p_bs = a.p_bs; p.p_ls = a.p_ls; p.wide = a.wide;
+    p.w = static_cast<const __nv_bfloat16 *>(a.w);
+    p.r = {a.freq, a.rot, a.layout, a.factor};
+    p.eps = a.eps; p.B = a.B; p.L = a.L; p.H = a.H; p.D = a.D;
+    if (a.dtype == 0) return rotary::pick<__nv_bfloat16>(p, st);
+    if (a.dtype == 1) return rotary::pick<__half>(p, st);
+    return rotary::pick<float>(p, st);
+}
+
+cudaError_t launch_append_rotated(const CacheArgs &c, int layer, const AppendRotatedArgs &a, cudaStream_t st) {
+    rotary::AppendParams p;
+    const int64_t tokens = (int64_t)layer * c.meta.pages * c.heads * c.meta.page;
+    const int row_bytes = c.ks ? 128 : 256;
+    for (int i = 0; i < 3; ++i) {
+        p.x[i] = static_cast<const __nv_bfloat16 *>(a.x[i]);
+        p.bs[i] = a.bs[i]; p.ts[i] = a.ts[i]; p.hs[i] = a.hs[i];
+    }
+    p.out = static_cast<__nv_bfloat16 *>(a.out);
+    p.pool[0] = static_cast<uint8_t *>(c.k) + tokens * row_bytes;
+    p.pool[1] = static_cast<uint8_t *>(c.v) + tokens * row_bytes;
+    p.scale[0] = c.ks ? c.ks + tokens : nullptr;
+    p.scale[1] = c.ks ? c.vs + tokens : nullptr;
+    p.rows = a.rows; p.pos = a.pos; p.p_bs = a.p_bs; p.p_ts = a.p_ts; p.wide = a.wide;
+    for (int i = 0; i < 2; ++i) p.w[i] = static_cast<const __nv_bfloat16 *>(a.w[i]);
+    p.r = {a.freq, a.rot, a.layout, a.factor};
+    p.eps = a.eps; p.B = a.B; p.n = a.n; p.H = a.H; p.heads = c.heads;
+    const int64_t count = (int64_t)a.B * a.n, passes = cdiv(a.H + 2 * c.heads, 2), want = (int64_t)num_sms() * 32;
+    int64_t each = cdiv(count * passes, want);
+    if (each > passes) each = passes;
+    p.per = (int)(2 * each);
+    p.groups = (int)cdiv(a.H + 2 * c.heads, p.per);
+    const int64_t grid = cdiv(count * p.groups, rotary::WARPS), most = (int64_t)num_sms() * 8;
+    const unsigned g = (unsigned)(grid < most ? grid : most);
+    if (c.ks) rotary::k_append_rotated<true><<<g, 32 * rotary::WARPS, 0, st>>>(p, c.meta);
+    else rotary::k_append_rotated<false><<<g, 32 * rotary::WARPS, 0, st>>>(p, c.meta);
+    return cudaGetLastError();
+}
+
+} // namespace hn

@@ -19,6 +19,7 @@ STATUS = {0: "HN_OK", 1: "HN_ERR_SHAPE", 2: "HN_ERR_ALIGN", 3: "HN_ERR_ARCH", 4:
 
 DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.int32: 3}
 KIND = {"int8": 0, "fp8": 1}
+FP4_KIND = {"mxfp4": 2, "nvfp4": 3}
 SCALE_MODE = {"group": 0, "row": 1, "block": 2}
 
 # name -> argtypes (all entry points return int)
@@ -57,6 +58,13 @@ SIGNATURES = {
     "hn_paged_attention_workspace": [_V, _I64, _I64, _I64, _I64, _I32, ctypes.POINTER(ctypes.c_int64)],
     "hn_paged_attention": [_V, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I32, _F32, _V, _I64, _I64,
                            _I64, _V, _V, _I64, _V],
+    "hn_quantize_fp4": [_V, _I64, _I32, _I64, _I64, _I32, _V, _I64, _V, _V, _V],
+    "hn_dequantize_fp4": [_V, _I64, _V, _V, _I64, _I64, _I64, _I32, _V, _I64, _I32, _V],
+    "hn_fp4_gemm": [_V, _I64, _V, _V, _V, _I64, _V, _V, _V, _I32, _V, _I64, _I32, _I64, _I64, _I64, _I32, _V],
+    "hn_rotate": [_V, _I64, _I64, _I64, _I32, _V, _I64, _I64, _I32, _V, _I64, _I32, _F32, _V, _F32, _I64, _I64, _I64, _I64, _V,
+                  _I64, _I64, _I64, _V],
+    "hn_cache_append_rotated": [_V, _I64, _V, _I64, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64,
+                                _V, _I64, _I64, _I32, _V, _I64, _I32, _F32, _V, _V, _F32, _V, _V],
     "hn_attention": [_V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                      _F32, _V, _I64, _I64, _I64, _V, _V, _V],
     "hn_attn_merge": [_V, _V, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _V, _I64, _I64, _I64,

@@ -147,3 +147,141 @@ def block_linear(x, qw, sw, bias=None, kind="int8"):
 def int8_g128_linear(x, qw, sw, bias=None):
     """hy_nomas/kernels.py:225-226."""
     return block_linear(x, qw, sw, bias, kind="int8")
+
+
+# ----------------------------------------------------------------------------------------------- 4-bit codes with block scales
+
+FP4_SPAN = {"mxfp4": 128, "nvfp4": 64}      # columns of a scale tile
+
+
+def _fp4_kind(kind, what):
+    if kind not in FP4_SPAN:
+        raise ValueError(f"{what}: kind {kind!r} (mxfp4 or nvfp4)")
+    return _lib.FP4_KIND[kind]
+
+
+def _fp4_operand(q, s, r, kind, what, name):
+    """The checks of one operand -> (codes whose rows start on 16 bytes, scales, row scales)."""
+    if q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] % 16 or not q.shape[1]:
+        raise ValueError(f"{what}: the codes of {name} must be uint8 [rows, K / 2] with K a multiple of 32, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    rows, kp = q.shape[0], 2 * q.shape[1]
+    span = FP4_SPAN[kind]
+    want = ((rows + 127) // 128, (kp + span - 1) // span, 512)
+    if s.dtype != torch.uint8 or s.shape != want:
+        raise ValueError(f"{what}: the scales of {name} must be uint8 {want} for {kind}, got {s.dtype} {tuple(s.shape)}")
+    if r is not None:
+        if kind == "mxfp4":
+            raise ValueError(f"{what}: mxfp4 has no row scales")
+        if r.dtype != torch.float32 or r.shape != (rows,):
+            raise ValueError(f"{what}: the row scales of {name} must be fp32 [{rows}], got {r.dtype} {tuple(r.shape)}")
+        if not r.is_contiguous():
+            r = r.contiguous()
+    if s.device != q.device or (r is not None and r.device != q.device):
+        raise RuntimeError(f"{what}: codes and scales of {name} on different devices")
+    if not (q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1] and q.data_ptr() % 16 == 0):
+        q = _lib.dense(q)
+    if not (s.is_contiguous() and s.data_ptr() % 16 == 0):
+        s = _lib.dense(s)
+    return q, s, r
+
+
+def quantize_fp4(x, kind="nvfp4"):
+    """x [M, K] -> (codes, scales, row scales): e2m1 codes uint8 [M, Kp / 2], two to a byte (the even column in the low half), Kp =
+    K rounded up to 32; scale bytes uint8 [M / 128, tiles, 512] (rounded up) in the tensor cores' order (`ops.untile_fp4_scales`).
+
+    "nvfp4": an e4m3 scale per 16 columns and an fp32 scale per row, max|row| / 2688 (fp32 [M]), so no scale has to be known
+    beforehand. "mxfp4": a scale 2^e per 32 columns, e = floor(log2 max|x|) - 2; the row scales are None. A NaN or an infinity
+    makes its row (nvfp4) or its 32 columns (mxfp4) NaN; nvfp4 rows below 2^-100 count as zeros."""
+    code = _fp4_kind(kind, "quantize_fp4")
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"quantize_fp4: x must be [M, K], got {tuple(x.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        x = x.float()
+    m, k = x.shape
+    if x.stride(1) != 1 or x.stride(0) < k:
+        x = x.contiguous()
+    kp, device = (k + 31) // 32 * 32, x.device
+    span = FP4_SPAN[kind]
+    q = torch.empty((m, kp // 2), dtype=torch.uint8, device=device)
+    s = torch.empty(((m + 127) // 128, (kp + span - 1) // span, 512), dtype=torch.uint8, device=device)
+    r = torch.empty(m, dtype=torch.float32, device=device) if kind == "nvfp4" else None
+    _lib.check(_lib.launch("hn_quantize_fp4", device, x.data_ptr(), max(x.stride(0), k), _lib.DTYPE[x.dtype], m, k, code,
+                           q.data_ptr(), kp // 2, s.data_ptr(), None if r is None else r.data_ptr()), "quantize_fp4")
+    return q, s, r
+
+
+def dequantize_fp4(q, s, r=None, kind="nvfp4", dtype=torch.bfloat16, columns=None):
+    """What codes, scales and row scales (None: all 1) stand for: code * (scale * row scale), rounded once to `dtype` (bf16, fp16,
+    fp32) [M, columns]. `columns`: the K that was quantized, where it was no multiple of 32."""
+    code = _fp4_kind(kind, "dequantize_fp4")
+    _lib.require_cuda(q, s, r)
+    q, s, r = _fp4_operand(q, s, r, kind, "dequantize_fp4", "q")
+    m, kp = q.shape[0], 2 * q.shape[1]
+    k = kp if columns is None else columns
+    if not kp - 32 < k <= kp:
+        raise ValueError(f"dequantize_fp4: {k} columns of {kp}")
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"dequantize_fp4: dtype {dtype} (bf16, fp16 or fp32)")
+    if r is None and kind == "nvfp4":
+        r = torch.ones(m, dtype=torch.float32, device=q.device)
+    out = torch.empty((m, k), dtype=dtype, device=q.device)
+    _lib.check(_lib.launch("hn_dequantize_fp4", q.device, q.data_ptr(), q.stride(0), s.data_ptr(),
+                           None if r is None else r.data_ptr(), m, k, kp, code, out.data_ptr(), k, _lib.DTYPE[dtype]),
+               "dequantize_fp4")
+    return out
+
+
+def fp4_gemm(qa, sa, ra, qw, sw, rw, bias=None, out_dtype=torch.bfloat16, kind="nvfp4", out=None):
+    """The product of two operands of `quantize_fp4`: (qa, sa, ra) [M, K] activations, (qw, sw, rw) [N, K] weights -> [M, N] in
+    `out_dtype` (bf16, fp16, fp32), a . w^T (+ bias [N] in one of these types), summed in fp32 on the tensor cores with the block
+    scales, rounded once. `ra`, `rw` None: row scales of 1.
+
+    `out`: a caller-owned [M, N] destination of `out_dtype` with unit column stride (rows may be strided)."""
+    code = _fp4_kind(kind, "fp4_gemm")
+    if not (qa.is_cuda and qw.is_cuda and sa.is_cuda and sw.is_cuda):
+        _lib.require_cuda(qa, qw, sa, sw)
+    qa, sa, ra = _fp4_operand(qa, sa, ra, kind, "fp4_gemm", "a")
+    qw, sw, rw = _fp4_operand(qw, sw, rw, kind, "fp4_gemm", "w")
+    m, n, half = qa.shape[0], qw.shape[0], qa.shape[1]
+    device = qa.device
+    if qw.shape[1] != half:
+        raise ValueError(f"fp4_gemm: a has {2 * half} columns, w {2 * qw.shape[1]}")
+    if n == 0:
+        raise ValueError("fp4_gemm: w has no rows")
+    if qw.device != device:
+        raise RuntimeError(f"fp4_gemm: a on {device}, w on {qw.device}")
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"fp4_gemm: out_dtype {out_dtype} (bf16, fp16 or fp32)")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise ValueError(f"fp4_gemm: bias must be bf16, fp16 or fp32 [{n}], got {bias.dtype} {tuple(bias.shape)}")
+        if bias.device != device:
+            raise RuntimeError(f"fp4_gemm: a on {device}, bias on {bias.device}")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=device)
+    elif out.shape != (m, n) or out.dtype != out_dtype or out.device != device or (n > 1 and out.stride(1) != 1) or \
+            (m > 1 and out.stride(0) < n):
+        raise ValueError(f"fp4_gemm: out must be a {out_dtype} [{m}, {n}] tensor with unit column stride on {device}")
+    _lib.check(_lib.launch("hn_fp4_gemm", device, qa.data_ptr(), qa.stride(0), sa.data_ptr(),
+                           None if ra is None else ra.data_ptr(), qw.data_ptr(), qw.stride(0), sw.data_ptr(),
+                           None if rw is None else rw.data_ptr(), None if bias is None else bias.data_ptr(),
+                           0 if bias is None else _lib.DTYPE[bias.dtype], out.data_ptr(), max(out.stride(0), n),
+                           _lib.DTYPE[out_dtype], m, n, 2 * half, code), "fp4_gemm")
+    return out
+
+
+def fp4_linear(x, qw, sw, rw=None, bias=None, kind="nvfp4"):
+    """F.linear with 4-bit weights, as `block_linear` has it for 8-bit ones: x [..., K] -> [..., N] in x's dtype (bf16, fp16 or
+    fp32), the activations quantized on the way."""
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"fp4_linear: x must be bf16, fp16 or fp32, got {x.dtype}")
+    shape = x.shape
+    x2 = x.reshape(-1, shape[-1])
+    if qw.dim() != 2 or (shape[-1] + 31) // 32 * 16 != qw.shape[1]:
+        raise ValueError(f"fp4_linear: x {tuple(shape)} does not fit codes {tuple(qw.shape)}")
+    return fp4_gemm(*quantize_fp4(x2, kind), qw, sw, rw, bias, x.dtype, kind).reshape(*shape[:-1], qw.shape[0])

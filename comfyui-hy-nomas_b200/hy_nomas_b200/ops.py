@@ -93,3 +93,37 @@ def decoder_mlp(x, norm_weight, gate_up, down, eps=1e-6):
     hq, hs = fused.silu_mul_quant(gu[:, :inter], gu[:, inter:], kind="fp8")
     y = block_gemm(hq, hs, down[0], down[1], kind="fp8")
     return x + y.view(shape)
+
+
+def tile_fp4_scales(scales):
+    """Block scales [rows, groups] of 4-bit codes, one byte each (uint8, or float8_e4m3fn), as a checkpoint stores them, in the
+    tensor cores' order: uint8 [rows / 128, groups / 4, 512] (rounded up, zeros behind the ends), where row 32 i + r of a block of 128
+    and group j of a block of four are byte 16 r + 4 i + j. Done once, when weights are loaded."""
+    if scales.dim() != 2 or scales.element_size() != 1:
+        raise ValueError(f"tile_fp4_scales: one byte per scale [rows, groups] expected, got {scales.dtype} {tuple(scales.shape)}")
+    b = scales.contiguous().view(torch.uint8)
+    rows, groups = b.shape
+    b = F.pad(b, (0, -groups % 4, 0, -rows % 128))
+    return b.view(b.shape[0] // 128, 4, 32, b.shape[1] // 4, 4).permute(0, 3, 2, 1, 4).reshape(
+        b.shape[0] // 128, b.shape[1] // 4, 512).contiguous()
+
+
+def untile_fp4_scales(tiled, rows, groups):
+    """`tile_fp4_scales` back: uint8 [rows, groups]."""
+    if tiled.dtype != torch.uint8 or tiled.dim() != 3 or tiled.shape[2] != 512 or not 0 <= rows <= 128 * tiled.shape[0] or \
+            not 0 <= groups <= 4 * tiled.shape[1]:
+        raise ValueError(f"untile_fp4_scales: no [{rows}, {groups}] scales in {tiled.dtype} {tuple(tiled.shape)}")
+    a, b, _ = tiled.shape
+    return tiled.reshape(a, b, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(a * 128, b * 4)[:rows, :groups].contiguous()
+
+
+def stack_fp4_linears(*linears):
+    """4-bit linears (codes, scales, row scales) with the same K, stacked along N into one, as `stack_fp8_linears`. All but the last
+    need whole scale tiles: N a multiple of 128."""
+    if any(q.shape[0] % 128 for q, _, _ in linears[:-1]):
+        raise ValueError("stack_fp4_linears: all linears but the last need a multiple of 128 channels")
+    rows = [r for _, _, r in linears]
+    if any(r is None for r in rows) and any(r is not None for r in rows):
+        raise ValueError("stack_fp4_linears: row scales on some of the linears only")
+    return (torch.cat([q for q, _, _ in linears]), torch.cat([s for _, s, _ in linears]),
+            None if rows[0] is None else torch.cat(rows))

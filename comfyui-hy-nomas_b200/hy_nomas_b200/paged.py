@@ -7,6 +7,7 @@ and a branch of a sequence shares its parent's full pages instead of copying the
     cache = KVCache(layers, pages, heads, page, slots, width, kind="int8")
     cache.extend(rows, n)                        # room for n more tokens of each row
     cache.append(layer, k, v, rows)              # k, v [B, n, heads, 128]: those tokens, layer by layer
+    q = cache.append_rotated(layer, q, k, v, rows, rot, q_norm, k_norm)   # ... or with norm and rotation on the way
     cache.fork(parents, children)                # children become branches: only a partial last page is copied
     out = attention(q, cache, layer, rows, shared=tokens)     # the shared tokens are read once for all rows
     cache.free(rows)
@@ -23,7 +24,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, rotary
 
 HEAD_DIM = 128
 
@@ -138,6 +139,42 @@ class KVCache:
         vb, vt, vh, _ = v.stride()
         _lib.check(_lib.launch("hn_cache_append", self.device, self._ref, layer, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt,
                                vh, rows.data_ptr(), k.shape[0], k.shape[1]), "cache.append")
+
+    def append_rotated(self, layer, q, k, v, rows, rot, q_norm=None, k_norm=None, eps=1e-6, positions=None):
+        """`append` of k with its per-head RMSNorm (`k_norm` [128], None: none) and rotation (`rotary.Rotary`), and of v as it is, in
+        one pass with the norm and rotation of q [B, n, H, 128] -> q' [B, n, H, 128] bf16, for `attention`. Positions are the
+        tokens' places in their rows, or `positions` [B, n] or [n]. All in fp32; K is rounded once, to the cache's format.
+        Rows that `append` leaves out are left out and counted in the same way; their q' means nothing."""
+        what = "append_rotated"
+        if not (q.is_cuda and k.is_cuda and v.is_cuda):
+            _lib.require_cuda(q, k, v)
+        rows, device = self._ids(rows, what), self.device
+        if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+            raise TypeError(f"{what}: bf16 expected, got {q.dtype}, {k.dtype} and {v.dtype}")
+        b = rows.numel()
+        if k.dim() != 4 or k.shape != v.shape or k.shape[2] != self.heads or k.shape[3] != HEAD_DIM or k.shape[0] != b or \
+                q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != HEAD_DIM or q.shape[2] == 0:
+            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must be "
+                             f"[{b}, n, H, {HEAD_DIM}] and [{b}, n, {self.heads}, {HEAD_DIM}]")
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"{what}: layer {layer} of {self.layers}")
+        if any(t.device != device for t in (q, k, v)):
+            raise RuntimeError(f"{what}: q on {q.device}, k on {k.device} and v on {v.device}, the cache is on {device}")
+        rotary.check_rotary(rot, HEAD_DIM, device, what)
+        n, h = k.shape[1], q.shape[2]
+        ptr, pb, pt, wide, positions = (None, 0, 0, 0, None) if positions is None else \
+            rotary.positions_of(positions, b, n, device, what)
+        wq, wk = rotary.norm_weight(q_norm, HEAD_DIM, device, what), rotary.norm_weight(k_norm, HEAD_DIM, device, what)
+        q, k, v = _operand(q), _operand(k), _operand(v)
+        out = torch.empty((b, n, h, HEAD_DIM), dtype=torch.bfloat16, device=device)
+        dim, layout, factor = rot._args
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        _lib.check(_lib.launch(
+            "hn_cache_append_rotated", device, self._ref, layer, q.data_ptr(), qs[0], qs[1], qs[2], h, k.data_ptr(), ks[0], ks[1],
+            ks[2], v.data_ptr(), vs[0], vs[1], vs[2], rows.data_ptr(), b, n, ptr, pb, pt, wide, rot.freq.data_ptr(), dim, layout,
+            factor, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, out.data_ptr()),
+            "cache.append_rotated")
+        return out
 
     def free(self, rows):
         """The listed rows drop their pages and become empty (a row listed twice, once). A page is free again when its last row

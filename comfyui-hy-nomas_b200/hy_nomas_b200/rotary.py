@@ -1,0 +1,171 @@
+"""Rotary positions computed on the way: heads of any width up to 256, both pair layouts, a part of the head, scaled contexts.
+
+`fused.qk_norm_rope` and `fused.pixelumm_qk` take tables of cos and sin [tokens, 128], as the reference makes them
+(hy_nomas/fused.py:65-186). Here a call takes the tokens' positions, so that no table is made or read, and a token far into
+a long context is turned as exactly as the first:
+
+    rot = Rotary(128, theta=10000.0, layout="half")                          # once
+    q = rotate(q, positions, rot, q_norm)                                    # RMSNorm per head, then the rotation
+    q = cache.append_rotated(layer, q, k, v, rows, rot, q_norm, k_norm)      # paged.KVCache: k and v into the pages, too
+
+Inference only, as the rest of the framework.
+"""
+import math
+
+import torch
+
+from . import _lib
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {"linear": {"factor"}, "ntk": {"factor"}, "yarn": {"factor", "original", "beta_fast", "beta_slow", "attention_factor"}}
+
+
+def frequencies(dim, theta=10000.0, scaling=None):
+    """(radians per position of the dim / 2 pairs in 64 bits, on the CPU; the factor on cos and sin). `scaling`: None, or a dict
+    {"type": ..., "factor": f}:
+      "linear"  positions divided by f
+      "ntk"     theta * f^(dim / (dim - 2)): the slowest pair is slowed f times, the fastest kept
+      "yarn"    (Peng et al., arXiv 2309.00071) pairs that turn more than `beta_fast` (32) times over `original` positions are kept,
+                those that turn less than `beta_slow` (1) times are slowed f times, a ramp between; cos and sin times
+                `attention_factor` (0.1 ln f + 1)"""
+    if dim < 8 or dim > 256 or dim % 8:
+        raise ValueError(f"rotary: {dim} rotated columns (a multiple of 8 up to 256)")
+    if not (math.isfinite(theta) and theta > 1):
+        raise ValueError(f"rotary: theta {theta}")
+    scaling = dict(scaling or {})
+    kind = scaling.pop("type", None)
+    if kind not in _SCALINGS and (kind is not None or scaling):
+        raise ValueError(f"rotary: scaling type {kind!r} (linear, ntk or yarn)")
+    if kind is not None and (set(scaling) - _SCALINGS[kind] or "factor" not in scaling or (kind == "yarn" and "original" not in scaling)):
+        raise ValueError(f"rotary: scaling {kind} with {sorted(scaling)}")
+    if any(not (math.isfinite(v) and v > 0) for v in scaling.values()):
+        raise ValueError(f"rotary: scaling {scaling} must be positive numbers")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    factor = scaling.get("factor", 1.0)
+    if kind == "ntk":
+        theta = theta * factor ** (dim / (dim - 2))
+        if theta <= 1:
+            raise ValueError(f"rotary: ntk factor {factor} leaves theta {theta}")
+    freq = theta ** (-2.0 * i / dim)
+    if kind == "linear":
+        freq = freq / factor
+    if kind != "yarn":
+        return freq, 1.0
+
+    def column(turns):      # the (fractional) pair that turns so many times over the original context, in columns / 2
+        return dim * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
+    low = max(math.floor(column(scaling.get("beta_fast", 32.0))), 0)
+    high = min(math.ceil(column(scaling.get("beta_slow", 1.0))), dim - 1)
+    ramp = ((i - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+    return freq * (1 - ramp) + freq / factor * ramp, scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0)
+
+
+class Rotary:
+    """What turns the first `dim` columns of a head by position. `layout` "half": column i pairs with i + dim / 2; "interleaved": 2 i
+    with 2 i + 1. `scaling`: see `frequencies`; or give `freq`, radians per position [dim / 2], and `factor` yourself."""
+
+    def __init__(self, dim, theta=10000.0, layout="half", scaling=None, device="cuda", freq=None, factor=1.0):
+        if layout not in LAYOUTS:
+            raise ValueError(f"Rotary: layout {layout!r} (half or interleaved)")
+        if freq is None:
+            freq, factor = frequencies(dim, theta, scaling)
+        else:
+            if scaling is not None:
+                raise ValueError("Rotary: freq and scaling")
+            frequencies(dim)                                    # the checks of dim
+            freq = torch.as_tensor(freq, dtype=torch.float64).cpu()
+            if freq.shape != (dim // 2,) or not bool(torch.isfinite(freq).all()):
+                raise ValueError(f"Rotary: freq must be {dim // 2} finite numbers")
+        if not math.isfinite(factor):
+            raise ValueError(f"Rotary: factor {factor}")
+        self.dim, self.layout, self.factor, self.radians = dim, layout, float(factor), freq
+        # fractions of a turn times 2^64, as signed 64-bit integers: what is past a whole turn does not matter
+        turns = [round(math.ldexp(f / (2 * math.pi), 64)) % 2 ** 64 for f in freq.tolist()]
+        self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self._args = (dim, LAYOUTS[layout], self.factor)
+
+
+def positions_of(p, batch, tokens, device, what):
+    """(pointer, batch stride, token stride, 1 if int64, the tensor) of positions [batch, tokens] or [tokens]."""
+    if not isinstance(p, torch.Tensor) or p.is_floating_point() or p.is_complex() or p.dtype == torch.bool:
+        raise TypeError(f"{what}: positions must be a tensor of integers")
+    if p.dtype not in (torch.int32, torch.int64):
+        p = p.to(torch.int32 if p.element_size() < 4 else torch.int64)
+    if p.device != device:
+        raise RuntimeError(f"{what}: positions on {p.device}, the heads on {device}")
+    if p.shape == (tokens,):
+        return p.data_ptr(), 0, p.stride(0), int(p.dtype == torch.int64), p
+    if p.shape != (batch, tokens):
+        raise ValueError(f"{what}: positions {tuple(p.shape)} must be [{batch}, {tokens}] or [{tokens}]")
+    return p.data_ptr(), p.stride(0), p.stride(1), int(p.dtype == torch.int64), p
+
+
+def norm_weight(w, dim, device, what):
+    """A per-head norm weight as an aligned bf16 tensor, or None."""
+    if w is None:
+        return None
+    if w.shape != (dim,):
+        raise ValueError(f"{what}: norm weight {tuple(w.shape)} must be [{dim}]")
+    if w.device != device:
+        raise RuntimeError(f"{what}: norm weight on {w.device}, the heads on {device}")
+    if w.dtype != torch.bfloat16:
+        w = w.to(torch.bfloat16)
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else _lib.dense(w)
+
+
+def check_rotary(rot, dim, device, what):
+    if not isinstance(rot, Rotary):
+        raise TypeError(f"{what}: a Rotary is needed, got {type(rot).__name__}")
+    if rot.dim > dim:
+        raise ValueError(f"{what}: {rot.dim} rotated columns of a head of {dim}")
+    if rot.freq.device != device:
+        raise RuntimeError(f"{what}: the Rotary is on {rot.freq.device}, the heads on {device}")
+
+
+def _steps8(t):
+    return t.stride(3) == 1 and not (t.stride(0) | t.stride(1) | t.stride(2)) % 8 and t.data_ptr() % 16 == 0
+
+
+def _span(t):
+    """First byte and the byte after the last of a tensor that is not empty."""
+    at = t.data_ptr()
+    lo = sum(min(0, s * (n - 1)) for s, n in zip(t.stride(), t.shape))
+    hi = sum(max(0, s * (n - 1)) for s, n in zip(t.stride(), t.shape))
+    return at + lo * t.element_size(), at + (hi + 1) * t.element_size()
+
+
+def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
+    """x [B, L, H, D] (bf16, fp16 or fp32; D a multiple of 8 up to 256; any strides in steps of 8 elements, the last dimension
+    contiguous) at integer positions [B, L] or [L] -> [B, L, H, D] of x's dtype: RMSNorm over each head times `weight` [D] (None: no
+    norm), then the rotation of its first rot.dim columns, in fp32 with one rounding. `out`: a caller-owned tensor like x, or x."""
+    what = "rotate"
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    device = x.device
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"rotate: x must be bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() != 4 or x.shape[3] % 8 or not 8 <= x.shape[3] <= 256:
+        raise ValueError(f"rotate: x must be [B, L, H, D] with D a multiple of 8 up to 256, got {tuple(x.shape)}")
+    b, l, h, d = x.shape
+    check_rotary(rot, d, device, what)
+    ptr, pb, pl, wide, keep = positions_of(positions, b, l, device, what)
+    w = norm_weight(weight, d, device, what)
+    src = x if _steps8(x) else _lib.dense(x)
+    if out is None:
+        out = torch.empty((b, l, h, d), dtype=x.dtype, device=device)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != device or not _steps8(out):
+            raise ValueError(f"rotate: out must be {x.dtype} {tuple(x.shape)} on {device} in steps of 8 elements, 16-byte aligned")
+        if out.numel():
+            if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+                raise ValueError("rotate: the heads of out overlap")
+            same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
+            (a0, a1), (b0, b1) = _span(src), _span(out)
+            if not same and a0 < b1 and b0 < a1:
+                raise ValueError("rotate: out must be x itself or lie apart from it")
+    dim, layout, factor = rot._args
+    xs, os = src.stride(), out.stride()
+    _lib.check(_lib.launch("hn_rotate", device, src.data_ptr(), xs[0], xs[1], xs[2], _lib.DTYPE[x.dtype], ptr, pb, pl, wide,
+                           rot.freq.data_ptr(), dim, layout, factor, None if w is None else w.data_ptr(), eps, b, l, h, d,
+                           out.data_ptr(), os[0], os[1], os[2]), what)
+    return out

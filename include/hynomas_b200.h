@@ -61,6 +61,10 @@ typedef enum {
 /* quantized code types */
 #define HN_KIND_INT8 0
 #define HN_KIND_FP8E4M3 1
+/* 4-bit code types (hn_quantize_fp4, hn_dequantize_fp4, hn_fp4_gemm): e2m1 codes with a scale 2^e per 32 columns, or an e4m3
+ * scale per 16 columns and an fp32 scale per row */
+#define HN_KIND_MXFP4 2
+#define HN_KIND_NVFP4 3
 
 /* scale layouts of the block-scaled GEMM (hn_block_gemm) */
 #define HN_SCALE_GROUP 0  /* one fp32 per row and 128-wide K group: [rows, K/128] (the reference layout) */
@@ -71,6 +75,10 @@ typedef enum {
 #define HN_EPI_NONE 0
 #define HN_EPI_GELU 1
 #define HN_EPI_GELU_QUANT 2
+
+/* columns of a head that a rotation pairs: i with i + rot / 2, or 2 i with 2 i + 1 */
+#define HN_ROPE_HALF 0
+#define HN_ROPE_INTERLEAVED 1
 
 /* Message of the last failed call on this thread ("" if none). */
 const char *hn_last_error(void);
@@ -405,6 +413,53 @@ int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, i
                        const int32_t *rows, int64_t B, int64_t Lq, int64_t H, int64_t D, int64_t shared, int causal,
                        float scale, void *out, int64_t o_bs, int64_t o_ls, int64_t o_hs, float *lse, void *ws,
                        int64_t ws_bytes, void *stream);
+
+/*
+ * Linears on 4-bit codes with block scales. No reference counterpart: its linears are int8 and e4m3 (hy_nomas/kernels.py:19-226).
+ * A row of K columns is stored as Kp = K rounded up to 32, the codes beyond K zero: q [rows][Kp / 2] bytes, the even column in
+ * the low four bits, rows ldq (lda, ldw) BYTES apart, 16-byte aligned. A code is e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign.
+ * Scale bytes lie in tiles of 128 rows x 4 groups, 512 bytes each, 16-byte aligned, [ceil(rows / 128)][ceil(Kp / span)] of them,
+ * span = 128 columns (HN_KIND_MXFP4) or 64 (HN_KIND_NVFP4); row r of a tile, group g: byte 16 (r % 32) + 4 (r / 32) + g. Groups
+ * between Kp and the last tile's end hold zeros.
+ *   HN_KIND_MXFP4: 2^(byte - 127) per 32 columns, byte 255: NaN; row scales NULL
+ *   HN_KIND_NVFP4: e4m3 per 16 columns, and an fp32 scale per row (r, ra, rw [rows]; NULL in hn_fp4_gemm: all 1)
+ *
+ * hn_quantize_fp4: x [M, K] bf16, fp16 or fp32, rows ldx elements apart. MX: s = 2^(floor(log2 max|x|) - 2) of the group, 1 for
+ *   zeros; codes of x / s, to the nearest, ties to the even code, beyond 6 to 6. NV: top = max|row|, r = top / 2688; s = e4m3((0.875
+ *   max|x|) / (top 2^-9)), codes of (0.65625 x) / (s top 2^-12); a row with top < 2^-100 counts as zeros (r = 1). A NaN or an
+ *   infinity makes its group's scale (MX) or its row's (NV) NaN, with zero codes. Rows of the last tile past M get zero scales.
+ * hn_dequantize_fp4: code * RN(scale * row scale), rounded to out_dtype; K columns of rows of Kp codes.
+ * hn_fp4_gemm: out[m, n] = ra[m] rw[n] sum_k a w (+ bias[n]), the sum with its block scales in fp32 on the tensor cores (few rows:
+ *   a read of the weights without them), one rounding to out_dtype (bf16, fp16, fp32). K is the operands' Kp, a multiple of 32.
+ */
+int hn_quantize_fp4(const void *x, int64_t ldx, int x_dtype, int64_t M, int64_t K, int kind, void *q, int64_t ldq, void *s,
+                    float *r, void *stream);
+int hn_dequantize_fp4(const void *q, int64_t ldq, const void *s, const float *r, int64_t M, int64_t K, int64_t Kp, int kind,
+                      void *out, int64_t ldo, int out_dtype, void *stream);
+int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, const void *qw, int64_t ldw, const void *sw,
+                const float *rw, const void *bias, int bias_dtype, void *out, int64_t ldo, int out_dtype, int64_t M, int64_t N,
+                int64_t K, int kind, void *stream);
+
+/*
+ * Rotation of heads by their tokens' positions, with the per-head RMSNorm before it (hy_nomas/fused.py:65-186 takes tables of
+ * cos and sin instead): y = R(pos) (x / sqrt(mean x^2 + eps) * weight), in fp32, rounded once. Pair i of the first `rot` columns
+ * turns by pos * freq[i] / 2^64 of a turn (the product modulo one turn is exact), cos and sin times `factor`; the other columns
+ * pass. layout HN_ROPE_*. weight bf16 [D], or NULL: no norm. pos int32, or int64 with pos_wide 1; any sign.
+ * x, out [B, L, H, D] of `dtype` (bf16, fp16, fp32), element strides for batch, token, head, multiples of 8; out may be x itself,
+ * else they do not overlap. D and rot multiples of 8, rot <= D <= 256. 16-byte aligned x, out, weight.
+ *
+ * hn_cache_append_rotated: hn_cache_append of R(pos) norm(k) and v, and R(pos) norm(q) into out [B, n, H, 128], dense bf16. pos
+ *   NULL: a token's place in its row (the first is 0); else [B, n] as above. q, k, v bf16 as in hn_cache_append; norm weights [128]
+ *   or NULL each. K is rounded once, to the cache's format. q is rotated for rows that are left out, too.
+ */
+int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype, const void *pos, int64_t p_bs, int64_t p_ls,
+              int pos_wide, const int64_t *freq, int64_t rot, int layout, float factor, const void *weight, float eps, int64_t B,
+              int64_t L, int64_t H, int64_t D, void *out, int64_t o_bs, int64_t o_ls, int64_t o_hs, void *stream);
+int hn_cache_append_rotated(const hn_kv_cache *cache, int64_t layer, const void *q, int64_t q_bs, int64_t q_ts, int64_t q_hs,
+                            int64_t H, const void *k, int64_t k_bs, int64_t k_ts, int64_t k_hs, const void *v, int64_t v_bs,
+                            int64_t v_ts, int64_t v_hs, const int32_t *rows, int64_t B, int64_t n, const void *pos, int64_t p_bs,
+                            int64_t p_ts, int pos_wide, const int64_t *freq, int64_t rot, int layout, float factor,
+                            const void *q_weight, const void *k_weight, float eps, void *out, void *stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
