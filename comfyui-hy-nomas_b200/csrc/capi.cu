@@ -120,13 +120,18 @@ static bool scale_strides_ok(int64_t rows, int64_t groups, int64_t rs, int64_t g
 
 // The device that owns `stream` made current for the duration of an entry point (the caller's current device
 // is put back on exit), so a launch, the SM count and the architecture check all refer to the stream's
-// device whichever device the calling thread had current. The NULL stream keeps the current device.
+// device whichever device the calling thread had current. The NULL stream keeps the current device, and so does a
+// stream that is being captured into a graph, which may not be asked for its device (a launch from another
+// device is then refused by the check of the data's device, or by CUDA).
 struct StreamDevice {
     int prev = -1;
     cudaError_t err = cudaSuccess;
     explicit StreamDevice(void *stream) {
         if (stream == nullptr) return;
         int want = 0, cur = 0;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        err = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture);
+        if (err != cudaSuccess || capture != cudaStreamCaptureStatusNone) return;
         err = cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &want);
         if (err != cudaSuccess) return;
         err = cudaGetDevice(&cur);
