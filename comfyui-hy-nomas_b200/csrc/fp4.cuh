@@ -71,15 +71,16 @@ struct Result {
     int64_t ldo;
     int out_dtype;
 };
+__device__ __forceinline__ float bias_at(const Result &o, int64_t n) {
+    return o.bias_dtype == 2 ? static_cast<const float *>(o.bias)[n]
+         : o.bias_dtype == 0 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(o.bias)[n])
+                             : __half2float(static_cast<const __half *>(o.bias)[n]);
+}
 // fp32 result of column n; ra: the row's scale, or 1
 __device__ __forceinline__ float finish(const Result &o, float sum, float ra, int64_t n) {
     if (o.ra) sum = __fmul_rn(sum, ra);
     if (o.rb) sum = __fmul_rn(sum, o.rb[n]);
-    if (!o.bias) return sum;
-    const float b = o.bias_dtype == 2 ? static_cast<const float *>(o.bias)[n]
-                  : o.bias_dtype == 0 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(o.bias)[n])
-                                      : __half2float(static_cast<const __half *>(o.bias)[n]);
-    return __fadd_rn(sum, b);
+    return o.bias ? __fadd_rn(sum, bias_at(o, n)) : sum;
 }
 __device__ __forceinline__ void store_result(const Result &o, int64_t at, float v) {
     if (o.out_dtype == 0) static_cast<__nv_bfloat16 *>(o.out)[at] = __float2bfloat16_rn(v);

@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
             tc_fence_after();
             if (lane == 0) {
                 const uint32_t at = sbase + stage * C::STAGE, sf = tmem + C::SFC + stage * 8 * C::TILES;
-                const int left = p.Kp - kt * KB;            // a stage's scale columns are its own: the MMAs that read them last
-#pragma unroll                                              // are done when its operands are
+                // a stage's scale columns are its own: the MMAs that read them last are done when its operands are
+#pragma unroll
                 for (int j = 0; j < C::TILES; ++j) {
                     copy_scale(sf + 4 * j, sdesc_scale(at + 2 * C::OP + j * TILE));
                     copy_scale(sf + 4 * (C::TILES + j), sdesc_scale(at + 2 * C::OP + C::SF + j * TILE));
@@ -171,7 +171,6 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
                 const uint64_t ad = sdesc(at), bd = sdesc(at + C::OP);
 #pragma unroll
                 for (int k = 0; k < KB / 64; ++k) {
-                    if (64 * k >= left) break;
                     const int j = KIND == NV ? k : k >> 1;
                     const uint32_t id = KIND == NV ? idesc : idesc | (k & 1) << 5 | (uint32_t)(k & 1) << 30;
                     mma<KIND>(tmem + C::ACC, ad + 2 * k, bd + 2 * k, id, sf + 4 * j, sf + 4 * (C::TILES + j),
@@ -246,6 +245,406 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
 }
 
 // ---------------------------------------------------------------------------------------------------
+// Many rows: tiles of 256 x 256 outputs, a pair of CTAs (cta_group::2) on each, one pair per two SMs, over the tiles in turn.
+// Each CTA brings 128 rows of A and 128 of B into its shared memory, the pair's MMA reads both halves, so an operand byte from
+// L2 serves twice the outputs of a tile that one SM holds alone. A step is 256 columns; the full barriers are the first CTA's, on
+// which the copies of both complete. Scales of all 256 rows of B are brought to both CTAs.
+//   warps 0, 1, 2   codes of A, codes of B, scales (each CTA its own; a request costs its thread some 35 ns and a wait 100 and
+//                   more, so one warp for all three would be the bound: 412 ns a step)
+//   warps 4 to 7    (first CTA) scales to tensor memory, every fourth step each: a tcgen05.cp of 512 bytes takes its thread some
+//                   30 ns, 12 of them a step. A stage has scale columns of its own, so they run ahead of the MMAs
+//   warp 3          (first CTA) the MMAs. It meets warps 4 to 7 at named barriers: its own look at a barrier in shared memory would
+//                   wait until its MMAs have read their operands. Its four MMAs a step have no branch between them
+//   warps 8 to 15   the sums: a thread holds 128 columns of a row in registers, hands tensor memory back, and only then scales,
+//                   rounds and writes, beside the next tile's MMAs; 64 bytes of a row at a time go through shared memory, so that a
+//                   row's outputs leave as whole sectors
+// Bound by the tensor cores and what keeps them waiting. A step's MMAs are 512 clocks. Measured, 18944 x 4096 x 16384 NV (16 tiles
+// a pair, 1024 steps): 495 us. Timed apart, in ns a step: MMAs alone 332, with their commits 362, with the barriers 399, with the
+// loads 418, with the scales' copies 483; a tile's end costs 2 us (the wake of the epilogue, tensor memory's read, the issuer's
+// wake). Tried and slower (20240 x 4096 x 16384 NV, us): scale copies by the MMAs' thread 877, by one other warp 699, by two 593;
+// a branch for the last columns between the MMAs 600 (without: 552); scales written to tensor memory from registers 1676.
+template <int KIND> struct Wide {
+    static constexpr int BM = 256, BN = 256;
+    static constexpr int TILES = KB / SPAN<KIND>;
+    static constexpr int OP = 128 * 128, SFA = TILES * TILE, SFB = 2 * TILES * TILE;
+    static constexpr int STAGES = 5, STAGE = 2 * OP;            // codes of both operands
+    static constexpr int SLOTS = 6, SLOT = SFA + SFB;           // scales on their way to tensor memory
+    static constexpr int ACC = 0, SFC = BN, SFW = 12 * TILES;   // tensor memory columns; SFW: a stage's scales
+    static_assert(SFC + STAGES * SFW <= 512, "tensor memory");
+    static constexpr int EPI = 8, PITCH = 80;                   // warps; bytes a row of their chunks of 64
+    static constexpr int OFF_SF = STAGES * STAGE, OFF_EPI = OFF_SF + SLOTS * SLOT;
+    static constexpr int OFF_COLS = OFF_EPI + EPI * 32 * PITCH;                             // column scales and bias: [2][2][256]
+    static constexpr int OFF_BAR = OFF_COLS + 2 * 2 * 256 * 4;
+    static constexpr int OFF_MISC = OFF_BAR + 8 * (2 * STAGES + 2 * SLOTS + 3);
+    static constexpr int SMEM = OFF_MISC + 16 + 1024;
+    static_assert(SMEM <= 232448, "shared memory");
+    static constexpr int THREADS = 256 + 32 * EPI;
+    static constexpr int CP = 4;                                // warps that copy scales
+    // registers a thread: launched with 128 (512 x 128 = 65536), the epilogue's warps take over what the others leave
+    static constexpr int REGS = 56, EPI_REGS = 200;
+    static_assert(THREADS == 512 && 256 * REGS + 32 * EPI * EPI_REGS <= THREADS * 128, "registers");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+// tile loads into this CTA's shared memory that complete on a barrier of either CTA of the pair
+__device__ __forceinline__ void pair_load_2d(const CUtensorMap *map, uint32_t dst, uint32_t bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_load_3d(const CUtensorMap *map, uint32_t dst, uint32_t bar, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(bar), "r"(0), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_copy_scale(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int KIND>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+    if (KIND == NV)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                     ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                     ::"r"(d), "l"(ad), "l"(bd), "r"(idesc), "r"(acc), "r"(sa), "r"(sb) : "memory");
+}
+// arrives on the barrier at this offset in both CTAs when the MMAs so far are done
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// ... in this CTA alone
+__device__ __forceinline__ void pair_commit1(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// a wait of a step's chain: some looks before the clock of the bounded wait is read (504 -> 495 us at 18944 x 4096 x 16384)
+__device__ __forceinline__ bool spin_wait(int lane, uint32_t bar, uint32_t parity, volatile int *abort_flag, int *err) {
+    bool ok = true;
+    if (lane == 0) {
+        bool in = false;
+#pragma unroll 1
+        for (int i = 0; i < 200 && !in; ++i) in = mbar_try(bar, parity);
+        if (!in) ok = mbar_wait(bar, parity, abort_flag, WAIT_NS, err);
+    }
+    return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+// W warps meet at named barrier 1: whether `stop` holds in any of them
+template <int W> __device__ __forceinline__ bool any_of(bool stop) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(stop ? 1u : 0u), "n"(32 * W) : "memory");
+    return r != 0;
+}
+// after a wait that gave up: time for the copies in flight, of both CTAs, to land
+__device__ __forceinline__ void land() {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 10000000ull) { }
+}
+
+// tile t -> (row tile, column tile): groups of `gn` column tiles, whose weights stay in L2 while the rows pass
+struct Raster {
+    int m_tiles, n_tiles, gn;
+};
+__device__ __forceinline__ void tile_at(const Raster &r, int t, int &mt, int &nt) {
+    const int g = t / (r.m_tiles * r.gn), in = t - g * r.m_tiles * r.gn;
+    const int width = r.n_tiles - g * r.gn < r.gn ? r.n_tiles - g * r.gn : r.gn;
+    mt = in / width;
+    nt = g * r.gn + in - mt * width;
+}
+
+// a pair's steps: the stages of its tiles, tile by tile
+struct Step {
+    int tile, kt, mt, nt;
+};
+__device__ __forceinline__ Step first_step(const Raster &r, int tile) {
+    Step s;
+    s.tile = tile; s.kt = 0;
+    tile_at(r, tile, s.mt, s.nt);
+    return s;
+}
+__device__ __forceinline__ void next_step(const Raster &r, Step &s, int kts, int pairs) {
+    if (++s.kt < kts) return;
+    s.kt = 0;
+    s.tile += pairs;
+    if (s.tile < r.m_tiles * r.n_tiles) tile_at(r, s.tile, s.mt, s.nt);
+}
+
+struct WideParams {
+    Result o;
+    int vec;
+    int M, N, Kp, tiles;
+    Raster raster;
+    int *err;
+};
+
+// EB: bytes of an output
+template <int KIND, int EB>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS, 1)
+    k_fp4_gemm_wide(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const WideParams p) {
+    using C = Wide<KIND>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sbase = smem_u32(smem);
+    const uint32_t bar_full = sbase + C::OFF_BAR, bar_empty = bar_full + 8 * C::STAGES;
+    const uint32_t bar_sfull = bar_empty + 8 * C::STAGES, bar_sempty = bar_sfull + 8 * C::SLOTS;
+    const uint32_t bar_tfull = bar_sempty + 8 * C::SLOTS, bar_tempty = bar_tfull + 8, bar_drain = bar_tempty + 8;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int kts = (p.Kp + KB - 1) / KB;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(bar_full + 8 * s, 3);         // A, B, and their scales in tensor memory
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int s = 0; s < C::SLOTS; ++s) { mbar_init(bar_sfull + 8 * s, 1); mbar_init(bar_sempty + 8 * s, 1); }
+        mbar_init(bar_tfull, 1);
+        mbar_init(bar_tempty, 2 * C::EPI);
+        mbar_init(bar_drain, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();                       // the other CTA's barriers are there before a copy completes on them
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int steps = (p.tiles - pair + pairs - 1) / pairs * kts;      // of this pair's tiles, one after the other
+    if (warp < 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS));
+    if (warp < 2) {
+        int stage = 0;
+        uint32_t phase = 0;
+        Step s = first_step(p.raster, pair);
+        bool ok = true;
+        for (int i = 0; i < steps; ++i) {
+            ok = spin_wait(lane, bar_empty + 8 * stage, phase ^ 1, abort_flag, p.err);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t at = sbase + stage * C::STAGE + warp * C::OP, fb = in_cta(bar_full + 8 * stage, 0);
+                if (rank == 0) mbar_arrive_tx(bar_full + 8 * stage, 2 * C::OP);
+                pair_load_2d(warp == 0 ? &tmA : &tmB, at, fb, s.kt * 128, (warp == 0 ? s.mt : s.nt) * 256 + rank * 128);
+            }
+            __syncwarp();
+            next_step(p.raster, s, kts, pairs);
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) land();
+    } else if (warp == 2) {
+        int slot = 0;
+        uint32_t phase = 0;
+        Step s = first_step(p.raster, pair);
+        bool ok = true;
+        for (int i = 0; i < steps; ++i) {
+            ok = spin_wait(lane, bar_sempty + 8 * slot, phase ^ 1, abort_flag, p.err);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t at = sbase + C::OFF_SF + slot * C::SLOT, fb = in_cta(bar_sfull + 8 * slot, 0);
+                if (rank == 0) mbar_arrive_tx(bar_sfull + 8 * slot, 2 * C::SLOT);
+                pair_load_3d(&tmSA, at, fb, s.kt * C::TILES, 2 * s.mt + rank);
+                pair_load_3d(&tmSB, at + C::SFA, fb, s.kt * C::TILES, 2 * s.nt);
+            }
+            __syncwarp();
+            next_step(p.raster, s, kts, pairs);
+            if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
+        }
+        if (!ok) land();
+    } else if (warp >= 4 && warp < 8 && rank == 0) {
+        // step i, every C::CP-th: its scales into the columns of its stage, when the MMAs that read them last are done; then, when they
+        // and the codes are in, the issuer's release. After a wait that gave up the steps that are left are only met, so that
+        // the issuer comes to its end.
+        int stage = (warp - 4) % C::STAGES, slot = (warp - 4) % C::SLOTS, last = -1;
+        uint32_t phase = (warp - 4) / C::STAGES & 1, sphase = (warp - 4) / C::SLOTS & 1, last_phase = 0;
+        bool ok = true;
+        for (int i = warp - 4; i < steps; i += C::CP) {
+            ok = ok && spin_wait(lane, bar_sfull + 8 * slot, sphase, abort_flag, p.err);
+            ok = ok && spin_wait(lane, bar_empty + 8 * stage, phase ^ 1, abort_flag, p.err);
+            if (ok) {
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t at = sbase + C::OFF_SF + slot * C::SLOT, sf = tmem + C::SFC + stage * C::SFW;
+#pragma unroll
+                    for (int j = 0; j < C::TILES; ++j) {        // of A 4 columns, of B 8 (its two blocks of 128 rows) a tile
+                        pair_copy_scale(sf + 4 * j, sdesc_scale(at + j * TILE));
+                        pair_copy_scale(sf + 4 * C::TILES + 8 * j, sdesc_scale(at + C::SFA + j * TILE));
+                        pair_copy_scale(sf + 4 * C::TILES + 8 * j + 4, sdesc_scale(at + C::SFA + (C::TILES + j) * TILE));
+                    }
+                    pair_commit1(bar_full + 8 * stage);
+                    pair_commit(bar_sempty + 8 * slot);
+                }
+                __syncwarp();
+                last = slot; last_phase = sphase;
+                ok = spin_wait(lane, bar_full + 8 * stage, phase, abort_flag, p.err);
+            }
+            if (ok) asm volatile("barrier.cta.arrive %0, 64;" ::"r"(2 + stage) : "memory");
+            else asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + stage) : "memory");
+            if ((stage += C::CP) >= C::STAGES) { stage -= C::STAGES; phase ^= 1; }
+            if ((slot += C::CP) >= C::SLOTS) { slot -= C::SLOTS; sphase ^= 1; }
+        }
+        if (last >= 0 && lane == 0) {
+            volatile int never = 0;
+            mbar_wait(bar_sempty + 8 * last, last_phase, &never, 100000000ull, p.err);
+        }
+        __syncwarp();
+    } else if (warp == 3 && rank == 0) {
+        constexpr uint32_t idesc = instruction<KIND, C::BM, C::BN>();
+        int stage = 0, kt = 0;
+        uint32_t tphase = 0;
+        bool ok = true;
+        for (int i = 0; i < steps; ++i) {
+            if (kt == 0 && ok) {
+                ok = warp_wait(lane, bar_tempty, tphase ^ 1, abort_flag, WAIT_NS, p.err);
+                tphase ^= 1;
+            }
+            asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + stage) : "memory");
+            if (ok) {
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t at = sbase + stage * C::STAGE, sf = tmem + C::SFC + stage * C::SFW;
+                    const uint64_t ad = sdesc(at), bd = sdesc(at + C::OP);
+#pragma unroll
+                    for (int k = 0; k < KB / 64; ++k) {
+                        const int j = KIND == NV ? k : k >> 1;
+                        const uint32_t id = KIND == NV ? idesc : idesc | (k & 1) << 5 | (uint32_t)(k & 1) << 30;
+                        pair_mma<KIND>(tmem + C::ACC, ad + 2 * k, bd + 2 * k, id, sf + 4 * j, sf + 4 * C::TILES + 8 * j,
+                                       (uint32_t)(kt > 0 || k > 0));
+                    }
+                    pair_commit(bar_empty + 8 * stage);
+                    if (kt == kts - 1) pair_commit(bar_tfull);
+                }
+                __syncwarp();
+            }
+            if (++kt == kts) kt = 0;
+            if (++stage == C::STAGES) stage = 0;
+        }
+        // what was issued finishes before tensor memory is released
+        if (lane == 0) {
+            volatile int never = 0;
+            pair_commit1(bar_drain);
+            mbar_wait(bar_drain, 0, &never, 100000000ull, p.err);
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::EPI_REGS));
+        const int q = warp & 3, half = (warp - 8) >> 2, thread = threadIdx.x - 256;
+        const uint32_t tcol = tmem + C::ACC + 128 * half + ((uint32_t)(32 * q) << 16);
+        const uint32_t tempty = in_cta(bar_tempty, 0);
+        uint8_t *chunk = smem + C::OFF_EPI + (warp - 8) * 32 * C::PITCH;
+        uint32_t tphase = 0;
+        int it = 0;
+        bool ok = true;
+        for (int tile = pair; tile < p.tiles; tile += pairs, ++it) {
+            int mt, nt;
+            tile_at(p.raster, tile, mt, nt);
+            const int m0 = mt * 256 + rank * 128 + 32 * q, n0 = nt * 256 + 128 * half;
+            // the tile's column scales and bias into shared memory (two tiles' places in turn) and the row's scale, beside its MMAs
+            float *cols = reinterpret_cast<float *>(smem + C::OFF_COLS) + (it & 1) * 512;
+            const int n = nt * 256 + thread;
+            cols[thread] = p.o.rb && n < p.N ? p.o.rb[n] : 1.0f;
+            cols[256 + thread] = p.o.bias && n < p.N ? bias_at(p.o, n) : 0.0f;
+            const float ra = p.o.ra && m0 + lane < p.M ? p.o.ra[m0 + lane] : 1.0f;
+            if (any_of<C::EPI>(!ok)) break;                 // all warps leave together: each waits for the others here
+            ok = warp_wait(lane, bar_tfull, tphase, abort_flag, 2 * WAIT_NS, p.err);
+            if (!ok) continue;
+            tphase ^= 1;
+            tc_fence_after();
+            uint32_t r[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(tcol + 32 * c, r[c]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(tempty);
+            const float *rb = cols + 128 * half, *bias = rb + 256;
+            constexpr int COLS = 64 / EB;               // of a chunk: 64 bytes a row
+#pragma unroll
+            for (int c = 0; c < 128 / COLS; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < COLS; j += 4) {
+                    const float4 s = *reinterpret_cast<const float4 *>(rb + COLS * c + j), b = *reinterpret_cast<const float4 *>(bias + COLS * c + j);
+                    const uint32_t *x = &r[(COLS * c + j) >> 5][(COLS * c + j) & 31];
+                    float v[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+                    if (KIND == NV) {
+                        v[0] = __fmul_rn(__fmul_rn(v[0], ra), s.x); v[1] = __fmul_rn(__fmul_rn(v[1], ra), s.y);
+                        v[2] = __fmul_rn(__fmul_rn(v[2], ra), s.z); v[3] = __fmul_rn(__fmul_rn(v[3], ra), s.w);
+                    }
+                    v[0] = __fadd_rn(v[0], b.x); v[1] = __fadd_rn(v[1], b.y); v[2] = __fadd_rn(v[2], b.z); v[3] = __fadd_rn(v[3], b.w);
+                    if (EB == 4) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[j + i] = __float_as_uint(v[i]);
+                    } else if (p.o.out_dtype == 0) {
+                        w[j >> 1] = pack_bf16_rn(v[0], v[1]);
+                        w[(j >> 1) + 1] = pack_bf16_rn(v[2], v[3]);
+                    } else {
+                        w[j >> 1] = pack_f16_rn(v[0], v[1]);
+                        w[(j >> 1) + 1] = pack_f16_rn(v[2], v[3]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4 *>(chunk + lane * C::PITCH + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                __syncwarp();
+                const int nc = n0 + COLS * c;
+                uint8_t *out = static_cast<uint8_t *>(p.o.out) + ((int64_t)m0 * p.o.ldo + nc) * EB;
+                if (p.vec) {
+                    const bool in = nc + 16 / EB * (lane & 3) < p.N;
+                    uint4 y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint4 *>(chunk + (8 * i + (lane >> 2)) * C::PITCH + 16 * (lane & 3));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 8 * i + (lane >> 2);
+                        if (in && m0 + row < p.M) *reinterpret_cast<uint4 *>(out + (int64_t)row * p.o.ldo * EB + 16 * (lane & 3)) = y[i];
+                    }
+                } else {
+#pragma unroll 8
+                    for (int i = 0; i < COLS; ++i) {
+                        const int row = (32 * i + lane) / COLS, col = (32 * i + lane) % COLS;
+                        if (nc + col >= p.N || m0 + row >= p.M) continue;
+                        if (EB == 2) *reinterpret_cast<uint16_t *>(out + ((int64_t)row * p.o.ldo + col) * 2) = *reinterpret_cast<uint16_t *>(chunk + row * C::PITCH + 2 * col);
+                        else *reinterpret_cast<uint32_t *>(out + ((int64_t)row * p.o.ldo + col) * 4) = *reinterpret_cast<uint32_t *>(chunk + row * C::PITCH + 4 * col);
+                    }
+                }
+            }
+        }
+        if (!ok) *abort_flag = 1;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();                       // neither CTA leaves while the other may reach its shared or tensor memory
+    cluster_wait();
+    tc_fence_after();
+    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---------------------------------------------------------------------------------------------------
 // host side
 
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -280,37 +679,82 @@ static bool map_scales(CUtensorMap *map, const void *base, uint64_t blocks, uint
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// outputs may be stored `bytes` at a time: rows begin on that boundary and are whole units
+static int whole_stores(const Fp4GemmArgs &a, int bytes) {
+    const int size = a.out_dtype == 2 ? 4 : 2;
+    return a.N * size % bytes == 0 && a.ldo * size % bytes == 0 && reinterpret_cast<uintptr_t>(a.out) % bytes == 0;
+}
+template <int KIND, typename C> static bool maps(const Fp4GemmArgs &a, int b_blocks, CUtensorMap (&m)[4]) {
+    const uint64_t sp = (uint64_t)cdiv(a.K, SPAN<KIND>);
+    return map_codes(&m[0], a.qa, a.M, a.K / 2, a.lda, 128) && map_codes(&m[1], a.qw, a.N, a.K / 2, a.ldw, 128) &&
+           map_scales(&m[2], a.sa, cdiv(a.M, 128), sp, C::TILES, 1) &&
+           map_scales(&m[3], a.sw, cdiv(a.N, 128), sp, C::TILES, b_blocks);
+}
+// the shared-memory opt-in, once per kernel and device
+template <typename K> static cudaError_t opt_in(K kernel, int bytes, bool (&done)[HN_MAX_DEV]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
+    if (done[dev]) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    done[dev] = e == cudaSuccess;
+    return e;
+}
+
+template <int KIND> static cudaError_t launch_wide(const Fp4GemmArgs &a, cudaStream_t st, const char **msg) {
+    using C = Wide<KIND>;
+    WideParams p;
+    cudaError_t e = device_error_word(err_slot(st), &p.err);
+    if (e != cudaSuccess) return e;
+    p.o = {a.ra, a.rw, a.bias, a.bias_dtype, a.out, a.ldo, a.out_dtype};
+    p.M = (int)a.M; p.N = (int)a.N; p.Kp = (int)a.K;
+    p.vec = whole_stores(a, 16);
+    p.raster.m_tiles = (int)cdiv(a.M, C::BM);
+    p.raster.n_tiles = (int)cdiv(a.N, C::BN);
+    p.tiles = p.raster.m_tiles * p.raster.n_tiles;
+    // the weights of a group of column tiles: 32 MB at most, so that they stay in L2
+    const int64_t fit = (32LL << 20) / (C::BN * (a.K / 2));
+    p.raster.gn = (int)(fit < 1 ? 1 : fit > p.raster.n_tiles ? p.raster.n_tiles : fit);
+    CUtensorMap m[4];
+    if (!maps<KIND, C>(a, 2, m)) {
+        *msg = "cuTensorMapEncodeTiled failed (pointer/stride alignment or driver entry point)";
+        return cudaErrorInvalidValue;
+    }
+    int pairs = num_sms() / 2;
+    if (pairs > p.tiles) pairs = p.tiles;
+    auto go = [&](auto kernel, bool (&done)[HN_MAX_DEV]) {
+        cudaError_t e = opt_in(kernel, C::SMEM, done);
+        if (e != cudaSuccess) return e;
+        kernel<<<2 * pairs, C::THREADS, C::SMEM, st>>>(m[0], m[1], m[2], m[3], p);
+        return cudaGetLastError();
+    };
+    static bool done2[HN_MAX_DEV], done4[HN_MAX_DEV];
+    return a.out_dtype == 2 ? go(k_fp4_gemm_wide<KIND, 4>, done4) : go(k_fp4_gemm_wide<KIND, 2>, done2);
+}
+
 template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t st, const char **msg) {
     using C = Cfg<KIND>;
+    if (cdiv(a.M, 256) * cdiv(a.N, 256) >= num_sms() / 2) return launch_wide<KIND>(a, st, msg);
     Params p;
     cudaError_t e = device_error_word(err_slot(st), &p.err);
     if (e != cudaSuccess) return e;
     p.o = {a.ra, a.rw, a.bias, a.bias_dtype, a.out, a.ldo, a.out_dtype};
     p.M = (int)a.M; p.N = (int)a.N; p.Kp = (int)a.K;
-    const int64_t out_bytes = a.out_dtype == 2 ? 16 : 8;                        // of four outputs
-    p.vec = a.N % 4 == 0 && a.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % out_bytes == 0;
+    p.vec = whole_stores(a, a.out_dtype == 2 ? 16 : 8);
     p.m_tiles = (int)cdiv(a.M, C::BM);
     const int64_t tiles = p.m_tiles * cdiv(a.N, C::BN), kts = cdiv(a.K, KB);
     // K is split over a cluster while the tiles leave SMs idle
     p.parts = 1;
     while (p.parts < 8 && tiles * p.parts * 2 <= 2 * num_sms() && kts >= 4 * p.parts) p.parts *= 2;
-    CUtensorMap ma, mb, msa, msb;
-    const uint64_t sp = (uint64_t)cdiv(a.K, SPAN<KIND>);
-    if (!map_codes(&ma, a.qa, a.M, a.K / 2, a.lda, 128) || !map_codes(&mb, a.qw, a.N, a.K / 2, a.ldw, 128) ||
-        !map_scales(&msa, a.sa, cdiv(a.M, 128), sp, C::TILES, 1) || !map_scales(&msb, a.sw, cdiv(a.N, 128), sp, C::TILES, 1)) {
+    CUtensorMap m[4];
+    if (!maps<KIND, C>(a, 1, m)) {
         *msg = "cuTensorMapEncodeTiled failed (pointer/stride alignment or driver entry point)";
         return cudaErrorInvalidValue;
     }
-    static bool configured[HN_MAX_DEV];
-    int dev = 0;
-    e = cudaGetDevice(&dev);
+    static bool done[HN_MAX_DEV];
+    e = opt_in(k_fp4_gemm<KIND>, C::SMEM, done);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= HN_MAX_DEV) return cudaErrorInvalidDevice;
-    if (!configured[dev]) {
-        e = cudaFuncSetAttribute(k_fp4_gemm<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) return e;
-        configured[dev] = true;
-    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * p.parts));
     cfg.blockDim = dim3(C::THREADS);
@@ -321,7 +765,7 @@ template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t
     at[0].val.clusterDim.x = p.parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<KIND>, ma, mb, msa, msb, p);
+    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<KIND>, m[0], m[1], m[2], m[3], p);
 }
 
 } // namespace fp4g

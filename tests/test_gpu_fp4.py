@@ -218,3 +218,12 @@ def test_product(hn, cuda, kind, m, n, k):
     a, w = operands(hn, m, n, k, kind, 12)
     for dtype in DTYPES:
         check_product(hn, hn.kernels.fp4_gemm(*a, *w, kind=kind, out_dtype=dtype), a, w, kind)
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(2304, 2304, 256), (2100, 2300, 160), (20000, 130, 64), (257, 9500, 2080), (4700, 1101, 4128),
+                                   (9472, 512, 96)])
+def test_product_many_rows(hn, cuda, kind, m, n, k):
+    a, w = operands(hn, m, n, k, kind, 13)
+    for dtype in DTYPES:
+        check_product(hn, hn.kernels.fp4_gemm(*a, *w, kind=kind, out_dtype=dtype), a, w, kind)
