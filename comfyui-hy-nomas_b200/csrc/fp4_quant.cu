@@ -7,9 +7,9 @@
 // A NaN or an infinity makes its block's scale NaN (MX) or its row's (NV), with zero codes, so that what reads it gives NaN.
 //
 // Bound by HBM: 2 B read (bf16) and 0.5 B + 1/16 B written per element. NV needs the row's top before its first code, so T
-// threads hold a row in registers, NCH chunks of 8 columns each (chunk i T + t), and x is read once; rows of more than 16384
-// columns are read twice. A chunk's block is 2 (NV) or 4 (MX) neighbouring lanes, and the lanes of a scale tile's word (8 or
-// 16) gather its bytes before the one store.
+// threads hold a row in registers as it was loaded, NCH chunks of 16 columns each (chunk i T + t), and x is read once; rows of more
+// than 16384 columns are read twice. A chunk is a block of NV and half a block of MX; the lanes of a scale tile's word (4 or
+// 8) gather its bytes before the one store.
 #include "fp4.cuh"
 #include "hn_kernels.h"
 
@@ -22,71 +22,129 @@ struct Params {
     const void *x;
     int64_t ldx, M, rows;       // rows: M rounded up to whole scale tiles; those from M on get zero scales
     int K, nch, tiles;          // chunks of the padded row, group blocks
-    uint32_t *q;                // [M][nch] words of eight codes
-    int64_t ldq;                // in words
+    uint8_t *q;
+    int64_t ldq;
     uint8_t *s;
     float *r;
 };
 
-// columns 8 c to 8 c + 7 of a row, zeros behind its end. VEC: the row starts on 16 bytes
-template <typename E, bool VEC> __device__ __forceinline__ void load_chunk(const E *row, int c, int K, float (&v)[8]) {
-    if (VEC && 8 * c + 8 <= K) {
-        Elem<E>::load8(row + 8 * c, v);
+// sixteen columns as loaded, widened when they are used
+template <typename E> struct Chunk {                // two to a word
+    uint32_t w[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const E *p) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 8);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+    __device__ __forceinline__ void put(int j, const E *p) { w[j >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p) << (16 * (j & 1)); }
+    __device__ __forceinline__ void widen(float (&v)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = pair(w[i], E());
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float2 pair(uint32_t x, __nv_bfloat16) { return make_float2(bf16_lo(x), bf16_hi(x)); }
+    static __device__ __forceinline__ float2 pair(uint32_t x, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
+};
+template <> struct Chunk<float> {
+    float w[16];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = 0.0f;
+    }
+    __device__ __forceinline__ void load(const float *p) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(p + i);
+            w[i] = a.x; w[i + 1] = a.y; w[i + 2] = a.z; w[i + 3] = a.w;
+        }
+    }
+    __device__ __forceinline__ void put(int j, const float *p) { w[j] = *p; }
+    __device__ __forceinline__ void widen(float (&v)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = w[i];
+    }
+};
+
+// columns 16 c to 16 c + 15 of a row, zeros behind its end. VEC: the row starts on 16 bytes
+template <typename E, bool VEC> __device__ __forceinline__ void load_chunk(const E *row, int c, int K, Chunk<E> &v) {
+    v.clear();
+    if (VEC && 16 * c + 16 <= K) {
+        v.load(row + 16 * c);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 8 * c + j < K ? Elem<E>::load1(row + 8 * c + j) : 0.0f;
+        for (int j = 0; j < 16; ++j)
+            if (16 * c + j < K) v.put(j, row + 16 * c + j);
     }
 }
-__device__ __forceinline__ float peak8(const float (&v)[8]) {
-    float p = nanmax_abs3(0.0f, v[0], v[1]);
-    p = nanmax_abs3(p, v[2], v[3]);
-    p = nanmax_abs3(p, v[4], v[5]);
-    return nanmax_abs3(p, v[6], v[7]);
+template <typename E> __device__ __forceinline__ float peak16(const Chunk<E> &c) {
+    float v[16], p = 0.0f;
+    c.widen(v);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) p = nanmax_abs3(p, v[j], v[j + 1]);
+    return p;
+}
+__device__ __forceinline__ uint2 pack16(const float (&v)[16]) {
+    return make_uint2(pack8_e2m1(*reinterpret_cast<const float(*)[8]>(v)), pack8_e2m1(*reinterpret_cast<const float(*)[8]>(v + 8)));
 }
 
 // MX: codes and scale byte of a chunk whose block's largest magnitude is `peak`
-__device__ __forceinline__ uint32_t chunk_mx(float (&v)[8], float peak, uint32_t &byte) {
+template <typename E> __device__ __forceinline__ uint2 chunk_mx(const Chunk<E> &c, float peak, uint32_t &byte) {
     const uint32_t be = __float_as_uint(peak) >> 23;
-    if (be == 255) { byte = 255; return 0; }
+    if (be == 255) { byte = 255; return make_uint2(0, 0); }
     byte = peak == 0.0f ? 127 : be < 2 ? 0 : be - 2;
-    const float inv = __uint_as_float((254 - byte) << 23);      // 2^(127 - byte): byte <= 252
+    const uint64_t inv = x2_splat(__uint_as_float((254 - byte) << 23));     // 2^(127 - byte): byte <= 252
+    float v[16];
+    c.widen(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= inv;
-    return pack8_e2m1(v);
+    for (int j = 0; j < 16; j += 2) x2_split(x2_mul(x2(v[j], v[j + 1]), inv), v[j], v[j + 1]);
+    return pack16(v);
 }
 
 // what a row's top fixes
 struct RowNV {
-    float div, den;      // top 2^-9 and top 2^-12
+    float ndiv, rdiv, den;      // -top 2^-9, its reciprocal, top 2^-12
     bool live;
 };
 __device__ __forceinline__ RowNV row_nv(float top, float *r) {
     RowNV n;
     n.live = top >= 0x1p-100f && top < INFINITY;
-    n.div = top * 0x1p-9f;
+    n.ndiv = top * -0x1p-9f;
+    n.rdiv = __frcp_rn(top * 0x1p-9f);
     n.den = top * 0x1p-12f;
     *r = n.live ? __fdiv_rn(top, 2688.0f) : top < 0x1p-100f ? 1.0f : __int_as_float(0x7fffffff);
     return n;
 }
-__device__ __forceinline__ uint32_t chunk_nv(float (&v)[8], float peak, const RowNV &n, uint32_t &byte) {
-    byte = n.live ? e4m3_byte(__fdiv_rn(0.875f * peak, n.div)) : 0;
-    if (byte == 0) return 0;
+template <typename E> __device__ __forceinline__ uint2 chunk_nv(const Chunk<E> &c, float peak, const RowNV &n, uint32_t &byte) {
+    byte = 0;
+    if (!n.live) return make_uint2(0, 0);
+    // RN(0.875 peak / (top 2^-9)): the quotient corrected once, as in x2_quot (what a remainder loses below 2^-126 is far below
+    // the smallest scale)
+    const float a = 0.875f * peak, q0 = a * n.rdiv;
+    byte = e4m3_byte(fmaf(fmaf(q0, n.ndiv, a), n.rdiv, q0));
+    if (byte == 0) return make_uint2(0, 0);
     const float den = scale_value<NV>(byte) * n.den;
+    float v[16];
+    c.widen(v);
     if (den >= 0x1p-90f) {
         const uint64_t ns = x2_splat(-den), rs = x2_splat(__frcp_rn(den));
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const uint64_t p = x2_mul(x2(v[j], v[j + 1]), x2_splat(0.65625f));
+        for (int j = 0; j < 16; j += 2) {
             float a, b;
-            x2_split(x2_quot(p, ns, rs), a, b);
+            x2_split(x2_quot(x2_mul(x2(v[j], v[j + 1]), x2_splat(0.65625f)), ns, rs), a, b);
             v[j] = copysignf(a, v[j]);          // of a zero
             v[j + 1] = copysignf(b, v[j + 1]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(0.65625f * v[j], den);
+        for (int j = 0; j < 16; ++j) v[j] = __fdiv_rn(0.65625f * v[j], den);
     }
-    return pack8_e2m1(v);
+    return pack16(v);
 }
 
 // the bytes of W neighbouring lanes' blocks (B lanes each) -> one word in every lane
@@ -100,29 +158,28 @@ template <int W, int B> __device__ __forceinline__ uint32_t gather_word(uint32_t
 // T threads a row (below 32: so many lanes of a warp), the row in registers
 template <typename E, int KIND, bool VEC, int T, int NCH>
 __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quant_fp4(Params p) {
-    constexpr int BLK = GROUP<KIND> / 8, LANES = SPAN<KIND> / 8, W = LANES < T ? LANES : T;
+    constexpr int BLK = GROUP<KIND> / 16, LANES = SPAN<KIND> / 16, W = LANES < T ? LANES : T;
     __shared__ float red[T < 128 ? 1 : T / 32];
     const int t = threadIdx.x % T, lane = threadIdx.x & 31, warp = (threadIdx.x % T) >> 5;
     const int64_t m = T < 128 ? (int64_t)blockIdx.x * (128 / T) + threadIdx.x / T : (int64_t)blockIdx.x;
     const bool row = m < p.M;                   // p.rows is whole blocks of threads, so no thread leaves before a shuffle
-    float v[NCH][8], peak[NCH];
+    Chunk<E> v[NCH];
+    float peak[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int c = i * T + t;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        if (row && c < p.nch) load_chunk<E, VEC>(static_cast<const E *>(p.x) + m * p.ldx, c, p.K, v[i]);
+        load_chunk<E, VEC>(static_cast<const E *>(p.x) + m * p.ldx, c, row ? p.K : 0, v[i]);
     }
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        peak[i] = lanes_max<BLK>(peak8(v[i]));
+        peak[i] = lanes_max<BLK>(peak16(v[i]));
         top = nanmax(top, peak[i]);
     }
     RowNV n;
     if (KIND == NV) {
 #pragma unroll
-        for (int o = BLK; o < (T < 32 ? T : 32); o <<= 1) top = nanmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 1; o < (T < 32 ? T : 32); o <<= 1) top = nanmax(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (T >= 128) {
             if (lane == 0) red[warp] = top;
             __syncthreads();
@@ -138,7 +195,8 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quant_fp4(Params p) {
     for (int i = 0; i < NCH; ++i) {
         const int c = i * T + t;
         uint32_t byte = 0;
-        if (row && c < p.nch) p.q[m * p.ldq + c] = KIND == MX ? chunk_mx(v[i], peak[i], byte) : chunk_nv(v[i], peak[i], n, byte);
+        if (row && c < p.nch)
+            *reinterpret_cast<uint2 *>(p.q + m * p.ldq + 8 * c) = KIND == MX ? chunk_mx(v[i], peak[i], byte) : chunk_nv(v[i], peak[i], n, byte);
         const uint32_t word = gather_word<W, BLK>(byte);
         if (t % W == 0 && c / LANES < p.tiles) *reinterpret_cast<uint32_t *>(p.s + scale_word(m, c / LANES, p.tiles)) = word;
     }
@@ -146,7 +204,7 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quant_fp4(Params p) {
 
 // any row length: the row's top in a pass of its own (NV)
 template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256) k_quant_fp4_long(Params p) {
-    constexpr int BLK = GROUP<KIND> / 8, LANES = SPAN<KIND> / 8, T = 256;
+    constexpr int BLK = GROUP<KIND> / 16, LANES = SPAN<KIND> / 16, T = 256;
     __shared__ float red[T / 32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t m = blockIdx.x;
@@ -155,10 +213,11 @@ template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256)
     RowNV n;
     if (KIND == NV) {
         float top = 0.0f;
-        for (int c = t; row && c < p.nch; c += T) {
-            float v[8];
+#pragma unroll 4
+        for (int c = t; c < (row ? p.nch : 0); c += T) {
+            Chunk<E> v;
             load_chunk<E, VEC>(x, c, p.K, v);
-            top = nanmax(top, peak8(v));
+            top = nanmax(top, peak16(v));
         }
         top = lanes_max<32>(top);
         if (lane == 0) red[warp] = top;
@@ -172,11 +231,12 @@ template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256)
     }
     for (int c0 = 0; c0 < p.tiles * LANES; c0 += T) {           // whole warps: the words' lanes stay together
         const int c = c0 + t;
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (row && c < p.nch) load_chunk<E, VEC>(x, c, p.K, v);
-        const float peak = lanes_max<BLK>(peak8(v));
+        Chunk<E> v;
+        load_chunk<E, VEC>(x, c, row ? p.K : 0, v);
+        const float peak = lanes_max<BLK>(peak16(v));
         uint32_t byte = 0;
-        if (row && c < p.nch) p.q[m * p.ldq + c] = KIND == MX ? chunk_mx(v, peak, byte) : chunk_nv(v, peak, n, byte);
+        if (row && c < p.nch)
+            *reinterpret_cast<uint2 *>(p.q + m * p.ldq + 8 * c) = KIND == MX ? chunk_mx(v, peak, byte) : chunk_nv(v, peak, n, byte);
         const uint32_t word = gather_word<LANES, BLK>(byte);
         if (t % LANES == 0 && c / LANES < p.tiles) *reinterpret_cast<uint32_t *>(p.s + scale_word(m, c / LANES, p.tiles)) = word;
     }
@@ -188,17 +248,17 @@ template <typename E, int KIND, bool VEC, int T, int NCH> cudaError_t go(const P
     return cudaGetLastError();
 }
 
-// T by the row's length alone, as the residual's norm and quantizer have it
+// T by the row's length alone
 template <typename E, int KIND, bool VEC> cudaError_t pick(const Params &p, cudaStream_t st) {
-    if (p.nch <= 4) return go<E, KIND, VEC, 4, 1>(p, st);
+    if (p.nch <= 2) return go<E, KIND, VEC, 2, 1>(p, st);
+    if (p.nch <= 8) return go<E, KIND, VEC, 8, 1>(p, st);
     if (p.nch <= 16) return go<E, KIND, VEC, 16, 1>(p, st);
     if (p.nch <= 32) return go<E, KIND, VEC, 32, 1>(p, st);
     if (p.nch <= 64) return go<E, KIND, VEC, 32, 2>(p, st);
     if (p.nch <= 128) return go<E, KIND, VEC, 32, 4>(p, st);
     if (p.nch <= 256) return go<E, KIND, VEC, 128, 2>(p, st);
     if (p.nch <= 512) return go<E, KIND, VEC, 128, 4>(p, st);
-    if (p.nch <= 1024) return go<E, KIND, VEC, 256, 4>(p, st);
-    if (p.nch <= 2048) return go<E, KIND, VEC, 256, 8>(p, st);
+    if (p.nch <= 1024) return go<E, KIND, VEC, 512, 2>(p, st);
     k_quant_fp4_long<E, KIND, VEC><<<(unsigned)p.rows, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
@@ -209,70 +269,78 @@ template <typename E> cudaError_t pick_kind(const Params &p, int kind, cudaStrea
 }
 
 struct BackParams {
-    const uint32_t *q;
+    const uint8_t *q;
     int64_t ldq, M;
-    int K, nch, tiles;
+    int K, nch, tiles;          // chunks of 8 columns
     const uint8_t *s;
     const float *r;
     void *out;
     int64_t ldo;
 };
 
-// code * RN(scale * row scale), one rounding to the output type. A thread takes a chunk of 8 columns; VEC: 16-byte stores
 template <typename E> __device__ __forceinline__ void store1(E *p, float v);
 template <> __device__ __forceinline__ void store1(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ void store1(__half *p, float v) { *p = __float2half_rn(v); }
 template <> __device__ __forceinline__ void store1(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store8(__nv_bfloat16 *o, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(o) = make_uint4(pack_bf16_rn(v[0], v[1]), pack_bf16_rn(v[2], v[3]), pack_bf16_rn(v[4], v[5]), pack_bf16_rn(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(__half *o, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(o) = make_uint4(pack_f16_rn(v[0], v[1]), pack_f16_rn(v[2], v[3]), pack_f16_rn(v[4], v[5]), pack_f16_rn(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(float *o, const float (&v)[8]) {
+    *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
 
-template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256) k_dequant_fp4(BackParams p) {
-    const int64_t n = p.M * p.nch;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = div_nonneg(i, p.nch);
-        const int c = (int)(i - m * p.nch), g = 8 * c / GROUP<KIND>;
-        if (8 * c >= p.K) continue;
-        const uint32_t w = p.q[m * p.ldq + c];
-        float d = scale_value<KIND>(p.s[scale_word(m, g >> 2, p.tiles) + (g & 3)]);
-        if (KIND == NV) d = __fmul_rn(d, p.r[m]);
+// code * RN(scale * row scale), one rounding to the output type. T threads a row, which take its chunks of 8 columns in turn (16
+// bytes out, neighbouring lanes write on), so that a row's address and scale are worked out once. VEC: 16-byte stores
+template <typename E, int KIND, bool VEC, int T> __global__ void __launch_bounds__(256) k_dequant_fp4(BackParams p) {
+    const int64_t m = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T;
+    if (m >= p.M) return;
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p.q + m * p.ldq);
+    const uint8_t *s = p.s + scale_word(m, 0, p.tiles);
+    const float r = KIND == NV ? p.r[m] : 1.0f;
+    E *out = static_cast<E *>(p.out) + m * p.ldo;
+#pragma unroll 2
+    for (int c = threadIdx.x % T; c < p.nch; c += T) {
+        const int g = 8 * c / GROUP<KIND>;
+        const uint32_t w = q[c];
+        float d = scale_value<KIND>(s[(int64_t)(g >> 2) * TILE + (g & 3)]);
+        if (KIND == NV) d = __fmul_rn(d, r);
         uint32_t h[4];
         unpack8_e2m1(w, h);
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-            v[2 * j] = f.x * d;
-            v[2 * j + 1] = f.y * d;
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[k]));
+            v[2 * k] = f.x * d;
+            v[2 * k + 1] = f.y * d;
         }
-        E *o = static_cast<E *>(p.out) + m * p.ldo + 8 * c;
         if (VEC && 8 * c + 8 <= p.K) {
-            if (sizeof(E) == 4) {
-                *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4 *>(reinterpret_cast<float *>(o) + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-                E e[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) store1(&e[j], v[j]);
-                *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<uint4 *>(e);
-            }
+            store8(out + 8 * c, v);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (8 * c + j < p.K) store1(o + j, v[j]);
+            for (int k = 0; k < 8; ++k)
+                if (8 * c + k < p.K) store1(out + 8 * c + k, v[k]);
         }
     }
 }
 
+template <typename E, int KIND, bool VEC> cudaError_t back_rows(const BackParams &p, cudaStream_t st) {
+    auto go = [&](auto kernel, int per) {
+        kernel<<<(unsigned)cdiv(p.M, per), 256, 0, st>>>(p);
+        return cudaGetLastError();
+    };
+    if (p.nch <= 8) return go(k_dequant_fp4<E, KIND, VEC, 4>, 64);
+    if (p.nch <= 32) return go(k_dequant_fp4<E, KIND, VEC, 16>, 16);
+    if (p.nch <= 256) return go(k_dequant_fp4<E, KIND, VEC, 64>, 4);
+    return go(k_dequant_fp4<E, KIND, VEC, 256>, 1);
+}
 template <typename E> cudaError_t back(const BackParams &p, int kind, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * (int64_t)sizeof(E) % 16 == 0;
-    const int64_t want = cdiv(p.M * p.nch, 256), most = (int64_t)num_sms() * 8;
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    if (kind == MX) {
-        if (vec) k_dequant_fp4<E, MX, true><<<grid, 256, 0, st>>>(p);
-        else k_dequant_fp4<E, MX, false><<<grid, 256, 0, st>>>(p);
-    } else {
-        if (vec) k_dequant_fp4<E, NV, true><<<grid, 256, 0, st>>>(p);
-        else k_dequant_fp4<E, NV, false><<<grid, 256, 0, st>>>(p);
-    }
-    return cudaGetLastError();
+    if (kind == MX) return vec ? back_rows<E, MX, true>(p, st) : back_rows<E, MX, false>(p, st);
+    return vec ? back_rows<E, NV, true>(p, st) : back_rows<E, NV, false>(p, st);
 }
 
 } // namespace fp4q
@@ -281,9 +349,9 @@ cudaError_t launch_quant_fp4(const void *x, int64_t ldx, int x_dtype, int64_t M,
                              void *s, float *r, cudaStream_t st) {
     fp4q::Params p;
     p.x = x; p.ldx = ldx; p.M = M; p.rows = cdiv(M, 128) * 128; p.K = (int)K;
-    p.nch = (int)(cdiv(K, 32) * 4);
+    p.nch = (int)(cdiv(K, 32) * 2);
     p.tiles = (int)cdiv(K, kind == fp4::MX ? 128 : 64);
-    p.q = static_cast<uint32_t *>(q); p.ldq = ldq / 4; p.s = static_cast<uint8_t *>(s); p.r = r;
+    p.q = static_cast<uint8_t *>(q); p.ldq = ldq; p.s = static_cast<uint8_t *>(s); p.r = r;
     if (x_dtype == 0) return fp4q::pick_kind<__nv_bfloat16>(p, kind, st);
     if (x_dtype == 1) return fp4q::pick_kind<__half>(p, kind, st);
     return fp4q::pick_kind<float>(p, kind, st);
@@ -292,7 +360,7 @@ cudaError_t launch_quant_fp4(const void *x, int64_t ldx, int x_dtype, int64_t M,
 cudaError_t launch_dequant_fp4(const void *q, int64_t ldq, const void *s, const float *r, int64_t M, int64_t K, int64_t Kp,
                                int kind, void *out, int64_t ldo, int out_dtype, cudaStream_t st) {
     fp4q::BackParams p;
-    p.q = static_cast<const uint32_t *>(q); p.ldq = ldq / 4; p.M = M; p.K = (int)K; p.nch = (int)cdiv(K, 8);
+    p.q = static_cast<const uint8_t *>(q); p.ldq = ldq; p.M = M; p.K = (int)K; p.nch = (int)cdiv(K, 8);
     p.tiles = (int)cdiv(Kp, kind == fp4::MX ? 128 : 64);
     p.s = static_cast<const uint8_t *>(s); p.r = r; p.out = out; p.ldo = ldo;
     if (out_dtype == 0) return fp4q::back<__nv_bfloat16>(p, kind, st);

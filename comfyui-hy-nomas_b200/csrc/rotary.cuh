@@ -143,5 +143,140 @@ __device__ __forceinline__ void head_norm(float (&v)[8], float (&o)[8], const We
             for (int i = 4 * j; i < 4 * j + 4; ++i) o[i] = o[i] * inv * w.other[i];
 }
 
+// ---------------------------------------------------------------------------------------------------
+// Sixteen columns a lane: two runs of eight that hold eight whole pairs, so that no partner stands elsewhere. Heads whose width and
+// rotated part are multiples of 16. In the half layout a rotated lane's runs are half the rotated part apart, in the interleaved
+// one they follow each other, as they do in lanes that are not rotated.
+struct Lane16 {
+    int a, b;                       // first columns of the two runs
+    bool on;                        // rotated
+    int pair;                       // its first pair
+};
+template <bool INTER> __device__ __forceinline__ Lane16 lane16(const Rotation &r, int sub) {
+    Lane16 l;
+    l.on = 16 * sub < r.rot;
+    l.a = INTER || !l.on ? 16 * sub : 8 * sub;
+    l.b = INTER || !l.on ? l.a + 8 : l.a + (r.rot >> 1);
+    l.pair = 8 * sub;
+    return l;
+}
+// A lane's columns as eight f32x2: x[i] the first columns of pairs 2 i and 2 i + 1, y[i] their partners. Products and fused
+// multiply-adds on them take one instruction for two columns.
+struct Cols {
+    uint64_t x[4], y[4];
+};
+struct Turn16 {
+    uint64_t c[4], s[4], ns[4];
+};
+__device__ __forceinline__ void turn16_of(const Lane16 &l, const float *table, Turn16 &t) {
+    if (!l.on) return;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2 *>(table + l.pair + 2 * i);
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2 *>(table + MAX_PAIRS + l.pair + 2 * i);
+        t.c[i] = c.x; t.c[i + 1] = c.y;
+        t.s[i] = s.x; t.s[i + 1] = s.y;
+        t.ns[i] = s.x ^ 0x8000000080000000ull; t.ns[i + 1] = s.y ^ 0x8000000080000000ull;
+    }
+}
+__device__ __forceinline__ void turn16(const Lane16 &l, const Turn16 &t, Cols &v) {
+    if (!l.on) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t u = x2_fma(v.y[i], t.ns[i], x2_mul(v.x[i], t.c[i]));
+        v.y[i] = x2_fma(v.x[i], t.s[i], x2_mul(v.y[i], t.c[i]));
+        v.x[i] = u;
+    }
+}
+// x / sqrt(mean x^2 + eps) * w over the P lanes of a head; v is 0 in lanes behind it. rd = 1 / D
+template <int P> __device__ __forceinline__ void norm16(Cols &v, const Cols &w, float rd, float eps) {
+    uint64_t a = x2_mul(v.x[0], v.x[0]), b = x2_mul(v.y[0], v.y[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        a = x2_fma(v.x[i], v.x[i], a);
+        b = x2_fma(v.y[i], v.y[i], b);
+    }
+    float a0, a1, b0, b1;
+    x2_split(a, a0, a1);
+    x2_split(b, b0, b1);
+    float ss = (a0 + a1) + (b0 + b1);
+#pragma unroll
+    for (int i = 1; i < P; i <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, i);
+    const uint64_t inv = x2_splat(rsqrtf(fmaf(ss, rd, eps)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v.x[i] = x2_mul(x2_mul(v.x[i], inv), w.x[i]);
+        v.y[i] = x2_mul(x2_mul(v.y[i], inv), w.y[i]);
+    }
+}
+// eight columns in order <-> half of a lane's: run `r` (0 or 1)
+template <bool INTER> __device__ __forceinline__ void put_run(Cols &c, int r, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!INTER) (r ? c.y : c.x)[i] = x2(v[2 * i], v[2 * i + 1]);
+        else if (i < 2) c.x[2 * r + i] = x2(v[4 * i], v[4 * i + 2]);
+        else c.y[2 * r + i - 2] = x2(v[4 * i - 7], v[4 * i - 5]);
+    }
+}
+template <bool INTER> __device__ __forceinline__ void take_run(const Cols &c, int r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!INTER) x2_split((r ? c.y : c.x)[i], v[2 * i], v[2 * i + 1]);
+        else if (i < 2) x2_split(c.x[2 * r + i], v[4 * i], v[4 * i + 2]);
+        else x2_split(c.y[2 * r + i - 2], v[4 * i - 7], v[4 * i - 5]);
+    }
+}
+// eight columns as loaded, to be widened later
+template <typename E> struct Raw8 {
+    uint4 w;
+    __device__ __forceinline__ void load(const E *p) { w = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void widen(float (&v)[8]) const;
+};
+template <> __device__ __forceinline__ void Raw8<__nv_bfloat16>::widen(float (&v)[8]) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(x[i]); v[2 * i + 1] = bf16_hi(x[i]); }
+}
+template <> __device__ __forceinline__ void Raw8<__half>::widen(float (&v)[8]) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+template <> struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = *reinterpret_cast<const float4 *>(p);
+        b = *reinterpret_cast<const float4 *>(p + 4);
+    }
+    __device__ __forceinline__ void clear() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <bool INTER, typename E> __device__ __forceinline__ void widen16(const Raw8<E> (&raw)[2], Cols &c) {
+    float v[8];
+    raw[0].widen(v);
+    put_run<INTER>(c, 0, v);
+    raw[1].widen(v);
+    put_run<INTER>(c, 1, v);
+}
+template <bool INTER, typename E> __device__ __forceinline__ void store_runs(E *p, const Lane16 &l, const Cols &c) {
+    float v[8];
+    take_run<INTER>(c, 0, v);
+    store8(p + l.a, v);
+    take_run<INTER>(c, 1, v);
+    store8(p + l.b, v);
+}
+template <bool INTER> __device__ __forceinline__ void load_weights16(const __nv_bfloat16 *w, const Lane16 &l, Cols &c) {
+    Raw8<__nv_bfloat16> raw[2];
+    raw[0].load(w + l.a);
+    raw[1].load(w + l.b);
+    widen16<INTER>(raw, c);
+}
+
 } // namespace rotary
 } // namespace hn
