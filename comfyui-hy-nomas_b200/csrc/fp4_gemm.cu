@@ -7,6 +7,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "fp4.cuh"
 #include "hn_kernels.h"
 #include "hn_tc.cuh"
@@ -22,8 +24,9 @@ constexpr int KB = 256;                         // columns of a stage: 128 bytes
 
 // Tiles of 128 x 128 outputs. A cluster of S CTAs shares one: each takes a part of K, leaves its fp32 sums in its shared memory,
 // and CTA r of the cluster adds those of its 128 / S rows, in the CTAs' order, and writes them.
-template <int KIND> struct Cfg {
-    static constexpr int BM = 128, BN = 128, STAGES = 3;
+template <int KIND, int STAGES_> struct Cfg {
+    static constexpr int BM = 128, BN = 128, STAGES = STAGES_;
+    static constexpr int CTAS = STAGES > 3 ? 1 : 2;             // an SM
     static constexpr int TILES = KB / SPAN<KIND>;               // scale tiles of an operand in a stage
     static constexpr int OP = 128 * 128, SF = TILES * TILE;     // bytes of a stage: codes and scales of an operand
     static constexpr int STAGE = 2 * OP + 2 * SF;
@@ -33,10 +36,10 @@ template <int KIND> struct Cfg {
     static constexpr int OFF_MISC = OFF_BAR + 8 * (2 * STAGES + 1);
     static constexpr int SMEM = OFF_MISC + 16 + 1024;           // + alignment slack
     static constexpr int ACC = 0, SFC = BN;                     // tensor memory columns: sums, then 8 x TILES a stage
-    static constexpr int COLS = 256;
+    static constexpr int COLS = CTAS == 1 ? 512 : 256;
     static constexpr int THREADS = 192;                         // producer, issuer, four warps that empty tensor memory
     static_assert(SFC + STAGES * 8 * TILES <= COLS, "tensor memory");
-    static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
 };
 
 struct Params {
@@ -92,11 +95,72 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
+// Rows [r0, r1) of a tile's sums: P CTAs' partial sums added in their order, scales, bias, rounding. A warp takes every WARPS-th
+// row, U of them at a time so that their loads overlap; a lane has the same four columns throughout (VEC: neighbours, one store).
+template <int P, bool VEC, int WARPS>
+__device__ __forceinline__ void write_rows(const Params &p, const float *tile, int pitch, int m0, int n0, int r0, int r1) {
+    constexpr int U = P == 8 ? 2 : 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float cs[4], cb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int n = n0 + (VEC ? 4 * lane + j : lane + 32 * j);
+        cs[j] = p.o.rb && n < p.N ? p.o.rb[n] : 1.0f;
+        cb[j] = p.o.bias && n < p.N ? bias_at(p.o, n) : 0.0f;
+    }
+    for (int r = r0 + warp; r < r1; r += U * WARPS) {
+        float v[U][P][4], ra[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = r + u * WARPS < r1 ? r + u * WARPS : r;
+            ra[u] = p.o.ra ? p.o.ra[m0 + row] : 1.0f;
+            const float *at = tile + row * pitch;
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (VEC) {
+                    const float4 x = P == 1 ? *reinterpret_cast<const float4 *>(at + 4 * lane) : ld_cluster4(smem_u32(at + 4 * lane), i);
+                    v[u][i][0] = x.x; v[u][i][1] = x.y; v[u][i][2] = x.z; v[u][i][3] = x.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[u][i][j] = P == 1 ? at[lane + 32 * j] : ld_cluster1(smem_u32(at + lane + 32 * j), i);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = r + u * WARPS;
+            if (row >= r1) break;
+            float o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = v[u][0][j];
+#pragma unroll
+                for (int i = 1; i < P; ++i) o[j] += v[u][i][j];
+                o[j] = __fadd_rn(__fmul_rn(__fmul_rn(o[j], ra[u]), cs[j]), cb[j]);
+            }
+            const int64_t off = (int64_t)(m0 + row) * p.o.ldo + n0;
+            if (VEC) {
+                if (n0 + 4 * lane >= p.N) continue;
+                if (p.o.out_dtype == 2)
+                    *reinterpret_cast<float4 *>(static_cast<float *>(p.o.out) + off + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
+                else
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.o.out) + off + 4 * lane) =
+                        p.o.out_dtype == 0 ? make_uint2(pack_bf16_rn(o[0], o[1]), pack_bf16_rn(o[2], o[3]))
+                                           : make_uint2(pack_f16_rn(o[0], o[1]), pack_f16_rn(o[2], o[3]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n0 + lane + 32 * j < p.N) store_result(p.o, off + lane + 32 * j, o[j]);
+            }
+        }
+    }
+}
+
+template <int KIND, int STAGES>
+__global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>::CTAS)
     k_fp4_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const Params p) {
-    using C = Cfg<KIND>;
+    using C = Cfg<KIND, STAGES>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = smem_u32(smem);
@@ -109,12 +173,22 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
     const int kts = (p.Kp + KB - 1) / KB;
     const int kt0 = (int)((int64_t)kts * part / p.parts), kt1 = (int)((int64_t)kts * (part + 1) / p.parts);
 
+    auto load = [&](int kt, int stage) {
+        // boxes that run past the operand are zero-filled and count their full bytes
+        const uint32_t at = sbase + stage * C::STAGE, fb = bar_full + 8 * stage;
+        mbar_arrive_tx(fb, C::STAGE);
+        tma_load_2d(&tmA, at, fb, kt * 128, m0);
+        tma_load_2d(&tmB, at + C::OP, fb, kt * 128, n0);
+        tma_load_3d(&tmSA, at + 2 * C::OP, fb, kt * C::TILES, m0 >> 7);
+        tma_load_3d(&tmSB, at + 2 * C::OP + C::SF, fb, kt * C::TILES, n0 >> 7);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        for (int s = 0; s < C::STAGES && kt0 + s < kt1; ++s) load(kt0 + s, s);      // the first stages, while the others prepare
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::COLS)
@@ -128,20 +202,13 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
 
     bool ok = true;
     if (warp == 0) {
-        int stage = 0, issued = 0;
-        uint32_t phase = 0;
-        for (int kt = kt0; kt < kt1; ++kt) {
+        int stage = 0, issued = min(C::STAGES, kt1 - kt0);
+        uint32_t phase = 1;
+        if (issued < C::STAGES) { stage = issued; phase = 0; }
+        for (int kt = kt0 + issued; kt < kt1; ++kt) {
             ok = warp_wait(lane, bar_empty + 8 * stage, phase ^ 1, abort_flag, WAIT_NS, p.err);
             if (!ok) break;
-            if (lane == 0) {
-                // boxes that run past the operand are zero-filled and count their full bytes
-                const uint32_t at = sbase + stage * C::STAGE, fb = bar_full + 8 * stage;
-                mbar_arrive_tx(fb, C::STAGE);
-                tma_load_2d(&tmA, at, fb, kt * 128, m0);
-                tma_load_2d(&tmB, at + C::OP, fb, kt * 128, n0);
-                tma_load_3d(&tmSA, at + 2 * C::OP, fb, kt * C::TILES, m0 >> 7);
-                tma_load_3d(&tmSB, at + 2 * C::OP + C::SF, fb, kt * C::TILES, n0 >> 7);
-            }
+            if (lane == 0) load(kt, stage);
             ++issued;
             if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
         }
@@ -203,39 +270,16 @@ __global__ void __launch_bounds__(Cfg<KIND>::THREADS, 2)
     cluster_arrive();                               // every CTA of the cluster comes by, a failed one too
     cluster_wait();
     if (ok) {
-        const int rows = C::BM / p.parts, first = part * rows;
-        for (int r = first + warp; r < first + rows && m0 + r < p.M; r += C::THREADS / 32) {
-            const int64_t off = (int64_t)(m0 + r) * p.o.ldo + n0;
-            const float ra = p.o.ra ? p.o.ra[m0 + r] : 1.0f;
-            if (p.vec) {
-                const int n = n0 + 4 * lane;
-                const uint32_t addr = smem_u32(tile_s + r * C::PITCH + 4 * lane);
-                float4 v = p.parts == 1 ? *reinterpret_cast<float4 *>(tile_s + r * C::PITCH + 4 * lane) : ld_cluster4(addr, 0);
-                for (int i = 1; i < p.parts; ++i) {
-                    const float4 w = ld_cluster4(addr, i);
-                    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-                }
-                if (n < p.N) {
-                    v.x = finish(p.o, v.x, ra, n); v.y = finish(p.o, v.y, ra, n + 1);
-                    v.z = finish(p.o, v.z, ra, n + 2); v.w = finish(p.o, v.w, ra, n + 3);
-                    if (p.o.out_dtype == 2)
-                        *reinterpret_cast<float4 *>(static_cast<float *>(p.o.out) + off + 4 * lane) = v;
-                    else
-                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.o.out) + off + 4 * lane) =
-                            p.o.out_dtype == 0 ? make_uint2(pack_bf16_rn(v.x, v.y), pack_bf16_rn(v.z, v.w))
-                                               : make_uint2(pack_f16_rn(v.x, v.y), pack_f16_rn(v.z, v.w));
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = lane + 32 * j;
-                    const uint32_t addr = smem_u32(tile_s + r * C::PITCH + n);
-                    float v = p.parts == 1 ? tile_s[r * C::PITCH + n] : ld_cluster1(addr, 0);
-                    for (int i = 1; i < p.parts; ++i) v += ld_cluster1(addr, i);
-                    if (n0 + n < p.N) store_result(p.o, off + n, finish(p.o, v, ra, n0 + n));
-                }
-            }
-        }
+        const int rows = min(C::BM, p.M - m0), r0 = rows * part / p.parts, r1 = rows * (part + 1) / p.parts;
+        auto write = [&](auto parts) {
+            constexpr int P = decltype(parts)::value, W = C::THREADS / 32;
+            if (p.vec) write_rows<P, true, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
+            else write_rows<P, false, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
+        };
+        if (p.parts == 1) write(std::integral_constant<int, 1>());
+        else if (p.parts == 2) write(std::integral_constant<int, 2>());
+        else if (p.parts == 4) write(std::integral_constant<int, 4>());
+        else write(std::integral_constant<int, 8>());
     }
     __syncwarp();
     cluster_arrive();                               // nobody leaves while its sums are read
@@ -733,9 +777,8 @@ template <int KIND> static cudaError_t launch_wide(const Fp4GemmArgs &a, cudaStr
     return a.out_dtype == 2 ? go(k_fp4_gemm_wide<KIND, 4>, done4) : go(k_fp4_gemm_wide<KIND, 2>, done2);
 }
 
-template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t st, const char **msg) {
-    using C = Cfg<KIND>;
-    if (cdiv(a.M, 256) * cdiv(a.N, 256) >= num_sms() / 2) return launch_wide<KIND>(a, st, msg);
+template <int KIND, int STAGES> static cudaError_t launch_narrow(const Fp4GemmArgs &a, int64_t tiles, int parts, cudaStream_t st, const char **msg) {
+    using C = Cfg<KIND, STAGES>;
     Params p;
     cudaError_t e = device_error_word(err_slot(st), &p.err);
     if (e != cudaSuccess) return e;
@@ -743,17 +786,14 @@ template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t
     p.M = (int)a.M; p.N = (int)a.N; p.Kp = (int)a.K;
     p.vec = whole_stores(a, a.out_dtype == 2 ? 16 : 8);
     p.m_tiles = (int)cdiv(a.M, C::BM);
-    const int64_t tiles = p.m_tiles * cdiv(a.N, C::BN), kts = cdiv(a.K, KB);
-    // K is split over a cluster while the tiles leave SMs idle
-    p.parts = 1;
-    while (p.parts < 8 && tiles * p.parts * 2 <= 2 * num_sms() && kts >= 4 * p.parts) p.parts *= 2;
+    p.parts = parts;
     CUtensorMap m[4];
     if (!maps<KIND, C>(a, 1, m)) {
         *msg = "cuTensorMapEncodeTiled failed (pointer/stride alignment or driver entry point)";
         return cudaErrorInvalidValue;
     }
     static bool done[HN_MAX_DEV];
-    e = opt_in(k_fp4_gemm<KIND>, C::SMEM, done);
+    e = opt_in(k_fp4_gemm<KIND, STAGES>, C::SMEM, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * p.parts));
@@ -765,7 +805,23 @@ template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t
     at[0].val.clusterDim.x = p.parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<KIND>, m[0], m[1], m[2], m[3], p);
+    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<KIND, STAGES>, m[0], m[1], m[2], m[3], p);
+}
+
+template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t st, const char **msg) {
+    const int sms = num_sms();
+    const int64_t tiles = cdiv(a.M, 128) * cdiv(a.N, 128), kts = cdiv(a.K, KB);
+    // Tiles of 128 x 128 while all of them run at once, two CTAs an SM; pairs of CTAs beyond. Measured (us, 128 x 128 / pairs):
+    // 777 x 5000 x 2080 (280 tiles) 16.3 / 18.6; 1024 x 5120 x 4096 (320) 33.8 / 25.2; 2560 x 2048 x 1024 (320) 16.8 / 14.8
+    if (tiles > 2 * sms) return launch_wide<KIND>(a, st, msg);
+    // K is split over a cluster while SMs are idle and each part keeps two stages; over a second CTA on each SM only where a part
+    // keeps eight. Measured (us, 1 / 2 / 4 / 8 parts): 48 x 8192 x 4096 MX 13.1 / 9.9 / 11.6 / -; 128 x 4096 x 4096 NV 16.4 / 11.5 /
+    // 10.1 / 16.5; 16 x 4096 x 16384 NV 43 / 25 / 17 / 15
+    int parts = 1;
+    while (parts < 8 && kts >= 4 * parts && (tiles * parts * 2 <= sms || (tiles * parts * 2 <= 2 * sms && kts >= 16 * parts))) parts *= 2;
+    // a CTA alone on its SM has twice the stages in flight
+    if (tiles * parts <= sms) return launch_narrow<KIND, 6>(a, tiles, parts, st, msg);
+    return launch_narrow<KIND, 3>(a, tiles, parts, st, msg);
 }
 
 } // namespace fp4g

@@ -40,7 +40,7 @@ __device__ __forceinline__ float dot16(const uint32_t *a, const uint32_t *b) {
     return f.x + f.y;
 }
 
-template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS) k_fp4_gemv(Params p) {
+template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS, MT == 1 ? 4 : 2) k_fp4_gemv(Params p) {
     __shared__ float sums[WARPS][ROWS * MT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t block = blockIdx.x >> 4;                      // of 128 rows
@@ -53,21 +53,8 @@ template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS) k_fp4_
     for (int c0 = warp * CHUNK; c0 < p.Kp; c0 += warps * CHUNK) {
         const int k = c0 + 32 * lane;
         const bool in = k < p.Kp;
-        uint4 w[ROWS];
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j) {                        // row 2 i + h of j is 32 i + pair + h of the block
-            const int64_t n = block * 128 + 32 * (j >> 1) + pair + (j & 1);
-            w[j] = make_uint4(0, 0, 0, 0);
-            if (in && n < p.N) w[j] = ldg_stream(p.qw + n * p.ldw + (k >> 1));
-        }
-        // the scale words of the eight rows for this lane's columns: NV a tile is two lanes' columns, MX four lanes'
-        const int tile = k / SPAN<KIND>;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;             // words of rows pair and pair + 1
-        if (in) {
-            const uint4 *s = reinterpret_cast<const uint4 *>(p.sw + (block * p.tiles + tile) * TILE + 16 * pair);
-            lo = __ldg(s);
-            hi = __ldg(s + 1);
-        }
+        const int tile = k / SPAN<KIND>;                        // NV: a tile is two lanes' columns, MX: four lanes'
+        const int g = KIND == NV ? 2 * (lane & 1) : lane & 3;   // the first of this lane's groups in it
         uint32_t x[MT][16];
         float xs[MT][2];
 #pragma unroll
@@ -79,27 +66,33 @@ template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS) k_fp4_
                 word = __ldg(reinterpret_cast<const uint32_t *>(p.sa + scale_word(i, tile, p.tiles)));
             }
             unpack32(a, x[i]);
-            const int g = KIND == NV ? 2 * (lane & 1) : lane & 3;
             xs[i][0] = scale_value<KIND>(word >> (8 * g) & 255);
             xs[i][1] = KIND == NV ? scale_value<KIND>(word >> (8 * g + 8) & 255) : 0.0f;
         }
+        const uint4 *scales = reinterpret_cast<const uint4 *>(p.sw + (block * p.tiles + tile) * TILE + 16 * pair);
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j) {
-            const uint4 sw = j & 1 ? hi : lo;
-            const uint32_t word = (j >> 1) == 0 ? sw.x : (j >> 1) == 1 ? sw.y : (j >> 1) == 2 ? sw.z : sw.w;
-            const int g = KIND == NV ? 2 * (lane & 1) : lane & 3;
-            const float s0 = scale_value<KIND>(word >> (8 * g) & 255);
-            const float s1 = KIND == NV ? scale_value<KIND>(word >> (8 * g + 8) & 255) : 0.0f;
-            uint32_t h[16];
-            unpack32(w[j], h);
+        for (int half = 0; half < 2; ++half) {                  // row `pair`, then `pair` + 1, of each 32: four rows in flight
+            uint4 w[4], s = make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const float d0 = dot16(h, x[i]), d1 = dot16(h + 8, x[i] + 8);
-                if (KIND == NV) {
-                    acc[i][j] = fmaf(d0, xs[i][0] * s0, acc[i][j]);
-                    acc[i][j] = fmaf(d1, xs[i][1] * s1, acc[i][j]);
-                } else {
-                    acc[i][j] = fmaf((d0 + d1) * xs[i][0], s0, acc[i][j]);
+            for (int j = 0; j < 4; ++j) {
+                const int64_t n = block * 128 + 32 * j + pair + half;
+                w[j] = make_uint4(0, 0, 0, 0);
+                if (in && n < p.N) w[j] = ldg_stream(p.qw + n * p.ldw + (k >> 1));
+            }
+            if (in) s = __ldg(scales + half);
+            const uint32_t words[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float s0 = scale_value<KIND>(words[j] >> (8 * g) & 255);
+                const float s1 = KIND == NV ? scale_value<KIND>(words[j] >> (8 * g + 8) & 255) : 0.0f;
+                uint32_t h[16];
+                unpack32(w[j], h);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const float d0 = dot16(h, x[i]), d1 = dot16(h + 8, x[i] + 8);
+                    float &sum = acc[i][2 * j + half];
+                    if (KIND == NV) sum = fmaf(d1, xs[i][1] * s1, fmaf(d0, xs[i][0] * s0, sum));
+                    else sum = fmaf((d0 + d1) * xs[i][0], s0, sum);
                 }
             }
         }
@@ -126,8 +119,7 @@ template <int KIND> cudaError_t go(const Params &p, cudaStream_t st) {
     const int chunks = (int)cdiv(p.Kp, CHUNK), warps = chunks < WARPS ? chunks : WARPS;
     const unsigned grid = (unsigned)(cdiv(p.N, 128) * 16);
     if (p.M == 1) k_fp4_gemv<KIND, 1><<<grid, 32 * warps, 0, st>>>(p);
-    else if (p.M == 2) k_fp4_gemv<KIND, 2><<<grid, 32 * warps, 0, st>>>(p);
-    else k_fp4_gemv<KIND, 4><<<grid, 32 * warps, 0, st>>>(p);
+    else k_fp4_gemv<KIND, 2><<<grid, 32 * warps, 0, st>>>(p);
     return cudaGetLastError();
 }
 

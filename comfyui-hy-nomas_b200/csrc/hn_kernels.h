@@ -152,7 +152,7 @@ struct Fp4GemmArgs {
     int64_t M, N, K;        // K: of the padded codes, a multiple of 32
     int kind;
 };
-constexpr int FP4_GEMV_MAX_M = 4;       // rows that run as a GEMV (fp4_gemv.cu)
+constexpr int FP4_GEMV_MAX_M = 2;       // rows that run as a GEMV (fp4_gemv.cu)
 bool fp4_gemv_applies(const Fp4GemmArgs &a);
 cudaError_t launch_fp4_gemv(const Fp4GemmArgs &a, cudaStream_t st);
 cudaError_t launch_fp4_gemm(const Fp4GemmArgs &a, cudaStream_t st, const char **msg);

@@ -152,38 +152,48 @@ def int8_g128_linear(x, qw, sw, bias=None):
 # ----------------------------------------------------------------------------------------------- 4-bit codes with block scales
 
 FP4_SPAN = {"mxfp4": 128, "nvfp4": 64}      # columns of a scale tile
+_FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _fp4_kind(kind, what):
-    if kind not in FP4_SPAN:
+    code = _lib.FP4_KIND.get(kind)
+    if code is None:
         raise ValueError(f"{what}: kind {kind!r} (mxfp4 or nvfp4)")
-    return _lib.FP4_KIND[kind]
+    return code
 
 
-def _fp4_operand(q, s, r, kind, what, name):
-    """The checks of one operand -> (codes whose rows start on 16 bytes, scales, row scales)."""
-    if q.dtype != torch.uint8 or q.dim() != 2 or q.shape[1] % 16 or not q.shape[1]:
+def _fp4_operand(q, s, r, kind, device, what, name):
+    """The checks of one operand -> (codes whose rows start on 16 bytes, their row pitch, scales, row scales, rows, K)."""
+    shape = q.shape
+    if len(shape) != 2 or shape[1] % 16 or not shape[1] or q.dtype != torch.uint8:
         raise ValueError(f"{what}: the codes of {name} must be uint8 [rows, K / 2] with K a multiple of 32, got {q.dtype} "
-                         f"{tuple(q.shape)}")
-    rows, kp = q.shape[0], 2 * q.shape[1]
-    span = FP4_SPAN[kind]
-    want = ((rows + 127) // 128, (kp + span - 1) // span, 512)
-    if s.dtype != torch.uint8 or s.shape != want:
+                         f"{tuple(shape)}")
+    rows, half = shape
+    span = FP4_SPAN[kind] // 2
+    want = ((rows + 127) // 128, (half + span - 1) // span, 512)
+    if s.shape != want or s.dtype != torch.uint8:
         raise ValueError(f"{what}: the scales of {name} must be uint8 {want} for {kind}, got {s.dtype} {tuple(s.shape)}")
+    if s.device != device:
+        raise RuntimeError(f"{what}: scales of {name} on {s.device}, the codes on {device}")
     if r is not None:
         if kind == "mxfp4":
             raise ValueError(f"{what}: mxfp4 has no row scales")
         if r.dtype != torch.float32 or r.shape != (rows,):
             raise ValueError(f"{what}: the row scales of {name} must be fp32 [{rows}], got {r.dtype} {tuple(r.shape)}")
+        if r.device != device:
+            raise RuntimeError(f"{what}: row scales of {name} on {r.device}, the codes on {device}")
         if not r.is_contiguous():
             r = r.contiguous()
-    if s.device != q.device or (r is not None and r.device != q.device):
-        raise RuntimeError(f"{what}: codes and scales of {name} on different devices")
-    if not (q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1] and q.data_ptr() % 16 == 0):
-        q = _lib.dense(q)
-    if not (s.is_contiguous() and s.data_ptr() % 16 == 0):
+    pitch = half
+    if not q.is_contiguous():
+        pitch = q.stride(0)
+        if q.stride(1) != 1 or pitch % 16 or pitch < half:
+            q, pitch = _lib.dense(q), half
+    if q.data_ptr() % 16:
+        q, pitch = _lib.dense(q), half
+    if not s.is_contiguous() or s.data_ptr() % 16:
         s = _lib.dense(s)
-    return q, s, r
+    return q, pitch, s, r, rows, 2 * half
 
 
 def quantize_fp4(x, kind="nvfp4"):
@@ -196,20 +206,25 @@ def quantize_fp4(x, kind="nvfp4"):
     code = _fp4_kind(kind, "quantize_fp4")
     if not x.is_cuda:
         _lib.require_cuda(x)
-    if x.dim() != 2 or x.shape[1] == 0:
-        raise ValueError(f"quantize_fp4: x must be [M, K], got {tuple(x.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        x = x.float()
-    m, k = x.shape
-    if x.stride(1) != 1 or x.stride(0) < k:
-        x = x.contiguous()
-    kp, device = (k + 31) // 32 * 32, x.device
-    span = FP4_SPAN[kind]
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"quantize_fp4: x must be [M, K], got {tuple(shape)}")
+    dtype = _FLOATS.get(x.dtype)
+    if dtype is None:
+        x, dtype = x.float(), 2
+    m, k = shape
+    pitch = k
+    if not x.is_contiguous():
+        if x.stride(1) == 1 and x.stride(0) >= k:
+            pitch = x.stride(0)
+        else:
+            x = x.contiguous()
+    kp, device, span = (k + 31) // 32 * 32, x.device, FP4_SPAN[kind]
     q = torch.empty((m, kp // 2), dtype=torch.uint8, device=device)
     s = torch.empty(((m + 127) // 128, (kp + span - 1) // span, 512), dtype=torch.uint8, device=device)
-    r = torch.empty(m, dtype=torch.float32, device=device) if kind == "nvfp4" else None
-    _lib.check(_lib.launch("hn_quantize_fp4", device, x.data_ptr(), max(x.stride(0), k), _lib.DTYPE[x.dtype], m, k, code,
-                           q.data_ptr(), kp // 2, s.data_ptr(), None if r is None else r.data_ptr()), "quantize_fp4")
+    r = torch.empty(m, dtype=torch.float32, device=device) if code == 3 else None
+    _lib.check(_lib.launch("hn_quantize_fp4", device, x.data_ptr(), pitch, dtype, m, k, code, q.data_ptr(), kp // 2, s.data_ptr(),
+                           None if r is None else r.data_ptr()), "quantize_fp4")
     return q, s, r
 
 
@@ -217,20 +232,20 @@ def dequantize_fp4(q, s, r=None, kind="nvfp4", dtype=torch.bfloat16, columns=Non
     """What codes, scales and row scales (None: all 1) stand for: code * (scale * row scale), rounded once to `dtype` (bf16, fp16,
     fp32) [M, columns]. `columns`: the K that was quantized, where it was no multiple of 32."""
     code = _fp4_kind(kind, "dequantize_fp4")
-    _lib.require_cuda(q, s, r)
-    q, s, r = _fp4_operand(q, s, r, kind, "dequantize_fp4", "q")
-    m, kp = q.shape[0], 2 * q.shape[1]
+    if not q.is_cuda:
+        _lib.require_cuda(q)
+    device = q.device
+    q, pitch, s, r, m, kp = _fp4_operand(q, s, r, kind, device, "dequantize_fp4", "q")
     k = kp if columns is None else columns
     if not kp - 32 < k <= kp:
         raise ValueError(f"dequantize_fp4: {k} columns of {kp}")
-    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if dtype not in _FLOATS:
         raise TypeError(f"dequantize_fp4: dtype {dtype} (bf16, fp16 or fp32)")
     if r is None and kind == "nvfp4":
-        r = torch.ones(m, dtype=torch.float32, device=q.device)
-    out = torch.empty((m, k), dtype=dtype, device=q.device)
-    _lib.check(_lib.launch("hn_dequantize_fp4", q.device, q.data_ptr(), q.stride(0), s.data_ptr(),
-                           None if r is None else r.data_ptr(), m, k, kp, code, out.data_ptr(), k, _lib.DTYPE[dtype]),
-               "dequantize_fp4")
+        r = torch.ones(m, dtype=torch.float32, device=device)
+    out = torch.empty((m, k), dtype=dtype, device=device)
+    _lib.check(_lib.launch("hn_dequantize_fp4", device, q.data_ptr(), pitch, s.data_ptr(), None if r is None else r.data_ptr(), m, k,
+                           kp, code, out.data_ptr(), k, _FLOATS[dtype]), "dequantize_fp4")
     return out
 
 
@@ -241,37 +256,40 @@ def fp4_gemm(qa, sa, ra, qw, sw, rw, bias=None, out_dtype=torch.bfloat16, kind="
 
     `out`: a caller-owned [M, N] destination of `out_dtype` with unit column stride (rows may be strided)."""
     code = _fp4_kind(kind, "fp4_gemm")
-    if not (qa.is_cuda and qw.is_cuda and sa.is_cuda and sw.is_cuda):
-        _lib.require_cuda(qa, qw, sa, sw)
-    qa, sa, ra = _fp4_operand(qa, sa, ra, kind, "fp4_gemm", "a")
-    qw, sw, rw = _fp4_operand(qw, sw, rw, kind, "fp4_gemm", "w")
-    m, n, half = qa.shape[0], qw.shape[0], qa.shape[1]
+    if not (qa.is_cuda and qw.is_cuda):
+        _lib.require_cuda(qa, qw)
     device = qa.device
-    if qw.shape[1] != half:
-        raise ValueError(f"fp4_gemm: a has {2 * half} columns, w {2 * qw.shape[1]}")
-    if n == 0:
-        raise ValueError("fp4_gemm: w has no rows")
     if qw.device != device:
         raise RuntimeError(f"fp4_gemm: a on {device}, w on {qw.device}")
-    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    qa, lda, sa, ra, m, k = _fp4_operand(qa, sa, ra, kind, device, "fp4_gemm", "a")
+    qw, ldw, sw, rw, n, kw = _fp4_operand(qw, sw, rw, kind, device, "fp4_gemm", "w")
+    if kw != k:
+        raise ValueError(f"fp4_gemm: a has {k} columns, w {kw}")
+    if n == 0:
+        raise ValueError("fp4_gemm: w has no rows")
+    dtype = _FLOATS.get(out_dtype)
+    if dtype is None:
         raise TypeError(f"fp4_gemm: out_dtype {out_dtype} (bf16, fp16 or fp32)")
     if bias is not None:
-        if bias.shape != (n,) or bias.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        if bias.shape != (n,) or bias.dtype not in _FLOATS:
             raise ValueError(f"fp4_gemm: bias must be bf16, fp16 or fp32 [{n}], got {bias.dtype} {tuple(bias.shape)}")
         if bias.device != device:
             raise RuntimeError(f"fp4_gemm: a on {device}, bias on {bias.device}")
         if not bias.is_contiguous():
             bias = bias.contiguous()
+    ldo = n
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype, device=device)
-    elif out.shape != (m, n) or out.dtype != out_dtype or out.device != device or (n > 1 and out.stride(1) != 1) or \
-            (m > 1 and out.stride(0) < n):
-        raise ValueError(f"fp4_gemm: out must be a {out_dtype} [{m}, {n}] tensor with unit column stride on {device}")
-    _lib.check(_lib.launch("hn_fp4_gemm", device, qa.data_ptr(), qa.stride(0), sa.data_ptr(),
-                           None if ra is None else ra.data_ptr(), qw.data_ptr(), qw.stride(0), sw.data_ptr(),
-                           None if rw is None else rw.data_ptr(), None if bias is None else bias.data_ptr(),
-                           0 if bias is None else _lib.DTYPE[bias.dtype], out.data_ptr(), max(out.stride(0), n),
-                           _lib.DTYPE[out_dtype], m, n, 2 * half, code), "fp4_gemm")
+    else:
+        if out.shape != (m, n) or out.dtype != out_dtype or out.device != device or (n > 1 and out.stride(1) != 1) or \
+                (m > 1 and out.stride(0) < n):
+            raise ValueError(f"fp4_gemm: out must be a {out_dtype} [{m}, {n}] tensor with unit column stride on {device}")
+        if m > 1:
+            ldo = out.stride(0)
+    _lib.check(_lib.launch("hn_fp4_gemm", device, qa.data_ptr(), lda, sa.data_ptr(), None if ra is None else ra.data_ptr(),
+                           qw.data_ptr(), ldw, sw.data_ptr(), None if rw is None else rw.data_ptr(),
+                           None if bias is None else bias.data_ptr(), 0 if bias is None else _FLOATS[bias.dtype], out.data_ptr(),
+                           ldo, dtype, m, n, k, code), "fp4_gemm")
     return out
 
 

@@ -148,20 +148,20 @@ class KVCache:
         what = "append_rotated"
         if not (q.is_cuda and k.is_cuda and v.is_cuda):
             _lib.require_cuda(q, k, v)
-        rows, device = self._ids(rows, what), self.device
-        if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        rows, device, bf16 = self._ids(rows, what), self.device, torch.bfloat16
+        if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
             raise TypeError(f"{what}: bf16 expected, got {q.dtype}, {k.dtype} and {v.dtype}")
-        b = rows.numel()
-        if k.dim() != 4 or k.shape != v.shape or k.shape[2] != self.heads or k.shape[3] != HEAD_DIM or k.shape[0] != b or \
-                q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != HEAD_DIM or q.shape[2] == 0:
-            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} must be "
+        b, qshape, shape = rows.shape[0], q.shape, k.shape
+        if len(shape) != 4 or shape != v.shape or shape[2] != self.heads or shape[3] != HEAD_DIM or shape[0] != b or \
+                len(qshape) != 4 or qshape[:2] != shape[:2] or qshape[3] != HEAD_DIM or qshape[2] == 0:
+            raise ValueError(f"{what}: q {tuple(qshape)}, k {tuple(shape)} and v {tuple(v.shape)} must be "
                              f"[{b}, n, H, {HEAD_DIM}] and [{b}, n, {self.heads}, {HEAD_DIM}]")
         if not 0 <= layer < self.layers:
             raise ValueError(f"{what}: layer {layer} of {self.layers}")
-        if any(t.device != device for t in (q, k, v)):
+        if q.device != device or k.device != device or v.device != device:
             raise RuntimeError(f"{what}: q on {q.device}, k on {k.device} and v on {v.device}, the cache is on {device}")
         rotary.check_rotary(rot, HEAD_DIM, device, what)
-        n, h = k.shape[1], q.shape[2]
+        n, h = shape[1], qshape[2]
         ptr, pb, pt, wide, positions = (None, 0, 0, 0, None) if positions is None else \
             rotary.positions_of(positions, b, n, device, what)
         wq, wk = rotary.norm_weight(q_norm, HEAD_DIM, device, what), rotary.norm_weight(k_norm, HEAD_DIM, device, what)

@@ -17,6 +17,7 @@ import torch
 from . import _lib
 
 LAYOUTS = {"half": 0, "interleaved": 1}
+_FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SCALINGS = {"linear": {"factor"}, "ntk": {"factor"}, "yarn": {"factor", "original", "beta_fast", "beta_slow", "attention_factor"}}
 
 
@@ -85,19 +86,25 @@ class Rotary:
         self._args = (dim, LAYOUTS[layout], self.factor)
 
 
+_WIDE = {torch.int32: 0, torch.int64: 1}
+
+
 def positions_of(p, batch, tokens, device, what):
     """(pointer, batch stride, token stride, 1 if int64, the tensor) of positions [batch, tokens] or [tokens]."""
-    if not isinstance(p, torch.Tensor) or p.is_floating_point() or p.is_complex() or p.dtype == torch.bool:
-        raise TypeError(f"{what}: positions must be a tensor of integers")
-    if p.dtype not in (torch.int32, torch.int64):
-        p = p.to(torch.int32 if p.element_size() < 4 else torch.int64)
+    wide = _WIDE.get(p.dtype) if isinstance(p, torch.Tensor) else None
+    if wide is None:
+        if not isinstance(p, torch.Tensor) or p.is_floating_point() or p.is_complex() or p.dtype == torch.bool:
+            raise TypeError(f"{what}: positions must be a tensor of integers")
+        p, wide = p.to(torch.int64), 1
     if p.device != device:
         raise RuntimeError(f"{what}: positions on {p.device}, the heads on {device}")
-    if p.shape == (tokens,):
-        return p.data_ptr(), 0, p.stride(0), int(p.dtype == torch.int64), p
-    if p.shape != (batch, tokens):
-        raise ValueError(f"{what}: positions {tuple(p.shape)} must be [{batch}, {tokens}] or [{tokens}]")
-    return p.data_ptr(), p.stride(0), p.stride(1), int(p.dtype == torch.int64), p
+    shape = p.shape
+    if shape == (tokens,):
+        return p.data_ptr(), 0, p.stride(0), wide, p
+    if shape != (batch, tokens):
+        raise ValueError(f"{what}: positions {tuple(shape)} must be [{batch}, {tokens}] or [{tokens}]")
+    pb, pt = p.stride()
+    return p.data_ptr(), pb, pt, wide, p
 
 
 def norm_weight(w, dim, device, what):
@@ -123,7 +130,8 @@ def check_rotary(rot, dim, device, what):
 
 
 def _steps8(t):
-    return t.stride(3) == 1 and not (t.stride(0) | t.stride(1) | t.stride(2)) % 8 and t.data_ptr() % 16 == 0
+    a, b, c, d = t.stride()
+    return d == 1 and not (a | b | c) % 8 and t.data_ptr() % 16 == 0
 
 
 def _span(t):
@@ -142,11 +150,13 @@ def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
     if not x.is_cuda:
         _lib.require_cuda(x)
     device = x.device
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    dtype = _FLOATS.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"rotate: x must be bf16, fp16 or fp32, got {x.dtype}")
-    if x.dim() != 4 or x.shape[3] % 8 or not 8 <= x.shape[3] <= 256:
-        raise ValueError(f"rotate: x must be [B, L, H, D] with D a multiple of 8 up to 256, got {tuple(x.shape)}")
-    b, l, h, d = x.shape
+    shape = x.shape
+    if len(shape) != 4 or shape[3] % 8 or not 8 <= shape[3] <= 256:
+        raise ValueError(f"rotate: x must be [B, L, H, D] with D a multiple of 8 up to 256, got {tuple(shape)}")
+    b, l, h, d = shape
     check_rotary(rot, d, device, what)
     ptr, pb, pl, wide, keep = positions_of(positions, b, l, device, what)
     w = norm_weight(weight, d, device, what)
@@ -165,7 +175,7 @@ def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
                 raise ValueError("rotate: out must be x itself or lie apart from it")
     dim, layout, factor = rot._args
     xs, os = src.stride(), out.stride()
-    _lib.check(_lib.launch("hn_rotate", device, src.data_ptr(), xs[0], xs[1], xs[2], _lib.DTYPE[x.dtype], ptr, pb, pl, wide,
+    _lib.check(_lib.launch("hn_rotate", device, src.data_ptr(), xs[0], xs[1], xs[2], dtype, ptr, pb, pl, wide,
                            rot.freq.data_ptr(), dim, layout, factor, None if w is None else w.data_ptr(), eps, b, l, h, d,
                            out.data_ptr(), os[0], os[1], os[2]), what)
     return out
