@@ -227,3 +227,109 @@ def test_product_many_rows(hn, cuda, kind, m, n, k):
     a, w = operands(hn, m, n, k, kind, 13)
     for dtype in DTYPES:
         check_product(hn, hn.kernels.fp4_gemm(*a, *w, kind=kind, out_dtype=dtype), a, w, kind)
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 96), (2, 300, 2080), (20, 300, 512), (130, 200, 4096), (2500, 2400, 128)])
+def test_product_nan_stays_in_its_row_and_column(hn, cuda, kind, m, n, k):
+    """A NaN or an infinity in a row of either operand: its outputs are NaN, all others as without it."""
+    x, y = randn((m, k), 1), randn((n, k), 2)
+    clean = hn.kernels.fp4_gemm(*hn.kernels.quantize_fp4(x, kind), *hn.kernels.quantize_fp4(y, kind), kind=kind, out_dtype=torch.float32)
+    x[m - 1, k - 1], y[n // 2, 0], y[n - 1, k // 2] = float("nan"), float("inf"), float("nan")
+    out = hn.kernels.fp4_gemm(*hn.kernels.quantize_fp4(x, kind), *hn.kernels.quantize_fp4(y, kind), kind=kind, out_dtype=torch.float32)
+    bad = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    bad[m - 1], bad[:, n // 2], bad[:, n - 1] = True, True, True
+    assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 512), (60, 301, 512), (600, 301, 96), (2500, 2401, 96), (2500, 2400, 96)])
+def test_product_bias_out_and_views(hn, cuda, kind, m, n, k):
+    """Biases of all types at odd addresses, outputs with strided rows at odd addresses, codes with strided rows."""
+    a, w = operands(hn, m, n, k, kind, 21)
+    wide = torch.zeros((m, k), dtype=torch.uint8, device="cuda")
+    wide[:, :k // 2] = a[0]
+    av = (wide[:, :k // 2], a[1], a[2])
+    for bias_dtype in DTYPES:
+        for out_dtype in DTYPES:
+            bias = randn((n + 1,), 3, bias_dtype, loud=False)[1:]
+            base = torch.full((m, n + 6), 7.0, dtype=out_dtype, device="cuda")
+            out = base[:, 3:n + 3]
+            assert hn.kernels.fp4_gemm(*av, *w, bias, out_dtype, kind, out) is out
+            check_product(hn, out, a, w, kind, bias)
+            assert bool((base[:, :3] == 7).all()) and bool((base[:, n + 3:] == 7).all())
+
+
+def test_product_without_row_scales(hn, cuda):
+    a, w = operands(hn, 70, 50, 320, "nvfp4", 5)
+    one = lambda t: (t[0], t[1], torch.ones_like(t[2]))  # noqa: E731
+    for m in (1, 70):
+        q, s, r = hn.kernels.quantize_fp4(randn((m, 320), 9), "nvfp4")
+        assert torch.equal(hn.kernels.fp4_gemm(q, s, None, w[0], w[1], None), hn.kernels.fp4_gemm(*one((q, s, r)), *one(w)))
+        assert torch.equal(hn.kernels.fp4_gemm(q, s, r, w[0], w[1], None), hn.kernels.fp4_gemm(q, s, r, *one(w)))
+
+
+def test_product_largest_scales(hn, cuda):
+    """MX scales from 2^-127 to 2^120. With s = 2^(ea + ew - 254) every partial sum is a multiple of s / 4 up to 2^14 s: exact in fp32
+    from ea + ew = 130 on (s / 4 = 2^-126) while 2^14 s stays finite (ea + ew < 366); below, each of 16 partial sums may lose what
+    lies under the smallest normal number; above, what is infinite is not finite (infinities of both signs may meet)."""
+    a, w = operands(hn, 5, 130, 256, "mxfp4", 6)
+    va, vw = (torch.from_numpy(VALUES[unpack(t[0])]).cuda() for t in (a, w))
+    sums = va @ vw.t()                                    # exact: small integers times 0.25
+    for ea, ew in ((1, 100), (0, 140), (127, 127), (200, 60), (247, 127), (247, 200), (0, 0)):
+        sa, sw = torch.full_like(a[1], ea), torch.full_like(w[1], ew)
+        want = (sums * 2.0 ** (ea + ew - 254)).float()
+        for m in (1, 5):
+            out = hn.kernels.fp4_gemm(a[0][:m].contiguous(), sa, None, w[0], sw, None, kind="mxfp4", out_dtype=torch.float32)
+            if 130 <= ea + ew < 366:
+                assert torch.equal(out, want[:m]), (ea, ew, m)
+            elif ea + ew < 130:
+                assert bool(((out - want[:m]).abs() <= 16 * 2.0 ** -126).all()), (ea, ew, m)
+            else:
+                assert not bool(out[want[:m].isinf()].isfinite().any()), (ea, ew, m)
+
+
+def test_linear(hn, cuda):
+    x = randn((3, 5, 100), 7)
+    w = hn.kernels.quantize_fp4(randn((40, 100), 8), "nvfp4")
+    bias = randn((40,), 9, loud=False)
+    y = hn.kernels.fp4_linear(x, *w, bias)
+    assert y.shape == (3, 5, 40) and y.dtype == torch.bfloat16
+    assert torch.equal(y.view(15, 40), hn.kernels.fp4_gemm(*hn.kernels.quantize_fp4(x.view(15, 100)), *w, bias))
+    assert hn.kernels.fp4_linear(x[:0], *w).shape == (0, 5, 40) and hn.kernels.fp4_linear(x[0, 0], *w).shape == (40,)
+    assert hn.kernels.fp4_linear(x.float(), *w).dtype == torch.float32
+    for bad, error in ((lambda: hn.kernels.fp4_linear(x[..., :60], *w), ValueError), (lambda: hn.kernels.fp4_linear(x.long(), *w), TypeError)):
+        with pytest.raises(error):
+            bad()
+
+
+def test_stacked(hn, cuda):
+    """Linears stacked along N give their outputs side by side, for every kernel."""
+    for m in (1, 30, 3000):
+        x = hn.kernels.quantize_fp4(randn((m, 288), m))
+        parts = [hn.kernels.quantize_fp4(randn((n, 288), n)) for n in (128, 1280, 1000)]
+        both = hn.kernels.fp4_gemm(*x, *hn.ops.stack_fp4_linears(*parts))
+        assert torch.equal(both, torch.cat([hn.kernels.fp4_gemm(*x, *p) for p in parts], 1))
+
+
+def test_refusals(hn, cuda):
+    K = hn.kernels
+    a, w = operands(hn, 5, 40, 96, "nvfp4", 3)
+    x = randn((5, 96), 1)
+    for bad, error in ((lambda: K.quantize_fp4(x, "fp4"), ValueError), (lambda: K.quantize_fp4(x[0]), ValueError),
+                       (lambda: K.quantize_fp4(x[:, :0]), ValueError), (lambda: K.dequantize_fp4(*a, columns=64), ValueError),
+                       (lambda: K.dequantize_fp4(*a, columns=97), ValueError), (lambda: K.dequantize_fp4(*a, dtype=torch.int8), TypeError),
+                       (lambda: K.dequantize_fp4(*a, "mxfp4"), ValueError), (lambda: K.dequantize_fp4(a[0], a[1], a[2][:4]), ValueError),
+                       (lambda: K.dequantize_fp4(a[0], a[1].cpu(), a[2]), RuntimeError),
+                       (lambda: K.fp4_gemm(*a, *w, kind="mxfp4"), ValueError), (lambda: K.fp4_gemm(*a, w[0][:, :32], w[1][:, :1], w[2]), ValueError),
+                       (lambda: K.fp4_gemm(*a, w[0][:0], w[1][:0], w[2][:0]), ValueError), (lambda: K.fp4_gemm(a[0].int(), *a[1:], *w), ValueError),
+                       (lambda: K.fp4_gemm(a[0], a[1][:, :1], a[2], *w), ValueError), (lambda: K.fp4_gemm(a[0], a[1], a[2].double(), *w), ValueError),
+                       (lambda: K.fp4_gemm(*a, *w, out_dtype=torch.int32), TypeError), (lambda: K.fp4_gemm(*a, *w, bias=x[0]), ValueError),
+                       (lambda: K.fp4_gemm(*a, *w, bias=x[0, :40].cpu()), RuntimeError), (lambda: K.fp4_gemm(*a, w[0].cpu(), *w[1:]), RuntimeError),
+                       (lambda: K.fp4_gemm(*a, *w, out=x), ValueError), (lambda: K.fp4_gemm(*a, *w, out=x[:1, :40].expand(5, 40)), ValueError)):
+        with pytest.raises(error):
+            bad()
+    assert K.fp4_gemm(*(t[:0] for t in a), *w).shape == (0, 40)
+    assert K.dequantize_fp4(*(t[:0] for t in a)).shape == (0, 96)
+    q = K.quantize_fp4(x[:0])
+    assert q[0].shape == (0, 48) and q[1].shape == (0, 2, 512) and q[2].shape == (0,)
