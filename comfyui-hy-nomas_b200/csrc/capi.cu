@@ -847,6 +847,7 @@ int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, co
     a.qw = qw; a.ldw = ldw; a.sw = sw; a.rw = rw;
     a.bias = bias; a.bias_dtype = bias_dtype; a.out = out; a.ldo = ldo; a.out_dtype = out_dtype;
     a.M = M; a.N = N; a.K = K; a.kind = kind - HN_KIND_MXFP4;
+    a.sm_reserve = gemm_sm_reserve();
     const char *msg = nullptr;
     cudaError_t e = launch_fp4_gemm(a, (cudaStream_t)stream, &msg);
     if (e != cudaSuccess && msg) return fail(HN_ERR_ALIGN, "hn_fp4_gemm: %s", msg);

@@ -765,8 +765,9 @@ template <int KIND> static cudaError_t launch_wide(const Fp4GemmArgs &a, cudaStr
         *msg = "cuTensorMapEncodeTiled failed (pointer/stride alignment or driver entry point)";
         return cudaErrorInvalidValue;
     }
-    int pairs = num_sms() / 2;
+    int pairs = (num_sms() - a.sm_reserve) / 2;
     if (pairs > p.tiles) pairs = p.tiles;
+    if (pairs < 1) pairs = 1;
     auto go = [&](auto kernel, bool (&done)[HN_MAX_DEV]) {
         cudaError_t e = opt_in(kernel, C::SMEM, done);
         if (e != cudaSuccess) return e;

@@ -151,6 +151,7 @@ struct Fp4GemmArgs {
     void *out; int64_t ldo; int out_dtype;
     int64_t M, N, K;        // K: of the padded codes, a multiple of 32
     int kind;
+    int sm_reserve;         // SMs that the persistent kernel leaves free
 };
 constexpr int FP4_GEMV_MAX_M = 2;       // rows that run as a GEMV (fp4_gemv.cu)
 bool fp4_gemv_applies(const Fp4GemmArgs &a);

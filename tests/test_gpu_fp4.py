@@ -333,3 +333,16 @@ def test_refusals(hn, cuda):
     assert K.dequantize_fp4(*(t[:0] for t in a)).shape == (0, 96)
     q = K.quantize_fp4(x[:0])
     assert q[0].shape == (0, 48) and q[1].shape == (0, 2, 512) and q[2].shape == (0,)
+
+
+def test_product_leaves_reserved_sms(hn, cuda):
+    """The GEMMs' SM reserve holds for the persistent kernel, too; its results do not depend on it."""
+    a, w = operands(hn, 2500, 2400, 96, "nvfp4", 30)
+    want = hn.kernels.fp4_gemm(*a, *w)
+    L, was = hn.lib.lib, hn.lib.lib.hn_get_gemm_sm_reserve()
+    try:
+        for n in (1, 20, 64):
+            assert L.hn_set_gemm_sm_reserve(n) == 0
+            assert torch.equal(hn.kernels.fp4_gemm(*a, *w), want)
+    finally:
+        L.hn_set_gemm_sm_reserve(was)
