@@ -39,6 +39,10 @@ template <typename E> struct Chunk {                // two to a word
         const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 8);
         w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     }
+    __device__ __forceinline__ void load4(const E *p) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+    }
     __device__ __forceinline__ void put(int j, const E *p) { w[j >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p) << (16 * (j & 1)); }
     __device__ __forceinline__ void widen(float (&v)[16]) const {
 #pragma unroll
@@ -64,6 +68,10 @@ template <> struct Chunk<float> {
             w[i] = a.x; w[i + 1] = a.y; w[i + 2] = a.z; w[i + 3] = a.w;
         }
     }
+    __device__ __forceinline__ void load4(const float *p) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = p[i];
+    }
     __device__ __forceinline__ void put(int j, const float *p) { w[j] = *p; }
     __device__ __forceinline__ void widen(float (&v)[16]) const {
 #pragma unroll
@@ -71,23 +79,44 @@ template <> struct Chunk<float> {
     }
 };
 
-// columns 16 c to 16 c + 15 of a row, zeros behind its end. VEC: the row starts on 16 bytes
-template <typename E, bool VEC> __device__ __forceinline__ void load_chunk(const E *row, int c, int K, Chunk<E> &v) {
+// columns 16 c to 16 c + 15 of a row, zeros behind its end. VEC: all rows start on 16 bytes (2), on 4 (1, 16-bit types), or
+// anywhere (0)
+template <typename E, int VEC> __device__ __forceinline__ void load_chunk(const E *row, int c, int K, Chunk<E> &v) {
     v.clear();
-    if (VEC && 16 * c + 16 <= K) {
+    if (VEC == 2 && 16 * c + 16 <= K) {
         v.load(row + 16 * c);
+    } else if (VEC == 1 && 16 * c + 16 <= K) {
+        v.load4(row + 16 * c);
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
             if (16 * c + j < K) v.put(j, row + 16 * c + j);
     }
 }
-template <typename E> __device__ __forceinline__ float peak16(const Chunk<E> &c) {
-    float v[16], p = 0.0f;
-    c.widen(v);
+// The largest magnitude of a chunk as a number that orders as magnitudes do, NaN above infinity: of 16-bit types the bits without
+// the sign (two columns an instruction), of fp32 the value. `magnitude` makes it a float (a NaN or an infinity of its own).
+__device__ __forceinline__ uint32_t peak_bits(const uint32_t (&w)[8]) {
+    uint32_t m = __vimax3_u16x2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu, w[2] & 0x7fff7fffu);
+    m = __vimax3_u16x2(m, w[3] & 0x7fff7fffu, w[4] & 0x7fff7fffu);
+    m = __vimax3_u16x2(m, w[5] & 0x7fff7fffu, w[6] & 0x7fff7fffu);
+    m = __vmaxu2(m, w[7] & 0x7fff7fffu);
+    return max(m & 0xffffu, m >> 16);
+}
+template <typename E> __device__ __forceinline__ uint32_t peak16(const Chunk<E> &c) { return peak_bits(c.w); }
+template <> __device__ __forceinline__ uint32_t peak16(const Chunk<float> &c) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < 16; j += 2) p = nanmax_abs3(p, v[j], v[j + 1]);
-    return p;
+    for (int j = 0; j < 16; j += 2) m = __vimax3_u32(m, __float_as_uint(c.w[j]) & 0x7fffffffu, __float_as_uint(c.w[j + 1]) & 0x7fffffffu);
+    return m;
+}
+template <typename E> __device__ __forceinline__ float magnitude(uint32_t bits);
+template <> __device__ __forceinline__ float magnitude<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <> __device__ __forceinline__ float magnitude<__half>(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+template <> __device__ __forceinline__ float magnitude<float>(uint32_t bits) { return __uint_as_float(bits); }
+template <int W> __device__ __forceinline__ uint32_t lanes_most(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < W; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 __device__ __forceinline__ uint2 pack16(const float (&v)[16]) {
     return make_uint2(pack8_e2m1(*reinterpret_cast<const float(*)[8]>(v)), pack8_e2m1(*reinterpret_cast<const float(*)[8]>(v + 8)));
@@ -132,13 +161,12 @@ template <typename E> __device__ __forceinline__ uint2 chunk_nv(const Chunk<E> &
     float v[16];
     c.widen(v);
     if (den >= 0x1p-90f) {
-        const uint64_t ns = x2_splat(-den), rs = x2_splat(__frcp_rn(den));
+        // x2_quot with the remainder's and the reciprocal's signs turned: a zero keeps its sign
+        const uint64_t d = x2_splat(den), nr = x2_splat(-__frcp_rn(den));
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-            float a, b;
-            x2_split(x2_quot(x2_mul(x2(v[j], v[j + 1]), x2_splat(0.65625f)), ns, rs), a, b);
-            v[j] = copysignf(a, v[j]);          // of a zero
-            v[j + 1] = copysignf(b, v[j + 1]);
+            const uint64_t np = x2_mul(x2(v[j], v[j + 1]), x2_splat(-0.65625f)), q0 = x2_mul(np, nr);
+            x2_split(x2_fma(x2_fma(q0, d, np), nr, q0), v[j], v[j + 1]);
         }
     } else {
 #pragma unroll
@@ -156,39 +184,40 @@ template <int W, int B> __device__ __forceinline__ uint32_t gather_word(uint32_t
 }
 
 // T threads a row (below 32: so many lanes of a warp), the row in registers
-template <typename E, int KIND, bool VEC, int T, int NCH>
+template <typename E, int KIND, int VEC, int T, int NCH>
 __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quant_fp4(Params p) {
     constexpr int BLK = GROUP<KIND> / 16, LANES = SPAN<KIND> / 16, W = LANES < T ? LANES : T;
-    __shared__ float red[T < 128 ? 1 : T / 32];
+    __shared__ uint32_t red[T < 128 ? 128 / T : 1][T < 32 ? 1 : T / 32];
     const int t = threadIdx.x % T, lane = threadIdx.x & 31, warp = (threadIdx.x % T) >> 5;
     const int64_t m = T < 128 ? (int64_t)blockIdx.x * (128 / T) + threadIdx.x / T : (int64_t)blockIdx.x;
     const bool row = m < p.M;                   // p.rows is whole blocks of threads, so no thread leaves before a shuffle
     Chunk<E> v[NCH];
-    float peak[NCH];
+    uint32_t peak[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
         const int c = i * T + t;
         load_chunk<E, VEC>(static_cast<const E *>(p.x) + m * p.ldx, c, row ? p.K : 0, v[i]);
     }
-    float top = 0.0f;
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        peak[i] = lanes_max<BLK>(peak16(v[i]));
-        top = nanmax(top, peak[i]);
+        peak[i] = lanes_most<BLK>(peak16(v[i]));
+        top = max(top, peak[i]);
     }
     RowNV n;
     if (KIND == NV) {
 #pragma unroll
-        for (int o = 1; o < (T < 32 ? T : 32); o <<= 1) top = nanmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (T >= 128) {
-            if (lane == 0) red[warp] = top;
+        for (int o = 1; o < (T < 32 ? T : 32); o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (T > 32) {
+            uint32_t *mine = red[T < 128 ? threadIdx.x / T : 0];
+            if (lane == 0) mine[warp] = top;
             __syncthreads();
-            top = red[0];
+            top = mine[0];
 #pragma unroll
-            for (int i = 1; i < T / 32; ++i) top = nanmax(top, red[i]);
+            for (int i = 1; i < T / 32; ++i) top = max(top, mine[i]);
         }
         float r;
-        n = row_nv(top, &r);
+        n = row_nv(magnitude<E>(top), &r);
         if (row && t == 0) p.r[m] = r;
     }
 #pragma unroll
@@ -196,44 +225,44 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) k_quant_fp4(Params p) {
         const int c = i * T + t;
         uint32_t byte = 0;
         if (row && c < p.nch)
-            *reinterpret_cast<uint2 *>(p.q + m * p.ldq + 8 * c) = KIND == MX ? chunk_mx(v[i], peak[i], byte) : chunk_nv(v[i], peak[i], n, byte);
+            *reinterpret_cast<uint2 *>(p.q + m * p.ldq + 8 * c) = KIND == MX ? chunk_mx(v[i], magnitude<E>(peak[i]), byte) : chunk_nv(v[i], magnitude<E>(peak[i]), n, byte);
         const uint32_t word = gather_word<W, BLK>(byte);
         if (t % W == 0 && c / LANES < p.tiles) *reinterpret_cast<uint32_t *>(p.s + scale_word(m, c / LANES, p.tiles)) = word;
     }
 }
 
 // any row length: the row's top in a pass of its own (NV)
-template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256) k_quant_fp4_long(Params p) {
+template <typename E, int KIND, int VEC> __global__ void __launch_bounds__(256) k_quant_fp4_long(Params p) {
     constexpr int BLK = GROUP<KIND> / 16, LANES = SPAN<KIND> / 16, T = 256;
-    __shared__ float red[T / 32];
+    __shared__ uint32_t red[T / 32];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int64_t m = blockIdx.x;
     const bool row = m < p.M;
     const E *x = static_cast<const E *>(p.x) + m * p.ldx;
     RowNV n;
     if (KIND == NV) {
-        float top = 0.0f;
+        uint32_t top = 0;
 #pragma unroll 4
         for (int c = t; c < (row ? p.nch : 0); c += T) {
             Chunk<E> v;
             load_chunk<E, VEC>(x, c, p.K, v);
-            top = nanmax(top, peak16(v));
+            top = max(top, peak16(v));
         }
-        top = lanes_max<32>(top);
+        top = lanes_most<32>(top);
         if (lane == 0) red[warp] = top;
         __syncthreads();
         top = red[0];
 #pragma unroll
-        for (int i = 1; i < T / 32; ++i) top = nanmax(top, red[i]);
+        for (int i = 1; i < T / 32; ++i) top = max(top, red[i]);
         float r;
-        n = row_nv(top, &r);
+        n = row_nv(magnitude<E>(top), &r);
         if (row && t == 0) p.r[m] = r;
     }
     for (int c0 = 0; c0 < p.tiles * LANES; c0 += T) {           // whole warps: the words' lanes stay together
         const int c = c0 + t;
         Chunk<E> v;
         load_chunk<E, VEC>(x, c, row ? p.K : 0, v);
-        const float peak = lanes_max<BLK>(peak16(v));
+        const float peak = magnitude<E>(lanes_most<BLK>(peak16(v)));
         uint32_t byte = 0;
         if (row && c < p.nch)
             *reinterpret_cast<uint2 *>(p.q + m * p.ldq + 8 * c) = KIND == MX ? chunk_mx(v, peak, byte) : chunk_nv(v, peak, n, byte);
@@ -242,30 +271,37 @@ template <typename E, int KIND, bool VEC> __global__ void __launch_bounds__(256)
     }
 }
 
-template <typename E, int KIND, bool VEC, int T, int NCH> cudaError_t go(const Params &p, cudaStream_t st) {
+template <typename E, int KIND, int VEC, int T, int NCH> cudaError_t go(const Params &p, cudaStream_t st) {
     constexpr int per = T < 128 ? 128 / T : 1;
     k_quant_fp4<E, KIND, VEC, T, NCH><<<(unsigned)cdiv(p.rows, per), T < 128 ? 128 : T, 0, st>>>(p);
     return cudaGetLastError();
 }
 
-// T by the row's length alone
-template <typename E, int KIND, bool VEC> cudaError_t pick(const Params &p, cudaStream_t st) {
+// T and NCH by the row's length alone: the fewest chunks that hold it
+template <typename E, int KIND, int VEC> cudaError_t pick(const Params &p, cudaStream_t st) {
     if (p.nch <= 2) return go<E, KIND, VEC, 2, 1>(p, st);
+    if (p.nch <= 4) return go<E, KIND, VEC, 4, 1>(p, st);
     if (p.nch <= 8) return go<E, KIND, VEC, 8, 1>(p, st);
     if (p.nch <= 16) return go<E, KIND, VEC, 16, 1>(p, st);
     if (p.nch <= 32) return go<E, KIND, VEC, 32, 1>(p, st);
     if (p.nch <= 64) return go<E, KIND, VEC, 32, 2>(p, st);
-    if (p.nch <= 128) return go<E, KIND, VEC, 32, 4>(p, st);
+    if (p.nch <= 96) return go<E, KIND, VEC, 32, 3>(p, st);
+    if (p.nch <= 128) return go<E, KIND, VEC, 64, 2>(p, st);
+    if (p.nch <= 192) return go<E, KIND, VEC, 64, 3>(p, st);
     if (p.nch <= 256) return go<E, KIND, VEC, 128, 2>(p, st);
-    if (p.nch <= 512) return go<E, KIND, VEC, 128, 4>(p, st);
+    if (p.nch <= 384) return go<E, KIND, VEC, 128, 3>(p, st);
+    if (p.nch <= 512) return go<E, KIND, VEC, 256, 2>(p, st);
+    if (p.nch <= 768) return go<E, KIND, VEC, 256, 3>(p, st);
     if (p.nch <= 1024) return go<E, KIND, VEC, 512, 2>(p, st);
     k_quant_fp4_long<E, KIND, VEC><<<(unsigned)p.rows, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 template <typename E> cudaError_t pick_kind(const Params &p, int kind, cudaStream_t st) {
-    const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx * (int64_t)sizeof(E) % 16 == 0;
-    if (kind == MX) return vec ? pick<E, MX, true>(p, st) : pick<E, MX, false>(p, st);
-    return vec ? pick<E, NV, true>(p, st) : pick<E, NV, false>(p, st);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * (int64_t)sizeof(E));
+    if (at % 16 == 0) return kind == MX ? pick<E, MX, 2>(p, st) : pick<E, NV, 2>(p, st);
+    if constexpr (sizeof(E) == 2)
+        if (at % 4 == 0) return kind == MX ? pick<E, MX, 1>(p, st) : pick<E, NV, 1>(p, st);
+    return kind == MX ? pick<E, MX, 0>(p, st) : pick<E, NV, 0>(p, st);
 }
 
 struct BackParams {

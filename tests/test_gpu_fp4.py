@@ -106,7 +106,8 @@ def randn(shape, seed, dtype=torch.bfloat16, loud=True):
 
 @pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 22), (5, 32), (130, 33), (129, 100), (40, 128), (33, 250), (2, 256), (70, 500),
-                                 (333, 1040), (9, 2080), (3, 4096), (2, 8190), (2, 16384), (3, 16400), (1, 40001), (1000, 64)])
+                                 (333, 1040), (9, 2080), (3, 4096), (2, 8190), (2, 16384), (3, 16400), (1, 40001), (1000, 64), (5, 1500), (6, 2040),
+                                 (3, 6001), (2, 12000)])
 def test_quantize_equals_its_definition(hn, cuda, kind, m, k):
     for dtype in DTYPES:
         x = randn((m, k), m * 7 + k, dtype)
@@ -141,7 +142,8 @@ def test_quantize_special_numbers(hn, cuda, kind):
 def test_quantize_views(hn, cuda, kind):
     """Rows at odd offsets and strides, columns that are not contiguous, an expanded row."""
     base = randn((40, 1000), 1)
-    for x in (base[:, 3:500], base[1::3, 8:648], base.t()[:100], base[:1].expand(5, 1000), base[:, :77].float().half()):
+    for x in (base[:, 3:500], base[1::3, 8:648], base.t()[:100], base[:1].expand(5, 1000), base[:, :77].float().half(),
+              base[:, 2:502], base[:, 2:99].float(), base[:, 998:]):
         check_quantized(hn, x, kind, hn.kernels.quantize_fp4(x, kind))
 
 
