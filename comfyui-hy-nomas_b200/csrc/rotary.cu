@@ -5,16 +5,19 @@
 // in fp32 from the loads to the one rounding. The first `rot` columns of a head are rotated, the others pass.
 //
 // Bound by HBM: each head read once and written once. A warp takes one token and several of its heads: cos and sin of the
-// token's pairs are computed once, by all lanes, and shared through shared memory; P lanes hold a head, eight columns each. In
-// the half layout a column's partner stands in another lane: it is loaded again (from L1), which costs less than an exchange
-// that the part-rotated heads, whose halves begin inside a lane, would need in several forms.
+// token's pairs are computed once, by all lanes, and shared through shared memory; the next heads are on their way while these
+// are turned. Heads and rotated parts of a multiple of 16: sixteen columns a lane, chosen so that whole pairs are a lane's own,
+// on packed arithmetic (20240 tokens x 32 heads of 128, bf16, with the norm: 58 us, 5.7 TB/s; one token: 2.5 us). Others: eight
+// columns a lane, and in the half layout, whose partner stands in another lane, possibly from the middle of its columns on, the
+// partners are loaded again, from L1 (128 with 120 rotated: 80 us).
 #include "hn_kernels.h"
 #include "rotary.cuh"
 
 namespace hn {
 namespace rotary {
 
-constexpr int WARPS = 8, CTAS = 2;
+constexpr int WARPS = 4, CTAS = 4;           // of a block; blocks an SM
+constexpr int AWARPS = 8, ACTAS = 2;         // the append's
 
 struct Params {
     const void *x;
@@ -30,7 +33,8 @@ struct Params {
     int B, L, H, D, per, groups;        // per: heads of a unit, a multiple of 32 / P; groups: units of a token
 };
 
-template <typename E, int P> __global__ void __launch_bounds__(32 * WARPS) k_rotate(Params p) {
+// Any head and rotated part: eight columns a lane
+template <typename E, int P, bool INTER, bool NORM> __global__ void __launch_bounds__(32 * WARPS, CTAS) k_rotate8(Params p) {
     __shared__ float tables[WARPS][2 * MAX_PAIRS];
     constexpr int HEADS = 32 / P, U = 2;
     const int lane = threadIdx.x & 31, sub = lane % P;
@@ -39,7 +43,8 @@ template <typename E, int P> __global__ void __launch_bounds__(32 * WARPS) k_rot
     Turn t;
     partners(p.r, sub, t);
     Weights w;
-    if (p.w != nullptr && in) load_weights(p.w + 8 * sub, t, w);
+    if (NORM && in) load_weights(p.w + 8 * sub, t, w);
+    const float rd = 1.0f / p.D;
     const int64_t units = (int64_t)p.B * p.L * p.groups, step = (int64_t)gridDim.x * WARPS;
     for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
         const int64_t token = div_nonneg(u, p.groups);
@@ -47,35 +52,57 @@ template <typename E, int P> __global__ void __launch_bounds__(32 * WARPS) k_rot
         const int64_t b = div_nonneg(token, p.L), l = token - b * p.L;
         const E *x = static_cast<const E *>(p.x) + b * p.x_bs + l * p.x_ls + 8 * sub;
         E *out = static_cast<E *>(p.out) + b * p.o_bs + l * p.o_ls + 8 * sub;
+        Raw8<E> raw[U];
+        Raw4<E> far[U][2];                      // the partners of the lane's two runs of four (half layout)
+        auto fetch = [&](int h0) {
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int h = h0 + i * HEADS;
+                raw[i].clear();
+                if (in && h < last) {
+                    const E *head = x + h * p.x_hs;
+                    raw[i].load(head);
+                    if (!INTER)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            if (t.off[j] != 0) far[i][j].load(head + 4 * j + t.off[j]);
+                }
+            }
+        };
+        fetch(first + lane / P);                // before the table: the loads do not depend on it
         const int64_t at = b * p.p_bs + l * p.p_ls;
         turn_table(p.r, p.wide ? static_cast<const int64_t *>(p.pos)[at] : static_cast<const int32_t *>(p.pos)[at], table, lane);
         turn_of(p.r, sub, table, t);
         for (int h0 = first + lane / P; h0 - lane / P < last; h0 += U * HEADS) {
-            float v[U][8], o[U][8];
+            Raw8<E> now[U];
+            Raw4<E> other[U][2];
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                const int h = h0 + i * HEADS;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-                if (in && h < last) {
-                    load8(x + h * p.x_hs, v[i]);
-                    load_partners(x + h * p.x_hs, t, o[i]);
-                }
+                now[i] = raw[i];
+                if (!INTER) { other[i][0] = far[i][0]; other[i][1] = far[i][1]; }
             }
-            __syncwarp();               // out may be x: the partners are read before they are written
+            // the next heads' loads; out may be x, whose heads are each read, partners and all, before they are written
+            if (h0 - lane / P + U * HEADS < last) fetch(h0 + U * HEADS);
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 const int h = h0 + i * HEADS;
-                if (p.w != nullptr) head_norm<P>(v[i], o[i], w, t, p.D, p.eps);
-                turn(t, v[i], o[i]);
-                if (in && h < last) store8(out + h * p.o_hs, v[i]);
+                float v[8], o[8];
+                now[i].widen(v);
+                if (!INTER)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (t.off[j] != 0) other[i][j].widen(o + 4 * j);
+                if (NORM) head_norm<P>(v, o, w, t, rd, p.eps);
+                turn<INTER>(t, v, o);
+                if (in && h < last) store8(out + h * p.o_hs, v);
             }
         }
     }
 }
 
 // heads and rotated parts of a multiple of 16: sixteen columns a lane
-template <typename E, int P, bool INTER, bool NORM> __global__ void __launch_bounds__(32 * WARPS, 2) k_rotate16(Params p) {
+template <typename E, int P, bool INTER, bool NORM> __global__ void __launch_bounds__(32 * WARPS, CTAS) k_rotate16(Params p) {
     __shared__ __align__(16) float tables[WARPS][2 * MAX_PAIRS];
     constexpr int HEADS = 32 / P, U = 2;
     const int lane = threadIdx.x & 31, sub = lane % P;
@@ -135,12 +162,16 @@ static unsigned plan(Params &p, int heads) {
     if (each > passes) each = passes;
     p.per = (int)(each * heads);
     p.groups = (int)cdiv(p.H, p.per);
-    const int64_t grid = cdiv(tokens * p.groups, WARPS), most = (int64_t)num_sms() * 2;
+    const int64_t grid = cdiv(tokens * p.groups, WARPS), most = (int64_t)num_sms() * CTAS;
     return (unsigned)(grid < most ? grid : most);
 }
 template <typename E, int P> cudaError_t go(Params p, cudaStream_t st) {
     const unsigned grid = plan(p, 32 / P);
-    k_rotate<E, P><<<grid, 32 * WARPS, 0, st>>>(p);
+    const bool inter = p.r.layout == INTERLEAVED;
+    if (inter && p.w) k_rotate8<E, P, true, true><<<grid, 32 * WARPS, 0, st>>>(p);
+    else if (inter) k_rotate8<E, P, true, false><<<grid, 32 * WARPS, 0, st>>>(p);
+    else if (p.w) k_rotate8<E, P, false, true><<<grid, 32 * WARPS, 0, st>>>(p);
+    else k_rotate8<E, P, false, false><<<grid, 32 * WARPS, 0, st>>>(p);
     return cudaGetLastError();
 }
 template <typename E, int P> cudaError_t go16(Params p, cudaStream_t st) {
@@ -189,15 +220,15 @@ struct AppendParams {
 // The rules of the plain append: a row whose last extend was refused, a page that several rows name, a row's listings after the
 // first keep what they hold, counted. q is rotated whatever becomes of the row. A unit is a warp's share of a token: some of
 // its q, k and v heads, in that order, two at a time (16 lanes each).
-template <bool I8> __global__ void __launch_bounds__(32 * WARPS) k_append_rotated(AppendParams p, Meta m) {
-    __shared__ float tables[WARPS][2 * MAX_PAIRS];
+template <bool I8> __global__ void __launch_bounds__(32 * AWARPS) k_append_rotated(AppendParams p, Meta m) {
+    __shared__ float tables[AWARPS][2 * MAX_PAIRS];
     const int lane = threadIdx.x & 31, sub = lane & 15, side = lane >> 4;
     float *table = tables[threadIdx.x >> 5];
     Turn t;
     partners(p.r, sub, t);
     const int all = p.H + 2 * p.heads;
-    const int64_t units = (int64_t)p.B * p.n * p.groups, step = (int64_t)gridDim.x * WARPS;
-    for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
+    const int64_t units = (int64_t)p.B * p.n * p.groups, step = (int64_t)gridDim.x * AWARPS;
+    for (int64_t u = (int64_t)blockIdx.x * AWARPS + (threadIdx.x >> 5); u < units; u += step) {
         const int64_t bt = div_nonneg(u, p.groups);
         const int first = (int)(u - bt * p.groups) * p.per, last = first + p.per < all ? first + p.per : all;
         const int b = (int)div_nonneg(bt, p.n), i = (int)(bt - (int64_t)b * p.n);
@@ -243,12 +274,15 @@ template <bool I8> __global__ void __launch_bounds__(32 * WARPS) k_append_rotate
                 for (int j = 0; j < 8; ++j) { n[j] = v[j]; no[j] = o[j]; }
                 Weights ww;
                 if (w != nullptr) load_weights(w + 8 * sub, t, ww);
-                head_norm<16>(n, no, ww, t, 128, p.eps);
+                head_norm<16>(n, no, ww, t, 1.0f / 128, p.eps);
                 if (w != nullptr)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) { v[j] = n[j]; o[j] = no[j]; }
             }
-            if (which < 2) turn(t, v, o);
+            if (which < 2) {
+                if (t.own) turn<true>(t, v, o);
+                else turn<false>(t, v, o);
+            }
             const int64_t to = ((int64_t)page * p.heads + head) * m.page + place;
             if (which == 0) {
                 if (in) store8(p.out + (bt * p.H + head) * 128 + 8 * sub, v);
@@ -273,7 +307,9 @@ template <bool I8> __global__ void __launch_bounds__(32 * WARPS) k_append_rotate
 }
 
 // ... with rotated parts of a multiple of 16: sixteen columns a lane, four heads of one kind (q, k or v) a pass. Bound by
-// instructions, not by HBM: the quantizer's above all, so each kind has a loop of its own, whose addresses only step on.
+// instructions, not by HBM, the int8 quantizer's above all (half of its cycles issue one), so each kind has a loop of its own,
+// whose addresses only step on. 2 x 4400 tokens, 16 + 16 + 16 heads, int8: 53 us of 28 for the bytes (61 with one loop that asks
+// for the kind); loads further ahead, through shared memory, and more warps of fewer registers changed nothing or cost more.
 // A row of K or V (16 columns of it in this lane) as codes and scale
 __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16 &l, const float (&a)[8], const float (&b)[8], bool in, bool lead) {
     float peak = nanmax_abs3(0.0f, a[0], a[1]);
@@ -293,14 +329,14 @@ __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16
     if (lead) *scale = sc;
 }
 
-template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * WARPS, CTAS) k_append_rotated16(AppendParams p, Meta m) {
-    __shared__ __align__(16) float tables[WARPS][2 * MAX_PAIRS];
+template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * AWARPS, ACTAS) k_append_rotated16(AppendParams p, Meta m) {
+    __shared__ __align__(16) float tables[AWARPS][2 * MAX_PAIRS];
     const int lane = threadIdx.x & 31, sub = lane & 7, side = lane >> 3;
     float *table = tables[threadIdx.x >> 5];
     const Lane16 at16 = lane16<INTER>(p.r, sub);
     const int nq = (p.H + 3) >> 2, nk = (p.heads + 3) >> 2, all = nq + 2 * nk;         // passes
-    const int64_t units = (int64_t)p.B * p.n * p.groups, step = (int64_t)gridDim.x * WARPS;
-    for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
+    const int64_t units = (int64_t)p.B * p.n * p.groups, step = (int64_t)gridDim.x * AWARPS;
+    for (int64_t u = (int64_t)blockIdx.x * AWARPS + (threadIdx.x >> 5); u < units; u += step) {
         const int64_t bt = div_nonneg(u, p.groups);
         const int first = (int)(u - bt * p.groups) * p.per, last = first + p.per < all ? first + p.per : all;
         const int b = (int)div_nonneg(bt, p.n), i = (int)(bt - (int64_t)b * p.n);
@@ -446,8 +482,8 @@ cudaError_t launch_append_rotated(const CacheArgs &c, int layer, const AppendRot
     if (each > passes) each = passes;
     p.groups = (int)cdiv(passes, each);
     p.per = (int)(wide ? each : 2 * each);
-    const int64_t grid = cdiv(count * p.groups, rotary::WARPS), most = (int64_t)num_sms() * rotary::CTAS;
-    const unsigned g = (unsigned)(grid < most ? grid : most), threads = 32 * rotary::WARPS;
+    const int64_t grid = cdiv(count * p.groups, rotary::AWARPS), most = (int64_t)num_sms() * rotary::ACTAS;
+    const unsigned g = (unsigned)(grid < most ? grid : most), threads = 32 * rotary::AWARPS;
     if (wide && a.layout == rotary::INTERLEAVED) {
         if (c.ks) rotary::k_append_rotated16<true, true><<<g, threads, 0, st>>>(p, c.meta);
         else rotary::k_append_rotated16<false, true><<<g, threads, 0, st>>>(p, c.meta);

@@ -65,21 +65,22 @@ __device__ __forceinline__ void turn_of(const Rotation &r, int sub, const float 
     }
 }
 // v: the lane's columns, o: their partners (half layout)
-__device__ __forceinline__ void turn(const Turn &t, float (&v)[8], const float (&o)[8]) {
-    if (t.own) {
+template <bool INTER> __device__ __forceinline__ void turn(const Turn &t, float (&v)[8], const float (&o)[8]) {
+    if constexpr (INTER) {
+        if (!t.own) return;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float a = v[2 * i], b = v[2 * i + 1];
             v[2 * i] = a * t.c[i] - b * t.s[i];
             v[2 * i + 1] = b * t.c[i] + a * t.s[i];
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        if (t.off[j] == 0) continue;
+        for (int j = 0; j < 2; ++j) {
+            if (t.off[j] == 0) continue;
 #pragma unroll
-        for (int i = 4 * j; i < 4 * j + 4; ++i) v[i] = v[i] * t.c[i] + o[i] * t.s[i];
+            for (int i = 4 * j; i < 4 * j + 4; ++i) v[i] = v[i] * t.c[i] + o[i] * t.s[i];
+        }
     }
 }
 
@@ -125,15 +126,15 @@ __device__ __forceinline__ void load_weights(const __nv_bfloat16 *w, const Turn 
     load8(w, out.own);
     load_partners(w, t, out.other);
 }
-// x / sqrt(mean x^2 + eps) * w over the P lanes of a head of D columns (v is 0 in lanes behind it)
+// x / sqrt(mean x^2 + eps) * w over the P lanes of a head (v is 0 in lanes behind it); rd = 1 / D
 template <int P>
-__device__ __forceinline__ void head_norm(float (&v)[8], float (&o)[8], const Weights &w, const Turn &t, int D, float eps) {
+__device__ __forceinline__ void head_norm(float (&v)[8], float (&o)[8], const Weights &w, const Turn &t, float rd, float eps) {
     float ss = v[0] * v[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
     for (int i = 1; i < P; i <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, i);
-    const float inv = rsqrt_cr(__fadd_rn(__fdiv_rn(ss, (float)D), eps));
+    const float inv = rsqrtf(fmaf(ss, rd, eps));
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w.own[i];
 #pragma unroll
@@ -256,6 +257,28 @@ template <> struct Raw8<float> {
     __device__ __forceinline__ void widen(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
+};
+// four columns as loaded
+template <typename E> struct Raw4 {
+    uint2 w;
+    __device__ __forceinline__ void load(const E *p) { w = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void widen(float *v) const;
+};
+template <> __device__ __forceinline__ void Raw4<__nv_bfloat16>::widen(float *v) const {
+    v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
+}
+template <> __device__ __forceinline__ void Raw4<__half>::widen(float *v) const {
+    const uint32_t x[2] = {w.x, w.y};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+template <> struct Raw4<float> {
+    float4 w;
+    __device__ __forceinline__ void load(const float *p) { w = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void widen(float *v) const { v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w; }
 };
 template <bool INTER, typename E> __device__ __forceinline__ void widen16(const Raw8<E> (&raw)[2], Cols &c) {
     float v[8];
