@@ -4,7 +4,9 @@
 // quarter of a scale tile's 128 (their scales are 32 neighbouring bytes), its warps the chunks of 1024 columns in turn, so a
 // lane has 16 bytes of every row in flight. Codes become fp16 pairs, exactly; the products of a block of 16 are
 // summed in fp16 pairs of eight products each, whose sum is exact too (at most 288 in steps of 0.25: 1152 of 2048), and leave
-// as fp32, times both scales. The order of the sums is fixed.
+// as fp32, times both scales. The order of the sums is fixed. Measured: one row over 4096 x 16384 NV: 9.7 us with its launch
+// (3.9 TB/s), two rows 14.2 (the tile kernel, three rows and more: 15). Four rows in flight and 64 registers, so that all CTAs of
+// that case are resident: 10.8 -> 9.7.
 #include "fp4.cuh"
 #include "hn_kernels.h"
 

@@ -9,7 +9,9 @@
 // Bound by HBM: 2 B read (bf16) and 0.5 B + 1/16 B written per element. NV needs the row's top before its first code, so T
 // threads hold a row in registers as it was loaded, NCH chunks of 16 columns each (chunk i T + t), and x is read once; rows of more
 // than 16384 columns are read twice. A chunk is a block of NV and half a block of MX; the lanes of a scale tile's word (4 or
-// 8) gather its bytes before the one store.
+// 8) gather its bytes before the one store. Measured, 20240 x 4096 bf16: MX 32 us (6.5 TB/s), NV 41 us (5.2 TB/s: its twelve
+// instructions a column, four of them the exact quotient, are what is left; a persistent loop over rows with the next one's loads
+// ahead did not help). Back to bf16: 44 us (4.8 TB/s, 16 bytes out a thread). One row of 4096: 2.6 us, a launch.
 #include "fp4.cuh"
 #include "hn_kernels.h"
 
