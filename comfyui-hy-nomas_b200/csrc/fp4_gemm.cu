@@ -303,23 +303,25 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
 //   warp 3          (first CTA) the MMAs. It meets warps 4 to 7 at named barriers: its own look at a barrier in shared memory would
 //                   wait until its MMAs have read their operands. Its four MMAs a step have no branch between them
 //   warps 8 to 15   the sums: a thread holds 128 columns of a row in registers, hands tensor memory back, and only then scales,
-//                   rounds and writes, beside the next tile's MMAs; 64 bytes of a row at a time go through shared memory, so that a
+//                   rounds and writes, beside the next tile's MMAs; 32 bytes of a row at a time go through shared memory, so that a
 //                   row's outputs leave as whole sectors
-// Bound by the tensor cores and what keeps them waiting. A step's MMAs are 512 clocks. Measured, 18944 x 4096 x 16384 NV (16 tiles
-// a pair, 1024 steps): 495 us. Timed apart, in ns a step: MMAs alone 332, with their commits 362, with the barriers 399, with the
-// loads 418, with the scales' copies 483; a tile's end costs 2 us (the wake of the epilogue, tensor memory's read, the issuer's
-// wake). Tried and slower (20240 x 4096 x 16384 NV, us): scale copies by the MMAs' thread 877, by one other warp 699, by two 593;
-// a branch for the last columns between the MMAs 600 (without: 552); scales written to tensor memory from registers 1676.
+// Bound by the tensor cores and what keeps them waiting. A step's MMAs are 512 clocks. Measured, 18944 x 4096 x 16384 (16 tiles a
+// pair, 1024 steps): NV 491 us (5.2 PFLOP/s), MX 453; under the power limit of a long run 7 - 8 of 10 of that. Timed apart with
+// an earlier build of 504 us, in ns a step: MMAs alone 332, with their commits 362, with the barriers 399, with the loads 418, with
+// the scales' copies 492; a tile's end costs 2 us (the wake of the epilogue, tensor memory's read, the issuer's wake). How far the
+// scales' loads run ahead counts: 4 slots 536 us, 8 slots 491. Tried and slower (20240 x 4096 x 16384 NV, us): scale copies by the
+// MMAs' thread 877, by one other warp 699, by two 593; a branch for the last columns between the MMAs 600 (without: 552); scales
+// written to tensor memory from registers 1676; codes released every other step 8% more.
 template <int KIND> struct Wide {
     static constexpr int BM = 256, BN = 256;
     static constexpr int TILES = KB / SPAN<KIND>;
     static constexpr int OP = 128 * 128, SFA = TILES * TILE, SFB = 2 * TILES * TILE;
     static constexpr int STAGES = 5, STAGE = 2 * OP;            // codes of both operands
     static constexpr int CP = 4;                                // warps that copy scales
-    static constexpr int SLOTS = CP, SLOT = SFA + SFB;          // scales on their way to tensor memory
+    static constexpr int SLOTS = 2 * CP, SLOT = SFA + SFB;      // scales on their way to tensor memory
     static constexpr int ACC = 0, SFC = BN, SFW = 12 * TILES;   // tensor memory columns; SFW: a stage's scales
     static_assert(SFC + STAGES * SFW <= 512, "tensor memory");
-    static constexpr int EPI = 8, PITCH = 80;                   // warps; bytes a row of their chunks of 64
+    static constexpr int EPI = 8, PITCH = 48;                   // warps; bytes a row of their chunks of 32
     static constexpr int OFF_SF = STAGES * STAGE, OFF_EPI = OFF_SF + SLOTS * SLOT;
     static constexpr int OFF_COLS = OFF_EPI + EPI * 32 * PITCH;                             // column scales and bias: [2][2][256]
     static constexpr int OFF_BAR = OFF_COLS + 2 * 2 * 256 * 4;
@@ -525,14 +527,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         // step i, every C::CP-th: its scales into the columns of its stage, when the MMAs that read them last are done; then, when they
         // and the codes are in, the issuer's release. After a wait that gave up the steps that are left are only met, so that
         // the issuer comes to its end.
-        // A parity tells a phase from its neighbours only, and these warps skip steps. So each has a slot of its own, whose phases it
-        // sees one after the other; that MMAs of step i - 2 STAGES are over, when those of i - STAGES are waited for, follows from
+        // A parity tells a phase from its neighbours only, and these warps skip steps. So each has two slots of its own, whose phases
+        // it sees one after the other; that MMAs of step i - 2 STAGES are over, when those of i - STAGES are waited for, follows from
         // step i - CP, whose codes the warp has seen in (they came after the MMAs of step i - CP - STAGES); and that the full
         // barrier's phase before is over follows from the MMAs of step i - STAGES.
-        static_assert(C::SLOTS == C::CP && C::CP <= C::STAGES, "phases that a warp may find");
-        const int slot = warp - 4;
-        int stage = slot % C::STAGES, last = -1;
-        uint32_t phase = slot / C::STAGES & 1, sphase = 0, last_phase = 0;
+        static_assert(C::SLOTS == 2 * C::CP && C::CP <= C::STAGES, "phases that a warp may find");
+        int stage = warp - 4, slot = warp - 4, last = -1;
+        uint32_t phase = 0, sphase = 0, last_phase = 0;
         bool ok = true;
         for (int i = warp - 4; i < steps; i += C::CP) {
             ok = ok && spin_wait(lane, bar_sfull + 8 * slot, sphase, abort_flag, p.err);
@@ -558,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
             if (ok) asm volatile("barrier.cta.arrive %0, 64;" ::"r"(2 + stage) : "memory");
             else asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + stage) : "memory");
             if ((stage += C::CP) >= C::STAGES) { stage -= C::STAGES; phase ^= 1; }
-            sphase ^= 1;
+            if ((slot += C::CP) >= C::SLOTS) { slot -= C::SLOTS; sphase ^= 1; }
         }
         if (last >= 0 && lane == 0) {
             volatile int never = 0;
@@ -634,10 +635,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
             __syncwarp();
             if (lane == 0) arrive_at(tempty);
             const float *rb = cols + 128 * half, *bias = rb + 256;
-            constexpr int COLS = 64 / EB;               // of a chunk: 64 bytes a row
+            constexpr int COLS = 32 / EB;               // of a chunk: 32 bytes a row
 #pragma unroll
             for (int c = 0; c < 128 / COLS; ++c) {
-                uint32_t w[16];
+                uint32_t w[8];
 #pragma unroll
                 for (int j = 0; j < COLS; j += 4) {
                     const float4 s = *reinterpret_cast<const float4 *>(rb + COLS * c + j), b = *reinterpret_cast<const float4 *>(bias + COLS * c + j);
@@ -661,20 +662,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
                 }
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 2; ++j)
                     *reinterpret_cast<uint4 *>(chunk + lane * C::PITCH + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 __syncwarp();
                 const int nc = n0 + COLS * c;
                 uint8_t *out = static_cast<uint8_t *>(p.o.out) + ((int64_t)m0 * p.o.ldo + nc) * EB;
                 if (p.vec) {
-                    const bool in = nc + 16 / EB * (lane & 3) < p.N;
-                    uint4 y[4];
+                    const bool in = nc + 16 / EB * (lane & 1) < p.N;
+                    uint4 y[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint4 *>(chunk + (8 * i + (lane >> 2)) * C::PITCH + 16 * (lane & 3));
+                    for (int i = 0; i < 2; ++i) y[i] = *reinterpret_cast<const uint4 *>(chunk + (16 * i + (lane >> 1)) * C::PITCH + 16 * (lane & 1));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = 8 * i + (lane >> 2);
-                        if (in && m0 + row < p.M) *reinterpret_cast<uint4 *>(out + (int64_t)row * p.o.ldo * EB + 16 * (lane & 3)) = y[i];
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 16 * i + (lane >> 1);
+                        if (in && m0 + row < p.M) *reinterpret_cast<uint4 *>(out + (int64_t)row * p.o.ldo * EB + 16 * (lane & 1)) = y[i];
                     }
                 } else {
 #pragma unroll 8
