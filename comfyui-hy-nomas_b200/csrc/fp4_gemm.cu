@@ -491,16 +491,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         uint32_t phase = 0;
         Step s = first_step(p.raster, pair);
         bool ok = true;
-        for (int i = 0; i < steps; ++i) {
+        for (int i = 0; i < steps + C::STAGES; ++i) {       // the last only wait: this CTA stays until their arrivals have reached it
             ok = spin_wait(lane, bar_empty + 8 * stage, phase ^ 1, abort_flag, p.err);
             if (!ok) break;
-            if (lane == 0) {
+            if (lane == 0 && i < steps) {
                 const uint32_t at = sbase + stage * C::STAGE + warp * C::OP, fb = in_cta(bar_full + 8 * stage, 0);
                 if (rank == 0) mbar_arrive_tx(bar_full + 8 * stage, 2 * C::OP);
                 pair_load_2d(warp == 0 ? &tmA : &tmB, at, fb, s.kt * 128, (warp == 0 ? s.mt : s.nt) * 256 + rank * 128);
             }
             __syncwarp();
-            next_step(p.raster, s, kts, pairs);
+            if (i < steps) next_step(p.raster, s, kts, pairs);
             if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) land();
@@ -509,17 +509,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         uint32_t phase = 0;
         Step s = first_step(p.raster, pair);
         bool ok = true;
-        for (int i = 0; i < steps; ++i) {
+        for (int i = 0; i < steps + C::SLOTS; ++i) {
             ok = spin_wait(lane, bar_sempty + 8 * slot, phase ^ 1, abort_flag, p.err);
             if (!ok) break;
-            if (lane == 0) {
+            if (lane == 0 && i < steps) {
                 const uint32_t at = sbase + C::OFF_SF + slot * C::SLOT, fb = in_cta(bar_sfull + 8 * slot, 0);
                 if (rank == 0) mbar_arrive_tx(bar_sfull + 8 * slot, 2 * C::SLOT);
                 pair_load_3d(&tmSA, at, fb, s.kt * C::TILES, 2 * s.mt + rank);
                 pair_load_3d(&tmSB, at + C::SFA, fb, s.kt * C::TILES, 2 * s.nt);
             }
             __syncwarp();
-            next_step(p.raster, s, kts, pairs);
+            if (i < steps) next_step(p.raster, s, kts, pairs);
             if (++slot == C::SLOTS) { slot = 0; phase ^= 1; }
         }
         if (!ok) land();
