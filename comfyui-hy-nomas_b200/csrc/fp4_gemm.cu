@@ -304,9 +304,10 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
 //                   wait until its MMAs have read their operands. Its four MMAs a step have no branch between them
 //   warps 8 to 15   the sums: a thread holds 128 columns of a row in registers, hands tensor memory back, and only then scales,
 //                   rounds and writes, beside the next tile's MMAs; 32 bytes of a row at a time go through shared memory, so that a
-//                   row's outputs leave as whole sectors
+//                   row's outputs leave as whole sectors, 16 bytes a store or as many as N and the rows' starts allow
+//                   (18944 rows, K = 4096: N = 4096 158 us, 4100 168, 4094 161, 4095 176; all but the first 217 - 229 one by one)
 // Bound by the tensor cores and what keeps them waiting. A step's MMAs are 512 clocks. Measured, 18944 x 4096 x 16384 (16 tiles a
-// pair, 1024 steps): NV 491 us (5.2 PFLOP/s), MX 453; under the power limit of a long run 7 - 8 of 10 of that. Timed apart with
+// pair, 1024 steps): NV 491 - 512 us from GPU to GPU (5.0 - 5.2 PFLOP/s), MX 453 - 465; under the power limit of a long run 7 - 8 of 10 of that. Timed apart with
 // an earlier build of 504 us, in ns a step: MMAs alone 332, with their commits 362, with the barriers 399, with the loads 418, with
 // the scales' copies 492; a tile's end costs 2 us (the wake of the epilogue, tensor memory's read, the issuer's wake). How far the
 // scales' loads run ahead counts: 4 slots 536 us, 8 slots 491. Tried and slower (20240 x 4096 x 16384 NV, us): scale copies by the
@@ -436,7 +437,7 @@ __device__ __forceinline__ void next_step(const Raster &r, Step &s, int kts, int
 
 struct WideParams {
     Result o;
-    int vec;
+    int unit;                   // bytes that are stored at a time: 16, 8, 4 or 2
     int M, N, Kp, tiles;
     Raster raster;
     int *err;
@@ -667,25 +668,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
                 __syncwarp();
                 const int nc = n0 + COLS * c;
                 uint8_t *out = static_cast<uint8_t *>(p.o.out) + ((int64_t)m0 * p.o.ldo + nc) * EB;
-                if (p.vec) {
-                    const bool in = nc + 16 / EB * (lane & 1) < p.N;
-                    uint4 y[2];
+                auto store = [&](auto zero) {           // units of U bytes: 32 / U lanes a row, U rows at a time
+                    using T = decltype(zero);
+                    constexpr int U = sizeof(T), G = U < 8 ? 8 : 32 / U;
+                    const int at = U * (lane % (32 / U)), row0 = lane / (32 / U);
+                    const bool in = nc + at / EB < p.N;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) y[i] = *reinterpret_cast<const uint4 *>(chunk + (16 * i + (lane >> 1)) * C::PITCH + 16 * (lane & 1));
+                    for (int g = 0; g < 32 / U; g += G) {
+                        T y[G];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = 16 * i + (lane >> 1);
-                        if (in && m0 + row < p.M) *reinterpret_cast<uint4 *>(out + (int64_t)row * p.o.ldo * EB + 16 * (lane & 1)) = y[i];
+                        for (int i = 0; i < G; ++i) y[i] = *reinterpret_cast<const T *>(chunk + (U * (g + i) + row0) * C::PITCH + at);
+#pragma unroll
+                        for (int i = 0; i < G; ++i) {
+                            const int row = U * (g + i) + row0;
+                            if (in && m0 + row < p.M) *reinterpret_cast<T *>(out + (int64_t)row * p.o.ldo * EB + at) = y[i];
+                        }
                     }
-                } else {
-#pragma unroll 8
-                    for (int i = 0; i < COLS; ++i) {
-                        const int row = (32 * i + lane) / COLS, col = (32 * i + lane) % COLS;
-                        if (nc + col >= p.N || m0 + row >= p.M) continue;
-                        if (EB == 2) *reinterpret_cast<uint16_t *>(out + ((int64_t)row * p.o.ldo + col) * 2) = *reinterpret_cast<uint16_t *>(chunk + row * C::PITCH + 2 * col);
-                        else *reinterpret_cast<uint32_t *>(out + ((int64_t)row * p.o.ldo + col) * 4) = *reinterpret_cast<uint32_t *>(chunk + row * C::PITCH + 4 * col);
-                    }
-                }
+                };
+                if (p.unit == 16) store(uint4());
+                else if (p.unit == 8) store(uint2());
+                else if (EB == 4 || p.unit == 4) store(uint32_t());
+                else store(uint16_t());
             }
         }
         if (!ok) *abort_flag = 1;
@@ -739,6 +742,11 @@ static int whole_stores(const Fp4GemmArgs &a, int bytes) {
     const int size = a.out_dtype == 2 ? 4 : 2;
     return a.N * size % bytes == 0 && a.ldo * size % bytes == 0 && reinterpret_cast<uintptr_t>(a.out) % bytes == 0;
 }
+static int store_unit(const Fp4GemmArgs &a) {
+    int bytes = 16;
+    while (!whole_stores(a, bytes)) bytes /= 2;
+    return bytes;
+}
 template <int KIND, typename C> static bool maps(const Fp4GemmArgs &a, int b_blocks, CUtensorMap (&m)[4]) {
     const uint64_t sp = (uint64_t)cdiv(a.K, SPAN<KIND>);
     return map_codes(&m[0], a.qa, a.M, a.K / 2, a.lda, 128) && map_codes(&m[1], a.qw, a.N, a.K / 2, a.ldw, 128) &&
@@ -764,7 +772,7 @@ template <int KIND> static cudaError_t launch_wide(const Fp4GemmArgs &a, cudaStr
     if (e != cudaSuccess) return e;
     p.o = {a.ra, a.rw, a.bias, a.bias_dtype, a.out, a.ldo, a.out_dtype};
     p.M = (int)a.M; p.N = (int)a.N; p.Kp = (int)a.K;
-    p.vec = whole_stores(a, 16);
+    p.unit = store_unit(a);
     p.raster.m_tiles = (int)cdiv(a.M, C::BM);
     p.raster.n_tiles = (int)cdiv(a.N, C::BN);
     p.tiles = p.raster.m_tiles * p.raster.n_tiles;
@@ -824,8 +832,12 @@ template <int KIND> static cudaError_t launch(const Fp4GemmArgs &a, cudaStream_t
     const int sms = num_sms();
     const int64_t tiles = cdiv(a.M, 128) * cdiv(a.N, 128), kts = cdiv(a.K, KB);
     // Tiles of 128 x 128 while all of them run at once, two CTAs an SM; pairs of CTAs beyond. Measured (us, 128 x 128 / pairs):
-    // 777 x 5000 x 2080 (280 tiles) 16.3 / 18.6; 1024 x 5120 x 4096 (320) 33.8 / 25.2; 2560 x 2048 x 1024 (320) 16.8 / 14.8
-    if (tiles > 2 * sms) return launch_wide<KIND>(a, st, msg);
+    // 777 x 5000 x 2080 (280 tiles) 16.3 / 18.6; 1024 x 5120 x 4096 (320) 33.8 / 25.2; 2560 x 2048 x 1024 (320) 16.8 / 14.8.
+    // Also pairs where SMs would get two tiles and the pairs one, in eight steps or more: 2048 x 2048 x 1024 11.6 / 11.9,
+    // x 2048 14.1 / 13.4, x 16384 50.5 / 37.3; 300 x 8192 x 4096 18.9 / 16.8; but 1024 x 2048 x 16384 (128 tiles) 29.1 / 34.7. Where
+    // outputs have to leave one by one, from 32 steps on: the pairs' epilogue is 4 us more then (2048 x 2041 x 2048 14.1 / 17.6)
+    const bool one_round = tiles > sms && cdiv(a.M, 256) * cdiv(a.N, 256) <= sms / 2 && kts >= (store_unit(a) > 2 ? 8 : 32);
+    if (tiles > 2 * sms || one_round) return launch_wide<KIND>(a, st, msg);
     // K is split over a cluster while SMs are idle and each part keeps two stages; over a second CTA on each SM only where a part
     // keeps eight. Measured (us, 1 / 2 / 4 / 8 parts): 48 x 8192 x 4096 MX 13.1 / 9.9 / 11.6 / -; 128 x 4096 x 4096 NV 16.4 / 11.5 /
     // 10.1 / 16.5; 16 x 4096 x 16384 NV 43 / 25 / 17 / 15

@@ -232,6 +232,21 @@ def test_product_many_rows(hn, cuda, kind, m, n, k):
 
 
 @pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("n", [2064, 2068, 2066, 2065])
+@pytest.mark.parametrize("m,k", [(1793, 2080), (2600, 96)])
+def test_product_rows_of_any_alignment(hn, cuda, kind, n, m, k):
+    """Pairs of CTAs, a tile each and several: outputs stored 16, 8, 4 and 2 bytes at a time."""
+    a, w = operands(hn, m, n, k, kind, 14)
+    for dtype in DTYPES:
+        for pad in (0, 16):
+            base = torch.full((m, n + pad), 7.0, dtype=dtype, device="cuda")
+            out = base[:, :n]
+            hn.kernels.fp4_gemm(*a, *w, None, dtype, kind, out)
+            check_product(hn, out, a, w, kind)
+            assert bool((base[:, n:] == 7).all())
+
+
+@pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("m,n,k", [(1, 40, 96), (2, 300, 2080), (20, 300, 512), (130, 200, 4096), (2500, 2400, 128)])
 def test_product_nan_stays_in_its_row_and_column(hn, cuda, kind, m, n, k):
     """A NaN or an infinity in a row of either operand: its outputs are NaN, all others as without it."""
