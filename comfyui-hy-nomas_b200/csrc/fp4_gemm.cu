@@ -306,13 +306,14 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
 //                   rounds and writes, beside the next tile's MMAs; 32 bytes of a row at a time go through shared memory, so that a
 //                   row's outputs leave as whole sectors, 16 bytes a store or as many as N and the rows' starts allow
 //                   (18944 rows, K = 4096: N = 4096 158 us, 4100 168, 4094 161, 4095 176; all but the first 217 - 229 one by one)
-// Bound by the tensor cores and what keeps them waiting. A step's MMAs are 512 clocks. Measured, 18944 x 4096 x 16384 (16 tiles a
-// pair, 1024 steps): NV 491 - 512 us from GPU to GPU (5.0 - 5.2 PFLOP/s), MX 453 - 465; under the power limit of a long run 7 - 8 of 10 of that. Timed apart with
-// an earlier build of 504 us, in ns a step: MMAs alone 332, with their commits 362, with the barriers 399, with the loads 418, with
-// the scales' copies 492; a tile's end costs 2 us (the wake of the epilogue, tensor memory's read, the issuer's wake). How far the
-// scales' loads run ahead counts: 4 slots 536 us, 8 slots 491. Tried and slower (20240 x 4096 x 16384 NV, us): scale copies by the
-// MMAs' thread 877, by one other warp 699, by two 593; a branch for the last columns between the MMAs 600 (without: 552); scales
-// written to tensor memory from registers 1676; codes released every other step 8% more.
+// Bound by what an SM takes from L2: a step brings 38 KB to each (MX 35), which is 76 (70) bytes a clock at the MMAs' rate of 512
+// clocks a step. Counters (NV, 9472 x 2048 x 16384): 48 bytes a clock over the kernel, tensor pipe active 63%; NV and MX times are
+// to one another as these bytes. Measured, 18944 x 4096 x 16384 (16 tiles a pair, 1024 steps): NV 491 - 512 us from GPU to GPU
+// (5.0 - 5.2 PFLOP/s), MX 453 - 465; 15% more under the power limit of a long run. A tile's end costs 2 us (the wake of the
+// epilogue, tensor memory's read, the issuer's wake). How far the scales' loads run ahead counts: 4 slots 536 us, 8 slots 491. Tried
+// and slower (20240 x 4096 x 16384 NV, us, of 552 then): scale copies by the MMAs' thread 877, by one other warp 699, by two 593; a
+// branch for the last columns between the MMAs 600; scales written to tensor memory from registers 1676; codes released every
+// other step 8% more.
 template <int KIND> struct Wide {
     static constexpr int BM = 256, BN = 256;
     static constexpr int TILES = KB / SPAN<KIND>;
