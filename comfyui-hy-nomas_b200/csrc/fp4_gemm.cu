@@ -625,9 +625,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
             cols[thread] = p.o.rb && n < p.N ? p.o.rb[n] : 1.0f;
             cols[256 + thread] = p.o.bias && n < p.N ? bias_at(p.o, n) : 0.0f;
             const float ra = p.o.ra && m0 + lane < p.M ? p.o.ra[m0 + lane] : 1.0f;
-            if (any_of<C::EPI>(!ok)) break;                 // all warps leave together: each waits for the others here
-            ok = warp_wait(lane, bar_tfull, tphase, abort_flag, 2 * WAIT_NS, p.err);
-            if (!ok) continue;
+            // one warp looks at the barrier, the others wait for it asleep; all leave together
+            if (warp == 8) ok = warp_wait(lane, bar_tfull, tphase, abort_flag, 2 * WAIT_NS, p.err);
+            ok = !any_of<C::EPI>(!ok);
+            if (!ok) break;
             tphase ^= 1;
             tc_fence_after();
             uint32_t r[4][32];
