@@ -11,7 +11,8 @@
 // than 16384 columns are read twice. A chunk is a block of NV and half a block of MX; the lanes of a scale tile's word (4 or
 // 8) gather its bytes before the one store. Measured, 20240 x 4096 bf16: MX 32 us (6.5 TB/s), NV 41 us (5.2 TB/s: its twelve
 // instructions a column, four of them the exact quotient, are what is left; a persistent loop over rows with the next one's loads
-// ahead did not help). Back to bf16: 44 us (4.8 TB/s, 16 bytes out a thread). One row of 4096: 2.6 us, a launch.
+// ahead did not help). Back to bf16: 35 us (6.0 TB/s, 16 bytes out a thread and chunk, up to
+// four chunks' loads under way). One row of 4096: 2.6 us, a launch.
 #include "fp4.cuh"
 #include "hn_kernels.h"
 
@@ -333,34 +334,44 @@ __device__ __forceinline__ void store8(float *o, const float (&v)[8]) {
 
 // code * RN(scale * row scale), one rounding to the output type. T threads a row, which take its chunks of 8 columns in turn (16
 // bytes out, neighbouring lanes write on), so that a row's address and scale are worked out once. VEC: 16-byte stores
-template <typename E, int KIND, bool VEC, int T> __global__ void __launch_bounds__(256) k_dequant_fp4(BackParams p) {
+template <typename E, int KIND, bool VEC, int T, int U> __global__ void __launch_bounds__(256) k_dequant_fp4(BackParams p) {
     const int64_t m = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T;
     if (m >= p.M) return;
     const uint32_t *q = reinterpret_cast<const uint32_t *>(p.q + m * p.ldq);
     const uint8_t *s = p.s + scale_word(m, 0, p.tiles);
     const float r = KIND == NV ? p.r[m] : 1.0f;
     E *out = static_cast<E *>(p.out) + m * p.ldo;
-#pragma unroll 2
-    for (int c = threadIdx.x % T; c < p.nch; c += T) {
-        const int g = 8 * c / GROUP<KIND>;
-        const uint32_t w = q[c];
-        float d = scale_value<KIND>(s[(int64_t)(g >> 2) * TILE + (g & 3)]);
-        if (KIND == NV) d = __fmul_rn(d, r);
-        uint32_t h[4];
-        unpack8_e2m1(w, h);
-        float v[8];
+    for (int c0 = threadIdx.x % T; c0 < p.nch; c0 += U * T) {
+        uint32_t w[U];
+        uint8_t sb[U];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[k]));
-            v[2 * k] = f.x * d;
-            v[2 * k + 1] = f.y * d;
+        for (int i = 0; i < U; ++i) {
+            const int c = c0 + i * T, g = 8 * c / GROUP<KIND>;
+            w[i] = c < p.nch ? q[c] : 0;
+            sb[i] = c < p.nch ? s[(int64_t)(g >> 2) * TILE + (g & 3)] : 0;
         }
-        if (VEC && 8 * c + 8 <= p.K) {
-            store8(out + 8 * c, v);
-        } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (8 * c + k < p.K) store1(out + 8 * c + k, v[k]);
+        for (int i = 0; i < U; ++i) {
+            const int c = c0 + i * T;
+            if (c >= p.nch) break;
+            float d = scale_value<KIND>(sb[i]);
+            if (KIND == NV) d = __fmul_rn(d, r);
+            uint32_t h[4];
+            unpack8_e2m1(w[i], h);
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[k]));
+                v[2 * k] = f.x * d;
+                v[2 * k + 1] = f.y * d;
+            }
+            if (VEC && 8 * c + 8 <= p.K) {
+                store8(out + 8 * c, v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (8 * c + k < p.K) store1(out + 8 * c + k, v[k]);
+            }
         }
     }
 }
@@ -370,10 +381,16 @@ template <typename E, int KIND, bool VEC> cudaError_t back_rows(const BackParams
         kernel<<<(unsigned)cdiv(p.M, per), 256, 0, st>>>(p);
         return cudaGetLastError();
     };
-    if (p.nch <= 8) return go(k_dequant_fp4<E, KIND, VEC, 4>, 64);
-    if (p.nch <= 32) return go(k_dequant_fp4<E, KIND, VEC, 16>, 16);
-    if (p.nch <= 256) return go(k_dequant_fp4<E, KIND, VEC, 64>, 4);
-    return go(k_dequant_fp4<E, KIND, VEC, 256>, 1);
+    // Two to eight chunks a thread where there are rows enough, all on their way together. Measured, bf16, against one to four, two at
+    // a time (us): 20240 x 4096 NV 44.2 -> 35.3, 80960 x 1024 44.1 -> 35.6, 20240 x 2080 30.7 -> 21.0. Few rows: more threads a row
+    // (1 x 4096: 2.2, as above 2.6)
+    const bool few = p.M < 8 * num_sms();
+    if (p.nch <= 4) return go(k_dequant_fp4<E, KIND, VEC, 4, 1>, 64);
+    if (p.nch <= 8) return go(k_dequant_fp4<E, KIND, VEC, 4, 2>, 64);
+    if (p.nch <= 32) return go(k_dequant_fp4<E, KIND, VEC, 16, 2>, 16);
+    if (p.nch <= 128 && !few) return go(k_dequant_fp4<E, KIND, VEC, 16, 4>, 16);
+    if (p.nch <= 256 || (p.nch <= 1024 && !few)) return go(k_dequant_fp4<E, KIND, VEC, 64, 4>, 4);
+    return go(k_dequant_fp4<E, KIND, VEC, 256, 4>, 1);
 }
 template <typename E> cudaError_t back(const BackParams &p, int kind, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * (int64_t)sizeof(E) % 16 == 0;
