@@ -215,7 +215,7 @@ def test_few_rows(hn, cuda, kind, m, n, k):
 @pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("m,n,k", [(5, 1, 32), (5, 128, 64), (16, 128, 256), (17, 130, 96), (48, 257, 512), (128, 128, 1024),
                                    (129, 100, 160), (130, 1001, 2080), (300, 5001, 320), (48, 256, 16384), (7, 8, 40000),
-                                   (700, 700, 700), (257, 512, 4096)])
+                                   (700, 700, 700), (257, 512, 4096), (9, 19000, 256), (777, 5001, 352), (1300, 1700, 2400)])
 def test_product(hn, cuda, kind, m, n, k):
     a, w = operands(hn, m, n, k, kind, 12)
     for dtype in DTYPES:
@@ -233,7 +233,7 @@ def test_product_many_rows(hn, cuda, kind, m, n, k):
 
 @pytest.mark.parametrize("kind", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("n", [2064, 2068, 2066, 2065])
-@pytest.mark.parametrize("m,k", [(1793, 2080), (2600, 96)])
+@pytest.mark.parametrize("m,k", [(1793, 2080), (2600, 96), (1200, 1312)])
 def test_product_rows_of_any_alignment(hn, cuda, kind, n, m, k):
     """Pairs of CTAs, a tile each and several: outputs stored 16, 8, 4 and 2 bytes at a time."""
     a, w = operands(hn, m, n, k, kind, 14)
