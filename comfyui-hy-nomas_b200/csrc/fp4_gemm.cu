@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "fp4.cuh"
+#include "fp4_handoff.h"
 #include "hn_kernels.h"
 #include "hn_tc.cuh"
 
@@ -321,8 +322,8 @@ template <int KIND> struct Wide {
     static constexpr int BM = 256, BN = 256;
     static constexpr int TILES = KB / SPAN<KIND>;
     static constexpr int OP = 128 * 128, SFA = TILES * TILE, SFB = 2 * TILES * TILE;
-    static constexpr int STAGES = 5, STAGE = 2 * OP;            // codes of both operands
-    static constexpr int CP = 4;                                // warps that copy scales
+    static constexpr int STAGES = Handoff::STAGES, STAGE = 2 * OP;      // codes of both operands
+    static constexpr int CP = Handoff::CP;                      // warps that copy scales
     static constexpr int SLOTS = 2 * CP, SLOT = SFA + SFB;      // scales on their way to tensor memory
     static constexpr int ACC = 0, SFC = BN, SFW = 12 * TILES;   // tensor memory columns; SFW: a stage's scales
     static_assert(SFC + STAGES * SFW <= 512, "tensor memory");
@@ -461,6 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
     const uint32_t bar_tfull = bar_sempty + 8 * C::SLOTS, bar_tempty = bar_tfull + 8, bar_drain = bar_tempty + 8;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
+    volatile int *taken = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 8);     // steps that the issuer has met
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int kts = (p.Kp + KB - 1) / KB;
@@ -475,6 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         mbar_init(bar_tempty, 2 * C::EPI);
         mbar_init(bar_drain, 1);
         *abort_flag = 0;
+        *taken = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -530,8 +533,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         if (!ok) land();
     } else if (warp >= 4 && warp < 8 && rank == 0) {
         // step i, every C::CP-th: its scales into the columns of its stage, when the MMAs that read them last are done; then, when they
-        // and the codes are in, the issuer's release. After a wait that gave up the steps that are left are only met, so that
-        // the issuer comes to its end.
+        // and the codes are in, the issuer's release. After a wait that gave up the steps that are left are only released, each not
+        // before the issuer has met the step that had its barrier before (Handoff), so that the issuer comes to its end: it needs
+        // steps i - CP to i - 1 for that, whose warps have released theirs or are themselves on the way, and its own wait is bounded.
         // A parity tells a phase from its neighbours only, and these warps skip steps. So each has two slots of its own, whose phases
         // it sees one after the other; that MMAs of step i - 2 STAGES are over, when those of i - STAGES are waited for, follows from
         // step i - CP, whose codes the warp has seen in (they came after the MMAs of step i - CP - STAGES); and that the full
@@ -561,8 +565,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
                 last_phase = sphase;
                 ok = spin_wait(lane, bar_full + 8 * stage, phase, abort_flag, p.err);
             }
-            if (ok) asm volatile("barrier.cta.arrive %0, 64;" ::"r"(2 + stage) : "memory");
-            else asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + stage) : "memory");
+            if (!ok) {
+                const uint64_t t0 = globaltimer_ns();
+                while (*taken < Handoff::taken_before(i) && globaltimer_ns() - t0 < 4 * WAIT_NS) { }
+                __syncwarp();
+            }
+            asm volatile("barrier.cta.arrive %0, 64;" ::"r"(2 + stage) : "memory");
             if ((stage += C::CP) >= C::STAGES) { stage -= C::STAGES; phase ^= 1; }
             if ((slot += C::CP) >= C::SLOTS) { slot -= C::SLOTS; sphase ^= 1; }
         }
@@ -582,6 +590,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
                 tphase ^= 1;
             }
             asm volatile("barrier.cta.sync %0, 64;" ::"r"(2 + stage) : "memory");
+            if (lane == 0) *taken = i + 1;
             if (ok) {
                 tc_fence_after();
                 if (lane == 0) {
