@@ -74,8 +74,8 @@ __device__ __forceinline__ float e4m3_scale(float peak) { return __fdiv_rn(fmaxf
 
 // RN(p / d) for a scale divisor d (127, 448) and p a bf16 value (or the 1e-12 floor): q0 = RN(p * RN(1/d)), the
 // exact remainder p - q0 * d in one fma, and one more fma corrects q0. tests/division_check.c checks it against
-// the IEEE quotient for every positive finite bf16 p. The same scales as i8_scale / e4m3_scale, for peaks that
-// are absmaxes of bf16 values.
+// the IEEE quotient for every positive finite bf16 p, tests/scale_quotient_check.c for every positive finite fp32 p
+// and 127. The same scales as i8_scale / e4m3_scale, for peaks that are absmaxes of bf16 values (127: of fp32 ones, too).
 __device__ __forceinline__ float quot_const(float p, float d, float rd) {
     const float q0 = __fmul_rn(p, rd);
     return __fmaf_rn(__fmaf_rn(-q0, d, p), rd, q0);

@@ -306,10 +306,6 @@ template <bool I8> __global__ void __launch_bounds__(32 * AWARPS) k_append_rotat
     }
 }
 
-// ... with rotated parts of a multiple of 16: sixteen columns a lane, four heads of one kind (q, k or v) a pass. Bound by
-// instructions, not by HBM, the int8 quantizer's above all (half of its cycles issue one), so each kind has a loop of its own,
-// whose addresses only step on. 2 x 4400 tokens, 16 + 16 + 16 heads, int8: 53 us of 28 for the bytes (61 with one loop that asks
-// for the kind); loads further ahead, through shared memory, and more warps of fewer registers changed nothing or cost more.
 // A row of K or V (16 columns of it in this lane) as codes and scale
 __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16 &l, const float (&a)[8], const float (&b)[8], bool in, bool lead) {
     float peak = nanmax_abs3(0.0f, a[0], a[1]);
@@ -318,8 +314,8 @@ __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16
 #pragma unroll
     for (int j = 0; j < 8; j += 2) peak = nanmax_abs3(peak, b[j], b[j + 1]);
     peak = lanes_max<8>(peak);
-    // a NaN or an infinity in the row: its scale is NaN, so that what reads it gives NaN. Of 16-bit values the quotient is exact
-    // (i8_scale_bf16), of others off by a unit at most
+    // a NaN or an infinity in the row: its scale is NaN, so that what reads it gives NaN. i8_scale_bf16 is the IEEE quotient of
+    // any finite fp32 peak, as i8_scale
     const float sc = peak < INFINITY ? i8_scale_bf16(peak) : __int_as_float(0x7fffffff);
     if (!in) return;
     const bool fast = sc >= 0x1p-90f;
@@ -329,6 +325,10 @@ __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16
     if (lead) *scale = sc;
 }
 
+// ... with rotated parts of a multiple of 16: sixteen columns a lane, four heads of one kind (q, k or v) a pass. Bound by
+// instructions, not by HBM, the int8 quantizer's above all (half of its cycles issue one), so each kind has a loop of its own,
+// whose addresses only step on. 2 x 4400 tokens, 16 + 16 + 16 heads, int8: 53 us of 28 for the bytes (61 with one loop that asks
+// for the kind); loads further ahead, through shared memory, and more warps of fewer registers changed nothing or cost more.
 template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * AWARPS, ACTAS) k_append_rotated16(AppendParams p, Meta m) {
     __shared__ __align__(16) float tables[AWARPS][2 * MAX_PAIRS];
     const int lane = threadIdx.x & 31, sub = lane & 7, side = lane >> 3;
