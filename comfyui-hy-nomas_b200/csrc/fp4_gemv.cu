@@ -4,7 +4,9 @@
 // quarter of a scale tile's 128 (their scales are 32 neighbouring bytes), its warps the chunks of 1024 columns in turn, so a
 // lane has 16 bytes of every row in flight. Codes become fp16 pairs, exactly; the products of a block of 16 are
 // summed in fp16 pairs of eight products each, whose sum is exact too (at most 288 in steps of 0.25: 1152 of 2048), and leave
-// as fp32, times both scales. The order of the sums is fixed. Measured: one row over 4096 x 16384 NV: 9.7 us with its launch
+// as fp32, times both scales. MX: these are powers of two that may be far apart, whose product with a sum need not be (2^125 and
+// 2^-27), so the activations' goes in two factors with exponents of one sign, half before the weights' and half after: no step
+// leaves fp32 unless the result does. The order of the sums is fixed. Measured: one row over 4096 x 16384 NV: 9.7 us with its launch
 // (3.9 TB/s), two rows 14.2 (the tile kernel, three rows and more: 15). Four rows in flight and 64 registers, so that all CTAs of
 // that case are resident: 10.8 -> 9.7.
 #include "fp4.cuh"
@@ -42,6 +44,13 @@ __device__ __forceinline__ float dot16(const uint32_t *a, const uint32_t *b) {
     return f.x + f.y;
 }
 
+// the value of an MX scale byte (2^(byte - 127), 255: NaN) as two factors, their exponents of one sign and half of its each
+__device__ __forceinline__ void halves(uint32_t byte, float (&f)[2]) {
+    const int e = (int)byte - 127, h = e / 2;
+    f[0] = byte == 255 ? __int_as_float(0x7fffffff) : __uint_as_float((uint32_t)(127 + h) << 23);
+    f[1] = __uint_as_float((uint32_t)(127 + e - h) << 23);
+}
+
 template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS, MT == 1 ? 4 : 2) k_fp4_gemv(Params p) {
     __shared__ float sums[WARPS][ROWS * MT];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -68,8 +77,12 @@ template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS, MT == 
                 word = __ldg(reinterpret_cast<const uint32_t *>(p.sa + scale_word(i, tile, p.tiles)));
             }
             unpack32(a, x[i]);
-            xs[i][0] = scale_value<KIND>(word >> (8 * g) & 255);
-            xs[i][1] = KIND == NV ? scale_value<KIND>(word >> (8 * g + 8) & 255) : 0.0f;
+            if (KIND == MX) {
+                halves(word >> (8 * g) & 255, xs[i]);
+            } else {
+                xs[i][0] = scale_value<KIND>(word >> (8 * g) & 255);
+                xs[i][1] = scale_value<KIND>(word >> (8 * g + 8) & 255);
+            }
         }
         const uint4 *scales = reinterpret_cast<const uint4 *>(p.sw + (block * p.tiles + tile) * TILE + 16 * pair);
 #pragma unroll
@@ -94,7 +107,7 @@ template <int KIND, int MT> __global__ void __launch_bounds__(32 * WARPS, MT == 
                     const float d0 = dot16(h, x[i]), d1 = dot16(h + 8, x[i] + 8);
                     float &sum = acc[i][2 * j + half];
                     if (KIND == NV) sum = fmaf(d1, xs[i][1] * s1, fmaf(d0, xs[i][0] * s0, sum));
-                    else sum = fmaf((d0 + d1) * xs[i][0], s0, sum);
+                    else sum = fmaf((d0 + d1) * xs[i][0] * s0, xs[i][1], sum);
                 }
             }
         }
