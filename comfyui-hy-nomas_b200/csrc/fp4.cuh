@@ -76,10 +76,16 @@ __device__ __forceinline__ float bias_at(const Result &o, int64_t n) {
          : o.bias_dtype == 0 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(o.bias)[n])
                              : __half2float(static_cast<const __half *>(o.bias)[n]);
 }
+// sum ra rb in an order that leaves fp32 only where the result does: the largest sum, 36 448^2 K, is below 2^53, so it bears a row
+// scale up to 2^60 at once, and a larger one after the column's
+__device__ __forceinline__ bool is_far(float ra) { return fabsf(ra) > 0x1p60f; }
+__device__ __forceinline__ float scaled(float sum, float ra, float rb) {
+    const bool far = is_far(ra);
+    return __fmul_rn(__fmul_rn(sum, far ? rb : ra), far ? ra : rb);
+}
 // fp32 result of column n; ra: the row's scale, or 1
 __device__ __forceinline__ float finish(const Result &o, float sum, float ra, int64_t n) {
-    if (o.ra) sum = __fmul_rn(sum, ra);
-    if (o.rb) sum = __fmul_rn(sum, o.rb[n]);
+    if (o.ra || o.rb) sum = scaled(sum, ra, o.rb ? o.rb[n] : 1.0f);
     return o.bias ? __fadd_rn(sum, bias_at(o, n)) : sum;
 }
 __device__ __forceinline__ void store_result(const Result &o, int64_t at, float v) {

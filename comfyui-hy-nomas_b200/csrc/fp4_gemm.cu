@@ -103,7 +103,8 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr, uint32_t rank) {
 
 // Rows [r0, r1) of a tile's sums: P CTAs' partial sums added in their order, scales, bias, rounding. A warp takes every WARPS-th
 // row, U of them at a time so that their loads overlap; a lane has the same four columns throughout (VEC: neighbours, one store).
-template <int P, bool VEC, int WARPS>
+// FAR: rows whose scales need an order of their own (`scaled`) may be among them
+template <int P, bool VEC, bool FAR, int WARPS>
 __device__ __forceinline__ void write_rows(const Params &p, const float *tile, int pitch, int m0, int n0, int r0, int r1) {
     constexpr int U = P == 8 ? 2 : 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -142,7 +143,7 @@ __device__ __forceinline__ void write_rows(const Params &p, const float *tile, i
                 o[j] = v[u][0][j];
 #pragma unroll
                 for (int i = 1; i < P; ++i) o[j] += v[u][i][j];
-                o[j] = __fadd_rn(__fmul_rn(__fmul_rn(o[j], ra[u]), cs[j]), cb[j]);
+                o[j] = __fadd_rn(FAR ? scaled(o[j], ra[u], cs[j]) : __fmul_rn(__fmul_rn(o[j], ra[u]), cs[j]), cb[j]);
             }
             const int64_t off = (int64_t)(m0 + row) * p.o.ldo + n0;
             if (VEC) {
@@ -173,6 +174,7 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
     const uint32_t bar_full = sbase + C::OFF_BAR, bar_empty = bar_full + 8 * C::STAGES, bar_done = bar_empty + 8 * C::STAGES;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::OFF_MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 4);
+    volatile int *far = reinterpret_cast<volatile int *>(smem + C::OFF_MISC + 8);       // a row's scale is_far
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile = blockIdx.x / p.parts, part = blockIdx.x - tile * p.parts;
     const int m0 = tile % p.m_tiles * C::BM, n0 = tile / p.m_tiles * C::BN;
@@ -192,6 +194,7 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
         mbar_init(bar_done, 1);
         *abort_flag = 0;
+        *far = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         for (int s = 0; s < C::STAGES && kt0 + s < kt1; ++s) load(kt0 + s, s);      // the first stages, while the others prepare
@@ -256,6 +259,9 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
         }
         if (lane == 0) mma_commit(bar_done);        // also after a wait that gave up: what was issued is awaited
         __syncwarp();
+    } else if (KIND == NV && p.o.ra) {              // beside the MMAs: the rows' loop below pays 1% for the test
+        const int row = m0 + threadIdx.x - 64;
+        if (row < p.M && is_far(p.o.ra[row])) *far = 1;
     }
     ok = warp_wait(lane, bar_done, 0, abort_flag, WAIT_NS + 1000000000ull, p.err) && ok;
     tc_fence_after();
@@ -279,8 +285,9 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
         const int rows = min(C::BM, p.M - m0), r0 = rows * part / p.parts, r1 = rows * (part + 1) / p.parts;
         auto write = [&](auto parts) {
             constexpr int P = decltype(parts)::value, W = C::THREADS / 32;
-            if (p.vec) write_rows<P, true, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
-            else write_rows<P, false, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
+            if (KIND == NV && *far) write_rows<P, false, true, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
+            else if (p.vec) write_rows<P, true, false, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
+            else write_rows<P, false, false, W>(p, tile_s, C::PITCH, m0, n0, r0, r1);
         };
         if (p.parts == 1) write(std::integral_constant<int, 1>());
         else if (p.parts == 2) write(std::integral_constant<int, 2>());
@@ -330,7 +337,8 @@ template <int KIND> struct Wide {
     static constexpr int EPI = 8, PITCH = 48;                   // warps; bytes a row of their chunks of 32
     static constexpr int OFF_SF = STAGES * STAGE, OFF_EPI = OFF_SF + SLOTS * SLOT;
     static constexpr int OFF_COLS = OFF_EPI + EPI * 32 * PITCH;                             // column scales and bias: [2][2][256]
-    static constexpr int OFF_BAR = OFF_COLS + 2 * 2 * 256 * 4;
+    static constexpr int OFF_ONES = OFF_COLS + 2 * 2 * 256 * 4;                            // 128 column scales of 1
+    static constexpr int OFF_BAR = OFF_ONES + 128 * 4;
     static constexpr int OFF_MISC = OFF_BAR + 8 * (2 * STAGES + 2 * SLOTS + 3);
     static constexpr int SMEM = OFF_MISC + 16 + 1024;
     static_assert(SMEM <= 232448, "shared memory");
@@ -481,6 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    if (warp >= 8 && warp < 12) reinterpret_cast<float *>(smem + C::OFF_ONES)[threadIdx.x - 256] = 1.0f;
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -636,7 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
             const int n = nt * 256 + thread;
             cols[thread] = p.o.rb && n < p.N ? p.o.rb[n] : 1.0f;
             cols[256 + thread] = p.o.bias && n < p.N ? bias_at(p.o, n) : 0.0f;
-            const float ra = p.o.ra && m0 + lane < p.M ? p.o.ra[m0 + lane] : 1.0f;
+            float ra = p.o.ra && m0 + lane < p.M ? p.o.ra[m0 + lane] : 1.0f;
             // one warp looks at the barrier, the others wait for it asleep; all leave together
             if (warp == 8) ok = warp_wait(lane, bar_tfull, tphase, abort_flag, 2 * WAIT_NS, p.err);
             ok = !any_of<C::EPI>(!ok);
@@ -650,6 +659,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<KIND>::THREADS,
             __syncwarp();
             if (lane == 0) arrive_at(tempty);
             const float *rb = cols + 128 * half, *bias = rb + 256;
+            if (KIND == NV && __any_sync(0xffffffffu, is_far(ra))) {
+                // rare, so apart: the scales in an order of their own here, and ones for them below (a test in the loop below:
+                // 157 -> 165 us at 18944 x 4096 x 4096; a second loop: 178 -> 187 at 18944 x 4095 x 4096)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[c][j] = __float_as_uint(scaled(__uint_as_float(r[c][j]), ra, rb[32 * c + j]));
+                ra = 1.0f;
+                rb = reinterpret_cast<const float *>(smem + C::OFF_ONES);
+            }
             constexpr int COLS = 32 / EB;               // of a chunk: 32 bytes a row
 #pragma unroll
             for (int c = 0; c < 128 / COLS; ++c) {

@@ -1,5 +1,5 @@
-"""The 4-bit product at the ends of its scales: powers of two far apart, every e4m3 block scale, NaN scales.
-By each of its kernels: one and two rows, some rows, many."""
+"""The 4-bit product at the ends of its scales: powers of two far apart, every e4m3 block scale, NaN scales, row scales whose product
+with a sum leaves fp32 though the output does not. By each of its kernels: one and two rows, some rows, many."""
 import numpy as np
 import pytest
 import torch
@@ -78,3 +78,18 @@ def test_nan_scale(hn, cuda, kind, nan, m, n, k):
     bad = torch.zeros(m, n, dtype=torch.bool, device="cuda")
     bad[m - 1], bad[:, n // 2] = True, True
     assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_row_scales_far_apart(hn, cuda, m, n, k):
+    """nvfp4 rows of activations near 2^120 against weights near 2^-60, and the other way: the sum times the larger row scale alone
+    leaves fp32, the output does not."""
+    for big, small in ((2.0 ** 118, 2.0 ** -60), (2.0 ** -60, 2.0 ** 118)):
+        x, y = randn((m, k), 1, loud=False).float() * big, randn((n, k), 2, loud=False).float() * small
+        if m > 2:
+            x[1::2] = randn((x[1::2].shape[0], k), 3, loud=False).float() * min(big, 1.0)      # rows of both sorts side by side
+        a, w = hn.kernels.quantize_fp4(x), hn.kernels.quantize_fp4(y)
+        for dtype in (torch.bfloat16, torch.float32):
+            out = hn.kernels.fp4_gemm(*a, *w, out_dtype=dtype)
+            assert bool(out.isfinite().all())
+            check_product(hn, out, a, w, "nvfp4")
