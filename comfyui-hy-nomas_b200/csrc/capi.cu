@@ -854,9 +854,11 @@ int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, co
     return launched(e, "hn_fp4_gemm launch");
 }
 
-// what the rotations have in common
-static int rotation_args(const char *what, const void *pos, int wide, const int64_t *freq, int64_t rot, int layout, float factor,
-                         const void *w0, const void *w1, float eps, int64_t D) {
+// what the rotations have in common; takes the weights' type out of `layout`
+static int rotation_args(const char *what, const void *pos, int wide, const int64_t *freq, int64_t rot, int &layout, float factor,
+                         const void *w0, const void *w1, float eps, int64_t D, int &w_wide) {
+    w_wide = layout == (HN_ROPE_HALF | HN_ROPE_NORM_FP32) || layout == (HN_ROPE_INTERLEAVED | HN_ROPE_NORM_FP32);
+    if (w_wide) layout &= ~HN_ROPE_NORM_FP32;
     REQUIRE(D >= 8 && D <= 256 && D % 8 == 0 && rot >= 8 && rot <= D && rot % 8 == 0, HN_ERR_SHAPE,
             "%s: need rot <= D <= 256, both multiples of 8 (rot=%lld D=%lld)", what, (long long)rot, (long long)D);
     REQUIRE(layout == HN_ROPE_HALF || layout == HN_ROPE_INTERLEAVED, HN_ERR_ARG, "%s: unknown layout %d", what, layout);
@@ -874,7 +876,8 @@ int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype
     REQUIRE(float_dtype(dtype), HN_ERR_ARG, "hn_rotate: bad dtype %d", dtype);
     REQUIRE(B >= 0 && L >= 0 && H >= 0 && B <= 0x7fffffff && L <= 0x7fffffff && H <= 65536, HN_ERR_SHAPE,
             "hn_rotate: bad shape (B=%lld L=%lld H=%lld)", (long long)B, (long long)L, (long long)H);
-    if (int rc = rotation_args("hn_rotate", pos, pos_wide, freq, rot, layout, factor, weight, nullptr, eps, D)) return rc;
+    int w_wide = 0;
+    if (int rc = rotation_args("hn_rotate", pos, pos_wide, freq, rot, layout, factor, weight, nullptr, eps, D, w_wide)) return rc;
     if (B == 0 || L == 0 || H == 0) return HN_OK;
     REQUIRE(B * L <= (1LL << 40) / H, HN_ERR_SHAPE, "hn_rotate: too many heads");
     REQUIRE(x && pos && out, HN_ERR_ARG, "hn_rotate: null pointer");
@@ -884,7 +887,7 @@ int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype
     RotateArgs a;
     a.x = x; a.x_bs = x_bs; a.x_ls = x_ls; a.x_hs = x_hs;
     a.out = out; a.o_bs = o_bs; a.o_ls = o_ls; a.o_hs = o_hs; a.dtype = dtype;
-    a.pos = pos; a.p_bs = p_bs; a.p_ls = p_ls; a.wide = pos_wide; a.w = weight;
+    a.pos = pos; a.p_bs = p_bs; a.p_ls = p_ls; a.wide = pos_wide; a.w = weight; a.w_wide = w_wide;
     a.freq = freq; a.rot = (int)rot; a.layout = layout; a.factor = factor; a.eps = eps;
     a.B = (int)B; a.L = (int)L; a.H = (int)H; a.D = (int)D;
     return launched(launch_rotate(a, (cudaStream_t)stream), "hn_rotate launch");
@@ -901,7 +904,8 @@ int hn_cache_append_rotated(const hn_kv_cache *cache, int64_t layer, const void 
             (long long)cache->layers);
     REQUIRE(B >= 0 && n >= 0 && B <= MAX_REQUESTS && n <= 0x3fffffff && H >= 1 && H <= 65536, HN_ERR_SHAPE,
             "hn_cache_append_rotated: bad count");
-    if (int rc = rotation_args("hn_cache_append_rotated", pos, pos_wide, freq, rot, layout, factor, q_weight, k_weight, eps, 128))
+    int w_wide = 0;
+    if (int rc = rotation_args("hn_cache_append_rotated", pos, pos_wide, freq, rot, layout, factor, q_weight, k_weight, eps, 128, w_wide))
         return rc;
     if (B == 0 || n == 0) return HN_OK;
     REQUIRE(q && k && v && rows && out, HN_ERR_ARG, "hn_cache_append_rotated: null pointer");
@@ -916,7 +920,7 @@ int hn_cache_append_rotated(const hn_kv_cache *cache, int64_t layer, const void 
     a.x[1] = k; a.bs[1] = k_bs; a.ts[1] = k_ts; a.hs[1] = k_hs;
     a.x[2] = v; a.bs[2] = v_bs; a.ts[2] = v_ts; a.hs[2] = v_hs;
     a.out = out; a.rows = rows; a.pos = pos; a.p_bs = p_bs; a.p_ts = p_ts; a.wide = pos_wide;
-    a.w[0] = q_weight; a.w[1] = k_weight;
+    a.w[0] = q_weight; a.w[1] = k_weight; a.w_wide = w_wide;
     a.freq = freq; a.rot = (int)rot; a.layout = layout; a.factor = factor; a.eps = eps;
     a.B = (int)B; a.n = (int)n; a.H = (int)H;
     return launched(launch_append_rotated(c, (int)layer, a, (cudaStream_t)stream), "hn_cache_append_rotated launch");

@@ -165,7 +165,7 @@ struct RotateArgs {
     void *out; int64_t o_bs, o_ls, o_hs;
     int dtype;
     const void *pos; int64_t p_bs, p_ls; int wide;
-    const void *w;          // bf16 [D], or null: no norm
+    const void *w; int w_wide;      // [D] bf16, or fp32 where w_wide; null: no norm
     const int64_t *freq; int rot, layout; float factor;
     float eps;
     int B, L, H, D;
@@ -176,7 +176,7 @@ struct AppendRotatedArgs {
     void *out;                                          // [B, n, H, 128]
     const int *rows;
     const void *pos; int64_t p_bs, p_ts; int wide;      // pos null: a token's place in its row
-    const void *w[2];                                   // bf16 [128] of q and k, or null
+    const void *w[2]; int w_wide;                       // [128] of q and k, as above
     const int64_t *freq; int rot, layout; float factor;
     float eps;
     int B, n, H;

@@ -27,7 +27,8 @@ struct Params {
     const void *pos;                    // int32 or int64
     int64_t p_bs, p_ls;
     int wide;
-    const __nv_bfloat16 *w;             // or null
+    const void *w;                      // bf16, fp32 with w_wide, or null
+    int w_wide;
     Rotation r;
     float eps;
     int B, L, H, D, per, groups;        // per: heads of a unit, a multiple of 32 / P; groups: units of a token
@@ -43,7 +44,7 @@ template <typename E, int P, bool INTER, bool NORM> __global__ void __launch_bou
     Turn t;
     partners(p.r, sub, t);
     Weights w;
-    if (NORM && in) load_weights(p.w + 8 * sub, t, w);
+    if (NORM && in) load_weights(p.w, p.w_wide, 8 * sub, t, w);
     const float rd = 1.0f / p.D;
     const int64_t units = (int64_t)p.B * p.L * p.groups, step = (int64_t)gridDim.x * WARPS;
     for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
@@ -110,7 +111,7 @@ template <typename E, int P, bool INTER, bool NORM> __global__ void __launch_bou
     const bool in = 16 * sub < p.D;
     const Lane16 at16 = lane16<INTER>(p.r, sub);
     Cols w;
-    if (NORM && in) load_weights16<INTER>(p.w, at16, w);
+    if (NORM && in) load_weights16<INTER>(p.w, p.w_wide, at16, w);
     const float rd = 1.0f / p.D;
     const int64_t units = (int64_t)p.B * p.L * p.groups, step = (int64_t)gridDim.x * WARPS;
     for (int64_t u = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5); u < units; u += step) {
@@ -211,7 +212,8 @@ struct AppendParams {
     const void *pos;                    // [B, n] int32 or int64, or null: a token's place in its row
     int64_t p_bs, p_ts;
     int wide;
-    const __nv_bfloat16 *w[2];          // norm weights of q and of k, or null
+    const void *w[2];                   // norm weights of q and of k, bf16, fp32 with w_wide, or null
+    int w_wide;
     Rotation r;
     float eps;
     int B, n, H, heads, per, groups;    // per: heads of a unit, of the token's H + 2 heads
@@ -267,13 +269,13 @@ template <bool I8> __global__ void __launch_bounds__(32 * AWARPS) k_append_rotat
                 load8(x, v);
                 if (which < 2) load_partners(x, t, o);
             }
-            const __nv_bfloat16 *w = which < 2 ? p.w[which] : nullptr;
+            const void *w = which < 2 ? p.w[which] : nullptr;
             if (p.w[0] != nullptr || p.w[1] != nullptr) {
                 float n[8], no[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) { n[j] = v[j]; no[j] = o[j]; }
                 Weights ww;
-                if (w != nullptr) load_weights(w + 8 * sub, t, ww);
+                if (w != nullptr) load_weights(w, p.w_wide, 8 * sub, t, ww);
                 head_norm<16>(n, no, ww, t, 1.0f / 128, p.eps);
                 if (w != nullptr)
 #pragma unroll
@@ -387,7 +389,7 @@ template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * AWARPS, AC
             turn16_of(at16, table, t);
             Cols w;
             if (first < nq) {
-                if (p.w[0] != nullptr) load_weights16<INTER>(p.w[0], at16, w);
+                if (p.w[0] != nullptr) load_weights16<INTER>(p.w[0], p.w_wide, at16, w);
                 __nv_bfloat16 *out = p.out + (bt * p.H + hq) * 128;
                 for (int h = hq; h - side < endq; h += 4, out += 512) {
                     Cols v;
@@ -401,7 +403,7 @@ template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * AWARPS, AC
                 }
             }
             if (last > nq) {
-                if (p.w[1] != nullptr) load_weights16<INTER>(p.w[1], at16, w);
+                if (p.w[1] != nullptr) load_weights16<INTER>(p.w[1], p.w_wide, at16, w);
                 int64_t to = token + (int64_t)hk * m.page;
                 for (int h = hk; h - side < endk; h += 4, to += 4 * m.page) {
                     Cols v;
@@ -449,7 +451,7 @@ cudaError_t launch_rotate(const RotateArgs &a, cudaStream_t st) {
     p.x = a.x; p.x_bs = a.x_bs; p.x_ls = a.x_ls; p.x_hs = a.x_hs;
     p.out = a.out; p.o_bs = a.o_bs; p.o_ls = a.o_ls; p.o_hs = a.o_hs;
     p.pos = a.pos; p.p_bs = a.p_bs; p.p_ls = a.p_ls; p.wide = a.wide;
-    p.w = static_cast<const __nv_bfloat16 *>(a.w);
+    p.w = a.w; p.w_wide = a.w_wide;
     p.r = {a.freq, a.rot, a.layout, a.factor};
     p.eps = a.eps; p.B = a.B; p.L = a.L; p.H = a.H; p.D = a.D;
     if (a.dtype == 0) return rotary::pick<__nv_bfloat16>(p, st);
@@ -471,7 +473,7 @@ cudaError_t launch_append_rotated(const CacheArgs &c, int layer, const AppendRot
     p.scale[0] = c.ks ? c.ks + tokens : nullptr;
     p.scale[1] = c.ks ? c.vs + tokens : nullptr;
     p.rows = a.rows; p.pos = a.pos; p.p_bs = a.p_bs; p.p_ts = a.p_ts; p.wide = a.wide;
-    for (int i = 0; i < 2; ++i) p.w[i] = static_cast<const __nv_bfloat16 *>(a.w[i]);
+    p.w[0] = a.w[0]; p.w[1] = a.w[1]; p.w_wide = a.w_wide;
     p.r = {a.freq, a.rot, a.layout, a.factor};
     p.eps = a.eps; p.B = a.B; p.n = a.n; p.H = a.H; p.heads = c.heads;
     // passes of a token: four heads of a kind at a time, or two of any; a unit takes all of them where there are tokens enough

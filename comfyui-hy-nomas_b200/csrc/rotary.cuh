@@ -122,9 +122,14 @@ template <typename E> __device__ __forceinline__ void load_partners(const E *x, 
 struct Weights {
     float own[8], other[8];
 };
-__device__ __forceinline__ void load_weights(const __nv_bfloat16 *w, const Turn &t, Weights &out) {
+// of columns from `first` on; w: bf16, or fp32 (`wide`), as the caller has them
+template <typename E> __device__ __forceinline__ void load_weights(const E *w, const Turn &t, Weights &out) {
     load8(w, out.own);
     load_partners(w, t, out.other);
+}
+__device__ __forceinline__ void load_weights(const void *w, int wide, int first, const Turn &t, Weights &out) {
+    if (wide) load_weights(static_cast<const float *>(w) + first, t, out);
+    else load_weights(static_cast<const __nv_bfloat16 *>(w) + first, t, out);
 }
 // x / sqrt(mean x^2 + eps) * w over the P lanes of a head (v is 0 in lanes behind it); rd = 1 / D
 template <int P>
@@ -294,11 +299,15 @@ template <bool INTER, typename E> __device__ __forceinline__ void store_runs(E *
     take_run<INTER>(c, 1, v);
     store8(p + l.b, v);
 }
-template <bool INTER> __device__ __forceinline__ void load_weights16(const __nv_bfloat16 *w, const Lane16 &l, Cols &c) {
-    Raw8<__nv_bfloat16> raw[2];
+template <bool INTER, typename E> __device__ __forceinline__ void load_weights16(const E *w, const Lane16 &l, Cols &c) {
+    Raw8<E> raw[2];
     raw[0].load(w + l.a);
     raw[1].load(w + l.b);
     widen16<INTER>(raw, c);
+}
+template <bool INTER> __device__ __forceinline__ void load_weights16(const void *w, int wide, const Lane16 &l, Cols &c) {
+    if (wide) load_weights16<INTER>(static_cast<const float *>(w), l, c);
+    else load_weights16<INTER>(static_cast<const __nv_bfloat16 *>(w), l, c);
 }
 
 } // namespace rotary

@@ -143,7 +143,8 @@ class KVCache:
     def append_rotated(self, layer, q, k, v, rows, rot, q_norm=None, k_norm=None, eps=1e-6, positions=None):
         """`append` of k with its per-head RMSNorm (`k_norm` [128], None: none) and rotation (`rotary.Rotary`), and of v as it is, in
         one pass with the norm and rotation of q [B, n, H, 128] -> q' [B, n, H, 128] bf16, for `attention`. Positions are the
-        tokens' places in their rows, or `positions` [B, n] or [n]. All in fp32; K is rounded once, to the cache's format.
+        tokens' places in their rows, or `positions` [B, n] or [n]. All in fp32, the weights in their own types (bf16, fp16, fp32); K is
+        rounded once, to the cache's format.
         Rows that `append` leaves out are left out and counted in the same way; their q' means nothing."""
         what = "append_rotated"
         if not (q.is_cuda and k.is_cuda and v.is_cuda):
@@ -164,15 +165,15 @@ class KVCache:
         n, h = shape[1], qshape[2]
         ptr, pb, pt, wide, positions = (None, 0, 0, 0, None) if positions is None else \
             rotary.positions_of(positions, b, n, device, what)
-        wq, wk = rotary.norm_weight(q_norm, HEAD_DIM, device, what), rotary.norm_weight(k_norm, HEAD_DIM, device, what)
+        (wq, wk), w_wide = rotary.norm_weights((q_norm, k_norm), HEAD_DIM, device, what)
         q, k, v = _operand(q), _operand(k), _operand(v)
         out = torch.empty((b, n, h, HEAD_DIM), dtype=torch.bfloat16, device=device)
         dim, layout, factor = rot._args
         qs, ks, vs = q.stride(), k.stride(), v.stride()
         _lib.check(_lib.launch(
             "hn_cache_append_rotated", device, self._ref, layer, q.data_ptr(), qs[0], qs[1], qs[2], h, k.data_ptr(), ks[0], ks[1],
-            ks[2], v.data_ptr(), vs[0], vs[1], vs[2], rows.data_ptr(), b, n, ptr, pb, pt, wide, rot.freq.data_ptr(), dim, layout,
-            factor, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, out.data_ptr()),
+            ks[2], v.data_ptr(), vs[0], vs[1], vs[2], rows.data_ptr(), b, n, ptr, pb, pt, wide, rot.freq.data_ptr(), dim,
+            layout | w_wide, factor, None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, out.data_ptr()),
             "cache.append_rotated")
         return out
 

@@ -17,6 +17,7 @@ import torch
 from . import _lib
 
 LAYOUTS = {"half": 0, "interleaved": 1}
+NORM_FP32 = 16
 _FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SCALINGS = {"linear": {"factor"}, "ntk": {"factor"}, "yarn": {"factor", "original", "beta_fast", "beta_slow", "attention_factor"}}
 
@@ -107,17 +108,28 @@ def positions_of(p, batch, tokens, device, what):
     return p.data_ptr(), pb, pt, wide, p
 
 
-def norm_weight(w, dim, device, what):
-    """A per-head norm weight as an aligned bf16 tensor, or None."""
-    if w is None:
-        return None
-    if w.shape != (dim,):
-        raise ValueError(f"{what}: norm weight {tuple(w.shape)} must be [{dim}]")
-    if w.device != device:
-        raise RuntimeError(f"{what}: norm weight on {w.device}, the heads on {device}")
-    if w.dtype != torch.bfloat16:
-        w = w.to(torch.bfloat16)
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else _lib.dense(w)
+def norm_weights(ws, dim, device, what):
+    """Per-head norm weights (each a tensor [dim], or None) as the kernels take them, all bf16 or all fp32 and aligned -> (the tensors,
+    what the layout is told). fp32 where any is not bf16: no weight loses bits (but those beyond fp32)."""
+    wide = 0
+    for w in ws:
+        if w is None:
+            continue
+        if w.shape != (dim,):
+            raise ValueError(f"{what}: norm weight {tuple(w.shape)} must be [{dim}]")
+        if w.device != device:
+            raise RuntimeError(f"{what}: norm weight on {w.device}, the heads on {device}")
+        if w.dtype != torch.bfloat16:
+            wide = NORM_FP32
+    dtype, out = torch.float32 if wide else torch.bfloat16, []
+    for w in ws:
+        if w is not None:
+            if w.dtype != dtype:
+                w = w.to(dtype)
+            if not w.is_contiguous() or w.data_ptr() % 16:
+                w = _lib.dense(w)
+        out.append(w)
+    return out, wide
 
 
 def check_rotary(rot, dim, device, what):
@@ -144,8 +156,9 @@ def _span(t):
 
 def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
     """x [B, L, H, D] (bf16, fp16 or fp32; D a multiple of 8 up to 256; any strides in steps of 8 elements, the last dimension
-    contiguous) at integer positions [B, L] or [L] -> [B, L, H, D] of x's dtype: RMSNorm over each head times `weight` [D] (None: no
-    norm), then the rotation of its first rot.dim columns, in fp32 with one rounding. `out`: a caller-owned tensor like x, or x."""
+    contiguous) at integer positions [B, L] or [L] -> [B, L, H, D] of x's dtype: RMSNorm over each head times `weight` [D] (bf16, fp16
+    or fp32, taken as it is; None: no norm), then the rotation of its first rot.dim columns, in fp32 with one rounding. `out`: a
+    caller-owned tensor like x, or x."""
     what = "rotate"
     if not x.is_cuda:
         _lib.require_cuda(x)
@@ -159,7 +172,7 @@ def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
     b, l, h, d = shape
     check_rotary(rot, d, device, what)
     ptr, pb, pl, wide, keep = positions_of(positions, b, l, device, what)
-    w = norm_weight(weight, d, device, what)
+    (w,), w_wide = norm_weights((weight,), d, device, what)
     src = x if _steps8(x) else _lib.dense(x)
     if out is None:
         out = torch.empty((b, l, h, d), dtype=x.dtype, device=device)
@@ -176,6 +189,6 @@ def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
     dim, layout, factor = rot._args
     xs, os = src.stride(), out.stride()
     _lib.check(_lib.launch("hn_rotate", device, src.data_ptr(), xs[0], xs[1], xs[2], dtype, ptr, pb, pl, wide,
-                           rot.freq.data_ptr(), dim, layout, factor, None if w is None else w.data_ptr(), eps, b, l, h, d,
+                           rot.freq.data_ptr(), dim, layout | w_wide, factor, None if w is None else w.data_ptr(), eps, b, l, h, d,
                            out.data_ptr(), os[0], os[1], os[2]), what)
     return out

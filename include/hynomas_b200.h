@@ -79,6 +79,8 @@ typedef enum {
 /* columns of a head that a rotation pairs: i with i + rot / 2, or 2 i with 2 i + 1 */
 #define HN_ROPE_HALF 0
 #define HN_ROPE_INTERLEAVED 1
+/* added to the layout: the norm weights of the call are fp32, not bf16 */
+#define HN_ROPE_NORM_FP32 16
 
 /* Message of the last failed call on this thread ("" if none). */
 const char *hn_last_error(void);
@@ -444,13 +446,14 @@ int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, co
  * Rotation of heads by their tokens' positions, with the per-head RMSNorm before it (hy_nomas/fused.py:65-186 takes tables of
  * cos and sin instead): y = R(pos) (x / sqrt(mean x^2 + eps) * weight), in fp32, rounded once. Pair i of the first `rot` columns
  * turns by pos * freq[i] / 2^64 of a turn (the product modulo one turn is exact), cos and sin times `factor`; the other columns
- * pass. layout HN_ROPE_*. weight bf16 [D], or NULL: no norm. pos int32, or int64 with pos_wide 1; any sign.
+ * pass. layout HN_ROPE_*. weight [D] bf16, or fp32 with HN_ROPE_NORM_FP32 in layout, or NULL: no norm. pos int32, or int64 with
+ * pos_wide 1; any sign.
  * x, out [B, L, H, D] of `dtype` (bf16, fp16, fp32), element strides for batch, token, head, multiples of 8; out may be x itself,
  * else they do not overlap. D and rot multiples of 8, rot <= D <= 256. 16-byte aligned x, out, weight.
  *
  * hn_cache_append_rotated: hn_cache_append of R(pos) norm(k) and v, and R(pos) norm(q) into out [B, n, H, 128], dense bf16. pos
  *   NULL: a token's place in its row (the first is 0); else [B, n] as above. q, k, v bf16 as in hn_cache_append; norm weights [128]
- *   or NULL each. K is rounded once, to the cache's format. q is rotated for rows that are left out, too.
+ *   or NULL each, both of one type. K is rounded once, to the cache's format. q is rotated for rows that are left out, too.
  */
 int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype, const void *pos, int64_t p_bs, int64_t p_ls,
               int pos_wide, const int64_t *freq, int64_t rot, int layout, float factor, const void *weight, float eps, int64_t B,
