@@ -84,18 +84,12 @@ template <bool INTER> __device__ __forceinline__ void turn(const Turn &t, float 
     }
 }
 
-// eight or four columns to fp32, and back with one rounding
+// eight or four columns to fp32 (of heads bf16, of norm weights fp32, too), and back with one rounding
 __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) { Elem<__nv_bfloat16>::load8(p, v); }
-__device__ __forceinline__ void load8(const __half *p, float (&v)[8]) { Elem<__half>::load8(p, v); }
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) { Elem<float>::load8(p, v); }
 __device__ __forceinline__ void load4(const __nv_bfloat16 *p, float *v) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
     v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
-}
-__device__ __forceinline__ void load4(const __half *p, float *v) {
-    uint2 w = *reinterpret_cast<const uint2 *>(p);
-    const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&w.y));
-    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
 }
 __device__ __forceinline__ void load4(const float *p, float *v) {
     const float4 w = *reinterpret_cast<const float4 *>(p);
