@@ -1,8 +1,9 @@
 // rotary.cuh - positions to rotations: what the rotation kernel and the rotating append share.
 //
 // The angle of pair i at position t is t f_i, and only its part of a turn matters. f_i is held as a fraction of a turn in 64
-// bits, so t f_i modulo one turn is the wrapped 64-bit product: exact for any position, where an fp32 product would be off by
-// t 2^-25 turns. Its upper 32 bits, signed, go to sincospi in fp32 (2^-25 of half a turn).
+// bits, so t f_i modulo one turn is the wrapped 64-bit product, which rounds nothing: what f_i was rounded by counts t times, t 2^-65
+// of a turn (an fp32 product would be off by t 2^-25). Its upper 32 bits, signed, go to sincospi in fp32 (2^-25 of half a
+// turn, so that far positions are turned as well as the first ones up to 2^39).
 #pragma once
 #include "hn_common.cuh"
 

@@ -2,7 +2,7 @@
 
 `fused.qk_norm_rope` and `fused.pixelumm_qk` take tables of cos and sin [tokens, 128], as the reference makes them
 (hy_nomas/fused.py:65-186). Here a call takes the tokens' positions, so that no table is made or read, and a token far into
-a long context is turned as exactly as the first:
+a long context is turned as exactly as the first (up to position 2^39; a frequency is held to 2^-65 of a turn):
 
     rot = Rotary(128, theta=10000.0, layout="half")                          # once
     q = rotate(q, positions, rot, q_norm)                                    # RMSNorm per head, then the rotation
@@ -11,6 +11,7 @@ a long context is turned as exactly as the first:
 Inference only, as the rest of the framework.
 """
 import math
+from decimal import Context, Decimal, localcontext
 
 import torch
 
@@ -22,14 +23,14 @@ _FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SCALINGS = {"linear": {"factor"}, "ntk": {"factor"}, "yarn": {"factor", "original", "beta_fast", "beta_slow", "attention_factor"}}
 
 
-def frequencies(dim, theta=10000.0, scaling=None):
-    """(radians per position of the dim / 2 pairs in 64 bits, on the CPU; the factor on cos and sin). `scaling`: None, or a dict
-    {"type": ..., "factor": f}:
-      "linear"  positions divided by f
-      "ntk"     theta * f^(dim / (dim - 2)): the slowest pair is slowed f times, the fastest kept
-      "yarn"    (Peng et al., arXiv 2309.00071) pairs that turn more than `beta_fast` (32) times over `original` positions are kept,
-                those that turn less than `beta_slow` (1) times are slowed f times, a ramp between; cos and sin times
-                `attention_factor` (0.1 ln f + 1)"""
+# enough digits for 64 bits of a turn of frequencies up to 1e20 radians a position
+_EXACT = Context(prec=60)
+_TURN = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+def _radians(dim, theta, scaling):
+    """`frequencies` with the radians as Decimals: a double's 53 bits would leave the fixed-point ones some 2^-56 of a turn a
+    position off."""
     if dim < 8 or dim > 256 or dim % 8:
         raise ValueError(f"rotary: {dim} rotated columns (a multiple of 8 up to 256)")
     if not (math.isfinite(theta) and theta > 1):
@@ -42,24 +43,37 @@ def frequencies(dim, theta=10000.0, scaling=None):
         raise ValueError(f"rotary: scaling {kind} with {sorted(scaling)}")
     if any(not (math.isfinite(v) and v > 0) for v in scaling.values()):
         raise ValueError(f"rotary: scaling {scaling} must be positive numbers")
-    i = torch.arange(dim // 2, dtype=torch.float64)
-    factor = scaling.get("factor", 1.0)
-    if kind == "ntk":
-        theta = theta * factor ** (dim / (dim - 2))
-        if theta <= 1:
-            raise ValueError(f"rotary: ntk factor {factor} leaves theta {theta}")
-    freq = theta ** (-2.0 * i / dim)
-    if kind == "linear":
-        freq = freq / factor
-    if kind != "yarn":
-        return freq, 1.0
+    theta, factor = float(theta), float(scaling.get("factor", 1.0))
+    with localcontext(_EXACT):
+        base, by = Decimal(theta).ln(), Decimal(factor)
+        if kind == "ntk":
+            base += by.ln() * dim / (dim - 2)
+            if base <= 0:
+                raise ValueError(f"rotary: ntk factor {factor} leaves theta {float(base.exp())}")
+        freq = [(-2 * i * base / dim).exp() for i in range(dim // 2)]
+        if kind == "linear":
+            freq = [f / by for f in freq]
+        if kind != "yarn":
+            return freq, 1.0
 
-    def column(turns):      # the (fractional) pair that turns so many times over the original context, in columns / 2
-        return dim * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
-    low = max(math.floor(column(scaling.get("beta_fast", 32.0))), 0)
-    high = min(math.ceil(column(scaling.get("beta_slow", 1.0))), dim - 1)
-    ramp = ((i - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
-    return freq * (1 - ramp) + freq / factor * ramp, scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0)
+        def column(turns):      # the (fractional) pair that turns so many times over the original context, in columns / 2
+            return dim * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(column(scaling.get("beta_fast", 32.0))), 0)
+        high = min(math.ceil(column(scaling.get("beta_slow", 1.0))), dim - 1)
+        ramp = [min(max((i - low) / Decimal(max(high - low, 0.001)), Decimal(0)), Decimal(1)) for i in range(dim // 2)]
+        return [f * (1 - r) + f / by * r for f, r in zip(freq, ramp)], scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0)
+
+
+def frequencies(dim, theta=10000.0, scaling=None):
+    """(radians per position of the dim / 2 pairs in 64 bits, on the CPU; the factor on cos and sin). `scaling`: None, or a dict
+    {"type": ..., "factor": f}:
+      "linear"  positions divided by f
+      "ntk"     theta * f^(dim / (dim - 2)): the slowest pair is slowed f times, the fastest kept
+      "yarn"    (Peng et al., arXiv 2309.00071) pairs that turn more than `beta_fast` (32) times over `original` positions are kept,
+                those that turn less than `beta_slow` (1) times are slowed f times, a ramp between; cos and sin times
+                `attention_factor` (0.1 ln f + 1)"""
+    freq, factor = _radians(dim, theta, scaling)
+    return torch.tensor([float(f) for f in freq], dtype=torch.float64), factor
 
 
 class Rotary:
@@ -70,19 +84,22 @@ class Rotary:
         if layout not in LAYOUTS:
             raise ValueError(f"Rotary: layout {layout!r} (half or interleaved)")
         if freq is None:
-            freq, factor = frequencies(dim, theta, scaling)
+            radians, factor = _radians(dim, theta, scaling)
+            freq = torch.tensor([float(f) for f in radians], dtype=torch.float64)
         else:
             if scaling is not None:
                 raise ValueError("Rotary: freq and scaling")
-            frequencies(dim)                                    # the checks of dim
+            _radians(dim, 10000.0, None)                        # the checks of dim
             freq = torch.as_tensor(freq, dtype=torch.float64).cpu()
             if freq.shape != (dim // 2,) or not bool(torch.isfinite(freq).all()):
                 raise ValueError(f"Rotary: freq must be {dim // 2} finite numbers")
+            radians = [Decimal(f) for f in freq.tolist()]
         if not math.isfinite(factor):
             raise ValueError(f"Rotary: factor {factor}")
         self.dim, self.layout, self.factor, self.radians = dim, layout, float(factor), freq
-        # fractions of a turn times 2^64, as signed 64-bit integers: what is past a whole turn does not matter
-        turns = [round(math.ldexp(f / (2 * math.pi), 64)) % 2 ** 64 for f in freq.tolist()]
+        # fractions of a turn times 2^64, to the nearest, as signed 64-bit integers: what is past a whole turn does not matter
+        with localcontext(_EXACT):
+            turns = [int((f / _TURN * 2 ** 64).to_integral_value()) % 2 ** 64 for f in radians]
         self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
         self._args = (dim, LAYOUTS[layout], self.factor)
 
