@@ -623,14 +623,14 @@ int hn_cache_copy(const hn_kv_cache *cache, const int32_t *src, const int32_t *d
     return launched(launch_cache_copy(a, src, dst, (int)n, (cudaStream_t)stream), "hn_cache_copy launch");
 }
 
-// rows of 128 elements at b * bs + l * ls + h * hs that do not overlap: each stride is past what the smaller ones reach (a
+// rows of `width` elements at b * bs + l * ls + h * hs that do not overlap: each stride is past what the smaller ones reach (a
 // dimension of one has none)
-static bool rows_apart(int64_t B, int64_t bs, int64_t Lq, int64_t ls, int64_t H, int64_t hs) {
+static bool rows_apart(int64_t B, int64_t bs, int64_t Lq, int64_t ls, int64_t H, int64_t hs, int64_t width = 128) {
     int64_t n[3] = {B, Lq, H}, s[3] = {bs < 0 ? -bs : bs, ls < 0 ? -ls : ls, hs < 0 ? -hs : hs};
     for (int i = 0; i < 2; ++i)
         for (int j = 0; j < 2 - i; ++j)
             if (s[j] > s[j + 1]) { std::swap(s[j], s[j + 1]); std::swap(n[j], n[j + 1]); }
-    int64_t reach = 128;
+    int64_t reach = width;
     for (int i = 0; i < 3; ++i) {
         if (n[i] == 1) continue;
         if (s[i] < reach) return false;
@@ -883,6 +883,7 @@ int hn_rotate(const void *x, int64_t x_bs, int64_t x_ls, int64_t x_hs, int dtype
     REQUIRE(x && pos && out, HN_ERR_ARG, "hn_rotate: null pointer");
     REQUIRE(al16(x) && al16(out) && (x_bs | x_ls | x_hs | o_bs | o_ls | o_hs) % 8 == 0, HN_ERR_ALIGN,
             "hn_rotate: x and out must be 16-byte aligned, strides multiples of 8 elements");
+    REQUIRE(rows_apart(B, o_bs, L, o_ls, H, o_hs, D), HN_ERR_SHAPE, "hn_rotate: the heads of out overlap");
     CHECK_DEVICE(x);
     RotateArgs a;
     a.x = x; a.x_bs = x_bs; a.x_ls = x_ls; a.x_hs = x_hs;

@@ -171,6 +171,16 @@ def _span(t):
     return at + lo * t.element_size(), at + (hi + 1) * t.element_size()
 
 
+def _apart(t):
+    """The heads of a tensor that is not empty do not overlap: each stride is past what the smaller ones reach."""
+    reach = t.shape[3]
+    for s, n in sorted((abs(s), n) for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+        if s < reach:
+            return False
+        reach += s * (n - 1)
+    return True
+
+
 def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
     """x [B, L, H, D] (bf16, fp16 or fp32; D a multiple of 8 up to 256; any strides in steps of 8 elements, the last dimension
     contiguous) at integer positions [B, L] or [L] -> [B, L, H, D] of x's dtype: RMSNorm over each head times `weight` [D] (bf16, fp16
@@ -197,7 +207,7 @@ def rotate(x, positions, rot, weight=None, eps=1e-6, out=None):
         if out.shape != x.shape or out.dtype != x.dtype or out.device != device or not _steps8(out):
             raise ValueError(f"rotate: out must be {x.dtype} {tuple(x.shape)} on {device} in steps of 8 elements, 16-byte aligned")
         if out.numel():
-            if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+            if not _apart(out):
                 raise ValueError("rotate: the heads of out overlap")
             same = out.data_ptr() == src.data_ptr() and out.stride() == src.stride()
             (a0, a1), (b0, b1) = _span(src), _span(out)

@@ -35,3 +35,19 @@ def test_far_positions(hn, cuda, layout, dim, theta):
         bound = (u.abs() + v.abs()) * (2.0 ** -20 + 2 * math.pi * abs(p) * 2.0 ** -65)
         assert bool(((out.double()[..., j] - (u * c - v * s)).abs() <= bound).all()), p
         assert bool(((out.double()[..., l] - (v * c + u * s)).abs() <= bound).all()), p
+
+
+def test_out_whose_heads_overlap_is_refused(hn, cuda):
+    from hy_nomas_b200 import rotary
+    rot, pos = rotary.Rotary(64), torch.arange(3, device="cuda")
+    base = randn((4096,), 1)
+    kept = base.clone()
+    x = randn((2, 3, 4, 64), 2)
+    for strides in ((768, 256, 56), (768, 192, 64), (256, 256, 64), (8, 1024, 64)):
+        out = base.as_strided((2, 3, 4, 64), strides + (1,))
+        for src in (x, out):                                    # another tensor, and in place
+            with pytest.raises(ValueError, match="overlap"):
+                rotary.rotate(src, pos, rot, out=out)
+    assert torch.equal(base, kept)
+    out = base.as_strided((2, 3, 4, 64), (64, 512, 128, 1))     # batches between heads: apart
+    assert torch.equal(rotary.rotate(x, pos, rot, out=out), rotary.rotate(x, pos, rot))

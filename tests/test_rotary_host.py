@@ -40,6 +40,22 @@ def test_layout_tells_the_weights_type(hn, paged):
         refused(hn, name, good, [(dict(layout=16, **{"w" if name == "hn_rotate" else "wq": FAKE + 8}), 2)])
 
 
+@pytest.mark.parametrize("strides,apart", [
+    ((1536, 512, 128), True), ((512, 1024, 128), True), ((128, 1024, 256), True), ((1536, 128, 384), True), ((-1536, -512, -128), True),
+    ((1536, 512, 64), False), ((1536, 512, 0), False), ((512, 512, 128), False), ((1024, 512, 128), False), ((0, 512, 128), False),
+    ((1536, 384, 128), False), ((120, 1024, 256), False), ((-1536, -504, 128), False)])
+def test_rotate_refuses_heads_of_out_that_overlap(hn, strides, apart):
+    """B = 2, L = 3, H = 4 heads of 128: refused in the library and seen in the Python layer."""
+    from hy_nomas_b200 import rotary
+    if not apart:
+        good = rotate_args()
+        refused(hn, "hn_rotate", good, [(dict(zip(("ob", "ol", "oh"), strides)), 1)])
+    low = -sum(min(0, s * (n - 1)) for s, n in zip(strides, (2, 3, 4)))
+    if low == 0:
+        assert rotary._apart(torch.empty(8192).as_strided((2, 3, 4, 128), strides + (1,))) == apart
+    assert rotary._apart(torch.empty(8192).as_strided((1, 1, 1, 128), (0, 8, 0, 1)))
+
+
 PI = Fraction(3141592653589793238462643383279502884197, 10 ** 39)           # cut, so pi is less than 10^-39 above
 
 
