@@ -25,7 +25,7 @@ _SCALINGS = {"linear": {"factor"}, "ntk": {"factor"}, "yarn": {"factor", "origin
 
 # enough digits for 64 bits of a turn of frequencies up to 1e20 radians a position
 _EXACT = Context(prec=60)
-_TURN = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+_UNITS = _EXACT.divide(2 ** 63, Decimal("3.14159265358979323846264338327950288419716939937510582097494459"))    # of a radian: 2^64 a turn
 
 
 def _radians(dim, theta, scaling):
@@ -50,7 +50,10 @@ def _radians(dim, theta, scaling):
             base += by.ln() * dim / (dim - 2)
             if base <= 0:
                 raise ValueError(f"rotary: ntk factor {factor} leaves theta {float(base.exp())}")
-        freq = [(-2 * i * base / dim).exp() for i in range(dim // 2)]
+        # powers of one ratio: 127 more roundings of 60 digits, and an exponential each would be most of a Rotary's time (2 ms)
+        step, freq = (-2 * base / dim).exp(), [Decimal(1)]
+        for _ in range(dim // 2 - 1):
+            freq.append(freq[-1] * step)
         if kind == "linear":
             freq = [f / by for f in freq]
         if kind != "yarn":
@@ -99,8 +102,8 @@ class Rotary:
         self.dim, self.layout, self.factor, self.radians = dim, layout, float(factor), freq
         # fractions of a turn times 2^64, to the nearest, as signed 64-bit integers: what is past a whole turn does not matter
         with localcontext(_EXACT):
-            turns = [int((f / _TURN * 2 ** 64).to_integral_value()) % 2 ** 64 for f in radians]
-        self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+            turns = [int((f * _UNITS).to_integral_value()) for f in radians]
+        self.freq = torch.tensor([(t + 2 ** 63) % 2 ** 64 - 2 ** 63 for t in turns], dtype=torch.int64, device=device)
         self._args = (dim, LAYOUTS[layout], self.factor)
 
 

@@ -8,6 +8,7 @@ from test_gpu_fp4 import VALUES, check_product, operands, randn, unpack
 
 pytestmark = pytest.mark.gpu
 SIZES = [(1, 130, 256), (2, 130, 256), (5, 130, 256), (300, 257, 96), (2500, 2400, 96)]
+PARTS = [(48, 300, 1024), (48, 300, 2048), (48, 300, 4096)]         # K over two, four and eight CTAs
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -38,7 +39,7 @@ def test_powers_far_apart_block_by_block(hn, cuda, m, n, k):
     assert torch.equal(out, (va @ vw.t() * 2.0 ** 98).float())
 
 
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + PARTS)
 def test_large_activations_small_weights(hn, cuda, m, n, k):
     """From the quantizer on: rows near 2^126 against weights near 2^-30, mxfp4."""
     x, y = randn((m, k), 1, loud=False).float() * 2.0 ** 124, randn((n, k), 2, loud=False).float() * 2.0 ** -30
@@ -47,7 +48,7 @@ def test_large_activations_small_weights(hn, cuda, m, n, k):
         check_product(hn, hn.kernels.fp4_gemm(*a, *w, kind="mxfp4", out_dtype=dtype), a, w, "mxfp4")
 
 
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + PARTS)
 def test_every_e4m3_scale(hn, cuda, m, n, k):
     """Block scales from all bytes 0 to 126: zero, the subnormals, 448."""
     a, w = operands(hn, m, n, k, "nvfp4", 42)
@@ -80,7 +81,7 @@ def test_nan_scale(hn, cuda, kind, nan, m, n, k):
     assert bool(out[bad].isnan().all()) and torch.equal(out[~bad], clean[~bad])
 
 
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + PARTS)
 def test_row_scales_far_apart(hn, cuda, m, n, k):
     """nvfp4 rows of activations near 2^120 against weights near 2^-60, and the other way: the sum times the larger row scale alone
     leaves fp32, the output does not."""
