@@ -28,7 +28,8 @@ constexpr int KB = 256;                         // columns of a stage: 128 bytes
 // launch, the same bits every time. Bound by latency: a stage's round trip is 1.8 us, so that a lone CTA has six of them (3 x 36 KB:
 // 0.6 us a step of 256 columns), and what does not depend on K, launch to store, is 6 us. Measured (us): 48 x 8192 x 4096 MX 9.9,
 // 777 x 5001 x 2080 NV fp32 out 17; the sums' reduction is 1 us of the former (its loads from the other CTAs go out together). Long K:
-// 0.32 us a step of 36 KB, all that an SM takes from L2. 128 x 256 outputs a CTA, one an SM, take a quarter less from L2, and the
+// 0.32 us a step of 36 KB, some 60 bytes a clock and SM, the most seen here. 48 x 8192 x 4096 from HBM (24 sets of operands in turn):
+// 11.1 (NV 12.4, from L2 10.8). 128 x 256 outputs a CTA, one an SM, take a quarter less from L2, and the
 // issuer's 12 copies of scales a step eat that up (2048 x 2048 x 4096 19.6 -> 21.7).
 template <int KIND, int STAGES_> struct Cfg {
     static constexpr int BM = 128, BN = 128, STAGES = STAGES_;
@@ -316,9 +317,11 @@ __global__ void __launch_bounds__(Cfg<KIND, STAGES>::THREADS, Cfg<KIND, STAGES>:
 //                   rounds and writes, beside the next tile's MMAs; 32 bytes of a row at a time go through shared memory, so that a
 //                   row's outputs leave as whole sectors, 16 bytes a store or as many as N and the rows' starts allow
 //                   (18944 rows, K = 4096: N = 4096 158 us, 4100 168, 4094 161, 4095 176; all but the first 217 - 229 one by one)
-// Bound by what an SM takes from L2: a step brings 38 KB to each (MX 35), which is 76 (70) bytes a clock at the MMAs' rate of 512
-// clocks a step. Counters (NV, 9472 x 2048 x 16384): 48 bytes a clock over the kernel, tensor pipe active 63%; NV and MX times are
-// to one another as these bytes. Measured, 18944 x 4096 x 16384 (16 tiles a pair, 1024 steps): NV 498 us (5.1 PFLOP/s), MX 456;
+// Bound by the operands' way from L2, whether by its latency or by an SM's port is open. A step brings 38 KB to each SM (MX 35), 76
+// (70) bytes a clock at the MMAs' rate of 512 clocks a step; 48 arrive (counters, NV, 9472 x 2048 x 16384: tensor pipe active
+// 63%, L2 44%), NV and MX times are to one another as these bytes, and the port has been seen to give 60 (the tiles above). For
+// latency: the 160 KB of codes under way over a round trip of 1.8 us are 48 bytes a clock, scales sent for further ahead were worth 8%,
+// and codes released later cost 8%. Measured, 18944 x 4096 x 16384 (16 tiles a pair, 1024 steps): NV 498 us (5.1 PFLOP/s), MX 456;
 // 15% more under the power limit of a long run. A tile's end costs 2 us (the wake of the epilogue, tensor memory's read 0.4, the
 // issuer's wake). How far the scales' loads run ahead counts: 4 slots 536 us, 8 slots 491 (another GPU). All warps of the epilogue
 // looking for the sums: 510; sleeps between the other looks change nothing. Groups of 8 column tiles (the rule below: 16 here): 520, of

@@ -11,7 +11,8 @@
 // than 16384 columns are read twice. A chunk is a block of NV and half a block of MX; the lanes of a scale tile's word (4 or
 // 8) gather its bytes before the one store. Measured, 20240 x 4096 bf16: MX 32 us (6.5 TB/s), NV 41 us (5.2 TB/s: its twelve
 // instructions a column, four of them the exact quotient, are what is left; a persistent loop over rows with the next one's loads
-// ahead did not help). Back to bf16: 35 us (6.0 TB/s, 16 bytes out a thread and chunk, up to
+// ahead did not help). Rows that start on 4 or 8 bytes: 40000 x 1500 44 us (floor 23), 20240 x 4100 65; on odd elements 20240 x 4095 96, of
+// fp32 163 (floor 58): one element a load. Back to bf16: 35 us (6.0 TB/s, 16 bytes out a thread and chunk, up to
 // four chunks' loads under way). One row of 4096: 2.6 us, a launch.
 #include "fp4.cuh"
 #include "hn_kernels.h"
@@ -280,7 +281,10 @@ template <typename E, int KIND, int VEC, int T, int NCH> cudaError_t go(const Pa
     return cudaGetLastError();
 }
 
-// T and NCH by the row's length alone: the fewest chunks that hold it
+// T and NCH by the row's length alone: the fewest chunks that hold it. Measured, bf16, NV (MX), us: fewer than 32 threads a row against
+// 32 for all: 400000 x 32 9 (7) / 130 (93), 400000 x 128 32 (24) / 132 (95), 300000 x 256 46 (34) / 100 (73). Three chunks against the
+// next power of two: 60000 x 1040 47 (35) / 60 (42), 30000 x 3008 47 (38) / 59 (42), 12000 x 6000 41 (31) / 48 (35),
+// 6000 x 12000 45 (30) / 67 (34)
 template <typename E, int KIND, int VEC> cudaError_t pick(const Params &p, cudaStream_t st) {
     if (p.nch <= 2) return go<E, KIND, VEC, 2, 1>(p, st);
     if (p.nch <= 4) return go<E, KIND, VEC, 4, 1>(p, st);

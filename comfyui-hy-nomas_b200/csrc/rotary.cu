@@ -9,7 +9,7 @@
 // are turned. Heads and rotated parts of a multiple of 16: sixteen columns a lane, chosen so that whole pairs are a lane's own,
 // on packed arithmetic (20240 tokens x 32 heads of 128, bf16, with the norm: 58 us, 5.7 TB/s; one token: 2.5 us). Others: eight
 // columns a lane, and in the half layout, whose partner stands in another lane, possibly from the middle of its columns on, the
-// partners are loaded again, from L1 (128 with 120 rotated: 80 us).
+// partners are loaded again, from L1 (128 with 120 rotated: 82 us, interleaved 75; 136 columns, 17 of 32 lanes at work: 142 and 127).
 #include "hn_kernels.h"
 #include "rotary.cuh"
 
@@ -221,7 +221,8 @@ struct AppendParams {
 
 // The rules of the plain append: a row whose last extend was refused, a page that several rows name, a row's listings after the
 // first keep what they hold, counted. q is rotated whatever becomes of the row. A unit is a warp's share of a token: some of
-// its q, k and v heads, in that order, two at a time (16 lanes each).
+// its q, k and v heads, in that order, two at a time (16 lanes each). Without loads ahead: 2 x 4400 tokens, 16 + 16 + 16 heads, 120 of
+// 128 columns rotated: bf16 116 us, int8 133.
 template <bool I8> __global__ void __launch_bounds__(32 * AWARPS) k_append_rotated(AppendParams p, Meta m) {
     __shared__ float tables[AWARPS][2 * MAX_PAIRS];
     const int lane = threadIdx.x & 31, sub = lane & 15, side = lane >> 4;
@@ -327,10 +328,11 @@ __device__ __forceinline__ void put_codes(uint8_t *o, float *scale, const Lane16
     if (lead) *scale = sc;
 }
 
-// ... with rotated parts of a multiple of 16: sixteen columns a lane, four heads of one kind (q, k or v) a pass. Bound by
-// instructions, not by HBM, the int8 quantizer's above all (half of its cycles issue one), so each kind has a loop of its own,
-// whose addresses only step on. 2 x 4400 tokens, 16 + 16 + 16 heads, int8: 53 us of 28 for the bytes (61 with one loop that asks
-// for the kind); loads further ahead, through shared memory, and more warps of fewer registers changed nothing or cost more.
+// ... with rotated parts of a multiple of 16: sixteen columns a lane, four heads of one kind (q, k or v) a pass. Each kind
+// has a loop of its own, whose addresses only step on (61 us with one loop that asks for the kind). 2 x 4400 tokens, 16 + 16 + 16
+// heads: int8 52 us of 28 for the bytes, bf16 51 of 33. So it is neither the quantizer nor HBM that bounds it: half of the issue slots
+// are empty, and the 16 warps of an SM wait for their chains (norm, turn, peak, codes). Loads further ahead, through shared memory,
+// and more warps of fewer registers changed nothing or cost more.
 template <bool I8, bool INTER> __global__ void __launch_bounds__(32 * AWARPS, ACTAS) k_append_rotated16(AppendParams p, Meta m) {
     __shared__ __align__(16) float tables[AWARPS][2 * MAX_PAIRS];
     const int lane = threadIdx.x & 31, sub = lane & 7, side = lane >> 3;

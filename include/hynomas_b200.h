@@ -424,7 +424,7 @@ int hn_paged_attention(const hn_kv_cache *cache, int64_t layer, const void *q, i
  * span = 128 columns (HN_KIND_MXFP4) or 64 (HN_KIND_NVFP4); row r of a tile, group g: byte 16 (r % 32) + 4 (r / 32) + g. Groups
  * between Kp and the last tile's end hold zeros.
  *   HN_KIND_MXFP4: 2^(byte - 127) per 32 columns, byte 255: NaN; row scales NULL
- *   HN_KIND_NVFP4: e4m3 per 16 columns, and an fp32 scale per row (r, ra, rw [rows]; NULL in hn_fp4_gemm: all 1)
+ *   HN_KIND_NVFP4: e4m3 per 16 columns, its sign bit 0, and an fp32 scale per row (r, ra, rw [rows]; NULL in hn_fp4_gemm: all 1)
  *
  * hn_quantize_fp4: x [M, K] bf16, fp16 or fp32, rows ldx elements apart. MX: s = 2^(floor(log2 max|x|) - 2) of the group, 1 for
  *   zeros; codes of x / s, to the nearest, ties to the even code, beyond 6 to 6. NV: top = max|row|, r = top / 2688; s = e4m3((0.875
