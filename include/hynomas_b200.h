@@ -449,7 +449,7 @@ int hn_fp4_gemm(const void *qa, int64_t lda, const void *sa, const float *ra, co
  * pass. layout HN_ROPE_*. weight [D] bf16, or fp32 with HN_ROPE_NORM_FP32 in layout, or NULL: no norm. pos int32, or int64 with
  * pos_wide 1; any sign.
  * x, out [B, L, H, D] of `dtype` (bf16, fp16, fp32), element strides for batch, token, head, multiples of 8; out may be x itself,
- * else they do not overlap. D and rot multiples of 8, rot <= D <= 256. 16-byte aligned x, out, weight.
+ * else they do not overlap; out's heads lie apart. D and rot multiples of 8, rot <= D <= 256. 16-byte aligned x, out, weight.
  *
  * hn_cache_append_rotated: hn_cache_append of R(pos) norm(k) and v, and R(pos) norm(q) into out [B, n, H, 128], dense bf16. pos
  *   NULL: a token's place in its row (the first is 0); else [B, n] as above. q, k, v bf16 as in hn_cache_append; norm weights [128]
